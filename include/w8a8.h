@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define W8A8_ABI_VERSION 14
+#define W8A8_ABI_VERSION 15
 
 typedef enum w8a8_status {
   W8A8_OK = 0,
@@ -504,12 +504,217 @@ int w8a8_dequantize(const W8A8DequantArgs* args);
 int w8a8_segment_labels(const int32_t* ends, const int32_t* values, int64_t count, int32_t* labels, int64_t rows,
                         void* stream);
 
-/* ABI version (W8A8_ABI_VERSION; 14 added w8a8_segment_labels). */
+/*
+ * The residual stream between two blocks, in one pass: the update by a
+ * block's branch (its own RMS norm, gate and scales), then the next block's
+ * RMS norm with its modulation, to normalized rows or INT8 codes.
+ * Replaces: patches/h3_tensor_flow.py:130-152 (residual_add, gated_add)
+ *   followed by :134-142 (modulated_norm), where the update cannot ride in a
+ *   GEMM epilogue: after the SUM exchange of rank partials, or behind a norm
+ *   of the branch (no counterpart in the reference).
+ * x: [rows, cols] F16 or BF16 (ldx); branch: [rows, cols] of branch_dtype
+ *   (x's, or F32), row stride ldb. Per row, in fp32 (round to nearest even):
+ *   n    = branch, or with post != 0 (branch * pinv) * post_weight,
+ *          pinv = 1 / sqrt(sum(branch^2) * fp32(1/cols) + post_eps)
+ *   u    = n * branch_scale;  r = x * residual_scale
+ *   x'   = x_dtype(gate ? fma(u, gate[l], r) : r + u)
+ *   then y, q and q_scale are those of w8a8_norm_quantize on the rows x'.
+ * sum(branch^2): the 16 squares of each unit of w8a8_norm_quantize's order in
+ *   order, each 64 units' partials in its butterfly, these sums in order.
+ * post_weight: optional [cols] fp32. gate: optional fp32 [gate_rows, ld_gate];
+ *   labels: int32 [rows], each row's row of gate, mod_shift and mod_scale
+ *   (clamped into each table's range).
+ * out: [rows, cols] x_dtype, the updated rows x'; may be x itself
+ *   (ldo == ldx), and may not otherwise overlap an input.
+ * y and q NULL: the update alone. weight, mod_shift, mod_scale, ld_mod,
+ *   mod_rows, eps, y, ldy, convrot, round_rotated, q, ldq, q_scale,
+ *   convrot_signs: as in W8A8NormArgs; y may not overlap x or branch.
+ * Requirements: as w8a8_norm_quantize, for every array.
+ */
+typedef struct W8A8ResidualNormArgs {
+  uint32_t struct_size;
+  int32_t x_dtype;
+  const void* x;
+  int64_t ldx;
+  int64_t rows;
+  int64_t cols;
+  const void* branch;
+  int64_t ldb;
+  int32_t branch_dtype;
+  int32_t post;
+  const float* post_weight;
+  float post_eps;
+  float branch_scale;
+  float residual_scale;
+  int32_t gate_rows;
+  const float* gate;
+  int64_t ld_gate;
+  const int32_t* labels;
+  void* out;
+  int64_t ldo;
+  const float* weight;
+  const float* mod_shift;
+  const float* mod_scale;
+  int64_t ld_mod;
+  int32_t mod_rows;
+  float eps;
+  void* y;
+  int64_t ldy;
+  int32_t convrot;
+  int32_t round_rotated;
+  int8_t* q;
+  int64_t ldq;
+  float* q_scale;
+  const uint32_t* convrot_signs;
+  void* stream;
+} W8A8ResidualNormArgs;
+
+int w8a8_residual_norm(const W8A8ResidualNormArgs* args);
+
+/*
+ * Rotary positions with several axes (time, height, width, ...) of Q and K,
+ * optionally after a per-head RMS norm. Where w8a8_rms_rope reads rotation
+ * matrices of every row, this takes the rows' positions.
+ * q: [rows, q_heads, dim], k: [rows, k_heads, dim] (NULL with k_heads 0) of
+ *   dtype (F16, BF16 or F32), element strides {row, head}, channels
+ *   contiguous; q_out and k_out likewise, of the same dtype; an output may be
+ *   its own input (same strides), and may not otherwise overlap an input.
+ * positions: [rows, axes] of pos_type, element strides {row, axis}.
+ * inv_freq: [pairs] fp64, axis: [pairs] int32 in [0, axes) (clamped); pair p
+ *   of a row turns by phi = position[axis[p]] * inv_freq[p], in fp64 to the
+ *   fraction of a revolution, whose sine and cosine are fp32:
+ *   (a, b) -> (a cos - b sin, b cos + a sin), where (a, b) is
+ *   W8A8_ROPE_HALF:     (x[p], x[p + pairs])
+ *   W8A8_ROPE_ADJACENT: (x[2p], x[2p + 1])
+ *   and channels from 2 * pairs on keep their value.
+ * q_gain, k_gain: optional [dim] fp32 (both or neither; k_gain only with k);
+ *   with them x is first (x * inv) * gain,
+ *   inv = 1 / sqrt(sum(x^2) * fp32(1/dim) + eps).
+ * All in fp32 (products and sums contracted to FMAs as written in the
+ *   kernel), rounded once at the end.
+ * Requirements: 2 <= dim <= 256 and even, 1 <= pairs <= dim / 2,
+ *   1 <= axes <= 16; every array aligned to its elements.
+ */
+enum { W8A8_ROPE_HALF = 0, W8A8_ROPE_ADJACENT = 1 };
+enum { W8A8_POS_I32 = 0, W8A8_POS_I64 = 1, W8A8_POS_F32 = 2 };
+typedef struct W8A8AxialRopeArgs {
+  uint32_t struct_size;
+  int32_t dtype;
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t rows;
+  int32_t q_heads;
+  int32_t k_heads;
+  int32_t dim;
+  int32_t pairs;
+  int32_t axes;
+  int32_t pairing;
+  int64_t q_strides[2];
+  int64_t k_strides[2];
+  int64_t q_out_strides[2];
+  int64_t k_out_strides[2];
+  const void* positions;
+  int64_t pos_strides[2];
+  int32_t pos_type;
+  float eps;
+  const double* inv_freq;
+  const int32_t* axis;
+  const float* q_gain;
+  const float* k_gain;
+  void* stream;
+} W8A8AxialRopeArgs;
+
+int w8a8_axial_rope(const W8A8AxialRopeArgs* args);
+
+/*
+ * The rotation matrices of the same positions, in the layouts that
+ * w8a8_rms_rope and the QKV epilogue read: freqs [rows, pairs, 2, 2]
+ * (W8A8_ROPE_MATRICES: cos, -sin, sin, cos) or [rows, 2, pairs, 2]
+ * (W8A8_ROPE_PAIRS: (cos, -sin) of every pair, then (cos, sin)) of freq_dtype
+ * (F16 or F32), contiguous. Other fields as in W8A8AxialRopeArgs.
+ */
+typedef struct W8A8AxialFreqsArgs {
+  uint32_t struct_size;
+  int32_t freq_dtype;
+  int32_t freq_layout;
+  int32_t pos_type;
+  const void* positions;
+  int64_t pos_strides[2];
+  int64_t rows;
+  int32_t pairs;
+  int32_t axes;
+  const double* inv_freq;
+  const int32_t* axis;
+  void* freqs;
+  void* stream;
+} W8A8AxialFreqsArgs;
+
+int w8a8_axial_freqs(const W8A8AxialFreqsArgs* args);
+
+/*
+ * Projection with 4-bit weights and group scales, 16-bit activations. No
+ * counterpart in the reference (its projections are INT8): the text
+ * encoder's projections at few rows are bound by the bytes of their weights.
+ *   y[m][n] = sum over groups g of scale[g][n] *
+ *             sum over k in g of (code[n][k] - zero[g][n]) * x[m][k]
+ *   out = dtype(y [+ bias[n]] [+ residual[m][n]]), or with gated != 0, where
+ *   rows [0, n / 2) of the weight are gate and the others up,
+ *   out[m][j] = dtype(g / (1 + exp(-g)) * u), g = y[m][j] [+ bias[j]],
+ *   u = y[m][n / 2 + j] [+ bias[n / 2 + j]].
+ * Products are exact and sums, scales and the epilogue fp32; one rounding at
+ * the end. The same call gives the same bits every time.
+ * x: [m, k] F16 or BF16 (ldx); out, bias and residual of the same dtype.
+ * codes: [n, k / 8] words (ldw words a row); word i of a row holds inputs
+ *   8 i .. 8 i + 7: nibbles 0-3 (from the low end) inputs 0, 2, 4, 6, nibbles
+ *   4-7 inputs 1, 3, 5, 7 of the eight.
+ * scales: [k / group, n] of dtype, contiguous; zeros: [k / group, n] uint8
+ *   (0..15), contiguous, or NULL: 8.
+ * workspace: device buffer of at least w8a8_linear_w4_workspace_size() bytes
+ *   (16-byte aligned, any contents; NULL where that is 0) for calls too small
+ *   to fill the GPU, which split k. Calls that share one must not overlap;
+ *   calls in sequence may, and a captured graph may replay it.
+ * Requirements: group 32, 64 or a multiple of 128, k % group == 0; gated:
+ *   n even, no residual; x and codes 16-byte aligned, ldx % 8 == 0,
+ *   ldw % 4 == 0.
+ */
+typedef struct W8A8LinearW4Args {
+  uint32_t struct_size;
+  int32_t dtype;
+  const void* x;
+  int64_t ldx;
+  const int32_t* codes;
+  int64_t ldw;
+  const void* scales;
+  const uint8_t* zeros;
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  int32_t group;
+  int32_t gated;
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* out;
+  int64_t ldo;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} W8A8LinearW4Args;
+
+int w8a8_linear_w4(const W8A8LinearW4Args* args);
+
+/* Workspace bytes of w8a8_linear_w4 for these sizes on the current device. */
+int64_t w8a8_linear_w4_workspace_size(int64_t m, int64_t n, int64_t k, int32_t group, int32_t gated);
+
+/* ABI version (W8A8_ABI_VERSION; 14 added w8a8_segment_labels, 15
+ * w8a8_residual_norm, w8a8_axial_rope, w8a8_axial_freqs and w8a8_linear_w4). */
 int w8a8_abi_version(void);
 
 /* sizeof of each argument struct, by index: 0 Quant, 1 Swiglu, 2 Gemm,
- * 3 Dequant, 4 Norm, 5 RmsRope, 6 AttnPrepare, 7 Attention; -1 for an
- * unknown index. Lets bindings verify their layout. */
+ * 3 Dequant, 4 Norm, 5 RmsRope, 6 AttnPrepare, 7 Attention, 8 ResidualNorm,
+ * 9 AxialRope, 10 AxialFreqs, 11 LinearW4; -1 for an unknown index. Lets bindings verify their layout. */
 int64_t w8a8_struct_size(int32_t which);
 
 /* Message describing the last error returned on the calling thread. */

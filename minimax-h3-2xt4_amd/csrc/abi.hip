@@ -26,6 +26,10 @@ static_assert(sizeof(W8A8NormArgs) == 152, "W8A8NormArgs layout");
 static_assert(sizeof(W8A8RmsRopeArgs) == 104, "W8A8RmsRopeArgs layout");
 static_assert(sizeof(W8A8AttnPrepareArgs) == 224, "W8A8AttnPrepareArgs layout");
 static_assert(sizeof(W8A8AttentionArgs) == 144, "W8A8AttentionArgs layout");
+static_assert(sizeof(W8A8ResidualNormArgs) == 232, "W8A8ResidualNormArgs layout");
+static_assert(sizeof(W8A8AxialRopeArgs) == 208, "W8A8AxialRopeArgs layout");
+static_assert(sizeof(W8A8AxialFreqsArgs) == 88, "W8A8AxialFreqsArgs layout");
+static_assert(sizeof(W8A8LinearW4Args) == 152, "W8A8LinearW4Args layout");
 
 extern "C" int w8a8_abi_version(void) { return W8A8_ABI_VERSION; }
 
@@ -39,6 +43,10 @@ extern "C" int64_t w8a8_struct_size(int32_t which) {
     case 5: return (int64_t)sizeof(W8A8RmsRopeArgs);
     case 6: return (int64_t)sizeof(W8A8AttnPrepareArgs);
     case 7: return (int64_t)sizeof(W8A8AttentionArgs);
+    case 8: return (int64_t)sizeof(W8A8ResidualNormArgs);
+    case 9: return (int64_t)sizeof(W8A8AxialRopeArgs);
+    case 10: return (int64_t)sizeof(W8A8AxialFreqsArgs);
+    case 11: return (int64_t)sizeof(W8A8LinearW4Args);
     default: return -1;
   }
 }

@@ -10,7 +10,7 @@
 // butterfly (offsets 32, 16, ..., 1); IEEE addition is commutative, so every
 // lane ends with the same total. rsqrtf is replaced by a correctly rounded
 // square root followed by a correctly rounded division.
-#include "w8a8_device.h"
+#include "norm_device.h"
 #include "w8a8_host.h"
 
 #include <type_traits>
@@ -45,59 +45,6 @@ struct NormParams {
 constexpr int kNormSigned = 4;
 template <int MODE>
 constexpr int rot_of() { return (MODE & 3) == 2 ? 1 : (MODE & 3) == 3 ? 2 : 0; }
-
-__device__ __forceinline__ void load16_f32(const float* p, float (&v)[16]) {
-  const float4* q = reinterpret_cast<const float4*>(p);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 t = q[i];
-    v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
-  }
-}
-
-// Table flags of a kernel: kGain (weight present), kMod (shift/scale
-// tables present), kAnyTables (decide per call from the pointers).
-enum NormTables { kGain = 1, kMod = 2, kAnyTables = 4 };
-
-// v: x on entry; on return the normalized, modulated value rounded to DT
-// (as fp32; times 1/16 when SCALED), with its storage bits packed in bits.
-template <int DT, int TB, bool SCALED>
-__device__ __forceinline__ void modulate16(float (&v)[16], uint32_t (&bits)[8], float inv, const float* w,
-                                           const float* sh, const float* sc, int64_t c0) {
-  const bool gain = (TB & kGain) || ((TB & kAnyTables) && w);
-  const bool mod = (TB & kMod) || ((TB & kAnyTables) && sh);
-  float wv[16], shv[16], scv[16];
-  if (gain) load16_f32(w + c0, wv);
-  if (mod) {
-    load16_f32(sc + c0, scv);
-    load16_f32(sh + c0, shv);
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float t = DT == kF16 ? mul_mix(v[i], inv) : v[i] * inv;
-    if (gain) t = t * wv[i];
-    if (mod) {
-      const float f = 1.0f + scv[i];
-      t = t * f;
-      t = t + shv[i];
-    }
-    v[i] = t;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if constexpr (DT == kF16) {
-      bits[i] = f2h2_of_f32(v[2 * i], v[2 * i + 1]);
-      v[2 * i] = h2f((uint16_t)(bits[i] & 0xffffu));
-      v[2 * i + 1] = h2f((uint16_t)(bits[i] >> 16));
-    } else {
-      const uint16_t lo = f2bf(v[2 * i]), hi = f2bf(v[2 * i + 1]);
-      bits[i] = (uint32_t)lo | ((uint32_t)hi << 16);
-      v[2 * i] = bf2f(lo);
-      v[2 * i + 1] = bf2f(hi);
-    }
-  }
-  if constexpr (SCALED) scale16(v);
-}
 
 // Waves per workgroup of the norm-only kernel with AdaLN tables: the
 // workgroup stages the gain and its first row's shift and scale rows in LDS,
@@ -419,12 +366,6 @@ static int launch_norm(const NormParams& p, hipStream_t stream) {
                        4 * (size_t)max(norm_lds_floats<MODE, kNormWaves, false>(0), 1), stream, p);
   }
   return launch_status("w8a8_norm_quantize");
-}
-
-// Whether [a, a + an) and [b, b + bn) share a byte.
-static bool spans_overlap(const void* a, int64_t an, const void* b, int64_t bn) {
-  const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
-  return pa < pb + (uintptr_t)bn && pb < pa + (uintptr_t)an;
 }
 
 }  // namespace w8a8

@@ -17,6 +17,31 @@ void set_error(const char* fmt, ...);
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+// Whether [a, a + an) and [b, b + bn) share a byte.
+inline bool spans_overlap(const void* a, int64_t an, const void* b, int64_t bn) {
+  const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+  return pa < pb + (uintptr_t)bn && pb < pa + (uintptr_t)an;
+}
+
+// The memory of rows of one stride, in bytes: a row's extent, and that of all.
+struct RowsOf {
+  const void* at;
+  int64_t row, extent, span;
+};
+
+inline RowsOf rows_of(const void* at, int64_t ld, int64_t rows, int64_t cols, int es) {
+  return {at, ld * es, cols * es, ((rows - 1) * ld + cols) * es};
+}
+
+// Whether two such views share no byte, as far as their spans and, for columns
+// of one buffer's rows, their columns tell.
+inline bool apart(const RowsOf& a, const RowsOf& b) {
+  if (!spans_overlap(a.at, a.span, b.at, b.span)) return true;
+  if (a.row != b.row || a.row == 0) return false;
+  const int64_t off = (((int64_t)((uintptr_t)b.at - (uintptr_t)a.at) % a.row) + a.row) % a.row;
+  return a.extent <= off && off + b.extent <= a.row;
+}
+
 inline int elem_size(int dt) {
   switch (dt) {
     case W8A8_F16: case W8A8_BF16: return 2;

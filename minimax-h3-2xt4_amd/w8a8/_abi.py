@@ -15,7 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / 'libw8a8.so'
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_LAUNCH = 0, 1, 2, 3
 F16, BF16, F32, I32, I8 = 1, 2, 3, 4, 5
 EPI_INT32, EPI_ROW, EPI_COLUMN = 0, 1, 2
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 _c = ctypes
 _p = ctypes.c_void_p
@@ -89,13 +89,54 @@ class AttentionArgs(ctypes.Structure):
                 ('out_strides', _c.c_int64 * 3), ('stream', _p)]
 
 
+class ResidualNormArgs(ctypes.Structure):
+    _fields_ = [('struct_size', _c.c_uint32), ('x_dtype', _c.c_int32), ('x', _p), ('ldx', _c.c_int64),
+                ('rows', _c.c_int64), ('cols', _c.c_int64), ('branch', _p), ('ldb', _c.c_int64),
+                ('branch_dtype', _c.c_int32), ('post', _c.c_int32), ('post_weight', _p), ('post_eps', _c.c_float),
+                ('branch_scale', _c.c_float), ('residual_scale', _c.c_float), ('gate_rows', _c.c_int32),
+                ('gate', _p), ('ld_gate', _c.c_int64), ('labels', _p), ('out', _p), ('ldo', _c.c_int64),
+                ('weight', _p), ('mod_shift', _p), ('mod_scale', _p), ('ld_mod', _c.c_int64),
+                ('mod_rows', _c.c_int32), ('eps', _c.c_float), ('y', _p), ('ldy', _c.c_int64),
+                ('convrot', _c.c_int32), ('round_rotated', _c.c_int32), ('q', _p), ('ldq', _c.c_int64),
+                ('q_scale', _p), ('convrot_signs', _p), ('stream', _p)]
+
+
+class AxialRopeArgs(ctypes.Structure):
+    _fields_ = [('struct_size', _c.c_uint32), ('dtype', _c.c_int32), ('q', _p), ('k', _p), ('q_out', _p),
+                ('k_out', _p), ('rows', _c.c_int64), ('q_heads', _c.c_int32), ('k_heads', _c.c_int32),
+                ('dim', _c.c_int32), ('pairs', _c.c_int32), ('axes', _c.c_int32), ('pairing', _c.c_int32),
+                ('q_strides', _c.c_int64 * 2), ('k_strides', _c.c_int64 * 2), ('q_out_strides', _c.c_int64 * 2),
+                ('k_out_strides', _c.c_int64 * 2), ('positions', _p), ('pos_strides', _c.c_int64 * 2),
+                ('pos_type', _c.c_int32), ('eps', _c.c_float), ('inv_freq', _p), ('axis', _p), ('q_gain', _p),
+                ('k_gain', _p), ('stream', _p)]
+
+
+class AxialFreqsArgs(ctypes.Structure):
+    _fields_ = [('struct_size', _c.c_uint32), ('freq_dtype', _c.c_int32), ('freq_layout', _c.c_int32),
+                ('pos_type', _c.c_int32), ('positions', _p), ('pos_strides', _c.c_int64 * 2), ('rows', _c.c_int64),
+                ('pairs', _c.c_int32), ('axes', _c.c_int32), ('inv_freq', _p), ('axis', _p), ('freqs', _p),
+                ('stream', _p)]
+
+
+class LinearW4Args(ctypes.Structure):
+    _fields_ = [('struct_size', _c.c_uint32), ('dtype', _c.c_int32), ('x', _p), ('ldx', _c.c_int64),
+                ('codes', _p), ('ldw', _c.c_int64), ('scales', _p), ('zeros', _p), ('m', _c.c_int64),
+                ('n', _c.c_int64), ('k', _c.c_int64), ('group', _c.c_int32), ('gated', _c.c_int32), ('bias', _p),
+                ('residual', _p), ('ldr', _c.c_int64), ('out', _p), ('ldo', _c.c_int64), ('workspace', _p),
+                ('workspace_bytes', _c.c_int64), ('stream', _p)]
+
+
 # Argument structs in w8a8_struct_size() index order, with their entry points.
 STRUCTS = (QuantArgs, SwigluArgs, GemmArgs, DequantArgs, NormArgs, RmsRopeArgs, AttnPrepareArgs, AttentionArgs)
 STRUCT_ENTRY_POINTS = ('w8a8_quantize_rows', 'w8a8_swiglu_quantize', 'w8a8_gemm', 'w8a8_dequantize',
                        'w8a8_norm_quantize', 'w8a8_rms_rope', 'w8a8_attention_prepare', 'w8a8_attention')
-ENTRY_POINTS = STRUCT_ENTRY_POINTS + ('w8a8_gemm_noalloc', 'w8a8_abi_version', 'w8a8_struct_size',
+# Those of the operators around the projections of a block follow (indices 8 on).
+BLOCK_STRUCTS = (ResidualNormArgs, AxialRopeArgs, AxialFreqsArgs, LinearW4Args)
+BLOCK_ENTRY_POINTS = ('w8a8_residual_norm', 'w8a8_axial_rope', 'w8a8_axial_freqs', 'w8a8_linear_w4')
+ENTRY_POINTS = STRUCT_ENTRY_POINTS + BLOCK_ENTRY_POINTS + ('w8a8_gemm_noalloc', 'w8a8_abi_version', 'w8a8_struct_size',
                                       'w8a8_last_error', 'w8a8_gemm_workspace_size',
-                                      'w8a8_attention_workspace_size', 'w8a8_segment_labels')
+                                      'w8a8_attention_workspace_size', 'w8a8_segment_labels',
+                                      'w8a8_linear_w4_workspace_size')
 GEMM_SCRATCH_BYTES = 64 << 20   # W8A8_GEMM_SCRATCH_BYTES: the no-allocation GEMM's split-K scratch per GPU
 
 _LIB = None
@@ -133,11 +174,14 @@ def load(path=None):
     lib.w8a8_attention_workspace_size.argtypes = [_c.c_int64, _c.c_int64, _c.c_int64]
     lib.w8a8_segment_labels.restype = _c.c_int
     lib.w8a8_segment_labels.argtypes = [_p, _p, _c.c_int64, _p, _c.c_int64, _p]
-    for name, st in zip(STRUCT_ENTRY_POINTS + ('w8a8_gemm_noalloc',), STRUCTS + (GemmArgs,)):
+    lib.w8a8_linear_w4_workspace_size.restype = _c.c_int64
+    lib.w8a8_linear_w4_workspace_size.argtypes = [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int32, _c.c_int32]
+    for name, st in zip(STRUCT_ENTRY_POINTS + BLOCK_ENTRY_POINTS + ('w8a8_gemm_noalloc',),
+                        STRUCTS + BLOCK_STRUCTS + (GemmArgs,)):
         fn = getattr(lib, name)
         fn.restype = _c.c_int
         fn.argtypes = [ctypes.POINTER(st)]
-    for i, st in enumerate(STRUCTS):
+    for i, st in enumerate(STRUCTS + BLOCK_STRUCTS):
         if lib.w8a8_struct_size(i) != ctypes.sizeof(st):
             raise RuntimeError(f'{st.__name__}: library size {lib.w8a8_struct_size(i)} != '
                                f'binding size {ctypes.sizeof(st)}')

@@ -571,3 +571,298 @@ def attention(prep, *, out_dtype=torch.float16, out=None):
                               stream=_abi.stream_of(q8))
     _abi.call('w8a8_attention', args)
     return out
+
+
+def _no_gradient(*tensors):
+    """The operators below have no backward pass (nothing here trains): an
+    input that asks for one is refused, so that no gradient is lost silently."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError('this operator has no gradient: detach its inputs or run under torch.no_grad()')
+
+
+def _vector(t, name, n):
+    """fp32 [n] contiguous and 16-byte aligned (None stays None)."""
+    if t is None:
+        return None
+    t = t.reshape(-1)
+    if t.dtype != torch.float32 or t.numel() != n:
+        raise ValueError(f'{name} must be float32 with {n} entries')
+    return _aligned16(t)
+
+
+def _aligned_rows(x, elem):
+    """A 2-D tensor whose rows start on 16-byte boundaries (a copy if need be)."""
+    x = _rows_2d(x)
+    if x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) * elem % 16 or x.stride(0) < x.shape[1])):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _ld(x):
+    """Row stride of a 2-D tensor; one row's is its length, rounded up to 16 bytes."""
+    if x.shape[0] > 1:
+        return x.stride(0)
+    per = 16 // x.element_size()
+    return -(-x.shape[1] // per) * per
+
+
+def residual_norm(x, branch, *, weight=None, eps=None, post_weight=None, post_eps=None, gate=None, shift=None,
+                  scale=None, labels=None, residual_scale=1.0, branch_scale=1.0, quantize=False, convrot=True,
+                  round_rotated=True, want_normalized=False, signs=None, out=None):
+    """Update of the residual stream by a block's branch, then the next
+    block's RMS norm, in one pass.
+
+    x [M, K] F16/BF16, branch [M, K] in x's dtype or FP32:
+      n  = branch, or with post_eps its RMS norm (times post_weight [K])
+      x' = x_dtype(x * residual_scale + n * branch_scale * gate[label])
+    and with eps the normalized rows of x', as norm_quantize(x', weight,
+    shift, scale, labels, eps=eps, ...) gives them, bit for bit. gate, shift,
+    scale: fp32 [R, K] AdaLN tables with labels int32 [M] (each row's table
+    row). Returns a dict with 'x' (x'; written into ``out`` when given, which
+    may be x itself), and with eps 'y' (unless quantize without
+    want_normalized) and, when quantize, 'q' and 'scale'.
+    """
+    _no_gradient(x, branch, weight, post_weight, gate, shift, scale)
+    _device(x, branch, weight, post_weight, gate, shift, scale, labels, signs, out)
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError('x must be float16 or bfloat16')
+    if branch.dtype not in (x.dtype, torch.float32):
+        raise ValueError('branch must have x\'s dtype or float32')
+    if x.ndim < 2 or branch.shape != x.shape:
+        raise ValueError('x and branch must be [rows, cols] of the same shape')
+    x, branch = _aligned_rows(x, 2), _aligned_rows(branch, branch.element_size())
+    rows, cols = x.shape
+    if eps is None and (quantize or want_normalized or weight is not None or shift is not None or scale is not None):
+        raise ValueError('the norm after the update needs eps')
+    if post_eps is None and post_weight is not None:
+        raise ValueError('post_weight needs post_eps')
+    if cols == 0 or cols % 16 or (quantize and convrot and cols % 256):
+        raise ValueError('features must be a positive multiple of 16 (256 with ConvRot256)')
+    weight, post_weight = _vector(weight, 'weight', cols), _vector(post_weight, 'post_weight', cols)
+    if (shift is None) != (scale is None):
+        raise ValueError('shift and scale go together')
+    if shift is not None:
+        shift, scale = _table(shift, 'shift', cols), _table(scale, 'scale', cols)
+        if scale.shape[0] != shift.shape[0]:
+            raise ValueError('shift and scale tables must have the same rows')
+        if scale.stride(0) != shift.stride(0):
+            shift, scale = shift.contiguous(), scale.contiguous()
+    if gate is not None:
+        gate = _table(gate, 'gate', cols)
+    if gate is not None or shift is not None:
+        if labels is None or labels.dtype != torch.int32 or labels.numel() != rows:
+            raise ValueError('gate and modulation tables need int32 labels, one per row')
+        if any(t is not None and t.shape[0] == 0 for t in (gate, shift)):
+            raise ValueError('gate and modulation tables need a row')
+        labels = labels.reshape(-1).contiguous()
+    if signs is not None and not (quantize and convrot):
+        raise ValueError('signs apply to the ConvRot256 rotation of the quantized output')
+    signs = _sign_words(signs, cols, x.device)
+    if out is None:
+        out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    elif (out.dtype != x.dtype or out.ndim != 2 or tuple(out.shape) != (rows, cols) or out.stride(1) != 1
+          or out.data_ptr() % 16 or (rows > 1 and (out.stride(0) < cols or out.stride(0) % 8))):
+        raise ValueError(f'out must be {x.dtype} [{rows}, {cols}] with unit column stride and 16-byte aligned rows')
+    res = {'x': out}
+    y = q = qs = None
+    if eps is not None and (want_normalized or not quantize):
+        y = res['y'] = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    if quantize:
+        q = res['q'] = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
+        qs = res['scale'] = torch.empty((rows, 1), dtype=torch.float32, device=x.device)
+    if rows == 0:
+        return res
+    args = _abi.ResidualNormArgs(
+        x_dtype=_abi.DTYPE_CODE[x.dtype], x=x.data_ptr(), ldx=_ld(x), rows=rows, cols=cols, branch=branch.data_ptr(),
+        ldb=_ld(branch), branch_dtype=_abi.DTYPE_CODE[branch.dtype], post=0 if post_eps is None else 1,
+        post_weight=_abi.ptr(post_weight), post_eps=float(post_eps or 0.0), branch_scale=float(branch_scale),
+        residual_scale=float(residual_scale), gate_rows=gate.shape[0] if gate is not None else 0,
+        gate=_abi.ptr(gate), ld_gate=_ld(gate) if gate is not None else 0, labels=_abi.ptr(labels),
+        out=out.data_ptr(), ldo=_ld(out), weight=_abi.ptr(weight), mod_shift=_abi.ptr(shift),
+        mod_scale=_abi.ptr(scale), ld_mod=_ld(shift) if shift is not None else 0,
+        mod_rows=shift.shape[0] if shift is not None else 0, eps=float(eps or 0.0), y=_abi.ptr(y), ldy=cols,
+        convrot=256 if quantize and convrot else 0, round_rotated=1 if round_rotated else 0, q=_abi.ptr(q), ldq=cols,
+        q_scale=_abi.ptr(qs), convrot_signs=_abi.ptr(signs), stream=_abi.stream_of(x))
+    _abi.call('w8a8_residual_norm', args)
+    return res
+
+
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _axial_table(positions, inv_freq, axis):
+    """Check positions [rows, axes], inv_freq [pairs] and axis [pairs]; inv_freq as fp64."""
+    if positions.ndim != 2 or positions.dtype not in _POSITION_TYPES:
+        raise ValueError('positions must be [rows, axes] of int32, int64 or float32')
+    if not 1 <= positions.shape[1] <= 16:
+        raise ValueError('1 to 16 axes required')
+    if inv_freq.ndim != 1 or axis.ndim != 1 or inv_freq.shape != axis.shape or not 1 <= inv_freq.numel() <= 128:
+        raise ValueError('inv_freq and axis must be [pairs], 1 to 128 pairs')
+    if inv_freq.dtype not in (torch.float64, torch.float32) or axis.dtype != torch.int32:
+        raise ValueError('inv_freq must be float64 or float32, axis int32')
+    return positions, inv_freq.double().contiguous(), axis.contiguous()
+
+
+def _head_view(t, name):
+    """A [rows, heads, dim] tensor with contiguous channels, and its strides."""
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        t = t.contiguous()
+    return t, _head_strides(t)
+
+
+def _head_strides(t):
+    rows, heads, dim = t.shape
+    head = t.stride(1) if heads > 1 else dim
+    return (t.stride(0) if rows > 1 else heads * head, head)
+
+
+def axial_rope(q, k, positions, inv_freq, axis, *, adjacent=False, q_gain=None, k_gain=None, eps=1e-6, out=None):
+    """Rotary positions with several axes of q [rows, heads, dim] and k
+    [rows, k_heads, dim] (or None), fp16, bf16 or fp32, optionally after a
+    per-head RMS norm (q_gain, k_gain: fp32 [dim]).
+
+    Pair p of a row turns by positions[row, axis[p]] * inv_freq[p]; the first
+    2 * pairs channels of a head are turned, pair p being channels (p,
+    p + pairs), or with adjacent (2 p, 2 p + 1). out: (q_out, k_out) to write
+    into, e.g. (q, k) themselves; else new contiguous tensors. Returns
+    (q_out, k_out), k_out None without k.
+    """
+    _no_gradient(q, k, q_gain, k_gain, inv_freq, positions)
+    _device(q, k, positions, inv_freq, axis, q_gain, k_gain)
+    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32) or (k is not None and k.dtype != q.dtype):
+        raise ValueError('q and k must share float16, bfloat16 or float32')
+    if q.ndim != 3 or (k is not None and (k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        raise ValueError('q and k must be [rows, heads, dim] with the same rows and dim')
+    rows, heads, dim = q.shape
+    if heads == 0 or (k is not None and k.shape[1] == 0):
+        raise ValueError('q and k need a head')
+    if not 2 <= dim <= 256 or dim % 2:
+        raise ValueError('dim must be even, 2 to 256')
+    positions, inv_freq, axis = _axial_table(positions, inv_freq, axis)
+    pairs = inv_freq.numel()
+    if positions.shape[0] != rows or 2 * pairs > dim:
+        raise ValueError('positions must have a row for each of q\'s, and at most dim / 2 pairs turn')
+    if (q_gain is None) != (k_gain is None) and not (k is None and k_gain is None):
+        raise ValueError('q_gain and k_gain go together')
+    q_gain, k_gain = _vector(q_gain, 'q_gain', dim), _vector(k_gain, 'k_gain', dim)
+    if out is None:
+        q_out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty(tuple(k.shape), dtype=q.dtype, device=q.device)
+    else:
+        q_out, k_out = out
+        if (k_out is None) != (k is None):
+            raise ValueError('out must hold a tensor for q and one for k')
+        _no_gradient(q_out, k_out)
+        _device(q, q_out, k_out)
+        for t, o in ((q, q_out), (k, k_out)):
+            if t is not None and (o.shape != t.shape or o.dtype != t.dtype or (dim > 1 and o.stride(2) != 1)):
+                raise ValueError('outputs must have their input\'s shape and dtype, with contiguous channels')
+    if rows == 0:
+        return q_out, k_out
+    q, q_st = _head_view(q, 'q')
+    k, k_st = _head_view(k, 'k') if k is not None else (None, (0, 0))
+    args = _abi.AxialRopeArgs(
+        dtype=_abi.DTYPE_CODE[q.dtype], q=q.data_ptr(), k=_abi.ptr(k), q_out=q_out.data_ptr(), k_out=_abi.ptr(k_out),
+        rows=rows, q_heads=heads, k_heads=k.shape[1] if k is not None else 0, dim=dim, pairs=pairs,
+        axes=positions.shape[1], pairing=1 if adjacent else 0, q_strides=q_st, k_strides=k_st,
+        q_out_strides=_head_strides(q_out), k_out_strides=_head_strides(k_out) if k is not None else (0, 0),
+        positions=positions.data_ptr(), pos_strides=tuple(positions.stride()),
+        pos_type=_POSITION_TYPES[positions.dtype], eps=float(eps), inv_freq=inv_freq.data_ptr(),
+        axis=axis.data_ptr(), q_gain=_abi.ptr(q_gain), k_gain=_abi.ptr(k_gain), stream=_abi.stream_of(q))
+    _abi.call('w8a8_axial_rope', args)
+    return q_out, k_out
+
+
+def axial_freqs(positions, inv_freq, axis, *, dtype=torch.float16, pairs_layout=False):
+    """The rotation matrices of axial_rope's angles: [rows, pairs, 2, 2] (cos,
+    -sin, sin, cos), or with pairs_layout the [rows, 2, pairs, 2] order of
+    rms_rope.pack_freqs, fp16 or fp32 - what rms_rope() and the QKV GEMM's
+    rope epilogue read."""
+    _no_gradient(positions, inv_freq)
+    _device(positions, inv_freq, axis)
+    positions, inv_freq, axis = _axial_table(positions, inv_freq, axis)
+    if dtype not in (torch.float16, torch.float32):
+        raise ValueError('frequencies must be float16 or float32')
+    rows, n = positions.shape[0], inv_freq.numel()
+    freqs = torch.empty((rows, 2, n, 2) if pairs_layout else (rows, n, 2, 2), dtype=dtype, device=positions.device)
+    if rows == 0:
+        return freqs
+    args = _abi.AxialFreqsArgs(
+        freq_dtype=_abi.DTYPE_CODE[dtype], freq_layout=1 if pairs_layout else 0,
+        pos_type=_POSITION_TYPES[positions.dtype], positions=positions.data_ptr(),
+        pos_strides=tuple(positions.stride()), rows=rows, pairs=n, axes=positions.shape[1],
+        inv_freq=inv_freq.data_ptr(), axis=axis.data_ptr(), freqs=freqs.data_ptr(),
+        stream=_abi.stream_of(positions))
+    _abi.call('w8a8_axial_freqs', args)
+    return freqs
+
+
+def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=False, out=None):
+    """y = x @ W.T with 4-bit weights and group scales, x [.., K] F16/BF16.
+
+    codes int32 [N, K / 8] (linear_w4.pack's words), scales [K / group, N] in
+    x's dtype, zeros uint8 [K / group, N] (0 to 15) or None for 8:
+    W[n, k] = scales[k // group, n] * (code[n, k] - zeros[k // group, n]).
+    bias [N] in x's dtype. residual [.., N] in x's dtype is added. gated: W's
+    first N / 2 rows are gate, the others up; returns silu(gate) * up
+    [.., N / 2]. out: [rows, width] in x's dtype to write into; it may be the
+    residual itself.
+    """
+    _no_gradient(x, codes, scales, bias, residual)
+    _device(x, codes, scales, zeros, bias, residual, out)
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError('x must be float16 or bfloat16')
+    if codes.ndim != 2 or codes.dtype != torch.int32 or scales.ndim != 2 or scales.dtype != x.dtype:
+        raise ValueError('codes must be int32 [N, K / 8], scales [K / group, N] in x\'s dtype')
+    n, k = codes.shape[0], 8 * codes.shape[1]
+    if x.ndim < 1 or x.shape[-1] != k:
+        raise ValueError('Input and weight inner dimensions must match')
+    groups = scales.shape[0]
+    if k == 0 or groups == 0 or k % groups or scales.shape[1] != n:
+        raise ValueError('scales must be [K / group, N]')
+    group = k // groups
+    if group not in (32, 64) and group % 128:
+        raise ValueError('group sizes are 32, 64 and multiples of 128')
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise ValueError('zeros must be uint8, of the scales\' shape')
+    if gated and (n % 2 or residual is not None):
+        raise ValueError('a gated projection has gate and up halves and takes no residual')
+    width = n // 2 if gated else n
+    if bias is not None and (bias.dtype != x.dtype or bias.numel() != n):
+        raise ValueError('bias must have one entry per weight row, in x\'s dtype')
+    lead = x.shape[:-1]
+    x = _aligned_rows(x if x.ndim > 1 else x[None], 2)
+    m = x.shape[0]
+    if codes.stride(1) != 1 or codes.data_ptr() % 16 or (n > 1 and (codes.stride(0) % 4 or codes.stride(0) < k // 8)):
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    scales = scales.contiguous()
+    zeros = zeros.contiguous() if zeros is not None else None
+    bias = bias.reshape(-1).contiguous() if bias is not None else None
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.numel() != m * n or residual.shape[-1] != n:
+            raise ValueError('residual must be [.., N] in x\'s dtype')
+        residual = residual.reshape(m, n)
+        if residual.stride(1) != 1 and n > 1:
+            residual = residual.contiguous()
+    y = out
+    if y is None:
+        y = torch.empty((m, width), dtype=x.dtype, device=x.device)
+    elif (y.dtype != x.dtype or y.ndim != 2 or tuple(y.shape) != (m, width) or (width > 1 and y.stride(1) != 1)
+          or (m > 1 and y.stride(0) < width)):
+        raise ValueError('out must be [rows, width] in x\'s dtype with unit column stride')
+    if m == 0 or n == 0:
+        return y if out is not None else y.reshape(*lead, width)
+    with torch.cuda.device(x.device):
+        nbytes = int(_abi.load().w8a8_linear_w4_workspace_size(m, n, k, group, 1 if gated else 0))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    args = _abi.LinearW4Args(
+        dtype=_abi.DTYPE_CODE[x.dtype], x=x.data_ptr(), ldx=_ld(x), codes=codes.data_ptr(),
+        ldw=codes.stride(0) if n > 1 else k // 8, scales=scales.data_ptr(), zeros=_abi.ptr(zeros), m=m, n=n, k=k,
+        group=group, gated=1 if gated else 0, bias=_abi.ptr(bias), residual=_abi.ptr(residual),
+        ldr=residual.stride(0) if residual is not None and m > 1 else n,
+        out=y.data_ptr(), ldo=y.stride(0) if m > 1 else width, workspace=_abi.ptr(ws), workspace_bytes=nbytes,
+        stream=_abi.stream_of(x))
+    _abi.call('w8a8_linear_w4', args)
+    return y if out is not None else y.reshape(*lead, width)
