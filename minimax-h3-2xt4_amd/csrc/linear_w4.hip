@@ -41,18 +41,31 @@ struct W4Params {
   int64_t ldr;
   uint16_t* out;
   int64_t ldo;
+  bool quads;   // scales, zeros and outputs of four neighbouring rows are read and written as one
 };
 
 // The eight weights of a word as 16 + c, in the order of their inputs.
+// (One constant out of the compiler's sight: it sits in a register, and mask and
+// exponent take one v_and_or_b32.)
 template <int DT>
 __device__ __forceinline__ v4u weights8(uint32_t w) {
+  uint32_t one = DT == kF16 ? 0x4c004c00u : 0x41804180u;
+  __asm__("" : "+s"(one));
   if constexpr (DT == kF16) {
-    constexpr uint32_t mask = 0x03c003c0u, one = 0x4c004c00u;
+    constexpr uint32_t mask = 0x03c003c0u;
     return v4u{((w << 6) & mask) | one, ((w << 2) & mask) | one, ((w >> 2) & mask) | one, ((w >> 6) & mask) | one};
   } else {
-    constexpr uint32_t mask = 0x00780078u, one = 0x41804180u;
+    constexpr uint32_t mask = 0x00780078u;
     return v4u{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one, ((w >> 9) & mask) | one};
   }
+}
+
+// Eight fp16 less one (in both halves of z).
+__device__ __forceinline__ v4u less(v4u a, uint32_t z) {
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  v8h v = __builtin_bit_cast(v8h, a);
+  const v2 y = __builtin_bit_cast(v2, z);
+  return __builtin_bit_cast(v4u, v - __builtin_shufflevector(y, y, 0, 1, 0, 1, 0, 1, 0, 1));
 }
 
 template <int DT>
@@ -72,18 +85,53 @@ __device__ __forceinline__ uint16_t slim(float f) { return DT == kF16 ? f2h(f) :
 // before the bias.
 template <int DT, bool GATED>
 __device__ __forceinline__ void finish4(const W4Params& p, int64_t m, int64_t n, int64_t width, v4f y, v4f up) {
+  uint16_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (n + i >= width) break;
+    const int64_t c = min(n + i, width - 1);
     float v = y[i];
-    if (p.bias) v = v + wide<DT>(p.bias[n + i]);
+    if (p.bias) v = v + wide<DT>(p.bias[c]);
     if constexpr (GATED) {
-      const float u = p.bias ? up[i] + wide<DT>(p.bias[width + n + i]) : up[i];
+      const float u = p.bias ? up[i] + wide<DT>(p.bias[width + c]) : up[i];
       v = swiglu(v, u);
     }
-    if (p.residual) v = v + wide<DT>(p.residual[m * p.ldr + n + i]);
-    p.out[m * p.ldo + n + i] = slim<DT>(v);
+    if (p.residual) v = v + wide<DT>(p.residual[m * p.ldr + c]);
+    o[i] = slim<DT>(v);
   }
+  uint16_t* dst = p.out + m * p.ldo + n;
+  if (p.quads) {
+    if (n < width)
+      *reinterpret_cast<uint2*>(dst) = make_uint2(o[0] | ((uint32_t)o[1] << 16), o[2] | ((uint32_t)o[3] << 16));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < width) dst[i] = o[i];
+  }
+}
+
+// Scale and 16 + zero of four neighbouring weight rows in group row `at` (the
+// row's offset in scales and zeros); past the last row its values again.
+template <int DT>
+__device__ __forceinline__ void scales4(const W4Params& p, int64_t at, int64_t n, v4f& s, v4f& z) {
+  if (p.quads) {
+    n = min(n, p.n - 4);
+    const uint2 u = *reinterpret_cast<const uint2*>(p.scales + at + n);
+    s = v4f{wide<DT>((uint16_t)u.x), wide<DT>((uint16_t)(u.x >> 16)), wide<DT>((uint16_t)u.y),
+            wide<DT>((uint16_t)(u.y >> 16))};
+    if (p.zeros) {
+      const uint32_t b = *reinterpret_cast<const uint32_t*>(p.zeros + at + n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = (float)((b >> (8 * i)) & 0xffu) + 16.0f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t c = at + min(n + i, p.n - 1);
+      s[i] = wide<DT>(p.scales[c]);
+      if (p.zeros) z[i] = (float)p.zeros[c] + 16.0f;
+    }
+  }
+  if (!p.zeros) z = v4f{24.0f, 24.0f, 24.0f, 24.0f};
 }
 
 // A workgroup of W waves takes 16 NT weight rows (gated: half of them gate, half
@@ -141,15 +189,13 @@ void linear_w4_kernel(W4Params p) {
     const int64_t grow = (int64_t)(b * GB / p.group) * p.n;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      v4f sc, z;
+      scales4<DT>(p, grow, nd[t], sc, z);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t n = min(nd[t] + i, p.n - 1);
-        const float s = wide<DT>(p.scales[grow + n]);
-        const float z = p.zeros ? (float)p.zeros[grow + n] + 16.0f : 24.0f;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int u = 0; u < MT; ++u)
-          tot[t][u][i] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[u][i], acc[t][u][i]), tot[t][u][i]);
-      }
+          tot[t][u][i] = __builtin_fmaf(sc[i], __builtin_fmaf(-z[i], sum[u][i], acc[t][u][i]), tot[t][u][i]);
     }
   }
 #pragma unroll
@@ -170,8 +216,234 @@ void linear_w4_kernel(W4Params p) {
   }
 }
 
+// Sum of a value over the aligned N lanes (4, 8 or 16) of a row of 16, in all of them.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = add_dpp<0xb1>(v);                       // xor 1 within a quad
+  v = add_dpp<0x4e>(v);                       // xor 2
+  if constexpr (N >= 8) v = add_dpp<0x141>(v);   // the other quad of eight
+  if constexpr (N >= 16) v = add_dpp<0x140>(v);  // the other eight of sixteen
+  return v;
+}
+
+// The sums of x over blocks of GB inputs, as three bf16 that add up to the fp32
+// sum: sums[block][m] = (hi, mid, lo, 0). One 16-byte run of x per thread.
+template <int DT, int GB>
+__global__ __launch_bounds__(256)
+void w4_sums_kernel(W4Params p, uint2* sums) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int runs = (int)(p.k / 8);
+  const int64_t m = i / runs;
+  const int run = (int)(i - m * runs);
+  if (m >= p.m) return;   // (whole groups of lanes: a row is whole blocks)
+  const v4u x = *reinterpret_cast<const v4u*>(reinterpret_cast<const uint16_t*>(p.x) + m * p.ldx + 8 * run);
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s = s + (wide<DT>((uint16_t)x[j]) + wide<DT>((uint16_t)(x[j] >> 16)));
+  s = lanes_sum<GB / 8>(s);
+  if (run % (GB / 8)) return;
+  const uint16_t hi = f2bf(s);
+  const float s1 = s - bf2f(hi);
+  const uint16_t mid = f2bf(s1);
+  const uint16_t lo = f2bf(s1 - bf2f(mid));
+  sums[(int64_t)(run / (GB / 8)) * p.m + m] = make_uint2(hi | ((uint32_t)mid << 16), lo);
+}
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+template <int DT>
+__device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
+  if constexpr (DT == kF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+}
+
+// Many rows: a workgroup of four waves takes 128 rows of x and 256 weight rows
+// (gated: 128 of gate and the same of up); each wave takes all of x's rows and 64
+// of the weight's, so that every code is unpacked once. The 32 x 32 x 16 MFMA's
+// first operand is x, from LDS, its second the weights, a word of codes a lane:
+// a lane's column is one weight row, whose scale it holds. x comes by DMA in
+// steps of 128 inputs, two in turn (16-byte run c of row r at run c ^ (r & 15)),
+// codes and scales into registers a step ahead.
+//
+// fp16 takes the zeros off its weights (packed subtraction, exact). bf16 has no
+// such instruction: there an MFMA puts -(16 + z) sum x into the accumulators
+// before a block's products, with the sum in three bf16 (exact) as three inputs.
 template <int DT, int GB, bool GATED>
-static int launch_w4(const W4Params& p, hipStream_t stream) {
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1)))
+void linear_w4_tiles_kernel(W4Params p, const uint2* sums, int mtiles, int tiles) {
+  constexpr int S = GB / 16, NB = 128 / GB, BN = GATED ? 128 : 256;
+  __shared__ __attribute__((aligned(16))) char xs[2][128 * 256];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t width = GATED ? p.n / 2 : p.n;
+  // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, the
+  // row tiles of a few weight tiles at a time.
+  const int per = (tiles + 7) / 8, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (tile >= tiles || (int)(blockIdx.x >> 3) >= per) return;
+  const int64_t m0 = (int64_t)(tile % mtiles) * 128, n0 = (int64_t)(tile / mtiles) * BN;
+  const int mrows = (int)min((int64_t)128, p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
+  const int ncol = GATED ? 32 * wave + c : 64 * wave + c;   // the lane's column of the tile (and 32 on, ungated)
+  const int64_t wr[2] = {n0 + min(ncol, nrows - 1), GATED ? width + n0 + min(ncol, nrows - 1) : n0 + min(ncol + 32, nrows - 1)};
+  const char* wrow[2] = {reinterpret_cast<const char*>(p.codes + wr[0] * p.ldw),
+                         reinterpret_cast<const char*>(p.codes + wr[1] * p.ldw)};
+  const char* xbase = reinterpret_cast<const char*>(reinterpret_cast<const uint16_t*>(p.x) + m0 * p.ldx);
+  uint32_t xoff[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) xoff[i] = (uint32_t)min(32 * wave + 4 * i + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
+  const int steps = (int)((p.k + 127) / 128), words = (int)(p.k / 8), blocks = (int)(p.k / GB);
+  const int per_group = p.group / GB;
+
+  uint32_t w[NB][2][S];
+  uint16_t sc[NB][2];
+  uint8_t zr[NB][2];
+  uint2 sm[NB][4];
+  auto load = [&](int step, int buf) {
+    // Past the end of k (the last step only) the last runs and codes again: their blocks are left out.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int run = (lane & 15) ^ ((4 * i + (lane >> 4)) & 15);
+      const char* src = xbase + (xoff[i] + (uint32_t)min(step * 256 + run * 16, (int)p.k * 2 - 16));
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                       (__attribute__((address_space(3))) void*)(xs[buf] + (32 * wave + 4 * i) * 256), 16,
+                                       0, 0);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int at = min(step * 16 + b * (GB / 8) + h * S, words - S) * 4;
+      const int64_t grow = (int64_t)(min(step * NB + b, blocks - 1) / per_group) * p.n;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (S >= 4) {
+#pragma unroll
+          for (int j = 0; j < S; j += 4)
+            *reinterpret_cast<v4u*>(&w[b][t][j]) = *reinterpret_cast<const v4u*>(wrow[t] + at + 4 * j);
+        } else {
+          *reinterpret_cast<uint2*>(&w[b][t][0]) = *reinterpret_cast<const uint2*>(wrow[t] + at);
+        }
+        sc[b][t] = p.scales[grow + wr[t]];
+        zr[b][t] = p.zeros ? p.zeros[grow + wr[t]] : (uint8_t)8;
+      }
+      if constexpr (DT == kBF16) {
+        const uint2* row = sums + (int64_t)min(step * NB + b, blocks - 1) * p.m + m0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sm[b][u] = row[min(32 * u + c, mrows - 1)];
+      }
+    }
+  };
+
+  v16f tot[2][4] = {};
+  load(0, 0);
+  for (int step = 0; step < steps; ++step) {
+    const int buf = step & 1;
+    __syncthreads();   // the step's loads have landed (vmcnt(0)); the last one's reads are done
+    uint32_t cw[NB][2][S];
+    float cs[NB][2];
+    uint32_t cz[NB][2];
+    uint2 cm[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int j = 0; j < S; ++j) cw[b][t][j] = w[b][t][j];
+        cs[b][t] = wide<DT>(sc[b][t]);
+        if constexpr (DT == kF16) cz[b][t] = (uint32_t)f2h(16.0f + (float)zr[b][t]) * 0x10001u;
+        else cz[b][t] = h ? 0 : (uint32_t)f2bf(-16.0f - (float)zr[b][t]) * 0x10001u;
+      }
+      if constexpr (DT == kBF16) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) cm[b][u] = sm[b][u];
+      }
+    }
+    if (step + 1 < steps) load(step + 1, buf ^ 1);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if (NB > 1 && step * NB + b >= blocks) break;
+      v4u wt[2][S];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+          wt[t][j] = weights8<DT>(cw[b][t][j]);
+          if constexpr (DT == kF16) wt[t][j] = less(wt[t][j], cz[b][t]);
+        }
+      v16f prev = {};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        v4u x[S];
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+          x[j] = *reinterpret_cast<const v4u*>(xs[buf] + (32 * u + c) * 256 + 16 * ((b * (GB / 8) + h * S + j) ^ (c & 15)));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          v16f acc = {};
+          if constexpr (DT == kBF16)
+            acc = mfma32<kBF16>(v4u{h ? 0 : cm[b][u].x, h ? 0 : cm[b][u].y, 0, 0}, v4u{cz[b][t], cz[b][t], 0, 0}, acc);
+#pragma unroll
+          for (int j = 0; j < S; ++j) acc = mfma32<DT>(x[j], wt[t][j], acc);
+          // The sums of the chain before, while this one runs. (Pinned here: the
+          // compiler would put them all at the end, with every accumulator alive.)
+          if (u + t > 0) {
+            v16f& d = tot[t ^ 1][t ? u : u - 1];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) d[i] = __builtin_fmaf(cs[b][t ^ 1], prev[i], d[i]);
+            __asm__ volatile("" : "+v"(d));
+          }
+          prev = acc;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) tot[1][3][i] = __builtin_fmaf(cs[b][1], prev[i], tot[1][3][i]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < (GATED ? 1 : 2); ++t) {
+    const int col = ncol + 32 * t;
+    if (col >= nrows) continue;
+    const int64_t n = n0 + col;
+    const float bias = p.bias ? wide<DT>(p.bias[n]) : 0.0f;
+    const float up_bias = GATED && p.bias ? wide<DT>(p.bias[width + n]) : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (m >= mrows) continue;
+        float v = tot[t][u][i] + bias;
+        if constexpr (GATED) v = swiglu(v, tot[1][u][i] + up_bias);
+        if (p.residual) v = v + wide<DT>(p.residual[(m0 + m) * p.ldr + n]);
+        p.out[(m0 + m) * p.ldo + n] = slim<DT>(v);
+      }
+  }
+}
+
+// Whether a call takes the tiles (offsets inside a tile are 32 bits there).
+static bool w4_tiled(int64_t m, int64_t ldx) { return m > 64 && ldx < (1 << 22); }
+
+template <int DT, int GB, bool GATED>
+static int launch_w4_tiles(const W4Params& p, void* workspace, hipStream_t stream) {
+  const int64_t width = GATED ? p.n / 2 : p.n, per = GATED ? 128 : 256;
+  const int mtiles = (int)((p.m + 127) / 128);
+  const int64_t tiles = (width + per - 1) / per * mtiles;
+  W8A8_REQUIRE(tiles < ((int64_t)1 << 24), "w8a8_linear_w4: too many outputs for one launch");
+  uint2* sums = reinterpret_cast<uint2*>(workspace);
+  if (DT == kBF16)
+    hipLaunchKernelGGL((w4_sums_kernel<DT, GB>), dim3((unsigned)((p.m * (p.k / 8) + 255) / 256)), dim3(256), 0, stream,
+                       p, sums);
+  hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, GATED>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0,
+                     stream, p, sums, mtiles, (int)tiles);
+  return launch_status("w8a8_linear_w4");
+}
+
+template <int DT, int GB, bool GATED>
+static int launch_w4(const W4Params& p, void* workspace, hipStream_t stream) {
+  if (w4_tiled(p.m, p.ldx)) return launch_w4_tiles<DT, GB, GATED>(p, workspace, stream);
   constexpr int NT = 2, W = 8;
   const int64_t width = GATED ? p.n / 2 : p.n, per = GATED ? 16 * NT / 2 : 16 * NT;
   const int mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
@@ -185,17 +457,21 @@ static int launch_w4(const W4Params& p, hipStream_t stream) {
 }
 
 template <int DT>
-static int launch_w4_group(const W4Params& p, bool gated, hipStream_t s) {
+static int launch_w4_group(const W4Params& p, bool gated, void* ws, hipStream_t s) {
   switch (p.group) {
-    case 32: return gated ? launch_w4<DT, 32, true>(p, s) : launch_w4<DT, 32, false>(p, s);
-    case 64: return gated ? launch_w4<DT, 64, true>(p, s) : launch_w4<DT, 64, false>(p, s);
-    default: return gated ? launch_w4<DT, 128, true>(p, s) : launch_w4<DT, 128, false>(p, s);
+    case 32: return gated ? launch_w4<DT, 32, true>(p, ws, s) : launch_w4<DT, 32, false>(p, ws, s);
+    case 64: return gated ? launch_w4<DT, 64, true>(p, ws, s) : launch_w4<DT, 64, false>(p, ws, s);
+    default: return gated ? launch_w4<DT, 128, true>(p, ws, s) : launch_w4<DT, 128, false>(p, ws, s);
   }
 }
 
 }  // namespace w8a8
 
-extern "C" int64_t w8a8_linear_w4_workspace_size(int64_t, int64_t, int64_t, int32_t, int32_t) { return 0; }
+// Many rows: the sums of x, 8 bytes a row and block (bf16; asked of fp16 alike).
+extern "C" int64_t w8a8_linear_w4_workspace_size(int64_t m, int64_t n, int64_t k, int32_t group, int32_t) {
+  if (m <= 64 || n <= 0 || k <= 0 || group <= 0) return 0;
+  return 8 * m * (k / (group < 128 ? group : 128));
+}
 
 extern "C" int w8a8_linear_w4(const W8A8LinearW4Args* a) {
   using namespace w8a8;
@@ -233,8 +509,10 @@ extern "C" int w8a8_linear_w4(const W8A8LinearW4Args* a) {
   const W4Params p{a->x, a->ldx, reinterpret_cast<const uint32_t*>(a->codes), a->ldw,
                    reinterpret_cast<const uint16_t*>(a->scales), a->zeros, a->m, a->n, a->k, a->group,
                    reinterpret_cast<const uint16_t*>(a->bias), reinterpret_cast<const uint16_t*>(a->residual), a->ldr,
-                   reinterpret_cast<uint16_t*>(a->out), a->ldo};
+                   reinterpret_cast<uint16_t*>(a->out), a->ldo,
+                   width % 4 == 0 && a->ldo % 4 == 0 && (uintptr_t)a->out % 8 == 0 && (uintptr_t)a->scales % 8 == 0 &&
+                       (uintptr_t)a->zeros % 4 == 0};
   hipStream_t s = reinterpret_cast<hipStream_t>(a->stream);
-  return a->dtype == W8A8_F16 ? launch_w4_group<kF16>(p, a->gated != 0, s)
-                              : launch_w4_group<kBF16>(p, a->gated != 0, s);
+  return a->dtype == W8A8_F16 ? launch_w4_group<kF16>(p, a->gated != 0, a->workspace, s)
+                              : launch_w4_group<kBF16>(p, a->gated != 0, a->workspace, s);
 }
