@@ -44,28 +44,40 @@ struct W4Params {
   bool quads;   // scales, zeros and outputs of four neighbouring rows are read and written as one
 };
 
-// The eight weights of a word as 16 + c, in the order of their inputs.
-// (One constant out of the compiler's sight: it sits in a register, and mask and
-// exponent take one v_and_or_b32.)
+// The eight weights of a word as 16 + c, in the order of their inputs: a shift
+// and a v_and_or_b32 for two, which takes one constant from a vector register
+// and one from a scalar one (both out of the compiler's sight, which would make
+// it two instructions with literals).
 template <int DT>
-__device__ __forceinline__ v4u weights8(uint32_t w) {
-  uint32_t one = DT == kF16 ? 0x4c004c00u : 0x41804180u;
-  __asm__("" : "+s"(one));
-  if constexpr (DT == kF16) {
-    constexpr uint32_t mask = 0x03c003c0u;
-    return v4u{((w << 6) & mask) | one, ((w << 2) & mask) | one, ((w >> 2) & mask) | one, ((w >> 6) & mask) | one};
-  } else {
-    constexpr uint32_t mask = 0x00780078u;
-    return v4u{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one, ((w >> 9) & mask) | one};
+struct Unpack {
+  uint32_t mask, one;
+  __device__ __forceinline__ Unpack() {
+    mask = DT == kF16 ? 0x03c003c0u : 0x00780078u;
+    one = DT == kF16 ? 0x4c004c00u : 0x41804180u;
+    __asm__("" : "+v"(mask));
+    __asm__("" : "+s"(one));
   }
-}
+  __device__ __forceinline__ uint32_t pick(uint32_t w) const {
+    uint32_t r;
+    __asm__("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "v"(mask), "s"(one));
+    return r;
+  }
+  __device__ __forceinline__ v4u operator()(uint32_t w) const {
+    if constexpr (DT == kF16) return v4u{pick(w << 6), pick(w << 2), pick(w >> 2), pick(w >> 6)};
+    else return v4u{pick(w << 3), pick(w >> 1), pick(w >> 5), pick(w >> 9)};
+  }
+};
 
-// Eight fp16 less one (in both halves of z).
+// Eight fp16 less one (in both halves of z), exact here.
 __device__ __forceinline__ v4u less(v4u a, uint32_t z) {
-  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-  v8h v = __builtin_bit_cast(v8h, a);
-  const v2 y = __builtin_bit_cast(v2, z);
-  return __builtin_bit_cast(v4u, v - __builtin_shufflevector(y, y, 0, 1, 0, 1, 0, 1, 0, 1));
+  const v2h y = __builtin_bit_cast(v2h, z);
+  v4u r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t e = a[i];
+    r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, e) - y);
+  }
+  return r;
 }
 
 template <int DT>
@@ -160,6 +172,7 @@ void linear_w4_kernel(W4Params p) {
     xrow[t] = reinterpret_cast<const uint16_t*>(p.x) + min(m0 + 16 * t + r, p.m - 1) * p.ldx + g * (GB / 4);
   const v4u ones = DT == kF16 ? v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u}
                               : v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  const Unpack<DT> unpack;
   v4f tot[NT][MT] = {};
   const int blocks = (int)(p.k / GB);
   for (int b = wave; b < blocks; b += W) {
@@ -181,7 +194,7 @@ void linear_w4_kernel(W4Params p) {
       for (int t = 0; t < MT; ++t) sum[t] = mfma<DT>(ones, x[t][j], sum[t]);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const v4u a = weights8<DT>(w[t][j]);
+        const v4u a = unpack(w[t][j]);
 #pragma unroll
         for (int u = 0; u < MT; ++u) acc[t][u] = mfma<DT>(a, x[u][j], acc[t][u]);
       }
@@ -263,19 +276,27 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
 }
 
-// Many rows: a workgroup of four waves takes 128 rows of x and 256 weight rows
-// (gated: 128 of gate and the same of up); each wave takes all of x's rows and 64
-// of the weight's, so that every code is unpacked once. The 32 x 32 x 16 MFMA's
-// first operand is x, from LDS, its second the weights, a word of codes a lane:
-// a lane's column is one weight row, whose scale it holds. x comes by DMA in
-// steps of 128 inputs, two in turn (16-byte run c of row r at run c ^ (r & 15)),
-// codes and scales into registers a step ahead.
+// -(16 + z) sum x into fresh accumulators: the three bf16 of a row's sum (from
+// lanes 0-31, inputs 0-2) times the zero's column (lanes 32-63 hold zeros there).
+__device__ __forceinline__ v16f mfma_zero(uint2 sum, uint2 z) {
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  return __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(__builtin_bit_cast(v4s, sum), __builtin_bit_cast(v4s, z), v16f{}, 0, 0, 0);
+}
+
+// Many rows: a workgroup of eight waves takes 128 rows of x and 256 weight rows
+// (gated: 128 of gate and the same of up); each wave takes all of x's rows and 32
+// of the weight's (gated: 16 of each), so that every code is unpacked once, and
+// the two waves of a SIMD do each other's unpacking and scaling in the shadow of
+// their MFMAs. The 32 x 32 x 16 MFMA's first operand is x, from LDS, its second the
+// weights, a word of codes a lane: a lane's column is one weight row, whose scale
+// it holds. x comes by DMA in steps of 128 inputs, two in turn (16-byte run c of
+// row r at run c ^ (r & 15)), codes and scales into registers a step ahead.
 //
 // fp16 takes the zeros off its weights (packed subtraction, exact). bf16 has no
 // such instruction: there an MFMA puts -(16 + z) sum x into the accumulators
 // before a block's products, with the sum in three bf16 (exact) as three inputs.
 template <int DT, int GB, bool GATED>
-__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(1, 1)))
+__global__ __launch_bounds__(512, 2)
 void linear_w4_tiles_kernel(W4Params p, const uint2* sums, int mtiles, int tiles) {
   constexpr int S = GB / 16, NB = 128 / GB, BN = GATED ? 128 : 256;
   __shared__ __attribute__((aligned(16))) char xs[2][128 * 256];
@@ -288,74 +309,68 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, int mtiles, int tiles
   if (tile >= tiles || (int)(blockIdx.x >> 3) >= per) return;
   const int64_t m0 = (int64_t)(tile % mtiles) * 128, n0 = (int64_t)(tile / mtiles) * BN;
   const int mrows = (int)min((int64_t)128, p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
-  const int ncol = GATED ? 32 * wave + c : 64 * wave + c;   // the lane's column of the tile (and 32 on, ungated)
-  const int64_t wr[2] = {n0 + min(ncol, nrows - 1), GATED ? width + n0 + min(ncol, nrows - 1) : n0 + min(ncol + 32, nrows - 1)};
-  const char* wrow[2] = {reinterpret_cast<const char*>(p.codes + wr[0] * p.ldw),
-                         reinterpret_cast<const char*>(p.codes + wr[1] * p.ldw)};
+  const int ncol = GATED ? 16 * wave + (c & 15) : 32 * wave + c;   // the lane's column of the tile
+  const int64_t wr = (GATED && c >= 16 ? width : 0) + n0 + min(ncol, nrows - 1);
+  const char* const wrow = reinterpret_cast<const char*>(p.codes + wr * p.ldw);
   const char* xbase = reinterpret_cast<const char*>(reinterpret_cast<const uint16_t*>(p.x) + m0 * p.ldx);
-  uint32_t xoff[8];
+  uint32_t xoff[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) xoff[i] = (uint32_t)min(32 * wave + 4 * i + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
+  for (int i = 0; i < 4; ++i) xoff[i] = (uint32_t)min(16 * wave + 4 * i + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
   const int steps = (int)((p.k + 127) / 128), words = (int)(p.k / 8), blocks = (int)(p.k / GB);
   const int per_group = p.group / GB;
 
-  uint32_t w[NB][2][S];
-  uint16_t sc[NB][2];
-  uint8_t zr[NB][2];
+  uint32_t w[NB][S];
+  uint16_t sc[NB];
+  uint8_t zr[NB];
   uint2 sm[NB][4];
   auto load = [&](int step, int buf) {
     // Past the end of k (the last step only) the last runs and codes again: their blocks are left out.
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int run = (lane & 15) ^ ((4 * i + (lane >> 4)) & 15);
       const char* src = xbase + (xoff[i] + (uint32_t)min(step * 256 + run * 16, (int)p.k * 2 - 16));
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                       (__attribute__((address_space(3))) void*)(xs[buf] + (32 * wave + 4 * i) * 256), 16,
+                                       (__attribute__((address_space(3))) void*)(xs[buf] + (16 * wave + 4 * i) * 256), 16,
                                        0, 0);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      const int block = min(step * NB + b, blocks - 1);
       const int at = min(step * 16 + b * (GB / 8) + h * S, words - S) * 4;
-      const int64_t grow = (int64_t)(min(step * NB + b, blocks - 1) / per_group) * p.n;
+      const int64_t grow = (int64_t)(block / per_group) * p.n + wr;
+      if constexpr (S >= 4) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if constexpr (S >= 4) {
-#pragma unroll
-          for (int j = 0; j < S; j += 4)
-            *reinterpret_cast<v4u*>(&w[b][t][j]) = *reinterpret_cast<const v4u*>(wrow[t] + at + 4 * j);
-        } else {
-          *reinterpret_cast<uint2*>(&w[b][t][0]) = *reinterpret_cast<const uint2*>(wrow[t] + at);
-        }
-        sc[b][t] = p.scales[grow + wr[t]];
-        zr[b][t] = p.zeros ? p.zeros[grow + wr[t]] : (uint8_t)8;
+        for (int j = 0; j < S; j += 4) *reinterpret_cast<v4u*>(&w[b][j]) = *reinterpret_cast<const v4u*>(wrow + at + 4 * j);
+      } else {
+        *reinterpret_cast<uint2*>(&w[b][0]) = *reinterpret_cast<const uint2*>(wrow + at);
       }
+      sc[b] = p.scales[grow];
+      zr[b] = p.zeros ? p.zeros[grow] : (uint8_t)8;
       if constexpr (DT == kBF16) {
-        const uint2* row = sums + (int64_t)min(step * NB + b, blocks - 1) * p.m + m0;
+        const uint2* row = sums + (int64_t)block * p.m + m0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) sm[b][u] = row[min(32 * u + c, mrows - 1)];
       }
     }
   };
 
-  v16f tot[2][4] = {};
+  const Unpack<DT> unpack;
+  v16f tot[4] = {};
   load(0, 0);
   for (int step = 0; step < steps; ++step) {
     const int buf = step & 1;
     __syncthreads();   // the step's loads have landed (vmcnt(0)); the last one's reads are done
-    uint32_t cw[NB][2][S];
-    float cs[NB][2];
-    uint32_t cz[NB][2];
+    uint32_t cw[NB][S];
+    float cs[NB];
+    uint32_t cz[NB];
     uint2 cm[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int j = 0; j < S; ++j) cw[b][t][j] = w[b][t][j];
-        cs[b][t] = wide<DT>(sc[b][t]);
-        if constexpr (DT == kF16) cz[b][t] = (uint32_t)f2h(16.0f + (float)zr[b][t]) * 0x10001u;
-        else cz[b][t] = h ? 0 : (uint32_t)f2bf(-16.0f - (float)zr[b][t]) * 0x10001u;
-      }
+      for (int j = 0; j < S; ++j) cw[b][j] = w[b][j];
+      cs[b] = wide<DT>(sc[b]);
+      const float z = 16.0f + (float)zr[b];
+      cz[b] = DT == kF16 ? (uint32_t)f2h(z) * 0x10001u : h ? 0 : (uint32_t)f2bf(-z) * 0x10001u;
       if constexpr (DT == kBF16) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) cm[b][u] = sm[b][u];
@@ -365,62 +380,43 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, int mtiles, int tiles
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       if (NB > 1 && step * NB + b >= blocks) break;
-      v4u wt[2][S];
+      v4u wt[S];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-          wt[t][j] = weights8<DT>(cw[b][t][j]);
-          if constexpr (DT == kF16) wt[t][j] = less(wt[t][j], cz[b][t]);
-        }
-      v16f prev = {};
+      for (int j = 0; j < S; ++j) {
+        wt[j] = unpack(cw[b][j]);
+        if constexpr (DT == kF16) wt[j] = less(wt[j], cz[b]);
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        v4u x[S];
+        v16f acc = {};
+        if constexpr (DT == kBF16) acc = mfma_zero(cm[b][u], make_uint2(cz[b], cz[b]));
 #pragma unroll
-        for (int j = 0; j < S; ++j)
-          x[j] = *reinterpret_cast<const v4u*>(xs[buf] + (32 * u + c) * 256 + 16 * ((b * (GB / 8) + h * S + j) ^ (c & 15)));
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          v16f acc = {};
-          if constexpr (DT == kBF16)
-            acc = mfma32<kBF16>(v4u{h ? 0 : cm[b][u].x, h ? 0 : cm[b][u].y, 0, 0}, v4u{cz[b][t], cz[b][t], 0, 0}, acc);
-#pragma unroll
-          for (int j = 0; j < S; ++j) acc = mfma32<DT>(x[j], wt[t][j], acc);
-          // The sums of the chain before, while this one runs. (Pinned here: the
-          // compiler would put them all at the end, with every accumulator alive.)
-          if (u + t > 0) {
-            v16f& d = tot[t ^ 1][t ? u : u - 1];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) d[i] = __builtin_fmaf(cs[b][t ^ 1], prev[i], d[i]);
-            __asm__ volatile("" : "+v"(d));
-          }
-          prev = acc;
+        for (int j = 0; j < S; ++j) {
+          const v4u x = *reinterpret_cast<const v4u*>(xs[buf] + (32 * u + c) * 256 + 16 * ((b * (GB / 8) + h * S + j) ^ (c & 15)));
+          acc = mfma32<DT>(x, wt[j], acc);
         }
-      }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) tot[1][3][i] = __builtin_fmaf(cs[b][1], prev[i], tot[1][3][i]);
+        for (int i = 0; i < 16; ++i) tot[u][i] = __builtin_fmaf(cs[b], acc[i], tot[u][i]);
+      }
+      // (Here, not at the end of the step, where the compiler would put the sums
+      // of all its blocks with every accumulator alive.)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) __asm__ volatile("" : "+v"(tot[u]));
     }
   }
+  const int64_t n = n0 + ncol;
+  const float bias = p.bias ? wide<DT>(p.bias[wr]) : 0.0f;
 #pragma unroll
-  for (int t = 0; t < (GATED ? 1 : 2); ++t) {
-    const int col = ncol + 32 * t;
-    if (col >= nrows) continue;
-    const int64_t n = n0 + col;
-    const float bias = p.bias ? wide<DT>(p.bias[n]) : 0.0f;
-    const float up_bias = GATED && p.bias ? wide<DT>(p.bias[width + n]) : 0.0f;
+  for (int u = 0; u < 4; ++u)
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-        if (m >= mrows) continue;
-        float v = tot[t][u][i] + bias;
-        if constexpr (GATED) v = swiglu(v, tot[1][u][i] + up_bias);
-        if (p.residual) v = v + wide<DT>(p.residual[(m0 + m) * p.ldr + n]);
-        p.out[(m0 + m) * p.ldo + n] = slim<DT>(v);
-      }
-  }
+    for (int i = 0; i < 16; ++i) {
+      const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+      float v = tot[u][i] + bias;
+      if constexpr (GATED) v = swiglu(v, __shfl_xor(v, 16, 64));
+      if (m >= mrows || ncol >= nrows || (GATED && c >= 16)) continue;
+      if (p.residual) v = v + wide<DT>(p.residual[(m0 + m) * p.ldr + n]);
+      p.out[(m0 + m) * p.ldo + n] = slim<DT>(v);
+    }
 }
 
 // Whether a call takes the tiles (offsets inside a tile are 32 bits there).
@@ -436,7 +432,7 @@ static int launch_w4_tiles(const W4Params& p, void* workspace, hipStream_t strea
   if (DT == kBF16)
     hipLaunchKernelGGL((w4_sums_kernel<DT, GB>), dim3((unsigned)((p.m * (p.k / 8) + 255) / 256)), dim3(256), 0, stream,
                        p, sums);
-  hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, GATED>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0,
+  hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, GATED>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(512), 0,
                      stream, p, sums, mtiles, (int)tiles);
   return launch_status("w8a8_linear_w4");
 }
