@@ -283,55 +283,64 @@ __device__ __forceinline__ v16f mfma_zero(uint2 sum, uint2 z) {
   return __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(__builtin_bit_cast(v4s, sum), __builtin_bit_cast(v4s, z), v16f{}, 0, 0, 0);
 }
 
-// Many rows: a workgroup of eight waves takes 128 rows of x and 256 weight rows
-// (gated: 128 of gate and the same of up); each wave takes all of x's rows and 32
-// of the weight's (gated: 16 of each), so that every code is unpacked once, and
-// the two waves of a SIMD do each other's unpacking and scaling in the shadow of
-// their MFMAs. The 32 x 32 x 16 MFMA's first operand is x, from LDS, its second the
-// weights, a word of codes a lane: a lane's column is one weight row, whose scale
-// it holds. x comes by DMA in steps of 128 inputs, two in turn (16-byte run c of
-// row r at run c ^ (r & 15)), codes and scales into registers a step ahead.
+// More than 16 rows: a workgroup of W waves takes 32 U rows of x and 32 W weight
+// rows (gated: 16 W of gate and the same of up); each wave takes all of x's rows
+// and 32 of the weight's (gated: 16 of each), so that every code is unpacked once
+// a workgroup, and the waves of a SIMD do each other's unpacking and scaling in
+// the shadow of their MFMAs. The 32 x 32 x 16 MFMA's first operand is x, from LDS,
+// its second the weights, a word of codes a lane: a lane's column is one weight
+// row, whose scale it holds. x comes by DMA in steps of 128 inputs, two in turn
+// (16-byte run c of row r at run c ^ (r & 15)), codes and scales into registers a
+// step ahead.
 //
 // fp16 takes the zeros off its weights (packed subtraction, exact). bf16 has no
-// such instruction: there an MFMA puts -(16 + z) sum x into the accumulators
-// before a block's products, with the sum in three bf16 (exact) as three inputs.
-template <int DT, int GB, bool GATED>
-__global__ __launch_bounds__(512, 2)
-void linear_w4_tiles_kernel(W4Params p, const uint2* sums, int mtiles, int tiles) {
-  constexpr int S = GB / 16, NB = 128 / GB, BN = GATED ? 128 : 256;
-  __shared__ __attribute__((aligned(16))) char xs[2][128 * 256];
+// such instruction. Where the rows are many an MFMA puts -(16 + z) sum x into the
+// accumulators before a block's products, with the sum in three bf16 (exact) as
+// three inputs; where they are few a second MFMA beside each product sums x, which
+// costs less than the launch that sums it beforehand.
+//
+// Where the tiles are too few for the GPU, the steps of k are split over `splits`
+// workgroups, whose sums linear_w4_join_kernel adds in order.
+template <int DT, int GB, int U, int W, bool GATED>
+__global__ __launch_bounds__(64 * W, U == 4 ? 2 : DT == kBF16 && U == 2 ? 3 : 4)
+void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mtiles, int tiles, int splits) {
+  constexpr int S = GB / 16, NB = 128 / GB, BN = GATED ? 16 * W : 32 * W, ROWS = 32 * U, DMAS = 8 * U / W;
+  constexpr bool SUMS = DT == kBF16 && U == 4, ONES = DT == kBF16 && U < 4;
+  __shared__ __attribute__((aligned(16))) char xs[2][ROWS * 256];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t width = GATED ? p.n / 2 : p.n;
-  // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, the
-  // row tiles of a few weight tiles at a time.
-  const int per = (tiles + 7) / 8, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (tile >= tiles || (int)(blockIdx.x >> 3) >= per) return;
-  const int64_t m0 = (int64_t)(tile % mtiles) * 128, n0 = (int64_t)(tile / mtiles) * BN;
-  const int mrows = (int)min((int64_t)128, p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
+  // Workgroups go to the eight XCDs in turn: each XCD takes a run of items, the
+  // row tiles (then the ranges of k) of a few weight tiles at a time.
+  const int items = tiles * splits, per = (items + 7) / 8, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (item >= items || (int)(blockIdx.x >> 3) >= per) return;
+  const int tile = item / splits, split = item - tile * splits;
+  const int64_t m0 = (int64_t)(tile % mtiles) * ROWS, n0 = (int64_t)(tile / mtiles) * BN;
+  const int mrows = (int)min((int64_t)ROWS, p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
   const int ncol = GATED ? 16 * wave + (c & 15) : 32 * wave + c;   // the lane's column of the tile
   const int64_t wr = (GATED && c >= 16 ? width : 0) + n0 + min(ncol, nrows - 1);
   const char* const wrow = reinterpret_cast<const char*>(p.codes + wr * p.ldw);
   const char* xbase = reinterpret_cast<const char*>(reinterpret_cast<const uint16_t*>(p.x) + m0 * p.ldx);
-  uint32_t xoff[4];
+  uint32_t xoff[DMAS];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) xoff[i] = (uint32_t)min(16 * wave + 4 * i + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
-  const int steps = (int)((p.k + 127) / 128), words = (int)(p.k / 8), blocks = (int)(p.k / GB);
+  for (int i = 0; i < DMAS; ++i)
+    xoff[i] = (uint32_t)min(4 * (DMAS * wave + i) + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
+  const int all = (int)((p.k + 127) / 128), words = (int)(p.k / 8), blocks = (int)(p.k / GB);
+  const int first = (int)((int64_t)all * split / splits), last = (int)((int64_t)all * (split + 1) / splits);
   const int per_group = p.group / GB;
 
   uint32_t w[NB][S];
   uint16_t sc[NB];
   uint8_t zr[NB];
-  uint2 sm[NB][4];
-  auto load = [&](int step, int buf) {
+  uint2 sm[NB][SUMS ? U : 1];
+  auto load = [&](int step) {
     // Past the end of k (the last step only) the last runs and codes again: their blocks are left out.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int run = (lane & 15) ^ ((4 * i + (lane >> 4)) & 15);
+    for (int i = 0; i < DMAS; ++i) {
+      const int row = 4 * (DMAS * wave + i), run = (lane & 15) ^ ((row + (lane >> 4)) & 15);
       const char* src = xbase + (xoff[i] + (uint32_t)min(step * 256 + run * 16, (int)p.k * 2 - 16));
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                       (__attribute__((address_space(3))) void*)(xs[buf] + (16 * wave + 4 * i) * 256), 16,
-                                       0, 0);
+                                       (__attribute__((address_space(3))) void*)(xs[step & 1] + row * 256), 16, 0, 0);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -346,37 +355,38 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, int mtiles, int tiles
       }
       sc[b] = p.scales[grow];
       zr[b] = p.zeros ? p.zeros[grow] : (uint8_t)8;
-      if constexpr (DT == kBF16) {
+      if constexpr (SUMS) {
         const uint2* row = sums + (int64_t)block * p.m + m0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sm[b][u] = row[min(32 * u + c, mrows - 1)];
+        for (int u = 0; u < U; ++u) sm[b][u] = row[min(32 * u + c, mrows - 1)];
       }
     }
   };
 
   const Unpack<DT> unpack;
-  v16f tot[4] = {};
-  load(0, 0);
-  for (int step = 0; step < steps; ++step) {
-    const int buf = step & 1;
-    __syncthreads();   // the step's loads have landed (vmcnt(0)); the last one's reads are done
+  v16f tot[U] = {};
+  load(first);
+  for (int step = first; step < last; ++step) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the step's loads have landed,
+    __syncthreads();                      // everyone's, and the last one's reads are done
     uint32_t cw[NB][S];
-    float cs[NB];
+    float cs[NB], fz[NB];
     uint32_t cz[NB];
-    uint2 cm[NB][4];
+    uint2 cm[NB][SUMS ? U : 1];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
       for (int j = 0; j < S; ++j) cw[b][j] = w[b][j];
       cs[b] = wide<DT>(sc[b]);
-      const float z = 16.0f + (float)zr[b];
-      cz[b] = DT == kF16 ? (uint32_t)f2h(z) * 0x10001u : h ? 0 : (uint32_t)f2bf(-z) * 0x10001u;
-      if constexpr (DT == kBF16) {
+      fz[b] = -16.0f - (float)zr[b];
+      cz[b] = DT == kF16 ? (uint32_t)f2h(-fz[b]) * 0x10001u
+                         : h ? 0 : (__float_as_uint(fz[b]) >> 16) * 0x10001u;   // (exact: a small integer)
+      if constexpr (SUMS) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) cm[b][u] = sm[b][u];
+        for (int u = 0; u < U; ++u) cm[b][u] = sm[b][u];
       }
     }
-    if (step + 1 < steps) load(step + 1, buf ^ 1);
+    if (step + 1 < last) load(step + 1);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       if (NB > 1 && step * NB + b >= blocks) break;
@@ -387,27 +397,43 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, int mtiles, int tiles
         if constexpr (DT == kF16) wt[j] = less(wt[j], cz[b]);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        v16f acc = {};
-        if constexpr (DT == kBF16) acc = mfma_zero(cm[b][u], make_uint2(cz[b], cz[b]));
+      for (int u = 0; u < U; ++u) {
+        v16f acc = {}, sum = {};
+        if constexpr (SUMS) acc = mfma_zero(cm[b][u], make_uint2(cz[b], cz[b]));
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-          const v4u x = *reinterpret_cast<const v4u*>(xs[buf] + (32 * u + c) * 256 + 16 * ((b * (GB / 8) + h * S + j) ^ (c & 15)));
+          const v4u x = *reinterpret_cast<const v4u*>(xs[step & 1] + (32 * u + c) * 256 +
+                                                      16 * ((b * (GB / 8) + h * S + j) ^ (c & 15)));
           acc = mfma32<DT>(x, wt[j], acc);
+          if constexpr (ONES) sum = mfma32<DT>(x, v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}, sum);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) tot[u][i] = __builtin_fmaf(cs[b], acc[i], tot[u][i]);
+        for (int i = 0; i < 16; ++i) {
+          const float v = ONES ? __builtin_fmaf(fz[b], sum[i], acc[i]) : acc[i];
+          tot[u][i] = __builtin_fmaf(cs[b], v, tot[u][i]);
+        }
       }
       // (Here, not at the end of the step, where the compiler would put the sums
       // of all its blocks with every accumulator alive.)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) __asm__ volatile("" : "+v"(tot[u]));
+      for (int u = 0; u < U; ++u) __asm__ volatile("" : "+v"(tot[u]));
     }
   }
   const int64_t n = n0 + ncol;
+  if (splits > 1) {
+    float* part = parts + (int64_t)split * p.m * p.n + wr;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (m < mrows && ncol < nrows) part[(m0 + m) * p.n] = tot[u][i];
+      }
+    return;
+  }
   const float bias = p.bias ? wide<DT>(p.bias[wr]) : 0.0f;
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -419,36 +445,92 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, int mtiles, int tiles
     }
 }
 
+// The outputs of a split call: the ranges' sums in order, then the epilogue. One
+// output a thread.
+template <int DT>
+__global__ __launch_bounds__(256)
+void linear_w4_join_kernel(W4Params p, const float* parts, int splits, bool gated) {
+  const int64_t width = gated ? p.n / 2 : p.n, n = (int64_t)blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+  if (n >= width) return;
+  const float* row = parts + m * p.n + n;
+  const int64_t stride = p.m * p.n;
+  float v = row[0], up = gated ? row[width] : 0.0f;
+  for (int s = 1; s < splits; ++s) {
+    v = v + row[s * stride];
+    if (gated) up = up + row[s * stride + width];
+  }
+  if (p.bias) v = v + wide<DT>(p.bias[n]);
+  if (gated) v = swiglu(v, p.bias ? up + wide<DT>(p.bias[width + n]) : up);
+  if (p.residual) v = v + wide<DT>(p.residual[m * p.ldr + n]);
+  p.out[m * p.ldo + n] = slim<DT>(v);
+}
+
+// How a call of more than 16 rows is cut: 32 u rows and 32 w weight rows a tile,
+// and the ranges of k. The ranges keep at least four steps, and their sums at
+// most 64 MB.
+struct W4Plan {
+  int u, w, mtiles, splits;
+  int64_t tiles;
+};
+
+static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int cus) {
+  W4Plan q;
+  q.u = m > 64 ? 4 : m > 32 ? 2 : 1;
+  q.w = q.u == 4 ? 8 : 4;
+  q.mtiles = (int)((m + 32 * q.u - 1) / (32 * q.u));
+  q.tiles = (n + 32 * q.w - 1) / (32 * q.w) * q.mtiles;
+  const int64_t steps = (k + 127) / 128, want = (q.u == 4 ? 1 : 2) * (int64_t)cus;
+  int64_t s = q.tiles < want ? want / q.tiles : 1;
+  if (s > steps / 4) s = steps / 4;
+  const int64_t most = (64ll << 20) / (4 * m * n);
+  if (s > most) s = most;
+  q.splits = s < 2 ? 1 : (int)s;
+  return q;
+}
+
 // Whether a call takes the tiles (offsets inside a tile are 32 bits there).
-static bool w4_tiled(int64_t m, int64_t ldx) { return m > 64 && ldx < (1 << 22); }
+static bool w4_tiled(int64_t m) { return m > 16; }
+
+// Bytes of the sums of x (bf16 with many rows; asked of fp16 alike) and, behind
+// them, of the ranges' sums.
+static int64_t w4_sums_bytes(const W4Plan& q, int64_t m, int64_t k, int group) {
+  return q.u == 4 ? (8 * m * (k / (group < 128 ? group : 128)) + 255) / 256 * 256 : 0;
+}
+
+template <int DT, int GB, int U, int W, bool GATED>
+static void launch_w4_plan(const W4Params& p, const W4Plan& q, void* workspace, hipStream_t stream) {
+  uint2* sums = reinterpret_cast<uint2*>(workspace);
+  float* parts = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + w4_sums_bytes(q, p.m, p.k, p.group));
+  if (DT == kBF16 && U == 4)
+    hipLaunchKernelGGL((w4_sums_kernel<DT, GB>), dim3((unsigned)((p.m * (p.k / 8) + 255) / 256)), dim3(256), 0, stream,
+                       p, sums);
+  const int64_t items = q.tiles * q.splits;
+  hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, U, W, GATED>), dim3((unsigned)((items + 7) / 8 * 8)),
+                     dim3(64 * W), 0, stream, p, sums, parts, q.mtiles, (int)q.tiles, q.splits);
+  if (q.splits > 1)
+    hipLaunchKernelGGL((linear_w4_join_kernel<DT>), dim3((unsigned)(((GATED ? p.n / 2 : p.n) + 255) / 256), (unsigned)p.m),
+                       dim3(256), 0, stream, p, parts, q.splits, GATED);
+}
 
 template <int DT, int GB, bool GATED>
 static int launch_w4_tiles(const W4Params& p, void* workspace, hipStream_t stream) {
-  const int64_t width = GATED ? p.n / 2 : p.n, per = GATED ? 128 : 256;
-  const int mtiles = (int)((p.m + 127) / 128);
-  const int64_t tiles = (width + per - 1) / per * mtiles;
-  W8A8_REQUIRE(tiles < ((int64_t)1 << 24), "w8a8_linear_w4: too many outputs for one launch");
-  uint2* sums = reinterpret_cast<uint2*>(workspace);
-  if (DT == kBF16)
-    hipLaunchKernelGGL((w4_sums_kernel<DT, GB>), dim3((unsigned)((p.m * (p.k / 8) + 255) / 256)), dim3(256), 0, stream,
-                       p, sums);
-  hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, GATED>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(512), 0,
-                     stream, p, sums, mtiles, (int)tiles);
+  const W4Plan q = w4_plan(p.m, p.n, p.k, current_device_cus());
+  W8A8_REQUIRE(q.tiles < ((int64_t)1 << 22) && p.ldx < (1 << 22), "w8a8_linear_w4: too many outputs for one launch");
+  switch (q.u) {
+    case 4: launch_w4_plan<DT, GB, 4, 8, GATED>(p, q, workspace, stream); break;
+    case 2: launch_w4_plan<DT, GB, 2, 4, GATED>(p, q, workspace, stream); break;
+    default: launch_w4_plan<DT, GB, 1, 4, GATED>(p, q, workspace, stream); break;
+  }
   return launch_status("w8a8_linear_w4");
 }
 
 template <int DT, int GB, bool GATED>
 static int launch_w4(const W4Params& p, void* workspace, hipStream_t stream) {
-  if (w4_tiled(p.m, p.ldx)) return launch_w4_tiles<DT, GB, GATED>(p, workspace, stream);
+  if (w4_tiled(p.m)) return launch_w4_tiles<DT, GB, GATED>(p, workspace, stream);
   constexpr int NT = 2, W = 8;
   const int64_t width = GATED ? p.n / 2 : p.n, per = GATED ? 16 * NT / 2 : 16 * NT;
-  const int mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)((width + per - 1) / per), (unsigned)((p.m + 16 * mt - 1) / (16 * mt)));
-  switch (mt) {
-    case 1: hipLaunchKernelGGL((linear_w4_kernel<DT, GB, NT, 1, W, GATED>), grid, dim3(64 * W), 0, stream, p); break;
-    case 2: hipLaunchKernelGGL((linear_w4_kernel<DT, GB, NT, 2, W, GATED>), grid, dim3(64 * W), 0, stream, p); break;
-    default: hipLaunchKernelGGL((linear_w4_kernel<DT, GB, NT, 4, W, GATED>), grid, dim3(64 * W), 0, stream, p); break;
-  }
+  hipLaunchKernelGGL((linear_w4_kernel<DT, GB, NT, 1, W, GATED>), dim3((unsigned)((width + per - 1) / per)),
+                     dim3(64 * W), 0, stream, p);
   return launch_status("w8a8_linear_w4");
 }
 
@@ -463,10 +545,11 @@ static int launch_w4_group(const W4Params& p, bool gated, void* ws, hipStream_t 
 
 }  // namespace w8a8
 
-// Many rows: the sums of x, 8 bytes a row and block (bf16; asked of fp16 alike).
 extern "C" int64_t w8a8_linear_w4_workspace_size(int64_t m, int64_t n, int64_t k, int32_t group, int32_t) {
-  if (m <= 64 || n <= 0 || k <= 0 || group <= 0) return 0;
-  return 8 * m * (k / (group < 128 ? group : 128));
+  using namespace w8a8;
+  if (!w4_tiled(m) || n <= 0 || k <= 0 || group <= 0) return 0;
+  const W4Plan q = w4_plan(m, n, k, current_device_cus());
+  return w4_sums_bytes(q, m, k, group) + (q.splits > 1 ? 4 * (int64_t)q.splits * m * n : 0);
 }
 
 extern "C" int w8a8_linear_w4(const W8A8LinearW4Args* a) {
