@@ -14,6 +14,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
@@ -24,6 +25,7 @@
 #include <algorithm>
 #include <array>
 #include <cmath>
+#include <initializer_list>
 #include <vector>
 
 #include "w8a8.h"
@@ -306,6 +308,312 @@ PyObject* segment_labels(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------- around the projections of a block
+
+// A tensor argument that may be None: `ok` turns false for anything but None or
+// a plain tensor.
+const at::Tensor* optional(PyObject* o, bool& ok) {
+  if (o == Py_None) return nullptr;
+  const at::Tensor* t = plain(o);
+  if (!t) ok = false;
+  return t;
+}
+
+// A float argument that may be None.
+bool optional_float(PyObject* o, float& v, bool& given) {
+  given = o != Py_None;
+  if (!given) return true;
+  if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+  v = (float)PyFloat_AsDouble(o);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+
+// Whether a gradient would be asked of a tensor: the Python route refuses it.
+bool wants_gradient(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+
+bool aligned(const at::Tensor& t, uintptr_t n) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % n == 0; }
+
+// [rows, cols] with contiguous 16-byte aligned rows; ld its row stride.
+bool aligned_rows(const at::Tensor& t, int64_t rows, int64_t cols, int64_t& ld) {
+  if (t.dim() != 2 || t.size(0) != rows || t.size(1) != cols || t.stride(1) != 1 || !aligned(t, 16)) return false;
+  const int64_t es = t.element_size();
+  ld = rows > 1 ? t.stride(0) : (cols * es + 15) / 16 * 16 / es;
+  return ld >= cols && ld * es % 16 == 0;
+}
+
+bool fp32_vector(const at::Tensor* t, int64_t n) {
+  return !t || (t->scalar_type() == at::kFloat && t->numel() == n && t->is_contiguous() && aligned(*t, 16));
+}
+
+bool set_item(PyObject* dict, const char* key, at::Tensor t) {
+  PyObject* o = THPVariable_Wrap(std::move(t));
+  const bool ok = o && PyDict_SetItemString(dict, key, o) == 0;
+  Py_XDECREF(o);
+  return ok;
+}
+
+// residual_norm(x, branch, weight, eps, post_weight, post_eps, gate, shift,
+// scale, labels, residual_scale, branch_scale, quantize, convrot,
+// round_rotated, want_normalized, out): kernels.residual_norm without signs.
+PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 17 || modes_active()) Py_RETURN_NONE;
+  bool ok = true;
+  const at::Tensor* x = plain(args[0]);
+  const at::Tensor* branch = plain(args[1]);
+  const at::Tensor* weight = optional(args[2], ok);
+  const at::Tensor* post_weight = optional(args[4], ok);
+  const at::Tensor* gate = optional(args[6], ok);
+  const at::Tensor* shift = optional(args[7], ok);
+  const at::Tensor* mscale = optional(args[8], ok);
+  const at::Tensor* labels = optional(args[9], ok);
+  const at::Tensor* out = optional(args[16], ok);
+  W8A8ResidualNormArgs a{};
+  bool pre = false, post = false, given = false;
+  if (!x || !branch || !ok || x->dim() != 2 || !optional_float(args[3], a.eps, pre) ||
+      !optional_float(args[5], a.post_eps, post) || !optional_float(args[10], a.residual_scale, given) || !given ||
+      !optional_float(args[11], a.branch_scale, given) || !given)
+    Py_RETURN_NONE;
+  for (int i = 12; i < 16; ++i)
+    if (!PyBool_Check(args[i])) Py_RETURN_NONE;
+  const bool quantize = args[12] == Py_True, convrot = args[13] == Py_True, want = args[15] == Py_True;
+  const int64_t rows = x->size(0), cols = x->size(1);
+  const at::ScalarType type = x->scalar_type();
+  if ((type != at::kHalf && type != at::kBFloat16) ||
+      (branch->scalar_type() != type && branch->scalar_type() != at::kFloat) || rows <= 0 || cols <= 0 ||
+      cols % (quantize && convrot ? 256 : 16) || !aligned_rows(*x, rows, cols, a.ldx) ||
+      !aligned_rows(*branch, rows, cols, a.ldb) || !fp32_vector(weight, cols) || !fp32_vector(post_weight, cols) ||
+      (post_weight && !post) || (!pre && (quantize || want || weight || shift || mscale)) ||
+      wants_gradient({x, branch, weight, post_weight, gate, shift, mscale}))
+    Py_RETURN_NONE;
+  if (gate) {
+    if (gate->scalar_type() != at::kFloat || gate->dim() != 2 || gate->size(0) < 1 ||
+        !aligned_rows(*gate, gate->size(0), cols, a.ld_gate))
+      Py_RETURN_NONE;
+    a.gate = ptr<float>(*gate);
+    a.gate_rows = (int32_t)gate->size(0);
+  }
+  if (shift || mscale) {
+    int64_t ld = 0;
+    if (!shift || !mscale || shift->scalar_type() != at::kFloat || mscale->scalar_type() != at::kFloat ||
+        shift->dim() != 2 || shift->size(0) < 1 || !aligned_rows(*shift, shift->size(0), cols, a.ld_mod) ||
+        !aligned_rows(*mscale, shift->size(0), cols, ld) || ld != a.ld_mod)
+      Py_RETURN_NONE;
+    a.mod_shift = ptr<float>(*shift);
+    a.mod_scale = ptr<float>(*mscale);
+    a.mod_rows = (int32_t)shift->size(0);
+  }
+  if (gate || shift) {
+    if (!labels || labels->scalar_type() != at::kInt || labels->numel() != rows || !labels->is_contiguous())
+      Py_RETURN_NONE;
+    a.labels = ptr<int32_t>(*labels);
+  }
+  if (out && (out->scalar_type() != type || !aligned_rows(*out, rows, cols, a.ldo) || wants_gradient({out})))
+    Py_RETURN_NONE;
+  const auto opt = at::TensorOptions().device(x->device());
+  at::Tensor fresh, y, q, qs;
+  if (!out) {
+    fresh = at::empty({rows, cols}, opt.dtype(type));
+    a.ldo = cols;
+  }
+  const bool want_y = pre && (want || !quantize);
+  if (want_y) y = at::empty({rows, cols}, opt.dtype(type));
+  if (quantize) {
+    q = at::empty({rows, cols}, opt.dtype(at::kChar));
+    qs = at::empty({rows, 1}, opt.dtype(at::kFloat));
+  }
+  a.x_dtype = dtype_code(type);
+  a.x = x->data_ptr();
+  a.rows = rows;
+  a.cols = cols;
+  a.branch = branch->data_ptr();
+  a.branch_dtype = dtype_code(branch->scalar_type());
+  a.post = post;
+  a.post_weight = post_weight ? ptr<float>(*post_weight) : nullptr;
+  a.out = out ? out->data_ptr() : fresh.data_ptr();
+  a.weight = weight ? ptr<float>(*weight) : nullptr;
+  a.y = want_y ? y.data_ptr() : nullptr;
+  a.ldy = cols;
+  a.convrot = quantize && convrot ? 256 : 0;
+  a.round_rotated = args[14] == Py_True;
+  a.q = quantize ? ptr<int8_t>(q) : nullptr;
+  a.ldq = cols;
+  a.q_scale = quantize ? ptr<float>(qs) : nullptr;
+  a.stream = stream_of(x->get_device());
+  const int rc = call(w8a8_residual_norm, a);
+  if (rc != W8A8_OK) return fail("w8a8_residual_norm", rc);
+  PyObject* d = PyDict_New();
+  if (!d) return nullptr;
+  ok = out ? PyDict_SetItemString(d, "x", args[16]) == 0 : set_item(d, "x", std::move(fresh));
+  if (ok && want_y) ok = set_item(d, "y", std::move(y));
+  if (ok && quantize) ok = set_item(d, "q", std::move(q)) && set_item(d, "scale", std::move(qs));
+  if (!ok) {
+    Py_DECREF(d);
+    return nullptr;
+  }
+  return d;
+  END_HANDLE_TH_ERRORS
+}
+
+// Element strides {row, head} of a [rows, heads, dim] tensor.
+bool head_strides(const at::Tensor& t, int64_t (&st)[2]) {
+  if (t.dim() != 3 || (t.size(2) > 1 && t.stride(2) != 1)) return false;
+  st[1] = t.size(1) > 1 ? t.stride(1) : t.size(2);
+  st[0] = t.size(0) > 1 ? t.stride(0) : t.size(1) * st[1];
+  return true;
+}
+
+// axial_rope(q, k, positions, inv_freq, axis, adjacent, q_gain, k_gain, eps,
+// q_out, k_out): kernels.axial_rope; returns (q_out, k_out).
+PyObject* axial_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11 || modes_active() || !PyBool_Check(args[5])) Py_RETURN_NONE;
+  bool ok = true, given = false;
+  const at::Tensor* q = plain(args[0]);
+  const at::Tensor* k = optional(args[1], ok);
+  const at::Tensor* pos = plain(args[2]);
+  const at::Tensor* inv = plain(args[3]);
+  const at::Tensor* axis = plain(args[4]);
+  const at::Tensor* gq = optional(args[6], ok);
+  const at::Tensor* gk = optional(args[7], ok);
+  const at::Tensor* qo = optional(args[9], ok);
+  const at::Tensor* ko = optional(args[10], ok);
+  W8A8AxialRopeArgs a{};
+  if (!q || !pos || !inv || !axis || !ok || !optional_float(args[8], a.eps, given) || !given ||
+      !head_strides(*q, a.q_strides) || (k && !head_strides(*k, a.k_strides)))
+    Py_RETURN_NONE;
+  const at::ScalarType type = q->scalar_type();
+  const int64_t rows = q->size(0), heads = q->size(1), dim = q->size(2), pairs = inv->numel();
+  const int64_t kheads = k ? k->size(1) : 0;
+  const auto pt = pos->scalar_type();
+  if (!dtype_code(type) || rows <= 0 || heads <= 0 || heads > 4096 || dim < 2 || dim > 256 || dim % 2 ||
+      (k && (k->scalar_type() != type || k->size(0) != rows || k->size(2) != dim || kheads <= 0 || kheads > 4096)) ||
+      pos->dim() != 2 || pos->size(0) != rows || pos->size(1) < 1 || pos->size(1) > 16 ||
+      (pt != at::kInt && pt != at::kLong && pt != at::kFloat) || inv->dim() != 1 || inv->scalar_type() != at::kDouble ||
+      !inv->is_contiguous() || pairs < 1 || 2 * pairs > dim || axis->dim() != 1 || axis->numel() != pairs ||
+      axis->scalar_type() != at::kInt || !axis->is_contiguous() || !fp32_vector(gq, dim) || !fp32_vector(gk, dim) ||
+      (gq && k && !gk) || (gk && !(gq && k)) || wants_gradient({q, k, pos, inv, gq, gk, qo, ko}))
+    Py_RETURN_NONE;
+  if ((qo || ko) && (!qo || (ko != nullptr) != (k != nullptr))) Py_RETURN_NONE;
+  if (qo && (qo->scalar_type() != type || qo->sizes() != q->sizes() || !head_strides(*qo, a.q_out_strides)))
+    Py_RETURN_NONE;
+  if (ko && (ko->scalar_type() != type || ko->sizes() != k->sizes() || !head_strides(*ko, a.k_out_strides)))
+    Py_RETURN_NONE;
+  const auto opt = at::TensorOptions().device(q->device()).dtype(type);
+  at::Tensor q_new, k_new;
+  if (!qo) {
+    q_new = at::empty({rows, heads, dim}, opt);
+    head_strides(q_new, a.q_out_strides);
+    if (k) {
+      k_new = at::empty({rows, kheads, dim}, opt);
+      head_strides(k_new, a.k_out_strides);
+    }
+  }
+  a.dtype = dtype_code(type);
+  a.q = q->data_ptr();
+  a.k = k ? k->data_ptr() : nullptr;
+  a.q_out = qo ? qo->data_ptr() : q_new.data_ptr();
+  a.k_out = !k ? nullptr : ko ? ko->data_ptr() : k_new.data_ptr();
+  a.rows = rows;
+  a.q_heads = (int32_t)heads;
+  a.k_heads = (int32_t)kheads;
+  a.dim = (int32_t)dim;
+  a.pairs = (int32_t)pairs;
+  a.axes = (int32_t)pos->size(1);
+  a.pairing = args[5] == Py_True ? W8A8_ROPE_ADJACENT : W8A8_ROPE_HALF;
+  a.positions = pos->data_ptr();
+  a.pos_strides[0] = pos->stride(0);
+  a.pos_strides[1] = pos->stride(1);
+  a.pos_type = pt == at::kInt ? W8A8_POS_I32 : pt == at::kLong ? W8A8_POS_I64 : W8A8_POS_F32;
+  a.inv_freq = ptr<double>(*inv);
+  a.axis = ptr<int32_t>(*axis);
+  a.q_gain = gq ? ptr<float>(*gq) : nullptr;
+  a.k_gain = gk ? ptr<float>(*gk) : nullptr;
+  a.stream = stream_of(q->get_device());
+  const int rc = call(w8a8_axial_rope, a);
+  if (rc != W8A8_OK) return fail("w8a8_axial_rope", rc);
+  PyObject* pq = qo ? Py_NewRef(args[9]) : THPVariable_Wrap(std::move(q_new));
+  PyObject* pk = !k ? Py_NewRef(Py_None) : ko ? Py_NewRef(args[10]) : THPVariable_Wrap(std::move(k_new));
+  PyObject* r = pq && pk ? PyTuple_Pack(2, pq, pk) : nullptr;
+  Py_XDECREF(pq);
+  Py_XDECREF(pk);
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_w4(x, codes, scales, zeros, bias, residual, gated): kernels.linear_w4
+// of contiguous tensors into a new output.
+PyObject* linear_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || modes_active() || !PyBool_Check(args[6])) Py_RETURN_NONE;
+  bool ok = true;
+  const at::Tensor* x = plain(args[0]);
+  const at::Tensor* codes = plain(args[1]);
+  const at::Tensor* scales = plain(args[2]);
+  const at::Tensor* zeros = optional(args[3], ok);
+  const at::Tensor* bias = optional(args[4], ok);
+  const at::Tensor* residual = optional(args[5], ok);
+  const bool gated = args[6] == Py_True;
+  if (!x || !codes || !scales || !ok || x->dim() < 1 || !x->is_contiguous() || codes->dim() != 2 ||
+      codes->scalar_type() != at::kInt || !codes->is_contiguous() || scales->dim() != 2 || !scales->is_contiguous())
+    Py_RETURN_NONE;
+  const at::ScalarType type = x->scalar_type();
+  const int64_t nn = codes->size(0), k = 8 * codes->size(1), groups = scales->size(0);
+  if ((type != at::kHalf && type != at::kBFloat16) || scales->scalar_type() != type || k <= 0 || nn <= 0 ||
+      x->size(-1) != k || x->numel() == 0 || groups <= 0 || k % groups || scales->size(1) != nn || !aligned(*x, 16) ||
+      !aligned(*codes, 16) || codes->size(1) % 4 || wants_gradient({x, scales, bias, residual}))
+    Py_RETURN_NONE;
+  const int64_t group = k / groups, m = x->numel() / k, width = gated ? nn / 2 : nn;
+  if ((group != 32 && group != 64 && group % 128) || (gated && (nn % 2 || residual)) ||
+      (zeros && (zeros->scalar_type() != at::kByte || zeros->sizes() != scales->sizes() || !zeros->is_contiguous())) ||
+      (bias && (bias->scalar_type() != type || bias->numel() != nn || !bias->is_contiguous())) ||
+      (residual && (residual->scalar_type() != type || residual->numel() != m * nn || residual->size(-1) != nn ||
+                    !residual->is_contiguous())))
+    Py_RETURN_NONE;
+  const auto opt = at::TensorOptions().device(x->device());
+  at::DimVector shape(x->sizes().begin(), x->sizes().end());
+  shape.back() = width;
+  at::Tensor out = at::empty(shape, opt.dtype(type));
+  W8A8LinearW4Args a{};
+  at::Tensor workspace;
+  a.workspace_bytes = w8a8_linear_w4_workspace_size(m, nn, k, (int32_t)group, gated);
+  if (a.workspace_bytes > 0) {
+    workspace = at::empty({a.workspace_bytes}, opt.dtype(at::kByte));
+    a.workspace = workspace.data_ptr();
+  }
+  a.dtype = dtype_code(type);
+  a.x = x->data_ptr();
+  a.ldx = k;
+  a.codes = ptr<int32_t>(*codes);
+  a.ldw = k / 8;
+  a.scales = scales->data_ptr();
+  a.zeros = zeros ? ptr<uint8_t>(*zeros) : nullptr;
+  a.m = m;
+  a.n = nn;
+  a.k = k;
+  a.group = (int32_t)group;
+  a.gated = gated;
+  a.bias = bias ? bias->data_ptr() : nullptr;
+  a.residual = residual ? residual->data_ptr() : nullptr;
+  a.ldr = nn;
+  a.out = out.data_ptr();
+  a.ldo = width;
+  a.stream = stream_of(x->get_device());
+  const int rc = call(w8a8_linear_w4, a);
+  if (rc != W8A8_OK) return fail("w8a8_linear_w4", rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_error_class(PyObject*, PyObject* cls) {
   Py_INCREF(cls);
   Py_XSETREF(g_error_class, cls);
@@ -322,6 +630,9 @@ PyMODINIT_FUNC PyInit__native() {
       {"linear", fast(linear), METH_FASTCALL, nullptr},
       {"int8_attention", fast(int8_attention), METH_FASTCALL, nullptr},
       {"segment_labels", fast(segment_labels), METH_FASTCALL, nullptr},
+      {"residual_norm", fast(residual_norm), METH_FASTCALL, nullptr},
+      {"axial_rope", fast(axial_rope), METH_FASTCALL, nullptr},
+      {"linear_w4", fast(linear_w4), METH_FASTCALL, nullptr},
       {"set_error_class", set_error_class, METH_O, nullptr},
       {nullptr, nullptr, 0, nullptr},
   };

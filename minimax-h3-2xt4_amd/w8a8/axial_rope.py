@@ -12,7 +12,7 @@ pair). ``ladder`` builds the usual ones.
 """
 import torch
 
-from . import kernels
+from . import _abi, kernels
 
 
 def ladder(sections, theta=10000.0, *, shared=False, interleaved=False, device=None):
@@ -58,6 +58,11 @@ def rotate(q, k, positions, inv_freq, axis, *, pairing='half', q_gain=None, k_ga
     'half' (p with p + pairs) or 'adjacent' (2 p with 2 p + 1). Inference only."""
     if pairing not in ('half', 'adjacent'):
         raise ValueError('pairing must be half or adjacent')
+    q_out, k_out = out if out is not None else (None, None)
+    r = _abi.native().axial_rope(q, k, positions, inv_freq, axis, pairing == 'adjacent', q_gain, k_gain, eps, q_out,
+                                 k_out)
+    if r is not None:
+        return r
     return kernels.axial_rope(q, k, positions, inv_freq, axis, adjacent=pairing == 'adjacent', q_gain=q_gain,
                               k_gain=k_gain, eps=eps, out=out)
 

@@ -8,7 +8,7 @@ branch has an RMS norm of its own, which the reference's blocks have not),
 residual_norm does both in one kernel, down to the next projection's INT8
 codes.
 """
-from . import kernels
+from . import _abi, kernels
 from .h3_tensor_flow import _norm_args
 
 
@@ -21,6 +21,12 @@ def residual_norm(x, branch, *, weight=None, eps=None, post_weight=None, post_ep
     A branch that a norm follows cannot carry the residual divisor c in its
     projection's weight scale: pass branch_scale=1/c. ``out=x`` updates the
     stream in place."""
+    if signs is None:
+        r = _abi.native().residual_norm(x, branch, weight, eps, post_weight, post_eps, gate, shift, scale, labels,
+                                        residual_scale, branch_scale, quantize, convrot, round_rotated,
+                                        want_normalized, out)
+        if r is not None:
+            return r
     return kernels.residual_norm(x, branch, weight=weight, eps=eps, post_weight=post_weight, post_eps=post_eps,
                                  gate=gate, shift=shift, scale=scale, labels=labels, residual_scale=residual_scale,
                                  branch_scale=branch_scale, quantize=quantize, convrot=convrot,

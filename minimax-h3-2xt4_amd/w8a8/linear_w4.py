@@ -13,7 +13,7 @@ that a shift and a mask leave two neighbouring inputs in a word's halves).
 import torch
 from torch import nn
 
-from . import kernels
+from . import _abi, kernels
 
 _NIBBLE_OF_INPUT = (0, 4, 1, 5, 2, 6, 3, 7)
 
@@ -73,6 +73,10 @@ def dequantize_weight(codes, scales, zeros=None):
 
 def linear(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=False, out=None):
     """x [.., K] times the 4-bit weight; see kernels.linear_w4. Inference only."""
+    if out is None:
+        y = _abi.native().linear_w4(x, codes, scales, zeros, bias, residual, gated)
+        if y is not None:
+            return y
     return kernels.linear_w4(x, codes, scales, zeros, bias=bias, residual=residual, gated=gated, out=out)
 
 

@@ -130,3 +130,33 @@ def test_two_streams_at_once(gpu):
         torch.cuda.synchronize()
         for outs, v in zip(got, want):
             assert all(torch.equal(o, v) for o in outs)
+
+
+def test_host_routes_agree(gpu):
+    """The native calls and the Python wrappers make the same call."""
+    w = _weights(gpu)
+    x, branch, pos = _inputs(37, gpu)
+    gate = torch.randn((3, HIDDEN), device=gpu)
+    labels = (torch.arange(37, device=gpu) % 3).int()
+    for kw in (dict(), dict(eps=1e-6), dict(eps=1e-6, weight=w['norm1'], quantize=True, post_eps=1e-5),
+               dict(eps=1e-6, gate=gate, labels=labels, shift=gate, scale=gate, quantize=True, want_normalized=True,
+                    convrot=False, residual_scale=2, branch_scale=0.5),
+               dict(eps=1e-6, quantize=True, round_rotated=False, post_eps=1e-5, post_weight=w['post1'])):
+        for b in (branch, branch.float()):
+            one, two = block_norm.residual_norm(x, b, **kw), kernels.residual_norm(x, b, **kw)
+            assert one.keys() == two.keys()
+            for key in one:
+                assert torch.equal(one[key], two[key]) and one[key].shape == two[key].shape, (kw.keys(), key)
+    q = torch.randn((37, 6, 128), device=gpu).half()
+    k = torch.randn((37, 2, 128), device=gpu).half()
+    for args, kw in (((q, k), {}), ((q, None), dict(q_gain=w['q_gain'])),
+                     ((q, k), dict(q_gain=w['q_gain'], k_gain=w['k_gain']))):
+        one = axial_rope.rotate(*args, pos, w['inv'], w['axis'], pairing='adjacent', **kw)
+        two = kernels.axial_rope(*args, pos, w['inv'], w['axis'], adjacent=True, **kw)
+        assert torch.equal(one[0], two[0]) and (one[1] is None) == (two[1] is None)
+        assert one[1] is None or torch.equal(one[1], two[1])
+    m = w['out']
+    a = torch.randn((3, 7, HEADS * 128), device=gpu).half()
+    r = torch.randn((3, 7, HIDDEN), device=gpu).half()
+    assert torch.equal(linear_w4.linear(a, m.codes, m.scales, m.zeros, residual=r),
+                       kernels.linear_w4(a, m.codes, m.scales, m.zeros, residual=r))
