@@ -514,10 +514,10 @@ int w8a8_segment_labels(const int32_t* ends, const int32_t* values, int64_t coun
  *   of the branch (no counterpart in the reference).
  * x: [rows, cols] F16 or BF16 (ldx); branch: [rows, cols] of branch_dtype
  *   (x's, or F32), row stride ldb. Per row, in fp32 (round to nearest even):
- *   n    = branch, or with post != 0 (branch * pinv) * post_weight,
+ *   n    = branch, or with post != 0 branch * pinv,
  *          pinv = 1 / sqrt(sum(branch^2) * fp32(1/cols) + post_eps)
- *   u    = n * branch_scale;  r = x * residual_scale
- *   x'   = x_dtype(gate ? fma(u, gate[l], r) : r + u)
+ *   g    = ([post_weight *] branch_scale) [* gate[l]]
+ *   x'   = x_dtype(fma(n, g, x * residual_scale))
  *   then y, q and q_scale are those of w8a8_norm_quantize on the rows x'.
  * sum(branch^2): the 16 squares of each unit of w8a8_norm_quantize's order in
  *   order, each 64 units' partials in its butterfly, these sums in order.
