@@ -315,10 +315,10 @@ void residual_norm_split_kernel(ResNormParams p) {
 // Many rows: a row per wave, all its units in the wave's registers. A row's tables
 // are up to five times its own bytes, and read from L2 for every row they bound the
 // kernel (53504 x 5376 fp16 with all tables: 629 us), so a workgroup of twelve
-// waves stages those of its middle row's label in LDS - the branch's factor, the
+// waves (eight where the branch is fp32: its units take twice the registers) stages those of its middle row's label in LDS - the branch's factor, the
 // gain, 1 + mod_scale and mod_shift - and takes `per` rows; a row of another label
 // reads its own from memory.
-constexpr int kStagedWaves = 12;
+constexpr int staged_waves(int bt) { return bt == kF32 ? 8 : 12; }
 
 // A unit's raw words out of the compiler's sight: it would otherwise keep what the
 // pass before widened them to, twice the registers.
@@ -455,17 +455,18 @@ __device__ __forceinline__ void norm_row(const ResNormParams& p, const Staged& s
 }
 
 template <int DT, int BT, int MODE, int J>
-__global__ __launch_bounds__(64 * kStagedWaves, 3)
+__global__ __launch_bounds__(64 * staged_waves(BT), staged_waves(BT) / 4)
 void residual_norm_staged_kernel(ResNormParams p, int per) {
+  constexpr int W = staged_waves(BT);
   extern __shared__ __attribute__((aligned(16))) float dsm[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t row0 = (int64_t)blockIdx.x * per, row1 = min(row0 + per, p.rows);
   float* const buf = MODE >= 2 ? rot_slot(dsm, wave, lane) : nullptr;
-  float* next = dsm + (MODE >= 2 ? kStagedWaves * kRotWave : 0);
+  float* next = dsm + (MODE >= 2 ? W * kRotWave : 0);
   const int label = p.labels ? p.labels[row0 + (row1 - row0) / 2] : 0, cols = (int)p.cols;
   const RowTables mid = tables_of(p, label);
   Staged st{};
-  for (int i = 16 * threadIdx.x; i < cols; i += 16 * 64 * kStagedWaves) {
+  for (int i = 16 * threadIdx.x; i < cols; i += 16 * 64 * W) {
     float* at = next + i;
     auto put = [&](const float (&v)[16]) {
 #pragma unroll
@@ -504,7 +505,7 @@ void residual_norm_staged_kernel(ResNormParams p, int per) {
     st.add = next + cols;
   }
   __syncthreads();
-  for (int64_t row = row0 + wave; row < row1; row += kStagedWaves) {
+  for (int64_t row = row0 + wave; row < row1; row += W) {
     // (Its addresses formed anew for each row: kept, they take some forty registers.)
     int own = lane;
     __asm__ volatile("" : "+v"(own));
@@ -623,7 +624,7 @@ static int launch_residual_norm(const ResNormParams& p, hipStream_t stream) {
     return launch_status("w8a8_residual_norm");
   }
   const int tables = (p.gate || p.post_weight ? 1 : 0) + (p.weight ? 1 : 0) + (p.shift ? 2 : 0);
-  const size_t lds = sizeof(float) * ((MODE >= 2 ? kStagedWaves * kRotWave : 0) + (size_t)tables * p.cols);
+  const size_t lds = sizeof(float) * ((MODE >= 2 ? staged_waves(BT) * kRotWave : 0) + (size_t)tables * p.cols);
   // As many rows to a workgroup as give each CU a whole number of them, 60 at
   // most (a workgroup whose rows have two labels holds up the others less).
   const int64_t cus = current_device_cus(), rounds = (p.rows + 60 * cus - 1) / (60 * cus);
@@ -632,7 +633,7 @@ static int launch_residual_norm(const ResNormParams& p, hipStream_t stream) {
     constexpr int J = decltype(j_tag)::value;
     constexpr int JJ = J == 3 ? 4 : J == 5 ? 6 : J;
     hipLaunchKernelGGL((residual_norm_staged_kernel<DT, BT, MODE, JJ>), dim3((unsigned)((p.rows + per - 1) / per)),
-                       dim3(64 * kStagedWaves), lds, stream, p, per);
+                       dim3(64 * staged_waves(BT)), lds, stream, p, per);
   });
   return launch_status("w8a8_residual_norm");
 }
