@@ -121,43 +121,22 @@ __device__ __forceinline__ void finish4(const W4Params& p, int64_t m, int64_t n,
   }
 }
 
-// Scale and 16 + zero of four neighbouring weight rows in group row `at` (the
-// row's offset in scales and zeros); past the last row its values again.
-template <int DT>
-__device__ __forceinline__ void scales4(const W4Params& p, int64_t at, int64_t n, v4f& s, v4f& z) {
-  if (p.quads) {
-    n = min(n, p.n - 4);
-    const uint2 u = *reinterpret_cast<const uint2*>(p.scales + at + n);
-    s = v4f{wide<DT>((uint16_t)u.x), wide<DT>((uint16_t)(u.x >> 16)), wide<DT>((uint16_t)u.y),
-            wide<DT>((uint16_t)(u.y >> 16))};
-    if (p.zeros) {
-      const uint32_t b = *reinterpret_cast<const uint32_t*>(p.zeros + at + n);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) z[i] = (float)((b >> (8 * i)) & 0xffu) + 16.0f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t c = at + min(n + i, p.n - 1);
-      s[i] = wide<DT>(p.scales[c]);
-      if (p.zeros) z[i] = (float)p.zeros[c] + 16.0f;
-    }
-  }
-  if (!p.zeros) z = v4f{24.0f, 24.0f, 24.0f, 24.0f};
-}
-
-// A workgroup of W waves takes 16 NT weight rows (gated: half of them gate, half
-// the same rows of up) and 16 MT rows of x; its waves share out the blocks of k
-// and add their sums in LDS, in the order of the waves.
-template <int DT, int GB, int NT, int MT, int W, bool GATED>
+// Up to eight rows of x: a workgroup of W waves takes 16 NT weight rows (gated: half
+// of them gate, half the same rows of up); its waves share out the blocks of k and
+// add their sums in LDS, in the order of the waves. A wave's next `AHEAD` blocks
+// are under way while one is multiplied: the weights' bytes are the call's time.
+// The MFMA's first operand is the weights here, so that a lane's four results are
+// neighbouring outputs of one row.
+template <int DT, int GB, int NT, int W, bool GATED, int AHEAD>
 __global__ __launch_bounds__(64 * W)
 void linear_w4_kernel(W4Params p) {
   constexpr int S = GB / 32;   // MFMA steps of a block, and a lane's words of it
-  __shared__ v4f part[W][NT * MT][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t width = GATED ? p.n / 2 : p.n;
   constexpr int TILES = GATED ? NT / 2 : NT;   // tiles of outputs
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * TILES), m0 = (int64_t)blockIdx.y * (16 * MT);
+  __shared__ v4f part[W][NT][64];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t width = GATED ? p.n / 2 : p.n;
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * TILES);
   const uint32_t* wrow[NT];
   int64_t nd[NT];      // the lane's first row of the tile's result
 #pragma unroll
@@ -166,66 +145,93 @@ void linear_w4_kernel(W4Params p) {
     wrow[t] = p.codes + (shift + min(base + r, width - 1)) * p.ldw + g * S;
     nd[t] = shift + base + 4 * g;
   }
-  const uint16_t* xrow[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-    xrow[t] = reinterpret_cast<const uint16_t*>(p.x) + min(m0 + 16 * t + r, p.m - 1) * p.ldx + g * (GB / 4);
+  const uint16_t* const xrow =
+      reinterpret_cast<const uint16_t*>(p.x) + min((int64_t)r, p.m - 1) * p.ldx + g * (GB / 4);
   const v4u ones = DT == kF16 ? v4u{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u}
                               : v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
   const Unpack<DT> unpack;
-  v4f tot[NT][MT] = {};
-  const int blocks = (int)(p.k / GB);
-  for (int b = wave; b < blocks; b += W) {
+  const int blocks = (int)(p.k / GB), per_group = p.group / GB;
+  struct Block {
     uint32_t w[NT][S];
-    v4u x[MT][S];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int j = 0; j < S; ++j) w[t][j] = wrow[t][(int64_t)b * (GB / 8) + j];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int j = 0; j < S; ++j)
-        x[t][j] = *reinterpret_cast<const v4u*>(xrow[t] + (int64_t)b * GB + 8 * j);
-    v4f acc[NT][MT] = {}, sum[MT] = {};
-#pragma unroll
-    for (int j = 0; j < S; ++j) {
-#pragma unroll
-      for (int t = 0; t < MT; ++t) sum[t] = mfma<DT>(ones, x[t][j], sum[t]);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const v4u a = unpack(w[t][j]);
-#pragma unroll
-        for (int u = 0; u < MT; ++u) acc[t][u] = mfma<DT>(a, x[u][j], acc[t][u]);
-      }
-    }
-    const int64_t grow = (int64_t)(b * GB / p.group) * p.n;
+    v4u x[S];
+    uint32_t s[NT][2], z[NT];   // four scales, four zeros
+  };
+  // The blocks go to the waves in pairs, neighbours to one wave in turn, so that it
+  // reads whole 128-byte lines of codes (14336 x 4096, one row: 12.9 -> 10.7 us).
+  auto at_of = [](int i) {
+    const int turn = i / W, w = i - turn * W;
+    return (turn >> 1) * (2 * W) + 2 * w + (turn & 1);
+  };
+  auto load = [&](int b, Block& o) {
+    b = min(at_of(b), blocks - 1);   // (past the last one: loaded and left)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      v4f sc, z;
-      scales4<DT>(p, grow, nd[t], sc, z);
+      const uint32_t* at = wrow[t] + (int64_t)b * (GB / 8);
+      if constexpr (S == 4) *reinterpret_cast<v4u*>(&o.w[t][0]) = *reinterpret_cast<const v4u*>(at);
+      else if constexpr (S == 2) *reinterpret_cast<uint2*>(&o.w[t][0]) = *reinterpret_cast<const uint2*>(at);
+      else o.w[t][0] = *at;
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < S; ++j) o.x[j] = *reinterpret_cast<const v4u*>(xrow + (int64_t)b * GB + 8 * j);
+    const int64_t grow = (int64_t)(b / per_group) * p.n;
 #pragma unroll
-        for (int u = 0; u < MT; ++u)
-          tot[t][u][i] = __builtin_fmaf(sc[i], __builtin_fmaf(-z[i], sum[u][i], acc[t][u][i]), tot[t][u][i]);
+    for (int t = 0; t < NT; ++t) {
+      // (Past the last row its values again.)
+      if (p.quads) {
+        const int64_t at = grow + min(nd[t], p.n - 4);
+        *reinterpret_cast<uint2*>(&o.s[t][0]) = *reinterpret_cast<const uint2*>(p.scales + at);
+        o.z[t] = p.zeros ? *reinterpret_cast<const uint32_t*>(p.zeros + at) : 0x08080808u;
+      } else {
+        uint32_t z = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t at = grow + min(nd[t] + i, p.n - 1);
+          o.s[t][i >> 1] = i & 1 ? o.s[t][i >> 1] | ((uint32_t)p.scales[at] << 16) : p.scales[at];
+          z |= (uint32_t)(p.zeros ? p.zeros[at] : 8) << (8 * i);
+        }
+        o.z[t] = z;
+      }
+    }
+  };
+  v4f tot[NT] = {};
+  Block q[AHEAD + 1];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(wave + i * W, q[i]);
+  const int turns = (blocks + 2 * W - 1) / (2 * W) * 2;
+  for (int turn = 0; turn < turns; turn += AHEAD + 1) {
+#pragma unroll
+    for (int i = 0; i <= AHEAD; ++i) {
+      const Block& f = q[i];
+      load(wave + (turn + i + AHEAD) * W, q[(i + AHEAD) % (AHEAD + 1)]);
+      if (turn + i >= turns || at_of(wave + (turn + i) * W) >= blocks) continue;
+      v4f sum = {}, acc[NT] = {};
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        sum = mfma<DT>(ones, f.x[j], sum);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] = mfma<DT>(unpack(f.w[t][j]), f.x[j], acc[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float s = wide<DT>((uint16_t)(f.s[t][e >> 1] >> (16 * (e & 1))));
+          const float z = (float)((f.z[t] >> (8 * e)) & 0xffu) + 16.0f;
+          tot[t][e] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[e], acc[t][e]), tot[t][e]);
+        }
     }
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int u = 0; u < MT; ++u) part[wave][t * MT + u][lane] = tot[t][u];
+  for (int t = 0; t < NT; ++t) part[wave][t][lane] = tot[t];
   __syncthreads();
-  for (int tu = wave; tu < TILES * MT; tu += W) {
-    const int t = tu / MT, u = tu - t * MT;
-    v4f y = part[0][tu][lane], up = {};
-    for (int v = 1; v < W; ++v) y = y + part[v][tu][lane];
+  for (int t = wave; t < TILES; t += W) {
+    v4f y = part[0][t][lane], up = {};
+    for (int v = 1; v < W; ++v) y = y + part[v][t][lane];
     if constexpr (GATED) {
-      up = part[0][TILES * MT + tu][lane];
-      for (int v = 1; v < W; ++v) up = up + part[v][TILES * MT + tu][lane];
+      up = part[0][TILES + t][lane];
+      for (int v = 1; v < W; ++v) up = up + part[v][TILES + t][lane];
     }
-    const int64_t m = m0 + 16 * u + r;
-    if (m < p.m) finish4<DT, GATED>(p, m, n0 + 16 * t + 4 * g, width, y, up);
+    if (r < p.m) finish4<DT, GATED>(p, r, n0 + 16 * t + 4 * g, width, y, up);
   }
 }
 
@@ -283,7 +289,7 @@ __device__ __forceinline__ v16f mfma_zero(uint2 sum, uint2 z) {
   return __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(__builtin_bit_cast(v4s, sum), __builtin_bit_cast(v4s, z), v16f{}, 0, 0, 0);
 }
 
-// More than 16 rows: a workgroup of W waves takes 32 U rows of x and 32 W weight
+// More than eight rows: a workgroup of W waves takes 32 U rows of x and 32 W weight
 // rows (gated: 16 W of gate and the same of up); each wave takes all of x's rows
 // and 32 of the weight's (gated: 16 of each), so that every code is unpacked once
 // a workgroup, and the waves of a SIMD do each other's unpacking and scaling in
@@ -465,7 +471,7 @@ void linear_w4_join_kernel(W4Params p, const float* parts, int splits, bool gate
   p.out[m * p.ldo + n] = slim<DT>(v);
 }
 
-// How a call of more than 16 rows is cut: 32 u rows and 32 w weight rows a tile,
+// How a call of more than eight rows is cut: 32 u rows and 32 w weight rows a tile,
 // and the ranges of k. The ranges keep at least four steps, and their sums at
 // most 64 MB.
 struct W4Plan {
@@ -489,7 +495,7 @@ static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int cus) {
 }
 
 // Whether a call takes the tiles (offsets inside a tile are 32 bits there).
-static bool w4_tiled(int64_t m) { return m > 16; }
+static bool w4_tiled(int64_t m) { return m > 8; }
 
 // Bytes of the sums of x (bf16 with many rows; asked of fp16 alike) and, behind
 // them, of the ranges' sums.
@@ -527,10 +533,17 @@ static int launch_w4_tiles(const W4Params& p, void* workspace, hipStream_t strea
 template <int DT, int GB, bool GATED>
 static int launch_w4(const W4Params& p, void* workspace, hipStream_t stream) {
   if (w4_tiled(p.m)) return launch_w4_tiles<DT, GB, GATED>(p, workspace, stream);
-  constexpr int NT = 2, W = 8;
-  const int64_t width = GATED ? p.n / 2 : p.n, per = GATED ? 16 * NT / 2 : 16 * NT;
-  hipLaunchKernelGGL((linear_w4_kernel<DT, GB, NT, 1, W, GATED>), dim3((unsigned)((width + per - 1) / per)),
-                     dim3(64 * W), 0, stream, p);
+  // Two tiles of weight rows share a wave's x, and four waves of ten or so blocks
+  // each cost less to set up than eight of five; but where that leaves CUs idle on
+  // long sums, one tile and eight waves (us, two tiles / one; one row of x: 14336 x
+  // 4096 10.7 / 13.9, 5120 x 5120 7.9 / 9.9, 4096 x 14336 18.4 / 11.4).
+  const int64_t width = GATED ? p.n / 2 : p.n, pairs = (width + (GATED ? 15 : 31)) / (GATED ? 16 : 32);
+  if (!GATED && pairs < current_device_cus() && p.k > 64 * 128) {
+    hipLaunchKernelGGL((linear_w4_kernel<DT, GB, 1, 8, false, 1>), dim3((unsigned)((width + 15) / 16)), dim3(512), 0,
+                       stream, p);
+  } else {
+    hipLaunchKernelGGL((linear_w4_kernel<DT, GB, 2, 4, GATED, 1>), dim3((unsigned)pairs), dim3(256), 0, stream, p);
+  }
   return launch_status("w8a8_linear_w4");
 }
 
