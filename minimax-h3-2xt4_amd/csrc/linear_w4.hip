@@ -25,6 +25,7 @@ namespace w8a8 {
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 struct W4Params {
@@ -250,7 +251,8 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // The sums of x over blocks of GB inputs, as three bf16 that add up to the fp32
-// sum: sums[block][m] = (hi, mid, lo, 0). One 16-byte run of x per thread.
+// sum: sums[block][m] = (hi, mid, lo, 0), rows padded to a multiple of 128. One
+// 16-byte run of x per thread.
 template <int DT, int GB>
 __global__ __launch_bounds__(256)
 void w4_sums_kernel(W4Params p, uint2* sums) {
@@ -269,7 +271,7 @@ void w4_sums_kernel(W4Params p, uint2* sums) {
   const float s1 = s - bf2f(hi);
   const uint16_t mid = f2bf(s1);
   const uint16_t lo = f2bf(s1 - bf2f(mid));
-  sums[(int64_t)(run / (GB / 8)) * p.m + m] = make_uint2(hi | ((uint32_t)mid << 16), lo);
+  sums[(int64_t)(run / (GB / 8)) * ((p.m + 127) & ~(int64_t)127) + m] = make_uint2(hi | ((uint32_t)mid << 16), lo);
 }
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -287,6 +289,61 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
 __device__ __forceinline__ v16f mfma_zero(uint2 sum, uint2 z) {
   typedef short v4s __attribute__((ext_vector_type(4)));
   return __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(__builtin_bit_cast(v4s, sum), __builtin_bit_cast(v4s, z), v16f{}, 0, 0, 0);
+}
+
+// A uniform base for dma(), and SIZE bytes a lane from `off` bytes behind it to LDS:
+// lane i's at l + 16 i, or a word each at l + 4 i (shorter values zero-extended).
+// (The global form counts as an LDS access with the compiler, which then waits for
+// every LDS read in flight before the first one's use.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t dma_base(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, -1, 0x00027000);
+}
+template <int SIZE>
+__device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t base, uint32_t off, char* l) {
+  auto* to = (__attribute__((address_space(3))) void*)l;
+  if constexpr (SIZE == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(base, to, 16, (int)off, 0, 0, 0);
+  else if constexpr (SIZE == 4) __builtin_amdgcn_raw_ptr_buffer_load_lds(base, to, 4, (int)off, 0, 0, 0);
+  else if constexpr (SIZE == 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(base, to, 2, (int)off, 0, 0, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(base, to, 1, (int)off, 0, 0, 0);
+}
+
+// A tile's outputs, or its sums over a range of k.
+template <int DT, int U, bool GATED>
+__device__ __forceinline__ void store_tile(const W4Params& p, const v16f (&tot)[U], float* parts, int split, int splits,
+                                           int64_t m0, int64_t n0, int mrows, int nrows, int64_t wr, int ncol, int c,
+                                           int h) {
+  const int64_t n = n0 + ncol;
+  if (splits > 1) {
+    float* part = parts + (int64_t)split * p.m * p.n + wr;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (m < mrows && ncol < nrows) part[(m0 + m) * p.n] = tot[u][i];
+      }
+    return;
+  }
+  const float bias = p.bias ? wide<DT>(p.bias[wr]) : 0.0f;
+  const int64_t nc = n0 + min(ncol, nrows - 1);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    // (Sixteen loads at once, of the last row and column where the tile ends.)
+    uint16_t r[16];
+    if (p.residual) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        r[i] = p.residual[(m0 + min(32 * u + 8 * (i >> 2) + 4 * h + (i & 3), mrows - 1)) * p.ldr + nc];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+      float v = tot[u][i] + bias;
+      if constexpr (GATED) v = swiglu(v, __shfl_xor(v, 16, 64));
+      if (p.residual) v = v + wide<DT>(r[i]);
+      if (m < mrows && ncol < nrows && (!GATED || c < 16)) p.out[(m0 + m) * p.ldo + n] = slim<DT>(v);
+    }
+  }
 }
 
 // More than eight rows: a workgroup of W waves takes 32 U rows of x and 32 W weight
@@ -308,10 +365,10 @@ __device__ __forceinline__ v16f mfma_zero(uint2 sum, uint2 z) {
 // Where the tiles are too few for the GPU, the steps of k are split over `splits`
 // workgroups, whose sums linear_w4_join_kernel adds in order.
 template <int DT, int GB, int U, int W, bool GATED>
-__global__ __launch_bounds__(64 * W, U == 4 ? 2 : DT == kBF16 && U == 2 ? 3 : 4)
-void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mtiles, int tiles, int splits) {
+__global__ __launch_bounds__(64 * W, DT == kBF16 && U == 2 ? 3 : 4)
+void linear_w4_tiles_kernel(W4Params p, float* parts, int mtiles, int tiles, int splits) {
   constexpr int S = GB / 16, NB = 128 / GB, BN = GATED ? 16 * W : 32 * W, ROWS = 32 * U, DMAS = 8 * U / W;
-  constexpr bool SUMS = DT == kBF16 && U == 4, ONES = DT == kBF16 && U < 4;
+  constexpr bool ONES = DT == kBF16;
   __shared__ __attribute__((aligned(16))) char xs[2][ROWS * 256];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -326,7 +383,7 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
   const int ncol = GATED ? 16 * wave + (c & 15) : 32 * wave + c;   // the lane's column of the tile
   const int64_t wr = (GATED && c >= 16 ? width : 0) + n0 + min(ncol, nrows - 1);
   const char* const wrow = reinterpret_cast<const char*>(p.codes + wr * p.ldw);
-  const char* xbase = reinterpret_cast<const char*>(reinterpret_cast<const uint16_t*>(p.x) + m0 * p.ldx);
+  const auto xbase = dma_base(reinterpret_cast<const uint16_t*>(p.x) + m0 * p.ldx);
   uint32_t xoff[DMAS];
 #pragma unroll
   for (int i = 0; i < DMAS; ++i)
@@ -338,15 +395,12 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
   uint32_t w[NB][S];
   uint16_t sc[NB];
   uint8_t zr[NB];
-  uint2 sm[NB][SUMS ? U : 1];
   auto load = [&](int step) {
     // Past the end of k (the last step only) the last runs and codes again: their blocks are left out.
 #pragma unroll
     for (int i = 0; i < DMAS; ++i) {
       const int row = 4 * (DMAS * wave + i), run = (lane & 15) ^ ((row + (lane >> 4)) & 15);
-      const char* src = xbase + (xoff[i] + (uint32_t)min(step * 256 + run * 16, (int)p.k * 2 - 16));
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                       (__attribute__((address_space(3))) void*)(xs[step & 1] + row * 256), 16, 0, 0);
+      dma<16>(xbase, xoff[i] + (uint32_t)min(step * 256 + run * 16, (int)p.k * 2 - 16), xs[step & 1] + row * 256);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -361,11 +415,6 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
       }
       sc[b] = p.scales[grow];
       zr[b] = p.zeros ? p.zeros[grow] : (uint8_t)8;
-      if constexpr (SUMS) {
-        const uint2* row = sums + (int64_t)block * p.m + m0;
-#pragma unroll
-        for (int u = 0; u < U; ++u) sm[b][u] = row[min(32 * u + c, mrows - 1)];
-      }
     }
   };
 
@@ -378,7 +427,6 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
     uint32_t cw[NB][S];
     float cs[NB], fz[NB];
     uint32_t cz[NB];
-    uint2 cm[NB][SUMS ? U : 1];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -387,10 +435,6 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
       fz[b] = -16.0f - (float)zr[b];
       cz[b] = DT == kF16 ? (uint32_t)f2h(-fz[b]) * 0x10001u
                          : h ? 0 : (__float_as_uint(fz[b]) >> 16) * 0x10001u;   // (exact: a small integer)
-      if constexpr (SUMS) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) cm[b][u] = sm[b][u];
-      }
     }
     if (step + 1 < last) load(step + 1);
 #pragma unroll
@@ -405,7 +449,6 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         v16f acc = {}, sum = {};
-        if constexpr (SUMS) acc = mfma_zero(cm[b][u], make_uint2(cz[b], cz[b]));
 #pragma unroll
         for (int j = 0; j < S; ++j) {
           const v4u x = *reinterpret_cast<const v4u*>(xs[step & 1] + (32 * u + c) * 256 +
@@ -425,30 +468,245 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
       for (int u = 0; u < U; ++u) __asm__ volatile("" : "+v"(tot[u]));
     }
   }
-  const int64_t n = n0 + ncol;
-  if (splits > 1) {
-    float* part = parts + (int64_t)split * p.m * p.n + wr;
+  store_tile<DT, U, GATED>(p, tot, parts, split, splits, m0, n0, mrows, nrows, wr, ncol, c, h);
+}
+
+// More than 64 rows: the same tiles with 128 rows of x and 256 weight rows, and
+// everything by DMA: x, codes, scales and zeros (sub-word loads, a word each in LDS)
+// into a ring of stages of one step each, RING - 1 steps ahead, so that a counted
+// wait leaves the later steps' loads in flight (a load into registers behind a DMA
+// waits for all of them). The sums of x come one step ahead. A step's work is laid
+// out product by product (below), since the compiler's own order reads each operand
+// right before its use and scales and unpacks between the chains of MFMAs. 2048 x
+// 14336 x 4096: bf16 in groups of 64 381 -> 294 us (817 TFLOP/s), fp16 in groups of
+// 128 294 -> 258. What bounds it: every wave reads all of x's tile, 256 KB of LDS a
+// step, as long as its MFMAs take, and the two waves of a SIMD do not fill the rest.
+template <int DT, int GB>
+struct W4Stage {
+  static constexpr int NB = 128 / GB, PAIRS = (NB + 1) / 2;
+  static constexpr int kRing = GB == 32 ? 2 : 3;                 // (what 160 KB hold)
+  static constexpr int kX = 128 * 256, kCodes = 8 * 2048, kMeta = 8 * 512 * PAIRS, kBytes = kX + kCodes + kMeta;
+  static constexpr int kDma = 4 + 2 + 2 * PAIRS;                 // instructions of a wave
+  static constexpr int kSums = DT == kBF16 ? NB * 1024 : 0;
+  static constexpr int kLds = kRing * kBytes + 2 * kSums;
+};
+
+template <int N>
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0f70); }
+
+// Workgroup barrier without a fence, which would wait for the DMA in flight: the
+// caller waits for what it needs, and every LDS read before it has been used.
+__device__ __forceinline__ void block_barrier() {
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __asm__ volatile("" ::: "memory");
+}
+
+template <int DT, int GB, bool GATED>
+__global__ __launch_bounds__(512, 2)
+void linear_w4_ring_kernel(W4Params p, const uint2* sums, float* parts, int mtiles, int tiles, int splits) {
+  using Stage = W4Stage<DT, GB>;
+  constexpr int S = GB / 16, NB = Stage::NB, BN = GATED ? 128 : 256, RING = Stage::kRing;
+  constexpr int DEEP = 4;   // (6 and 8 the same within 1 %)
+  __shared__ __attribute__((aligned(16))) char lds[Stage::kLds];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t width = GATED ? p.n / 2 : p.n;
+  const int items = tiles * splits, per = (items + 7) / 8, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (item >= items || (int)(blockIdx.x >> 3) >= per) return;
+  const int tile = item / splits, split = item - tile * splits;
+  const int64_t m0 = (int64_t)(tile % mtiles) * 128, n0 = (int64_t)(tile / mtiles) * BN;
+  const int mrows = (int)min((int64_t)128, p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
+  // The tile's column of the wave's column col (0..31: gated, 16 of gate and the same of up).
+  auto column = [&](int col) { return GATED ? 16 * wave + (col & 15) : 32 * wave + col; };
+  const int ncol = column(c), nclamped = min(ncol, nrows - 1);
+  const int64_t wr = (GATED && c >= 16 ? width : 0) + n0 + nclamped;
+  const auto xbase = dma_base(reinterpret_cast<const uint16_t*>(p.x) + m0 * p.ldx);
+  uint32_t xoff[4];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+  for (int i = 0; i < 4; ++i) xoff[i] = (uint32_t)min(4 * (4 * wave + i) + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
+  // A wave brings its own codes: instruction i rows 16 i .. 16 i + 15, four 16-byte
+  // runs a row, run q at q ^ (row >> 2 & 3).
+  __amdgpu_buffer_rsrc_t cbase[2];
+  uint32_t coff[2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-        if (m < mrows && ncol < nrows) part[(m0 + m) * p.n] = tot[u][i];
-      }
-    return;
+  for (int i = 0; i < 2; ++i) {
+    cbase[i] = dma_base(p.codes + ((GATED && i ? width : 0) + n0) * p.ldw);
+    coff[i] = (uint32_t)min(column(16 * i + (lane >> 2)), nrows - 1) * (uint32_t)(p.ldw * 4);
   }
-  const float bias = p.bias ? wide<DT>(p.bias[wr]) : 0.0f;
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-      float v = tot[u][i] + bias;
-      if constexpr (GATED) v = swiglu(v, __shfl_xor(v, 16, 64));
-      if (m >= mrows || ncol >= nrows || (GATED && c >= 16)) continue;
-      if (p.residual) v = v + wide<DT>(p.residual[(m0 + m) * p.ldr + n]);
-      p.out[(m0 + m) * p.ldo + n] = slim<DT>(v);
+  const int crun = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
+  const uint32_t roff = (uint32_t)wr;
+  // (Without zeros a byte of the scales is read and left.)
+  const uint8_t* const zrow = p.zeros ? p.zeros : reinterpret_cast<const uint8_t*>(p.scales);
+  const int all = (int)((p.k + 127) / 128), blocks = (int)(p.k / GB), kbytes = (int)(p.k / 2);
+  const int first = (int)((int64_t)all * split / splits), last = (int)((int64_t)all * (split + 1) / splits);
+  const int per_group = p.group / GB;
+  const int64_t mpad = (p.m + 127) & ~(int64_t)127;
+
+  // Piece i of a step's loads. A step past the last is the last again; past the end
+  // of k the last runs and codes again, whose blocks' scales are taken as zero.
+  auto load = [&](int step, char* to, int i) {
+    step = min(step, last - 1);
+    if (i < 4) {
+      const int row = 4 * (4 * wave + i), run = (lane & 15) ^ ((row + (lane >> 4)) & 15);
+      dma<16>(xbase, xoff[i] + (uint32_t)min(step * 256 + run * 16, (int)p.k * 2 - 16), to + row * 256);
+    } else if (i < 6) {
+      dma<16>(cbase[i - 4], coff[i - 4] + (uint32_t)min(step * 64 + crun, kbytes - 16), to + Stage::kX + 2048 * wave + 1024 * (i - 4));
+    } else {
+      const int j = (i - 6) / 2;
+      // (Two neighbouring blocks of less than 128 inputs, half the lanes each.)
+      const int one = min(step * NB + 2 * j, blocks - 1), two = min(step * NB + 2 * j + 1, blocks - 1);
+      const int64_t group = NB > 1 ? one : one / per_group;   // (blocks are groups below 128 inputs)
+      const uint32_t at = roff + (NB > 1 && h && two != one ? (uint32_t)p.n : 0);
+      char* const meta = to + Stage::kX + Stage::kCodes + 512 * (Stage::PAIRS * wave + j);
+      if (i & 1) dma<1>(dma_base(zrow + group * p.n), at, meta + 256);
+      else dma<2>(dma_base(p.scales + group * p.n), 2 * at, meta);
     }
+  };
+  auto load_sums = [&](int step, char* to) {
+    // (4 bytes a lane; the waves that are left load the same again. Rows past the
+    // last are never stored.)
+    if constexpr (DT == kBF16) {
+#pragma unroll
+      for (int i = 0; i < (NB + 1) / 2; ++i) {
+        const int part = (8 * i + wave) & (4 * NB - 1);
+        const int64_t block = min(min(step, last - 1) * NB + part / 4, blocks - 1);
+        dma<4>(dma_base(sums + block * mpad + m0), 256 * (part & 3) + 4 * lane, to + 256 * part);
+      }
+    }
+  };
+
+  const uint32_t zero_mask = p.zeros ? 0xffu : 0u, zero_else = p.zeros ? 0u : 8u, half_mask = h ? 0u : ~0u;
+  const Unpack<DT> unpack;
+  // A block's codes, scale and zero as they lie in LDS, and its weights, scale and
+  // zero (fp16: to take off the weights; bf16: its column) ready for the MFMAs.
+  struct Raw {
+    uint32_t w[S], scale, zero;
+  };
+  struct Ready {
+    v4u w[S];
+    float scale;
+    uint32_t zero;
+  };
+  auto fetch = [&](const char* at, int b, Raw& o) {
+    const char* const cw = at + Stage::kX + 2048 * wave + 64 * c;
+    if constexpr (S == 8) {
+      *reinterpret_cast<v4u*>(&o.w[0]) = *reinterpret_cast<const v4u*>(cw + 16 * ((2 * h) ^ ((c >> 2) & 3)));
+      *reinterpret_cast<v4u*>(&o.w[4]) = *reinterpret_cast<const v4u*>(cw + 16 * ((2 * h + 1) ^ ((c >> 2) & 3)));
+    } else if constexpr (S == 4) {
+      *reinterpret_cast<v4u*>(&o.w[0]) = *reinterpret_cast<const v4u*>(cw + 16 * ((2 * b + h) ^ ((c >> 2) & 3)));
+    } else {
+      *reinterpret_cast<v2u*>(&o.w[0]) = *reinterpret_cast<const v2u*>(cw + 16 * (b ^ ((c >> 2) & 3)) + 8 * h);
+    }
+    const char* const meta = at + Stage::kX + Stage::kCodes + 512 * (Stage::PAIRS * wave + b / 2) + 4 * (32 * (b & 1) + c);
+    o.scale = *reinterpret_cast<const uint32_t*>(meta);
+    o.zero = *reinterpret_cast<const uint32_t*>(meta + 256);
+  };
+  auto open = [&](int step, int b, const Raw& r, Ready& o) {
+    // (Selects by arithmetic: behind a branch the compiler waits for every load.)
+    o.scale = wide<DT>((uint16_t)r.scale) * (NB == 1 || step * NB + b < blocks ? 1.0f : 0.0f);
+    const float z = 16.0f + (float)((r.zero & zero_mask) | zero_else);
+    o.zero = DT == kF16 ? (uint32_t)f2h(z) * 0x10001u
+                        : ((__float_as_uint(-z) >> 16) * 0x10001u) & half_mask;   // (exact: a small integer)
+  };
+  auto weights = [&](const Raw& r, int j, Ready& o) {
+    o.w[j] = unpack(r.w[j]);
+    if constexpr (DT == kF16) o.w[j] = less(o.w[j], o.zero);
+  };
+
+  v16f tot[4] = {}, acc[2] = {};
+  float carry = 0.0f;             // the scale of the last chain, whose sums are in acc[1]
+  int at = 0, to = (RING - 1) * Stage::kBytes, sums_of = RING * Stage::kBytes, sums_to = sums_of + Stage::kSums;
+  auto next_stage = [&](int q) { return q == (RING - 1) * Stage::kBytes ? 0 : q + Stage::kBytes; };
+  // A step: 32 products of 32 x 32 x 16, in chains of a block's S for 32 rows of x.
+  // Each is followed, in the shadow of its MFMA, by the read of x for the product
+  // DEEP on, a piece of the loads for the step RING - 1 on, a share of the last
+  // chain's scaling, and in the second half of a block a share of unpacking the next.
+  auto run = [&](int step, Ready& fa, Ready& fb) {
+    block_barrier();
+    load_sums(step + 1, lds + sums_to);
+    const char* const xs = lds + at;
+    const int after = next_stage(at);
+    auto read = [&](int i) {
+      const int b = i / (4 * S), u = i / S % 4, j = i % S;
+      return *reinterpret_cast<const v4u*>(xs + (32 * u + c) * 256 + 16 * ((b * (GB / 8) + h * S + j) ^ (c & 15)));
+    };
+    auto read_sum = [&](int b, int u) {
+      // (Not as a uint2: the compiler would wait for every DMA in flight before it.)
+      const v2u q = *reinterpret_cast<const v2u*>(lds + sums_of + 1024 * b + 256 * u + 8 * c);
+      return make_uint2(q[0], q[1]);
+    };
+    v4u x[DEEP];
+    uint2 sum[2];
+    Raw raw;
+    if constexpr (DT == kBF16) sum[0] = read_sum(0, 0);
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) x[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int b = i / (4 * S), u = i / S % 4, j = i % S;
+      Ready& f = b & 1 ? fb : fa;
+      Ready& g = b & 1 ? fa : fb;
+      if (j == 0) {
+        if constexpr (DT == kBF16) acc[u & 1] = mfma_zero(sum[u & 1], make_uint2(f.zero, f.zero));
+        else acc[u & 1] = v16f{};
+      }
+      acc[u & 1] = mfma32<DT>(x[i % DEEP], f.w[j], acc[u & 1]);
+      if (i + DEEP < 32) x[i % DEEP] = read(i + DEEP);
+      if (DT == kBF16 && j == 0 && i + S < 32) sum[(u + 1) & 1] = read_sum((i + S) / (4 * S), (u + 1) % 4);
+      if (i < Stage::kDma) load(step + RING - 1, lds + to, i);
+      if (j > 0) {
+        const float scale = u ? f.scale : carry;
+#pragma unroll
+        for (int e = 16 * (j - 1) / (S - 1); e < 16 * j / (S - 1); ++e)
+          tot[(u + 3) & 3][e] = __builtin_fmaf(scale, acc[(u + 1) & 1][e], tot[(u + 3) & 3][e]);
+      }
+      const bool ends = b + 1 == NB;
+      if (u == 1 && j == 0) {
+        // (A wave's codes are its own DMA. Every load of the step RING - 1 on has been issued.)
+        if (ends) wait_loads<(RING - 2) * Stage::kDma>();
+        fetch(lds + (ends ? after : at), ends ? 0 : b + 1, raw);
+      }
+      if (u == 2 && j == 0) open(step + ends, ends ? 0 : b + 1, raw, g);
+      if (u >= 2 && (j & 1) == 0) weights(raw, (u - 2) * (S / 2) + j / 2, g);
+      if (u == 3 && j == S - 1) carry = f.scale;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    at = after;
+    to = next_stage(to);
+    const int q = sums_of;
+    sums_of = sums_to;
+    sums_to = q;
+  };
+  load_sums(first, lds + sums_of);
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i)
+#pragma unroll
+    for (int j = 0; j < Stage::kDma; ++j) load(first + i, lds + i * Stage::kBytes, j);
+  wait_loads<(RING - 2) * Stage::kDma>();
+  Ready f0, f1;
+  {
+    Raw raw;
+    fetch(lds, 0, raw);
+    open(first, 0, raw, f0);
+#pragma unroll
+    for (int j = 0; j < S; ++j) weights(raw, j, f0);
+  }
+  if constexpr (NB == 1) {
+    int step = first;
+    for (; step + 1 < last; step += 2) {
+      run(step, f0, f1);
+      run(step + 1, f1, f0);
+    }
+    if (step < last) run(step, f0, f1);
+  } else {
+    for (int step = first; step < last; ++step) run(step, f0, f1);
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) tot[3][e] = __builtin_fmaf(carry, acc[1][e], tot[3][e]);
+  wait_loads<0>();     // no DMA outlives the workgroup's LDS
+  store_tile<DT, 4, GATED>(p, tot, parts, split, splits, m0, n0, mrows, nrows, wr, ncol, c, h);
 }
 
 // The outputs of a split call: the ranges' sums in order, then the epilogue. One
@@ -500,7 +758,7 @@ static bool w4_tiled(int64_t m) { return m > 8; }
 // Bytes of the sums of x (bf16 with many rows; asked of fp16 alike) and, behind
 // them, of the ranges' sums.
 static int64_t w4_sums_bytes(const W4Plan& q, int64_t m, int64_t k, int group) {
-  return q.u == 4 ? (8 * m * (k / (group < 128 ? group : 128)) + 255) / 256 * 256 : 0;
+  return q.u == 4 ? 8 * ((m + 127) / 128 * 128) * (k / (group < 128 ? group : 128)) : 0;
 }
 
 template <int DT, int GB, int U, int W, bool GATED>
@@ -511,8 +769,13 @@ static void launch_w4_plan(const W4Params& p, const W4Plan& q, void* workspace, 
     hipLaunchKernelGGL((w4_sums_kernel<DT, GB>), dim3((unsigned)((p.m * (p.k / 8) + 255) / 256)), dim3(256), 0, stream,
                        p, sums);
   const int64_t items = q.tiles * q.splits;
-  hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, U, W, GATED>), dim3((unsigned)((items + 7) / 8 * 8)),
-                     dim3(64 * W), 0, stream, p, sums, parts, q.mtiles, (int)q.tiles, q.splits);
+  const dim3 grid((unsigned)((items + 7) / 8 * 8));
+  if constexpr (U == 4)
+    hipLaunchKernelGGL((linear_w4_ring_kernel<DT, GB, GATED>), grid, dim3(512), 0, stream, p, sums, parts, q.mtiles,
+                       (int)q.tiles, q.splits);
+  else
+    hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, U, W, GATED>), grid, dim3(64 * W), 0, stream, p, parts, q.mtiles,
+                       (int)q.tiles, q.splits);
   if (q.splits > 1)
     hipLaunchKernelGGL((linear_w4_join_kernel<DT>), dim3((unsigned)(((GATED ? p.n / 2 : p.n) + 255) / 256), (unsigned)p.m),
                        dim3(256), 0, stream, p, parts, q.splits, GATED);
@@ -521,7 +784,8 @@ static void launch_w4_plan(const W4Params& p, const W4Plan& q, void* workspace, 
 template <int DT, int GB, bool GATED>
 static int launch_w4_tiles(const W4Params& p, void* workspace, hipStream_t stream) {
   const W4Plan q = w4_plan(p.m, p.n, p.k, current_device_cus());
-  W8A8_REQUIRE(q.tiles < ((int64_t)1 << 22) && p.ldx < (1 << 22), "w8a8_linear_w4: too many outputs for one launch");
+  W8A8_REQUIRE(q.tiles < ((int64_t)1 << 22) && p.n < (1 << 30) && p.ldx < (1 << 22) && p.ldw < (1 << 22),
+               "w8a8_linear_w4: too many outputs, or rows too long, for more than eight rows of x");
   switch (q.u) {
     case 4: launch_w4_plan<DT, GB, 4, 8, GATED>(p, q, workspace, stream); break;
     case 2: launch_w4_plan<DT, GB, 2, 4, GATED>(p, q, workspace, stream); break;
