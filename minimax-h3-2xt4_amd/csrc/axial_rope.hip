@@ -5,15 +5,15 @@
 // The angle is needed modulo a revolution, so it is taken in fp64 (position
 // 10^6 times one radian is 1.6 * 10^5 revolutions: fp64 leaves 10^-10 of one,
 // fp32 would leave a hundredth) and its fraction's sine and cosine in fp32.
-// Each angle serves all heads of its row: a workgroup puts its rows' angles
-// into LDS once and turns its share of their heads from there.
+// Each angle serves all heads of its row: a workgroup takes a row, puts its
+// angles into LDS and turns all its heads from there.
 //
 // A head is split into chunks of 2 V channels: V pairs (V channels of each
 // side, or V adjacent pairs), or 2 V channels that are not turned. A lane
 // takes one chunk (C of them where V is 1), so a turn needs no other lane, and
 // a head's 2^n lanes meet in a butterfly for the norm's sum.
 //
-// Bound by memory: q and k are read and written once.
+// Bound by memory where rows are many: q and k are read and written once.
 #include "w8a8_device.h"
 #include "w8a8_host.h"
 
@@ -22,7 +22,7 @@
 namespace w8a8 {
 
 constexpr int kAxThreads = 256;
-constexpr int kAxAngles = 512;   // (row, pair) angles a workgroup holds
+constexpr int kAxPairs = 128;   // the most that a row has
 
 struct AxTable {
   const void* positions;
@@ -38,9 +38,8 @@ struct AxRopeParams {
   int64_t in_row[2], in_head[2], out_row[2], out_head[2];
   const float* gain[2];
   int heads[2];
-  int64_t rows;
   AxTable table;
-  int dim, lanes, rows_per_block, splits;
+  int dim, lanes;
   float eps, inv_dim;
 };
 
@@ -102,25 +101,20 @@ template <int DT, bool ADJ, int V, int C>
 __global__ __launch_bounds__(kAxThreads)
 void axial_rope_kernel(AxRopeParams p) {
   using T = std::conditional_t<DT == kF32, uint32_t, uint16_t>;
-  __shared__ float2 angle[kAxAngles];
+  __shared__ float2 angle[kAxPairs];
   const int pairs = p.table.pairs;
-  const int64_t block = blockIdx.x / p.splits;
-  const int split = (int)(blockIdx.x - block * p.splits);
-  const int64_t row0 = block * p.rows_per_block;
-  const int rows = (int)min((int64_t)p.rows_per_block, p.rows - row0);
-  for (int i = threadIdx.x; i < rows * pairs; i += kAxThreads)
-    angle[i] = rotation_of(p.table, row0 + i / pairs, i % pairs);
+  const int64_t row = blockIdx.x;
+  for (int i = threadIdx.x; i < pairs; i += kAxThreads) angle[i] = rotation_of(p.table, row, i);
   __syncthreads();
 
   const int lanes = p.lanes, lane = threadIdx.x & (lanes - 1);
   const int per_pass = kAxThreads / lanes, heads = p.heads[0] + p.heads[1];
   const int turned = pairs / V, chunks = p.dim / (2 * V);
-  // Items (row, head) of the block; all lanes of a head run the same passes.
-  for (int it = split * per_pass + threadIdx.x / lanes; it < rows * heads; it += p.splits * per_pass) {
-    const int r = it / heads, head = it - r * heads;
+  // (All lanes of a head run the same passes.)
+  for (int head = threadIdx.x / lanes; head < heads; head += per_pass) {
     const int w = head >= p.heads[0] ? 1 : 0, h = head - (w ? p.heads[0] : 0);
-    const T* src = reinterpret_cast<const T*>(p.x[w]) + (row0 + r) * p.in_row[w] + h * p.in_head[w];
-    T* dst = reinterpret_cast<T*>(p.out[w]) + (row0 + r) * p.out_row[w] + h * p.out_head[w];
+    const T* src = reinterpret_cast<const T*>(p.x[w]) + row * p.in_row[w] + h * p.in_head[w];
+    T* dst = reinterpret_cast<T*>(p.out[w]) + row * p.out_row[w] + h * p.out_head[w];
     float a[C][V], b[C][V];
     int at[C], bt[C];
     float ss = 0.0f;
@@ -165,7 +159,7 @@ void axial_rope_kernel(AxRopeParams p) {
       if (ch >= chunks) continue;
       Run<T, V> ra, rb;
       if (ch < turned) {
-        const float2* rot = angle + r * pairs + ch * V;
+        const float2* rot = angle + ch * V;
         if constexpr (ADJ) {
           // The 2 V channels a[0..V), b[0..V) hold pairs (2 i, 2 i + 1).
           float v[2 * V];
@@ -321,7 +315,6 @@ extern "C" int w8a8_axial_rope(const W8A8AxialRopeArgs* a) {
   W8A8_REQUIRE(!heads[1] || apart(vout[0], vout[1]), "w8a8_axial_rope: q_out and k_out overlap");
   p.gain[0] = a->q_gain;
   p.gain[1] = a->k_gain;
-  p.rows = a->rows;
   p.table = AxTable{a->positions, a->pos_strides[0], a->pos_strides[1], a->pos_type, a->pairs, a->axes, a->inv_freq, a->axis};
   p.dim = a->dim;
   p.eps = a->eps;
@@ -329,13 +322,10 @@ extern "C" int w8a8_axial_rope(const W8A8AxialRopeArgs* a) {
   const int chunks = a->dim / (2 * v), lane_chunks = v == 1 ? 2 : 1;
   p.lanes = 1;
   while (p.lanes * lane_chunks < chunks) p.lanes *= 2;
-  p.rows_per_block = 1;
-  p.splits = 1;
-  const int64_t blocks = (a->rows + p.rows_per_block - 1) / p.rows_per_block * p.splits;
-  W8A8_REQUIRE(blocks * kAxThreads < ((int64_t)1 << 32), "w8a8_axial_rope: too many rows for one launch");
+  W8A8_REQUIRE(a->rows * kAxThreads < ((int64_t)1 << 32), "w8a8_axial_rope: too many rows for one launch");
   hipStream_t s = reinterpret_cast<hipStream_t>(a->stream);
   const bool adj = a->pairing == W8A8_ROPE_ADJACENT;
-  const unsigned grid = (unsigned)blocks;
+  const unsigned grid = (unsigned)a->rows;
   switch (a->dtype) {
     case W8A8_F16: return adj ? launch_axial<kF16, true>(p, v, grid, s) : launch_axial<kF16, false>(p, v, grid, s);
     case W8A8_BF16: return adj ? launch_axial<kBF16, true>(p, v, grid, s) : launch_axial<kBF16, false>(p, v, grid, s);

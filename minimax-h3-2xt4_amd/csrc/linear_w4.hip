@@ -18,6 +18,7 @@
 #include "w8a8_device.h"
 #include "w8a8_host.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace w8a8 {
@@ -251,27 +252,28 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // The sums of x over blocks of GB inputs, as three bf16 that add up to the fp32
-// sum: sums[block][m] = (hi, mid, lo, 0), rows padded to a multiple of 128. One
-// 16-byte run of x per thread.
+// sum: sums[block][m] = (hi, mid, lo, 0), rows padded to a multiple of 128. A
+// thread takes a 16-byte run of x, and another a grid on.
+constexpr int64_t kSumsBlocks = 1 << 20;
 template <int DT, int GB>
 __global__ __launch_bounds__(256)
 void w4_sums_kernel(W4Params p, uint2* sums) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int runs = (int)(p.k / 8);
-  const int64_t m = i / runs;
-  const int run = (int)(i - m * runs);
-  if (m >= p.m) return;   // (whole groups of lanes: a row is whole blocks)
-  const v4u x = *reinterpret_cast<const v4u*>(reinterpret_cast<const uint16_t*>(p.x) + m * p.ldx + 8 * run);
-  float s = 0.0f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.m * runs; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / runs;   // (whole groups of lanes: a row is whole blocks)
+    const int run = (int)(i - m * runs);
+    const v4u x = *reinterpret_cast<const v4u*>(reinterpret_cast<const uint16_t*>(p.x) + m * p.ldx + 8 * run);
+    float s = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) s = s + (wide<DT>((uint16_t)x[j]) + wide<DT>((uint16_t)(x[j] >> 16)));
-  s = lanes_sum<GB / 8>(s);
-  if (run % (GB / 8)) return;
-  const uint16_t hi = f2bf(s);
-  const float s1 = s - bf2f(hi);
-  const uint16_t mid = f2bf(s1);
-  const uint16_t lo = f2bf(s1 - bf2f(mid));
-  sums[(int64_t)(run / (GB / 8)) * ((p.m + 127) & ~(int64_t)127) + m] = make_uint2(hi | ((uint32_t)mid << 16), lo);
+    for (int j = 0; j < 4; ++j) s = s + (wide<DT>((uint16_t)x[j]) + wide<DT>((uint16_t)(x[j] >> 16)));
+    s = lanes_sum<GB / 8>(s);
+    if (run % (GB / 8)) continue;
+    const uint16_t hi = f2bf(s);
+    const float s1 = s - bf2f(hi);
+    const uint16_t mid = f2bf(s1);
+    const uint16_t lo = f2bf(s1 - bf2f(mid));
+    sums[(int64_t)(run / (GB / 8)) * ((p.m + 127) & ~(int64_t)127) + m] = make_uint2(hi | ((uint32_t)mid << 16), lo);
+  }
 }
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -766,8 +768,8 @@ static void launch_w4_plan(const W4Params& p, const W4Plan& q, void* workspace, 
   uint2* sums = reinterpret_cast<uint2*>(workspace);
   float* parts = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + w4_sums_bytes(q, p.m, p.k, p.group));
   if (DT == kBF16 && U == 4)
-    hipLaunchKernelGGL((w4_sums_kernel<DT, GB>), dim3((unsigned)((p.m * (p.k / 8) + 255) / 256)), dim3(256), 0, stream,
-                       p, sums);
+    hipLaunchKernelGGL((w4_sums_kernel<DT, GB>), dim3((unsigned)std::min((p.m * (p.k / 8) + 255) / 256, kSumsBlocks)),
+                       dim3(256), 0, stream, p, sums);
   const int64_t items = q.tiles * q.splits;
   const dim3 grid((unsigned)((items + 7) / 8 * 8));
   if constexpr (U == 4)

@@ -594,8 +594,12 @@ void residual_norm_wide_kernel(ResNormParams p) {
   }
 }
 
-// Rows that a workgroup per row takes.
-constexpr int64_t kSplitRows = 1536;
+// Rows that a workgroup per row takes, about three a CU; more go to the staged
+// kernel (us, split / staged: 5120 columns with post norm to rows, 512 rows 7.3 /
+// 9.8, 768 11.0 / 10.9, 1536 21.2 / 16.2; 5376 columns with gate, modulation and
+// rotation to codes, fp32 branch, 512 rows 11.2 / 16.9, 768 15.7 / 19.4, 1024 25.1 /
+// 21.2).
+constexpr int64_t kSplitRows = 768;
 
 template <int DT, int BT, int MODE>
 static int launch_residual_norm(const ResNormParams& p, hipStream_t stream) {
