@@ -671,13 +671,17 @@ int w8a8_axial_freqs(const W8A8AxialFreqsArgs* args);
  *   4-7 inputs 1, 3, 5, 7 of the eight.
  * scales: [k / group, n] of dtype, contiguous; zeros: [k / group, n] uint8
  *   (0..15), contiguous, or NULL: 8.
+ * An infinity or NaN in a row of x makes that row's outputs infinite or NaN,
+ *   and no other row's.
  * workspace: device buffer of at least w8a8_linear_w4_workspace_size() bytes
- *   (16-byte aligned, any contents; NULL where that is 0) for calls too small
- *   to fill the GPU, which split k. Calls that share one must not overlap;
- *   calls in sequence may, and a captured graph may replay it.
+ *   (16-byte aligned, any contents; NULL where that is 0): sums of x where its
+ *   rows are many, and partial outputs of calls too small to fill the GPU,
+ *   which split k. Calls that share one must not overlap; calls in sequence
+ *   may, and a captured graph may replay it.
  * Requirements: group 32, 64 or a multiple of 128, k % group == 0; gated:
  *   n even, no residual; x and codes 16-byte aligned, ldx % 8 == 0,
- *   ldw % 4 == 0.
+ *   ldw % 4 == 0; m < 2^22; with more than eight rows n < 2^30, ldx and
+ *   ldw < 2^22.
  */
 typedef struct W8A8LinearW4Args {
   uint32_t struct_size;

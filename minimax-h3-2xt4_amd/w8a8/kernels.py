@@ -844,8 +844,8 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
         if residual.dtype != x.dtype or residual.numel() != m * n or residual.shape[-1] != n:
             raise ValueError('residual must be [.., N] in x\'s dtype')
         residual = residual.reshape(m, n)
-        if residual.stride(1) != 1 and n > 1:
-            residual = residual.contiguous()
+        if (n > 1 and residual.stride(1) != 1) or (m > 1 and residual.stride(0) < n):
+            residual = residual.contiguous()   # (a broadcast one too)
     y = out
     if y is None:
         y = torch.empty((m, width), dtype=x.dtype, device=x.device)

@@ -185,6 +185,12 @@ def test_linear_w4_refusals(change, fragment):
     _refused('w8a8_linear_w4', _abi.LinearW4Args(**{**W4, **change}), fragment)
 
 
+@pytest.mark.parametrize('change', [dict(ldw=1 << 22), dict(ldx=1 << 22), dict(n=1 << 30, ldo=1 << 30)])
+def test_linear_w4_many_rows_offsets_fit_32_bits(change):
+    case = {**W4, **change, 'm': 16, 'x': 1 << 50, 'out': 1 << 40, 'workspace': 1 << 45, 'workspace_bytes': 1 << 40}
+    _refused('w8a8_linear_w4', _abi.LinearW4Args(**case), 'too long')
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros((2, 256), dtype=torch.float16)
     with pytest.raises(ValueError):

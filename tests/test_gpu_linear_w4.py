@@ -74,6 +74,25 @@ def test_linear_w4(gpu, m, n, k, group, dtype, zeros, bias, residual, gated):
     assert bool((wide == 3.0).all())
 
 
+@pytest.mark.parametrize('group,dtype,k', [(128, F16, 1408), (128, BF16, 1536), (64, BF16, 1472), (64, F16, 2048),
+                                           (32, BF16, 1376), (32, F16, 1056)])
+@pytest.mark.parametrize('m', [8, 9, 32, 33, 64, 65, 129])
+def test_where_the_kernels_change(gpu, m, group, dtype, k):
+    # Odd and even numbers of 128-input steps, whole or not, split over k (few outputs).
+    print(f'linear_w4 {m} rows, k {k} group {group} {dtype}', flush=True)
+    codes, s = _case(m, 200, k, group, dtype, True, True, True, gpu)
+    y = _call(codes, s)
+    exact, slack = exact_w4(s['x'], codes, s['scales'], s['zeros'], bias=s['bias'], residual=s['residual'])
+    assert_close(y, exact, slack, 'outputs')
+
+
+def test_broadcast_residual(gpu):
+    codes, s = _case(5, 64, 256, 128, F16, False, False, True, gpu)
+    row = s['residual'][:1]
+    y = _call(codes, {**s, 'residual': row.expand(5, 64)})
+    assert torch.equal(y, _call(codes, {**s, 'residual': row.repeat(5, 1)}))
+
+
 def test_rows_of_ones_and_single_inputs(gpu):
     """Each weight alone: x a unit vector picks out one column of the weight, exactly."""
     g = torch.Generator().manual_seed(1)
