@@ -352,144 +352,38 @@ __device__ __forceinline__ void store_tile(const W4Params& p, const v16f (&tot)[
 // rows (gated: 16 W of gate and the same of up); each wave takes all of x's rows
 // and 32 of the weight's (gated: 16 of each), so that every code is unpacked once
 // a workgroup, and the waves of a SIMD do each other's unpacking and scaling in
-// the shadow of their MFMAs. The 32 x 32 x 16 MFMA's first operand is x, from LDS,
-// its second the weights, a word of codes a lane: a lane's column is one weight
-// row, whose scale it holds. x comes by DMA in steps of 128 inputs, two in turn
-// (16-byte run c of row r at run c ^ (r & 15)), codes and scales into registers a
-// step ahead.
+// the shadow of their MFMAs. The 32 x 32 x 16 MFMA's first operand is x, its second
+// the weights, a word of codes a lane: a lane's column is one weight row, whose
+// scale it holds.
+//
+// Everything comes by DMA: x (16-byte run c of row r at run c ^ (r & 15)), codes,
+// scales and zeros (sub-word loads, a word each in LDS), into a ring of stages of
+// 128 inputs each, RING - 1 ahead, so that a counted wait leaves the later stages'
+// loads in flight (a load into registers behind a DMA waits for all of them). A
+// step's work is laid out product by product (below), since the compiler's own
+// order reads each operand right before its use and scales and unpacks between the
+// chains of MFMAs. 2048 x 14336 x 4096: bf16 in groups of 64 381 -> 294 us (817
+// TFLOP/s), fp16 in groups of 128 294 -> 258. What bounds it there: every wave
+// reads all of x's tile, 256 KB of LDS a step, as long as its MFMAs take, and the
+// two waves of a SIMD do not fill the rest.
 //
 // fp16 takes the zeros off its weights (packed subtraction, exact). bf16 has no
-// such instruction. Where the rows are many an MFMA puts -(16 + z) sum x into the
-// accumulators before a block's products, with the sum in three bf16 (exact) as
-// three inputs; where they are few a second MFMA beside each product sums x, which
-// costs less than the launch that sums it beforehand.
+// such instruction. Where the rows are many (U = 4) an MFMA puts -(16 + z) sum x
+// into the accumulators before a block's products, with the sum in three bf16
+// (exact) as three inputs, loaded one step ahead; where they are few a second MFMA
+// beside each product sums x, which costs less than the launch that sums it
+// beforehand.
 //
 // Where the tiles are too few for the GPU, the steps of k are split over `splits`
 // workgroups, whose sums linear_w4_join_kernel adds in order.
-template <int DT, int GB, int U, int W, bool GATED>
-__global__ __launch_bounds__(64 * W, DT == kBF16 && U == 2 ? 3 : 4)
-void linear_w4_tiles_kernel(W4Params p, float* parts, int mtiles, int tiles, int splits) {
-  constexpr int S = GB / 16, NB = 128 / GB, BN = GATED ? 16 * W : 32 * W, ROWS = 32 * U, DMAS = 8 * U / W;
-  constexpr bool ONES = DT == kBF16;
-  __shared__ __attribute__((aligned(16))) char xs[2][ROWS * 256];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t width = GATED ? p.n / 2 : p.n;
-  // Workgroups go to the eight XCDs in turn: each XCD takes a run of items, the
-  // row tiles (then the ranges of k) of a few weight tiles at a time.
-  const int items = tiles * splits, per = (items + 7) / 8, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (item >= items || (int)(blockIdx.x >> 3) >= per) return;
-  const int tile = item / splits, split = item - tile * splits;
-  const int64_t m0 = (int64_t)(tile % mtiles) * ROWS, n0 = (int64_t)(tile / mtiles) * BN;
-  const int mrows = (int)min((int64_t)ROWS, p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
-  const int ncol = GATED ? 16 * wave + (c & 15) : 32 * wave + c;   // the lane's column of the tile
-  const int64_t wr = (GATED && c >= 16 ? width : 0) + n0 + min(ncol, nrows - 1);
-  const char* const wrow = reinterpret_cast<const char*>(p.codes + wr * p.ldw);
-  const auto xbase = dma_base(reinterpret_cast<const uint16_t*>(p.x) + m0 * p.ldx);
-  uint32_t xoff[DMAS];
-#pragma unroll
-  for (int i = 0; i < DMAS; ++i)
-    xoff[i] = (uint32_t)min(4 * (DMAS * wave + i) + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
-  const int all = (int)((p.k + 127) / 128), words = (int)(p.k / 8), blocks = (int)(p.k / GB);
-  const int first = (int)((int64_t)all * split / splits), last = (int)((int64_t)all * (split + 1) / splits);
-  const int per_group = p.group / GB;
-
-  uint32_t w[NB][S];
-  uint16_t sc[NB];
-  uint8_t zr[NB];
-  auto load = [&](int step) {
-    // Past the end of k (the last step only) the last runs and codes again: their blocks are left out.
-#pragma unroll
-    for (int i = 0; i < DMAS; ++i) {
-      const int row = 4 * (DMAS * wave + i), run = (lane & 15) ^ ((row + (lane >> 4)) & 15);
-      dma<16>(xbase, xoff[i] + (uint32_t)min(step * 256 + run * 16, (int)p.k * 2 - 16), xs[step & 1] + row * 256);
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int block = min(step * NB + b, blocks - 1);
-      const int at = min(step * 16 + b * (GB / 8) + h * S, words - S) * 4;
-      const int64_t grow = (int64_t)(block / per_group) * p.n + wr;
-      if constexpr (S >= 4) {
-#pragma unroll
-        for (int j = 0; j < S; j += 4) *reinterpret_cast<v4u*>(&w[b][j]) = *reinterpret_cast<const v4u*>(wrow + at + 4 * j);
-      } else {
-        *reinterpret_cast<uint2*>(&w[b][0]) = *reinterpret_cast<const uint2*>(wrow + at);
-      }
-      sc[b] = p.scales[grow];
-      zr[b] = p.zeros ? p.zeros[grow] : (uint8_t)8;
-    }
-  };
-
-  const Unpack<DT> unpack;
-  v16f tot[U] = {};
-  load(first);
-  for (int step = first; step < last; ++step) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): the step's loads have landed,
-    __syncthreads();                      // everyone's, and the last one's reads are done
-    uint32_t cw[NB][S];
-    float cs[NB], fz[NB];
-    uint32_t cz[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-#pragma unroll
-      for (int j = 0; j < S; ++j) cw[b][j] = w[b][j];
-      cs[b] = wide<DT>(sc[b]);
-      fz[b] = -16.0f - (float)zr[b];
-      cz[b] = DT == kF16 ? (uint32_t)f2h(-fz[b]) * 0x10001u
-                         : h ? 0 : (__float_as_uint(fz[b]) >> 16) * 0x10001u;   // (exact: a small integer)
-    }
-    if (step + 1 < last) load(step + 1);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      if (NB > 1 && step * NB + b >= blocks) break;
-      v4u wt[S];
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        wt[j] = unpack(cw[b][j]);
-        if constexpr (DT == kF16) wt[j] = less(wt[j], cz[b]);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        v16f acc = {}, sum = {};
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-          const v4u x = *reinterpret_cast<const v4u*>(xs[step & 1] + (32 * u + c) * 256 +
-                                                      16 * ((b * (GB / 8) + h * S + j) ^ (c & 15)));
-          acc = mfma32<DT>(x, wt[j], acc);
-          if constexpr (ONES) sum = mfma32<DT>(x, v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}, sum);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float v = ONES ? __builtin_fmaf(fz[b], sum[i], acc[i]) : acc[i];
-          tot[u][i] = __builtin_fmaf(cs[b], v, tot[u][i]);
-        }
-      }
-      // (Here, not at the end of the step, where the compiler would put the sums
-      // of all its blocks with every accumulator alive.)
-#pragma unroll
-      for (int u = 0; u < U; ++u) __asm__ volatile("" : "+v"(tot[u]));
-    }
-  }
-  store_tile<DT, U, GATED>(p, tot, parts, split, splits, m0, n0, mrows, nrows, wr, ncol, c, h);
-}
-
-// More than 64 rows: the same tiles with 128 rows of x and 256 weight rows, and
-// everything by DMA: x, codes, scales and zeros (sub-word loads, a word each in LDS)
-// into a ring of stages of one step each, RING - 1 steps ahead, so that a counted
-// wait leaves the later steps' loads in flight (a load into registers behind a DMA
-// waits for all of them). The sums of x come one step ahead. A step's work is laid
-// out product by product (below), since the compiler's own order reads each operand
-// right before its use and scales and unpacks between the chains of MFMAs. 2048 x
-// 14336 x 4096: bf16 in groups of 64 381 -> 294 us (817 TFLOP/s), fp16 in groups of
-// 128 294 -> 258. What bounds it: every wave reads all of x's tile, 256 KB of LDS a
-// step, as long as its MFMAs take, and the two waves of a SIMD do not fill the rest.
-template <int DT, int GB>
+template <int DT, int GB, int U, int W>
 struct W4Stage {
+  static constexpr bool kOnes = DT == kBF16 && U < 4, kPre = DT == kBF16 && U == 4;
   static constexpr int NB = 128 / GB, PAIRS = (NB + 1) / 2;
-  static constexpr int kRing = GB == 32 ? 2 : 3;                 // (what 160 KB hold)
-  static constexpr int kX = 128 * 256, kCodes = 8 * 2048, kMeta = 8 * 512 * PAIRS, kBytes = kX + kCodes + kMeta;
-  static constexpr int kDma = 4 + 2 + 2 * PAIRS;                 // instructions of a wave
-  static constexpr int kSums = DT == kBF16 ? NB * 1024 : 0;
+  static constexpr int kRing = U > 1 && GB == 32 ? 2 : 3;        // (what 160 KB hold; two workgroups a CU below U = 4)
+  static constexpr int kX = U * 32 * 256, kCodes = W * 2048, kMeta = W * 512 * PAIRS, kBytes = kX + kCodes + kMeta;
+  static constexpr int kXDma = 8 * U / W, kDma = kXDma + 2 + 2 * PAIRS;   // instructions of a wave
+  static constexpr int kSums = kPre ? NB * 1024 : 0;
   static constexpr int kLds = kRing * kBytes + 2 * kSums;
 };
 
@@ -504,11 +398,11 @@ __device__ __forceinline__ void block_barrier() {
   __asm__ volatile("" ::: "memory");
 }
 
-template <int DT, int GB, bool GATED>
-__global__ __launch_bounds__(512, 2)
-void linear_w4_ring_kernel(W4Params p, const uint2* sums, float* parts, int mtiles, int tiles, int splits) {
-  using Stage = W4Stage<DT, GB>;
-  constexpr int S = GB / 16, NB = Stage::NB, BN = GATED ? 128 : 256, RING = Stage::kRing;
+template <int DT, int GB, int U, int W, bool GATED>
+__global__ __launch_bounds__(64 * W, 2)
+void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mtiles, int tiles, int splits) {
+  using Stage = W4Stage<DT, GB, U, W>;
+  constexpr int S = GB / 16, NB = Stage::NB, BN = GATED ? 16 * W : 32 * W, RING = Stage::kRing;
   constexpr int DEEP = 4;   // (6 and 8 the same within 1 %)
   __shared__ __attribute__((aligned(16))) char lds[Stage::kLds];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
@@ -517,16 +411,17 @@ void linear_w4_ring_kernel(W4Params p, const uint2* sums, float* parts, int mtil
   const int items = tiles * splits, per = (items + 7) / 8, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (item >= items || (int)(blockIdx.x >> 3) >= per) return;
   const int tile = item / splits, split = item - tile * splits;
-  const int64_t m0 = (int64_t)(tile % mtiles) * 128, n0 = (int64_t)(tile / mtiles) * BN;
-  const int mrows = (int)min((int64_t)128, p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
+  const int64_t m0 = (int64_t)(tile % mtiles) * (32 * U), n0 = (int64_t)(tile / mtiles) * BN;
+  const int mrows = (int)min((int64_t)(32 * U), p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
   // The tile's column of the wave's column col (0..31: gated, 16 of gate and the same of up).
   auto column = [&](int col) { return GATED ? 16 * wave + (col & 15) : 32 * wave + col; };
   const int ncol = column(c), nclamped = min(ncol, nrows - 1);
   const int64_t wr = (GATED && c >= 16 ? width : 0) + n0 + nclamped;
   const auto xbase = dma_base(reinterpret_cast<const uint16_t*>(p.x) + m0 * p.ldx);
-  uint32_t xoff[4];
+  uint32_t xoff[Stage::kXDma];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) xoff[i] = (uint32_t)min(4 * (4 * wave + i) + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
+  for (int i = 0; i < Stage::kXDma; ++i)
+    xoff[i] = (uint32_t)min(4 * (Stage::kXDma * wave + i) + (lane >> 4), mrows - 1) * (uint32_t)(p.ldx * 2);
   // A wave brings its own codes: instruction i rows 16 i .. 16 i + 15, four 16-byte
   // runs a row, run q at q ^ (row >> 2 & 3).
   __amdgpu_buffer_rsrc_t cbase[2];
@@ -549,26 +444,28 @@ void linear_w4_ring_kernel(W4Params p, const uint2* sums, float* parts, int mtil
   // of k the last runs and codes again, whose blocks' scales are taken as zero.
   auto load = [&](int step, char* to, int i) {
     step = min(step, last - 1);
-    if (i < 4) {
-      const int row = 4 * (4 * wave + i), run = (lane & 15) ^ ((row + (lane >> 4)) & 15);
+    constexpr int X = Stage::kXDma;
+    if (i < X) {
+      const int row = 4 * (X * wave + i), run = (lane & 15) ^ ((row + (lane >> 4)) & 15);
       dma<16>(xbase, xoff[i] + (uint32_t)min(step * 256 + run * 16, (int)p.k * 2 - 16), to + row * 256);
-    } else if (i < 6) {
-      dma<16>(cbase[i - 4], coff[i - 4] + (uint32_t)min(step * 64 + crun, kbytes - 16), to + Stage::kX + 2048 * wave + 1024 * (i - 4));
+    } else if (i < X + 2) {
+      dma<16>(cbase[i - X], coff[i - X] + (uint32_t)min(step * 64 + crun, kbytes - 16),
+              to + Stage::kX + 2048 * wave + 1024 * (i - X));
     } else {
-      const int j = (i - 6) / 2;
+      const int j = (i - X - 2) / 2;
       // (Two neighbouring blocks of less than 128 inputs, half the lanes each.)
       const int one = min(step * NB + 2 * j, blocks - 1), two = min(step * NB + 2 * j + 1, blocks - 1);
       const int64_t group = NB > 1 ? one : one / per_group;   // (blocks are groups below 128 inputs)
       const uint32_t at = roff + (NB > 1 && h && two != one ? (uint32_t)p.n : 0);
       char* const meta = to + Stage::kX + Stage::kCodes + 512 * (Stage::PAIRS * wave + j);
-      if (i & 1) dma<1>(dma_base(zrow + group * p.n), at, meta + 256);
+      if ((i - X) & 1) dma<1>(dma_base(zrow + group * p.n), at, meta + 256);
       else dma<2>(dma_base(p.scales + group * p.n), 2 * at, meta);
     }
   };
   auto load_sums = [&](int step, char* to) {
     // (4 bytes a lane; the waves that are left load the same again. Rows past the
     // last are never stored.)
-    if constexpr (DT == kBF16) {
+    if constexpr (Stage::kPre) {
 #pragma unroll
       for (int i = 0; i < (NB + 1) / 2; ++i) {
         const int part = (8 * i + wave) & (4 * NB - 1);
@@ -581,7 +478,8 @@ void linear_w4_ring_kernel(W4Params p, const uint2* sums, float* parts, int mtil
   const uint32_t zero_mask = p.zeros ? 0xffu : 0u, zero_else = p.zeros ? 0u : 8u, half_mask = h ? 0u : ~0u;
   const Unpack<DT> unpack;
   // A block's codes, scale and zero as they lie in LDS, and its weights, scale and
-  // zero (fp16: to take off the weights; bf16: its column) ready for the MFMAs.
+  // zero (fp16: to take off the weights; bf16: the correction's column, or factor)
+  // ready for the MFMAs.
   struct Raw {
     uint32_t w[S], scale, zero;
   };
@@ -608,29 +506,36 @@ void linear_w4_ring_kernel(W4Params p, const uint2* sums, float* parts, int mtil
     // (Selects by arithmetic: behind a branch the compiler waits for every load.)
     o.scale = wide<DT>((uint16_t)r.scale) * (NB == 1 || step * NB + b < blocks ? 1.0f : 0.0f);
     const float z = 16.0f + (float)((r.zero & zero_mask) | zero_else);
-    o.zero = DT == kF16 ? (uint32_t)f2h(z) * 0x10001u
-                        : ((__float_as_uint(-z) >> 16) * 0x10001u) & half_mask;   // (exact: a small integer)
+    if constexpr (Stage::kOnes) o.zero = __float_as_uint(-z);
+    else o.zero = DT == kF16 ? (uint32_t)f2h(z) * 0x10001u
+                             : ((__float_as_uint(-z) >> 16) * 0x10001u) & half_mask;   // (exact: a small integer)
   };
   auto weights = [&](const Raw& r, int j, Ready& o) {
     o.w[j] = unpack(r.w[j]);
     if constexpr (DT == kF16) o.w[j] = less(o.w[j], o.zero);
   };
 
-  v16f tot[4] = {}, acc[2] = {};
-  float carry = 0.0f;             // the scale of the last chain, whose sums are in acc[1]
+  constexpr int P = U * S, N = NB * P;        // products of a block and a step
+  constexpr bool ODD = NB * U == 1;           // one chain a step: accumulators change places between steps
+  v16f tot[U] = {}, acc[2] = {}, ones[2] = {};
+  float carry = 0.0f, carry_zero = 0.0f;      // of the last chain, whose sums are still to be scaled
   int at = 0, to = (RING - 1) * Stage::kBytes, sums_of = RING * Stage::kBytes, sums_to = sums_of + Stage::kSums;
   auto next_stage = [&](int q) { return q == (RING - 1) * Stage::kBytes ? 0 : q + Stage::kBytes; };
-  // A step: 32 products of 32 x 32 x 16, in chains of a block's S for 32 rows of x.
-  // Each is followed, in the shadow of its MFMA, by the read of x for the product
-  // DEEP on, a piece of the loads for the step RING - 1 on, a share of the last
-  // chain's scaling, and in the second half of a block a share of unpacking the next.
-  auto run = [&](int step, Ready& fa, Ready& fb) {
+  auto scaled = [&](float scale, float zero, int a, int e, float t) {
+    const float v = Stage::kOnes ? __builtin_fmaf(zero, ones[a][e], acc[a][e]) : acc[a][e];
+    return __builtin_fmaf(scale, v, t);
+  };
+  // A step: products of 32 x 32 x 16, in chains of a block's S for 32 rows of x. Each
+  // is followed, in the shadow of its MFMA, by the read of x for the product DEEP on,
+  // its share of the loads for the step RING - 1 on, a share of the last chain's
+  // scaling, and in the second half of a block a share of unpacking the next.
+  auto run = [&](int step, Ready& fa, Ready& fb, auto swap) {
     block_barrier();
     load_sums(step + 1, lds + sums_to);
     const char* const xs = lds + at;
     const int after = next_stage(at);
     auto read = [&](int i) {
-      const int b = i / (4 * S), u = i / S % 4, j = i % S;
+      const int b = i / P, u = i / S % U, j = i % S;
       return *reinterpret_cast<const v4u*>(xs + (32 * u + c) * 256 + 16 * ((b * (GB / 8) + h * S + j) ^ (c & 15)));
     };
     auto read_sum = [&](int b, int u) {
@@ -641,38 +546,51 @@ void linear_w4_ring_kernel(W4Params p, const uint2* sums, float* parts, int mtil
     v4u x[DEEP];
     uint2 sum[2];
     Raw raw;
-    if constexpr (DT == kBF16) sum[0] = read_sum(0, 0);
+    if constexpr (Stage::kPre) sum[0] = read_sum(0, 0);
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) x[i] = read(i);
     __builtin_amdgcn_sched_barrier(0);
+    // The step's loads go out before the fetch of the next step's first codes, whose
+    // wait counts them.
+    constexpr int kFetch = P / 4, kEach = (Stage::kDma - 1) / ((NB - 1) * P + kFetch) + 1;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int b = i / (4 * S), u = i / S % 4, j = i % S;
+    for (int i = 0; i < N; ++i) {
+      const int b = i / P, u = i / S % U, j = i % S, in = i % P, a = (i / S + swap()) & 1;
       Ready& f = b & 1 ? fb : fa;
       Ready& g = b & 1 ? fa : fb;
-      if (j == 0) {
-        if constexpr (DT == kBF16) acc[u & 1] = mfma_zero(sum[u & 1], make_uint2(f.zero, f.zero));
-        else acc[u & 1] = v16f{};
+      if (in == kFetch) {
+        // (A wave's codes are its own DMA.)
+        if (b + 1 == NB) wait_loads<(RING - 2) * Stage::kDma>();
+        fetch(lds + (b + 1 == NB ? after : at), b + 1 == NB ? 0 : b + 1, raw);
       }
-      acc[u & 1] = mfma32<DT>(x[i % DEEP], f.w[j], acc[u & 1]);
-      if (i + DEEP < 32) x[i % DEEP] = read(i + DEEP);
-      if (DT == kBF16 && j == 0 && i + S < 32) sum[(u + 1) & 1] = read_sum((i + S) / (4 * S), (u + 1) % 4);
-      if (i < Stage::kDma) load(step + RING - 1, lds + to, i);
+      if (j == 0) {
+        if constexpr (Stage::kPre) acc[a] = mfma_zero(sum[u & 1], make_uint2(f.zero, f.zero));
+        else acc[a] = v16f{};
+        ones[a] = v16f{};
+      }
+      acc[a] = mfma32<DT>(x[i % DEEP], f.w[j], acc[a]);
+      if constexpr (Stage::kOnes)
+        ones[a] = mfma32<DT>(x[i % DEEP], v4u{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}, ones[a]);
+      if (i + DEEP < N) x[i % DEEP] = read(i + DEEP);
+      if (Stage::kPre && j == 0 && i + S < N) sum[(u + 1) & 1] = read_sum((i + S) / P, (u + 1) % U);
+#pragma unroll
+      for (int d = i * kEach; d < (i + 1) * kEach; ++d)
+        if (d < Stage::kDma) load(step + RING - 1, lds + to, d);
       if (j > 0) {
-        const float scale = u ? f.scale : carry;
+        const float scale = u ? f.scale : carry, zero = u ? __uint_as_float(f.zero) : carry_zero;
+        const int last_u = (u + U - 1) % U;
 #pragma unroll
         for (int e = 16 * (j - 1) / (S - 1); e < 16 * j / (S - 1); ++e)
-          tot[(u + 3) & 3][e] = __builtin_fmaf(scale, acc[(u + 1) & 1][e], tot[(u + 3) & 3][e]);
+          tot[last_u][e] = scaled(scale, zero, a ^ 1, e, tot[last_u][e]);
       }
-      const bool ends = b + 1 == NB;
-      if (u == 1 && j == 0) {
-        // (A wave's codes are its own DMA. Every load of the step RING - 1 on has been issued.)
-        if (ends) wait_loads<(RING - 2) * Stage::kDma>();
-        fetch(lds + (ends ? after : at), ends ? 0 : b + 1, raw);
+      if (in == P / 2) open(step + (b + 1 == NB), b + 1 == NB ? 0 : b + 1, raw, g);
+      const int past = in - P / 2;
+      if (past >= 0 && past * 2 % U == 0) weights(raw, past * 2 / U, g);
+      if (past >= 0 && U == 1) weights(raw, past * 2 + 1, g);
+      if (in == P - 1) {
+        carry = f.scale;
+        carry_zero = __uint_as_float(f.zero);
       }
-      if (u == 2 && j == 0) open(step + ends, ends ? 0 : b + 1, raw, g);
-      if (u >= 2 && (j & 1) == 0) weights(raw, (u - 2) * (S / 2) + j / 2, g);
-      if (u == 3 && j == S - 1) carry = f.scale;
       __builtin_amdgcn_sched_barrier(0);
     }
     at = after;
@@ -695,20 +613,30 @@ void linear_w4_ring_kernel(W4Params p, const uint2* sums, float* parts, int mtil
 #pragma unroll
     for (int j = 0; j < S; ++j) weights(raw, j, f0);
   }
+  // (The last chain's accumulators are acc[1], but after an odd number of steps of one chain.)
+  auto flush = [&](int a) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) tot[U - 1][e] = scaled(carry, carry_zero, a, e, tot[U - 1][e]);
+  };
+  constexpr std::integral_constant<int, 0> zero;
   if constexpr (NB == 1) {
     int step = first;
     for (; step + 1 < last; step += 2) {
-      run(step, f0, f1);
-      run(step + 1, f1, f0);
+      run(step, f0, f1, zero);
+      run(step + 1, f1, f0, std::integral_constant<int, ODD>{});
     }
-    if (step < last) run(step, f0, f1);
+    if (step < last) {
+      run(step, f0, f1, zero);
+      flush(ODD ? 0 : 1);
+    } else {
+      flush(1);
+    }
   } else {
-    for (int step = first; step < last; ++step) run(step, f0, f1);
+    for (int step = first; step < last; ++step) run(step, f0, f1, zero);
+    flush(1);
   }
-#pragma unroll
-  for (int e = 0; e < 16; ++e) tot[3][e] = __builtin_fmaf(carry, acc[1][e], tot[3][e]);
   wait_loads<0>();     // no DMA outlives the workgroup's LDS
-  store_tile<DT, 4, GATED>(p, tot, parts, split, splits, m0, n0, mrows, nrows, wr, ncol, c, h);
+  store_tile<DT, U, GATED>(p, tot, parts, split, splits, m0, n0, mrows, nrows, wr, ncol, c, h);
 }
 
 // The outputs of a split call: the ranges' sums in order, then the epilogue. One
@@ -721,7 +649,21 @@ void linear_w4_join_kernel(W4Params p, const float* parts, int splits, bool gate
   const float* row = parts + m * p.n + n;
   const int64_t stride = p.m * p.n;
   float v = row[0], up = gated ? row[width] : 0.0f;
-  for (int s = 1; s < splits; ++s) {
+  int s = 1;
+  for (; s + 4 <= splits; s += 4) {   // (four loads at once)
+    float a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = row[(s + i) * stride];
+      b[i] = gated ? row[(s + i) * stride + width] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v = v + a[i];
+      up = up + b[i];
+    }
+  }
+  for (; s < splits; ++s) {
     v = v + row[s * stride];
     if (gated) up = up + row[s * stride + width];
   }
@@ -732,8 +674,11 @@ void linear_w4_join_kernel(W4Params p, const float* parts, int splits, bool gate
 }
 
 // How a call of more than eight rows is cut: 32 u rows and 32 w weight rows a tile,
-// and the ranges of k. The ranges keep at least four steps, and their sums at
-// most 64 MB.
+// and the ranges of k, as many as give each CU one. The ranges keep at least four
+// steps, and their sums at most 64 MB. (Two ranges a CU cost more to join than they
+// hide: us, one / two, 64 x 4096 x 14336 21.3 / 24.2, 16 x 4096 x 14336 14.6 / 16.9,
+// 64 x 14336 x 4096 20.3 / 21.4; where they are few anyway the same, 32 x 14336 x
+// 4096 15.7 / 15.8.)
 struct W4Plan {
   int u, w, mtiles, splits;
   int64_t tiles;
@@ -745,7 +690,7 @@ static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int cus) {
   q.w = q.u == 4 ? 8 : 4;
   q.mtiles = (int)((m + 32 * q.u - 1) / (32 * q.u));
   q.tiles = (n + 32 * q.w - 1) / (32 * q.w) * q.mtiles;
-  const int64_t steps = (k + 127) / 128, want = (q.u == 4 ? 1 : 2) * (int64_t)cus;
+  const int64_t steps = (k + 127) / 128, want = cus;
   int64_t s = q.tiles < want ? want / q.tiles : 1;
   if (s > steps / 4) s = steps / 4;
   const int64_t most = (64ll << 20) / (4 * m * n);
@@ -772,12 +717,8 @@ static void launch_w4_plan(const W4Params& p, const W4Plan& q, void* workspace, 
                        dim3(256), 0, stream, p, sums);
   const int64_t items = q.tiles * q.splits;
   const dim3 grid((unsigned)((items + 7) / 8 * 8));
-  if constexpr (U == 4)
-    hipLaunchKernelGGL((linear_w4_ring_kernel<DT, GB, GATED>), grid, dim3(512), 0, stream, p, sums, parts, q.mtiles,
-                       (int)q.tiles, q.splits);
-  else
-    hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, U, W, GATED>), grid, dim3(64 * W), 0, stream, p, parts, q.mtiles,
-                       (int)q.tiles, q.splits);
+  hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, U, W, GATED>), grid, dim3(64 * W), 0, stream, p, sums, parts,
+                     q.mtiles, (int)q.tiles, q.splits);
   if (q.splits > 1)
     hipLaunchKernelGGL((linear_w4_join_kernel<DT>), dim3((unsigned)(((GATED ? p.n / 2 : p.n) + 255) / 256), (unsigned)p.m),
                        dim3(256), 0, stream, p, parts, q.splits, GATED);
