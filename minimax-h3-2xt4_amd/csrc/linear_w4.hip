@@ -309,20 +309,19 @@ __device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t base, uint32_t off, c
   else __builtin_amdgcn_raw_ptr_buffer_load_lds(base, to, 1, (int)off, 0, 0, 0);
 }
 
-// A tile's outputs, or its sums over a range of k.
+// A tile's outputs, or (part: the lane's column of the range's tile, rows `width`
+// apart) its sums over a range of k.
 template <int DT, int U, bool GATED>
-__device__ __forceinline__ void store_tile(const W4Params& p, const v16f (&tot)[U], float* parts, int split, int splits,
-                                           int64_t m0, int64_t n0, int mrows, int nrows, int64_t wr, int ncol, int c,
-                                           int h) {
+__device__ __forceinline__ void store_tile(const W4Params& p, const v16f (&tot)[U], float* part, int width, int64_t m0,
+                                           int64_t n0, int mrows, int nrows, int64_t wr, int ncol, int c, int h) {
   const int64_t n = n0 + ncol;
-  if (splits > 1) {
-    float* part = parts + (int64_t)split * p.m * p.n + wr;
+  if (part) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int m = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-        if (m < mrows && ncol < nrows) part[(m0 + m) * p.n] = tot[u][i];
+        if (m < mrows) part[m * width] = tot[u][i];
       }
     return;
   }
@@ -374,8 +373,9 @@ __device__ __forceinline__ void store_tile(const W4Params& p, const v16f (&tot)[
 // beside each product sums x, which costs less than the launch that sums it
 // beforehand.
 //
-// Where the tiles are too few for the GPU, the steps of k are split over `splits`
-// workgroups, whose sums linear_w4_join_kernel adds in order.
+// The tiles past the last whole round of the GPU (all of them, where they are few)
+// split the steps of k over `splits` workgroups each, whose sums
+// linear_w4_join_kernel adds in order.
 template <int DT, int GB, int U, int W>
 struct W4Stage {
   static constexpr bool kOnes = DT == kBF16 && U < 4, kPre = DT == kBF16 && U == 4;
@@ -400,7 +400,7 @@ __device__ __forceinline__ void block_barrier() {
 
 template <int DT, int GB, int U, int W, bool GATED>
 __global__ __launch_bounds__(64 * W, 2)
-void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mtiles, int tiles, int splits) {
+void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mtiles, int whole, int rest, int splits) {
   using Stage = W4Stage<DT, GB, U, W>;
   constexpr int S = GB / 16, NB = Stage::NB, BN = GATED ? 16 * W : 32 * W, RING = Stage::kRing;
   constexpr int DEEP = 4;   // (6 and 8 the same within 1 %)
@@ -408,9 +408,15 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t width = GATED ? p.n / 2 : p.n;
-  const int items = tiles * splits, per = (items + 7) / 8, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (item >= items || (int)(blockIdx.x >> 3) >= per) return;
-  const int tile = item / splits, split = item - tile * splits;
+  // Workgroups go to the eight XCDs in turn: each XCD takes a run of the whole tiles
+  // (the row tiles of a few weight tiles at a time), then one of the rest's ranges.
+  const int head = (whole + 7) & ~7;
+  const bool split_up = (int)blockIdx.x >= head;
+  const int at_block = split_up ? (int)blockIdx.x - head : (int)blockIdx.x, items = split_up ? rest * splits : whole;
+  const int per = (items + 7) / 8, item = (at_block & 7) * per + (at_block >> 3);
+  if (item >= items || (at_block >> 3) >= per) return;
+  const int left = split_up ? item / splits : 0, split = split_up ? item - left * splits : 0;
+  const int tile = split_up ? whole + left : item, ranges = split_up ? splits : 1;
   const int64_t m0 = (int64_t)(tile % mtiles) * (32 * U), n0 = (int64_t)(tile / mtiles) * BN;
   const int mrows = (int)min((int64_t)(32 * U), p.m - m0), nrows = (int)min((int64_t)BN, width - n0);
   // The tile's column of the wave's column col (0..31: gated, 16 of gate and the same of up).
@@ -436,7 +442,7 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
   // (Without zeros a byte of the scales is read and left.)
   const uint8_t* const zrow = p.zeros ? p.zeros : reinterpret_cast<const uint8_t*>(p.scales);
   const int all = (int)((p.k + 127) / 128), blocks = (int)(p.k / GB), kbytes = (int)(p.k / 2);
-  const int first = (int)((int64_t)all * split / splits), last = (int)((int64_t)all * (split + 1) / splits);
+  const int first = (int)((int64_t)all * split / ranges), last = (int)((int64_t)all * (split + 1) / ranges);
   const int per_group = p.group / GB;
   const int64_t mpad = (p.m + 127) & ~(int64_t)127;
 
@@ -636,26 +642,32 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
     flush(1);
   }
   wait_loads<0>();     // no DMA outlives the workgroup's LDS
-  store_tile<DT, U, GATED>(p, tot, parts, split, splits, m0, n0, mrows, nrows, wr, ncol, c, h);
+  float* const part =
+      split_up ? parts + ((int64_t)split * rest + left) * (32 * U * 32 * W) + 32 * wave + c : nullptr;
+  store_tile<DT, U, GATED>(p, tot, part, 32 * W, m0, n0, mrows, nrows, wr, ncol, c, h);
 }
 
-// The outputs of a split call: the ranges' sums in order, then the epilogue. One
+// The outputs of the split tiles: the ranges' sums in order, then the epilogue. One
 // output a thread.
-template <int DT>
+template <int DT, int U, int W, bool GATED>
 __global__ __launch_bounds__(256)
-void linear_w4_join_kernel(W4Params p, const float* parts, int splits, bool gated) {
-  const int64_t width = gated ? p.n / 2 : p.n, n = (int64_t)blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
-  if (n >= width) return;
-  const float* row = parts + m * p.n + n;
-  const int64_t stride = p.m * p.n;
-  float v = row[0], up = gated ? row[width] : 0.0f;
+void linear_w4_join_kernel(W4Params p, const float* parts, int mtiles, int whole, int rest, int splits) {
+  constexpr int BN = GATED ? 16 * W : 32 * W, BLOCKS = 32 * U * BN / 256;
+  const int64_t width = GATED ? p.n / 2 : p.n;
+  const int left = blockIdx.x / BLOCKS, tile = whole + left;
+  const int i = (blockIdx.x - left * BLOCKS) * 256 + threadIdx.x, row = i / BN, col = i - row * BN;
+  const int64_t m = (int64_t)(tile % mtiles) * (32 * U) + row, n = (int64_t)(tile / mtiles) * BN + col;
+  if (m >= p.m || n >= width) return;
+  const int64_t stride = (int64_t)rest * (32 * U * 32 * W);
+  const float* at = parts + ((int64_t)left * (32 * U) + row) * (32 * W) + (GATED ? 32 * (col / 16) + col % 16 : col);
+  float v = at[0], up = GATED ? at[16] : 0.0f;
   int s = 1;
   for (; s + 4 <= splits; s += 4) {   // (four loads at once)
     float a[4], b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      a[i] = row[(s + i) * stride];
-      b[i] = gated ? row[(s + i) * stride + width] : 0.0f;
+      a[i] = at[(s + i) * stride];
+      b[i] = GATED ? at[(s + i) * stride + 16] : 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -664,38 +676,41 @@ void linear_w4_join_kernel(W4Params p, const float* parts, int splits, bool gate
     }
   }
   for (; s < splits; ++s) {
-    v = v + row[s * stride];
-    if (gated) up = up + row[s * stride + width];
+    v = v + at[s * stride];
+    if (GATED) up = up + at[s * stride + 16];
   }
   if (p.bias) v = v + wide<DT>(p.bias[n]);
-  if (gated) v = swiglu(v, p.bias ? up + wide<DT>(p.bias[width + n]) : up);
+  if (GATED) v = swiglu(v, p.bias ? up + wide<DT>(p.bias[width + n]) : up);
   if (p.residual) v = v + wide<DT>(p.residual[m * p.ldr + n]);
   p.out[m * p.ldo + n] = slim<DT>(v);
 }
 
-// How a call of more than eight rows is cut: 32 u rows and 32 w weight rows a tile,
-// and the ranges of k, as many as give each CU one. The ranges keep at least four
-// steps, and their sums at most 64 MB. (Two ranges a CU cost more to join than they
-// hide: us, one / two, 64 x 4096 x 14336 21.3 / 24.2, 16 x 4096 x 14336 14.6 / 16.9,
-// 64 x 14336 x 4096 20.3 / 21.4; where they are few anyway the same, 32 x 14336 x
-// 4096 15.7 / 15.8.)
+// How a call of more than eight rows is cut: 32 u rows and 32 w weight rows a tile.
+// With 128 rows a tile a CU holds one workgroup, and the tiles past the last whole
+// round of the GPU take ranges of k, as many as give each CU one and of at least four
+// steps (300 tiles of 353 x 25600 x 5120 gated: 117 to 124 us, 152 to 156 with a second round of
+// 44 tiles). Smaller tiles do so where they are fewer than the CUs. (Two ranges a CU
+// cost more to join than they hide: us, one / two, 64 x 4096 x 14336 21.3 / 24.2, 16 x
+// 4096 x 14336 14.6 / 16.9, 64 x 14336 x 4096 20.3 / 21.4; 32 x 14336 x 4096 15.7 /
+// 15.8.)
 struct W4Plan {
   int u, w, mtiles, splits;
-  int64_t tiles;
+  int64_t whole, rest;   // tiles with all of k, and tiles in `splits` ranges
+  int64_t rows() const { return 32 * u; }
+  int64_t cols() const { return 32 * w; }
 };
 
 static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int cus) {
   W4Plan q;
   q.u = m > 64 ? 4 : m > 32 ? 2 : 1;
   q.w = q.u == 4 ? 8 : 4;
-  q.mtiles = (int)((m + 32 * q.u - 1) / (32 * q.u));
-  q.tiles = (n + 32 * q.w - 1) / (32 * q.w) * q.mtiles;
-  const int64_t steps = (k + 127) / 128, want = cus;
-  int64_t s = q.tiles < want ? want / q.tiles : 1;
-  if (s > steps / 4) s = steps / 4;
-  const int64_t most = (64ll << 20) / (4 * m * n);
-  if (s > most) s = most;
+  q.mtiles = (int)((m + q.rows() - 1) / q.rows());
+  const int64_t tiles = (n + q.cols() - 1) / q.cols() * q.mtiles, steps = (k + 127) / 128;
+  q.rest = q.u == 4 || tiles < cus ? tiles % cus : 0;
+  const int64_t s = q.rest ? std::min(cus / q.rest, steps / 4) : 1;
   q.splits = s < 2 ? 1 : (int)s;
+  if (q.splits == 1) q.rest = 0;
+  q.whole = tiles - q.rest;
   return q;
 }
 
@@ -715,19 +730,19 @@ static void launch_w4_plan(const W4Params& p, const W4Plan& q, void* workspace, 
   if (DT == kBF16 && U == 4)
     hipLaunchKernelGGL((w4_sums_kernel<DT, GB>), dim3((unsigned)std::min((p.m * (p.k / 8) + 255) / 256, kSumsBlocks)),
                        dim3(256), 0, stream, p, sums);
-  const int64_t items = q.tiles * q.splits;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8));
+  const dim3 grid((unsigned)((q.whole + 7) / 8 * 8 + (q.rest * q.splits + 7) / 8 * 8));
   hipLaunchKernelGGL((linear_w4_tiles_kernel<DT, GB, U, W, GATED>), grid, dim3(64 * W), 0, stream, p, sums, parts,
-                     q.mtiles, (int)q.tiles, q.splits);
-  if (q.splits > 1)
-    hipLaunchKernelGGL((linear_w4_join_kernel<DT>), dim3((unsigned)(((GATED ? p.n / 2 : p.n) + 255) / 256), (unsigned)p.m),
-                       dim3(256), 0, stream, p, parts, q.splits, GATED);
+                     q.mtiles, (int)q.whole, (int)q.rest, q.splits);
+  if (q.rest)
+    hipLaunchKernelGGL((linear_w4_join_kernel<DT, U, W, GATED>),
+                       dim3((unsigned)(q.rest * (32 * U * (GATED ? 16 * W : 32 * W) / 256))), dim3(256), 0, stream, p,
+                       parts, q.mtiles, (int)q.whole, (int)q.rest, q.splits);
 }
 
 template <int DT, int GB, bool GATED>
 static int launch_w4_tiles(const W4Params& p, void* workspace, hipStream_t stream) {
   const W4Plan q = w4_plan(p.m, p.n, p.k, current_device_cus());
-  W8A8_REQUIRE(q.tiles < ((int64_t)1 << 22) && p.n < (1 << 30) && p.ldx < (1 << 22) && p.ldw < (1 << 22),
+  W8A8_REQUIRE(q.whole + q.rest < ((int64_t)1 << 22) && p.n < (1 << 30) && p.ldx < (1 << 22) && p.ldw < (1 << 22),
                "w8a8_linear_w4: too many outputs, or rows too long, for more than eight rows of x");
   switch (q.u) {
     case 4: launch_w4_plan<DT, GB, 4, 8, GATED>(p, q, workspace, stream); break;
@@ -769,7 +784,7 @@ extern "C" int64_t w8a8_linear_w4_workspace_size(int64_t m, int64_t n, int64_t k
   using namespace w8a8;
   if (!w4_tiled(m) || n <= 0 || k <= 0 || group <= 0) return 0;
   const W4Plan q = w4_plan(m, n, k, current_device_cus());
-  return w4_sums_bytes(q, m, k, group) + (q.splits > 1 ? 4 * (int64_t)q.splits * m * n : 0);
+  return w4_sums_bytes(q, m, k, group) + 4 * q.splits * q.rest * q.rows() * q.cols();
 }
 
 extern "C" int w8a8_linear_w4(const W8A8LinearW4Args* a) {

@@ -86,6 +86,17 @@ def test_where_the_kernels_change(gpu, m, group, dtype, k):
     assert_close(y, exact, slack, 'outputs')
 
 
+@pytest.mark.parametrize('n,dtype,residual,gated', [(35837, F16, True, False), (35830, BF16, False, True)])
+def test_more_tiles_than_a_round(gpu, n, dtype, residual, gated):
+    # Whole tiles first, the last round's in ranges of k: 2 x 140 tiles of 128 x 256.
+    print(f'linear_w4 130x{n}x1024 {dtype} {residual} {gated}', flush=True)
+    codes, s = _case(130, n, 1024, 128, dtype, True, True, residual, gpu)
+    y = _call(codes, s, gated)
+    exact, slack = exact_w4(s['x'], codes, s['scales'], s['zeros'], bias=s['bias'], residual=s['residual'], gated=gated)
+    assert_close(y, exact, slack, 'outputs')
+    assert torch.equal(y, _call(codes, s, gated))
+
+
 def test_broadcast_residual(gpu):
     codes, s = _case(5, 64, 256, 128, F16, False, False, True, gpu)
     row = s['residual'][:1]
