@@ -582,6 +582,13 @@ def _no_gradient(*tensors):
                 raise ValueError('this operator has no gradient: detach its inputs or run under torch.no_grad()')
 
 
+def _call_on(device, name, args):
+    """_abi.call with the tensors' device as the current one: a launch, and its
+    choice by the number of CUs, belong to it."""
+    with torch.cuda.device(device):
+        _abi.call(name, args)
+
+
 def _vector(t, name, n):
     """fp32 [n] contiguous and 16-byte aligned (None stays None)."""
     if t is None:
@@ -685,7 +692,7 @@ def residual_norm(x, branch, *, weight=None, eps=None, post_weight=None, post_ep
         mod_rows=shift.shape[0] if shift is not None else 0, eps=float(eps or 0.0), y=_abi.ptr(y), ldy=cols,
         convrot=256 if quantize and convrot else 0, round_rotated=1 if round_rotated else 0, q=_abi.ptr(q), ldq=cols,
         q_scale=_abi.ptr(qs), convrot_signs=_abi.ptr(signs), stream=_abi.stream_of(x))
-    _abi.call('w8a8_residual_norm', args)
+    _call_on(x.device, 'w8a8_residual_norm', args)
     return res
 
 
@@ -771,7 +778,7 @@ def axial_rope(q, k, positions, inv_freq, axis, *, adjacent=False, q_gain=None, 
         positions=positions.data_ptr(), pos_strides=tuple(positions.stride()),
         pos_type=_POSITION_TYPES[positions.dtype], eps=float(eps), inv_freq=inv_freq.data_ptr(),
         axis=axis.data_ptr(), q_gain=_abi.ptr(q_gain), k_gain=_abi.ptr(k_gain), stream=_abi.stream_of(q))
-    _abi.call('w8a8_axial_rope', args)
+    _call_on(q.device, 'w8a8_axial_rope', args)
     return q_out, k_out
 
 
@@ -795,7 +802,7 @@ def axial_freqs(positions, inv_freq, axis, *, dtype=torch.float16, pairs_layout=
         pos_strides=tuple(positions.stride()), rows=rows, pairs=n, axes=positions.shape[1],
         inv_freq=inv_freq.data_ptr(), axis=axis.data_ptr(), freqs=freqs.data_ptr(),
         stream=_abi.stream_of(positions))
-    _abi.call('w8a8_axial_freqs', args)
+    _call_on(positions.device, 'w8a8_axial_freqs', args)
     return freqs
 
 
@@ -864,5 +871,5 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
         ldr=residual.stride(0) if residual is not None and m > 1 else n,
         out=y.data_ptr(), ldo=y.stride(0) if m > 1 else width, workspace=_abi.ptr(ws), workspace_bytes=nbytes,
         stream=_abi.stream_of(x))
-    _abi.call('w8a8_linear_w4', args)
+    _call_on(x.device, 'w8a8_linear_w4', args)
     return y if out is not None else y.reshape(*lead, width)

@@ -18,6 +18,13 @@ from . import _abi, kernels
 _NIBBLE_OF_INPUT = (0, 4, 1, 5, 2, 6, 3, 7)
 
 
+def _check_groups(features, group_size):
+    if group_size not in (32, 64) and (group_size <= 0 or group_size % 128):
+        raise ValueError('group sizes are 32, 64 and multiples of 128')
+    if features <= 0 or features % group_size:
+        raise ValueError('the input features must be a positive multiple of the group size')
+
+
 def pack(codes):
     """int32 [N, K / 8] words of codes [N, K] (integers 0 to 15)."""
     if codes.ndim != 2 or codes.shape[1] % 8 or codes.is_floating_point():
@@ -43,10 +50,9 @@ def quantize_weight(weight, group_size=128, *, symmetric=True, dtype=torch.float
     group of group_size inputs, with the scale already rounded to dtype.
     symmetric: scale = absmax / 7, zeros None (8); else the group's range,
     widened to hold 0, over 15 steps with a zero of its own."""
-    if weight.ndim != 2 or weight.shape[1] % group_size or weight.shape[1] == 0:
-        raise ValueError('weight must be [N, K] with K a multiple of the group size')
-    if group_size not in (32, 64) and group_size % 128:
-        raise ValueError('group sizes are 32, 64 and multiples of 128')
+    if weight.ndim != 2:
+        raise ValueError('weight must be [N, K]')
+    _check_groups(weight.shape[1], group_size)
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError('scales must be float16 or bfloat16')
     n, k = weight.shape
@@ -87,8 +93,9 @@ class LinearW4(nn.Module):
     def __init__(self, in_features, out_features, *, group_size=128, zeros=False, bias=False, gated=False,
                  dtype=torch.float16, device=None):
         super().__init__()
-        if in_features % group_size or (group_size not in (32, 64) and group_size % 128):
-            raise ValueError('group sizes are 32, 64 and multiples of 128, and divide the input features')
+        _check_groups(in_features, group_size)
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError('scales must be float16 or bfloat16')
         if gated and out_features % 2:
             raise ValueError('a gated projection has gate and up halves')
         self.in_features, self.out_features, self.group_size, self.gated = in_features, out_features, group_size, gated

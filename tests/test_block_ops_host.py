@@ -191,6 +191,21 @@ def test_linear_w4_many_rows_offsets_fit_32_bits(change):
     _refused('w8a8_linear_w4', _abi.LinearW4Args(**case), 'too long')
 
 
+@pytest.mark.parametrize('group', [0, -128, 16, 192])
+def test_group_sizes_are_refused(group):
+    with pytest.raises(ValueError):
+        linear_w4.quantize_weight(torch.zeros((4, 768)), group)
+    with pytest.raises(ValueError):
+        linear_w4.LinearW4(768, 4, group_size=group, device='cpu')
+
+
+@pytest.mark.parametrize('features,kw', [(0, {}), (100, {}), (256, dict(dtype=torch.float32)),
+                                         (256, dict(gated=True))])
+def test_modules_are_refused(features, kw):
+    with pytest.raises(ValueError):
+        linear_w4.LinearW4(features, 5, device='cpu', **kw)
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros((2, 256), dtype=torch.float16)
     with pytest.raises(ValueError):
