@@ -593,7 +593,8 @@ int w8a8_residual_norm(const W8A8ResidualNormArgs* args);
  * All in fp32 (products and sums contracted to FMAs as written in the
  *   kernel), rounded once at the end.
  * Requirements: 2 <= dim <= 256 and even, 1 <= pairs <= dim / 2,
- *   1 <= axes <= 16; every array aligned to its elements.
+ *   1 <= axes <= 16; rows < 2^24; at most 4096 heads each; every array
+ *   aligned to its elements.
  */
 enum { W8A8_ROPE_HALF = 0, W8A8_ROPE_ADJACENT = 1 };
 enum { W8A8_POS_I32 = 0, W8A8_POS_I64 = 1, W8A8_POS_F32 = 2 };
