@@ -647,42 +647,41 @@ void linear_w4_tiles_kernel(W4Params p, const uint2* sums, float* parts, int mti
   store_tile<DT, U, GATED>(p, tot, part, 32 * W, m0, n0, mrows, nrows, wr, ncol, c, h);
 }
 
-// The outputs of the split tiles: the ranges' sums in order, then the epilogue. One
-// output a thread.
+// The outputs of the split tiles: the ranges' sums in order, then the epilogue. Four
+// neighbouring outputs of a row a thread.
 template <int DT, int U, int W, bool GATED>
 __global__ __launch_bounds__(256)
 void linear_w4_join_kernel(W4Params p, const float* parts, int mtiles, int whole, int rest, int splits) {
-  constexpr int BN = GATED ? 16 * W : 32 * W, BLOCKS = 32 * U * BN / 256;
+  constexpr int BN = GATED ? 16 * W : 32 * W, BLOCKS = 32 * U * BN / 1024;
   const int64_t width = GATED ? p.n / 2 : p.n;
   const int left = blockIdx.x / BLOCKS, tile = whole + left;
-  const int i = (blockIdx.x - left * BLOCKS) * 256 + threadIdx.x, row = i / BN, col = i - row * BN;
+  const int i = (blockIdx.x - left * BLOCKS) * 256 + threadIdx.x, row = i / (BN / 4), col = 4 * (i - row * (BN / 4));
   const int64_t m = (int64_t)(tile % mtiles) * (32 * U) + row, n = (int64_t)(tile / mtiles) * BN + col;
   if (m >= p.m || n >= width) return;
   const int64_t stride = (int64_t)rest * (32 * U * 32 * W);
   const float* at = parts + ((int64_t)left * (32 * U) + row) * (32 * W) + (GATED ? 32 * (col / 16) + col % 16 : col);
-  float v = at[0], up = GATED ? at[16] : 0.0f;
+  auto of = [&](int s, int half) { return *reinterpret_cast<const v4f*>(at + s * stride + 16 * half); };
+  v4f v = of(0, 0), up = {};
+  if constexpr (GATED) up = of(0, 1);
   int s = 1;
   for (; s + 4 <= splits; s += 4) {   // (four loads at once)
-    float a[4], b[4];
+    v4f a[4], b[4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = at[(s + i) * stride];
-      b[i] = GATED ? at[(s + i) * stride + 16] : 0.0f;
+    for (int j = 0; j < 4; ++j) {
+      a[j] = of(s + j, 0);
+      if constexpr (GATED) b[j] = of(s + j, 1);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v = v + a[i];
-      up = up + b[i];
+    for (int j = 0; j < 4; ++j) {
+      v = v + a[j];
+      if constexpr (GATED) up = up + b[j];
     }
   }
   for (; s < splits; ++s) {
-    v = v + at[s * stride];
-    if (GATED) up = up + at[s * stride + 16];
+    v = v + of(s, 0);
+    if constexpr (GATED) up = up + of(s, 1);
   }
-  if (p.bias) v = v + wide<DT>(p.bias[n]);
-  if (GATED) v = swiglu(v, p.bias ? up + wide<DT>(p.bias[width + n]) : up);
-  if (p.residual) v = v + wide<DT>(p.residual[m * p.ldr + n]);
-  p.out[m * p.ldo + n] = slim<DT>(v);
+  finish4<DT, GATED>(p, m, n, width, v, up);
 }
 
 // How a call of more than eight rows is cut: 32 u rows and 32 w weight rows a tile.
@@ -735,7 +734,7 @@ static void launch_w4_plan(const W4Params& p, const W4Plan& q, void* workspace, 
                      q.mtiles, (int)q.whole, (int)q.rest, q.splits);
   if (q.rest)
     hipLaunchKernelGGL((linear_w4_join_kernel<DT, U, W, GATED>),
-                       dim3((unsigned)(q.rest * (32 * U * (GATED ? 16 * W : 32 * W) / 256))), dim3(256), 0, stream, p,
+                       dim3((unsigned)(q.rest * (32 * U * (GATED ? 16 * W : 32 * W) / 1024))), dim3(256), 0, stream, p,
                        parts, q.mtiles, (int)q.whole, (int)q.rest, q.splits);
 }
 
