@@ -581,8 +581,9 @@ int w8a8_residual_norm(const W8A8ResidualNormArgs* args);
  *   its own input (same strides), and may not otherwise overlap an input.
  * positions: [rows, axes] of pos_type, element strides {row, axis}.
  * inv_freq: [pairs] fp64, axis: [pairs] int32 in [0, axes) (clamped); pair p
- *   of a row turns by phi = position[axis[p]] * inv_freq[p], in fp64 to the
- *   fraction of a revolution, whose sine and cosine are fp32:
+ *   of a row turns by phi = position[axis[p]] * inv_freq[p], in fp64 down to
+ *   the nearest quarter turn, whose rest is rounded to fp32; sine and cosine
+ *   are fp32, within 1.3 * 2^-24:
  *   (a, b) -> (a cos - b sin, b cos + a sin), where (a, b) is
  *   W8A8_ROPE_HALF:     (x[p], x[p + pairs])
  *   W8A8_ROPE_ADJACENT: (x[2p], x[2p + 1])

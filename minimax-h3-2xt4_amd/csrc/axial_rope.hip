@@ -4,7 +4,8 @@
 //
 // The angle is needed modulo a revolution, so it is taken in fp64 (position
 // 10^6 times one radian is 1.6 * 10^5 revolutions: fp64 leaves 10^-10 of one,
-// fp32 would leave a hundredth) and its fraction's sine and cosine in fp32.
+// fp32 would leave a hundredth) down to the nearest quarter; what is left is
+// rounded to fp32, for its sine and cosine.
 // Each angle serves all heads of its row: a workgroup takes a row, puts its
 // angles into LDS and turns all its heads from there.
 //
@@ -50,12 +51,14 @@ __device__ __forceinline__ double position_of(const AxTable& t, int64_t row, int
   return (double)reinterpret_cast<const float*>(t.positions)[i];
 }
 
-// Sine and cosine of 2 pi f for a fraction |f| <= 1/2: the nearest quarter is
-// taken off (exact), which leaves |x| <= pi / 4, where the Taylor series to
-// x^9 and x^10 are within 2^-29 of sine and cosine.
-__device__ __forceinline__ float2 cos_sin_turns(float f) {
-  const float n = rintf(4.0f * f);
-  const float x = (f - 0.25f * n) * 6.28318530717958648f;
+// Cosine and sine of 2 pi t: whole turns and the nearest quarter are taken off
+// (exact), which leaves |x| <= pi / 4, rounded here to fp32 (2^-25), where the
+// Taylor series to x^9 and x^10 are within 2^-29 of sine and cosine. With the
+// roundings of their sums both are within 1.3 * 2^-24. (Rounded before the
+// quarter is off, the fraction alone would be 2^-23.3 off.)
+__device__ __forceinline__ float2 cos_sin_turns(double t) {
+  const double f = t - rint(t), n = rint(4.0 * f);
+  const float x = (float)((f - 0.25 * n) * 6.28318530717958647693);
   const float z = x * x;
   float s = __builtin_fmaf(z, 1.0f / 362880.0f, -1.0f / 5040.0f);
   s = __builtin_fmaf(z, s, 1.0f / 120.0f);
@@ -75,7 +78,7 @@ __device__ __forceinline__ float2 cos_sin_turns(float f) {
 __device__ __forceinline__ float2 rotation_of(const AxTable& t, int64_t row, int pair) {
   const int axis = min(max(t.axis[pair], 0), t.axes - 1);
   const double turns = position_of(t, row, axis) * t.inv_freq[pair] * 0.15915494309189533577;
-  return cos_sin_turns((float)(turns - rint(turns)));
+  return cos_sin_turns(turns);
 }
 
 template <typename T, int N>
