@@ -45,11 +45,24 @@ def unpack(words):
     return ((words[:, :, None] >> shifts) & 15).to(torch.uint8).reshape(words.shape[0], -1)
 
 
+def _scales(step, dtype):
+    """Steps (fp32) as values of dtype, never 0: to the nearest, but in the subnormal
+    range (where that may be a good part of a step) never below."""
+    info = torch.finfo(dtype)
+    spacing = info.smallest_normal * info.eps
+    scale = step.to(dtype).float()
+    short = (scale < step) & (scale < info.smallest_normal)
+    return torch.where(short, scale + spacing, scale).clamp_min(spacing)
+
+
 def quantize_weight(weight, group_size=128, *, symmetric=True, dtype=torch.float16):
     """(codes, scales, zeros) of a weight [N, K]: round to nearest within each
     group of group_size inputs, with the scale already rounded to dtype.
     symmetric: scale = absmax / 7, zeros None (8); else the group's range,
-    widened to hold 0, over 15 steps with a zero of its own."""
+    widened to hold 0, over 15 steps with a zero of its own. Scales may be
+    subnormal, so that small weights (those that carry a residual divisor, say)
+    keep their steps: below the smallest normal a scale that would fall short is
+    the next one up, at most one spacing (2^-24 in fp16) more."""
     if weight.ndim != 2:
         raise ValueError('weight must be [N, K]')
     _check_groups(weight.shape[1], group_size)
@@ -57,13 +70,12 @@ def quantize_weight(weight, group_size=128, *, symmetric=True, dtype=torch.float
         raise ValueError('scales must be float16 or bfloat16')
     n, k = weight.shape
     w = weight.detach().float().reshape(n, k // group_size, group_size)
-    tiny = torch.finfo(dtype).tiny
     if symmetric:
-        scale = (w.abs().amax(-1) / 7).to(dtype).float().clamp_min(tiny)
+        scale = _scales(w.abs().amax(-1) / 7, dtype)
         zero = torch.full_like(scale, 8)
     else:
         low, high = w.amin(-1).clamp_max(0), w.amax(-1).clamp_min(0)
-        scale = ((high - low) / 15).to(dtype).float().clamp_min(tiny)
+        scale = _scales((high - low) / 15, dtype)
         zero = (-low / scale).round().clamp(0, 15)
     codes = ((w / scale[:, :, None]).round() + zero[:, :, None]).clamp(0, 15).to(torch.uint8)
     return (pack(codes.reshape(n, k)), scale.t().contiguous().to(dtype),

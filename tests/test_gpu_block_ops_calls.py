@@ -3,7 +3,8 @@ operator do not make."""
 import pytest
 import torch
 
-from w8a8 import axial_rope
+from block_refs import assert_close, linear_w4 as exact_w4
+from w8a8 import axial_rope, linear_w4
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +24,24 @@ def test_sine_and_cosine_keep_their_bits(gpu, rows, sections, far):
     for got, exact in ((f[..., 0, 0], phi.cos()), (f[..., 1, 0], phi.sin()), (f[..., 0, 1], -phi.sin()),
                        (f[..., 1, 1], phi.cos())):
         assert bool(((got - exact).abs() <= bound).all()), float((got - exact).abs().max())
+
+
+@pytest.mark.parametrize('m', [1, 8, 30, 64, 130])
+@pytest.mark.parametrize('group,zeros', [(32, False), (64, True), (128, True)])
+def test_subnormal_scales(gpu, m, group, zeros):
+    """FP16 scales below 2^-14, as small weights have them, keep their value."""
+    g = torch.Generator().manual_seed(m)
+    n, k = 72, 384
+    codes = torch.randint(0, 16, (n, k), generator=g)
+    scales = (torch.randint(1, 1024, (k // group, n), generator=g).float() * 2.0 ** -24).half()
+    assert float(scales.max()) < 2.0 ** -14 and float(scales.min()) > 0
+    z = torch.randint(0, 16, (k // group, n), generator=g).to(torch.uint8) if zeros else None
+    x = (torch.randn((m, k), generator=g) * 300).half()
+    args = [t.to(gpu) if t is not None else None for t in (x, codes, scales, z)]
+    y = linear_w4.linear(args[0], linear_w4.pack(args[1]), args[2], args[3])
+    assert_close(y, *exact_w4(*args), 'outputs')
+    w = (torch.randn((n, k), generator=g) * 0.02).to(gpu)
+    mod = linear_w4.LinearW4(k, n, group_size=group, zeros=zeros, device=gpu).load_weight(w / 512)
+    assert float(mod.scales.max()) < 2.0 ** -14
+    y = mod(args[0])
+    assert_close(y, *exact_w4(args[0], linear_w4.unpack(mod.codes), mod.scales, mod.zeros), 'module')
