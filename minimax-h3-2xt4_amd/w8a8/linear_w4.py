@@ -77,6 +77,8 @@ def quantize_weight(weight, group_size=128, *, symmetric=True, dtype=torch.float
         low, high = w.amin(-1).clamp_max(0), w.amax(-1).clamp_min(0)
         scale = _scales((high - low) / 15, dtype)
         zero = (-low / scale).round().clamp(0, 15)
+    if not bool(torch.isfinite(scale).all()):
+        raise ValueError(f'weights that are not finite, or whose scale {dtype} does not hold')
     codes = ((w / scale[:, :, None]).round() + zero[:, :, None]).clamp(0, 15).to(torch.uint8)
     return (pack(codes.reshape(n, k)), scale.t().contiguous().to(dtype),
             None if symmetric else zero.t().contiguous().to(torch.uint8))

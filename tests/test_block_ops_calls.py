@@ -29,3 +29,14 @@ def test_small_weights_keep_their_steps(dtype, symmetric, size):
     step = ideal * (1 + info.eps / 2) + info.smallest_normal * info.eps
     assert bool(((groups - back).abs() <= step * (0.5 + 15 * info.eps / 2) * (1 + 2.0 ** -20)).all())
     assert bool((back[5, 0] == 0).all()) and bool((scales > 0).all())
+
+
+@pytest.mark.parametrize('symmetric', [True, False])
+@pytest.mark.parametrize('value', [float('nan'), float('inf'), -float('inf'), 1e6])
+def test_weights_past_the_scales_are_refused(symmetric, value):
+    w = torch.ones((4, 128))
+    w[2, 70] = value
+    with pytest.raises(ValueError, match='scale'):
+        linear_w4.quantize_weight(w, 64, symmetric=symmetric)
+    if value == 1e6:
+        linear_w4.quantize_weight(w, 64, symmetric=symmetric, dtype=torch.bfloat16)
