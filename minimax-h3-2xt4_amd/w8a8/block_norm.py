@@ -39,12 +39,14 @@ def update_and_prepare(x, branch, gate, segments, norm, shift, scale, *, post_no
     row_scale)), the codes being modulated_norm_quantize(norm, x', shift,
     scale, segments)'s. gate, shift and scale are [R, hidden] modulation
     tables, segments [(a, b, row)] tile the rows, norm is the next sublayer's
-    and post_norm the branch's own RMSNorm (or None)."""
+    and post_norm the branch's own RMSNorm (or None). Inference only: the norms'
+    weights are taken as constants, any other input that requires a gradient is
+    refused."""
     weight, eps, labels, shift, scale = _norm_args(norm, x, shift, scale, segments)
     post_weight = post_eps = None
     if post_norm is not None:
         post_weight, post_eps, _, _, _ = _norm_args(post_norm, x, None, None, None)
-    r = kernels.residual_norm(x, branch.detach(), weight=weight, eps=eps, post_weight=post_weight, post_eps=post_eps,
-                              gate=gate.detach().float(), shift=shift, scale=scale, labels=labels,
+    r = kernels.residual_norm(x, branch, weight=weight, eps=eps, post_weight=post_weight, post_eps=post_eps,
+                              gate=gate.float(), shift=shift, scale=scale, labels=labels,
                               branch_scale=branch_scale, quantize=True, convrot=convrot, out=out)
     return r['x'], (r['q'], r['scale'])

@@ -3,7 +3,7 @@ and the 4-bit quantizer's range."""
 import pytest
 import torch
 
-from w8a8 import linear_w4
+from w8a8 import block_norm, linear_w4
 
 
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
@@ -40,3 +40,19 @@ def test_weights_past_the_scales_are_refused(symmetric, value):
         linear_w4.quantize_weight(w, 64, symmetric=symmetric)
     if value == 1e6:
         linear_w4.quantize_weight(w, 64, symmetric=symmetric, dtype=torch.bfloat16)
+
+
+def _update_args(rows=4, hidden=256, table_rows=3):
+    x = torch.zeros((rows, hidden), dtype=torch.float16)
+    tables = [torch.zeros((table_rows, hidden)) for _ in range(3)]
+    return [x, torch.zeros_like(x), tables[0], [(0, rows, 1)], torch.nn.RMSNorm(hidden, eps=1e-6), tables[1], tables[2]]
+
+
+@pytest.mark.parametrize('which', [0, 1, 2, 5, 6])
+def test_update_and_prepare_loses_no_gradient(which):
+    args = _update_args()
+    args[which] = args[which].requires_grad_()
+    with pytest.raises(ValueError, match='no gradient'):
+        block_norm.update_and_prepare(*args)
+    with torch.no_grad(), pytest.raises(ValueError, match='HIP device'):
+        block_norm.update_and_prepare(*args)
