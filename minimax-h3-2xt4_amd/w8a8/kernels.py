@@ -574,8 +574,9 @@ def attention(prep, *, out_dtype=torch.float16, out=None):
 
 
 def _no_gradient(*tensors):
-    """The operators below have no backward pass (nothing here trains): an
-    input that asks for one is refused, so that no gradient is lost silently."""
+    """The operators below have no backward pass (nothing here trains): an input
+    or a given output that asks for one is refused, so that no gradient is lost
+    silently."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -631,7 +632,7 @@ def residual_norm(x, branch, *, weight=None, eps=None, post_weight=None, post_ep
     may be x itself), and with eps 'y' (unless quantize without
     want_normalized) and, when quantize, 'q' and 'scale'.
     """
-    _no_gradient(x, branch, weight, post_weight, gate, shift, scale)
+    _no_gradient(x, branch, weight, post_weight, gate, shift, scale, out)
     _device(x, branch, weight, post_weight, gate, shift, scale, labels, signs, out)
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError('x must be float16 or bfloat16')
@@ -817,7 +818,7 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
     [.., N / 2]. out: [rows, width] in x's dtype to write into; it may be the
     residual itself.
     """
-    _no_gradient(x, codes, scales, bias, residual)
+    _no_gradient(x, codes, scales, bias, residual, out)
     _device(x, codes, scales, zeros, bias, residual, out)
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError('x must be float16 or bfloat16')

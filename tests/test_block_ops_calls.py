@@ -56,3 +56,12 @@ def test_update_and_prepare_loses_no_gradient(which):
         block_norm.update_and_prepare(*args)
     with torch.no_grad(), pytest.raises(ValueError, match='HIP device'):
         block_norm.update_and_prepare(*args)
+
+
+def test_outputs_that_want_a_gradient_are_refused():
+    x = torch.zeros((2, 256), dtype=torch.float16)
+    with pytest.raises(ValueError, match='no gradient'):
+        block_norm.residual_norm(x, x.clone(), out=torch.zeros_like(x, requires_grad=True))
+    out = torch.zeros((2, 16), dtype=torch.float16, requires_grad=True)
+    with pytest.raises(ValueError, match='no gradient'):
+        linear_w4.linear(x, torch.zeros((16, 32), dtype=torch.int32), torch.ones((2, 16), dtype=torch.float16), out=out)
