@@ -332,11 +332,12 @@ bool optional_float(PyObject* o, float& v, bool& given) {
   return true;
 }
 
-// Whether a gradient would be asked of a tensor: the Python route refuses it.
+// Whether a gradient, backward or forward, would be asked of a tensor: the Python
+// route refuses it.
 bool wants_gradient(std::initializer_list<const at::Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool grad = at::GradMode::is_enabled();
   for (const at::Tensor* t : ts)
-    if (t && t->requires_grad()) return true;
+    if (t && ((grad && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
   return false;
 }
 

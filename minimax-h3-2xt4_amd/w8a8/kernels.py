@@ -8,6 +8,7 @@ contract violation; a failing library call raises W8A8Error.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi
 from ._abi import EPI_COLUMN, EPI_INT32, EPI_ROW  # noqa: F401
@@ -576,11 +577,15 @@ def attention(prep, *, out_dtype=torch.float16, out=None):
 def _no_gradient(*tensors):
     """The operators below have no backward pass (nothing here trains): an input
     or a given output that asks for one is refused, so that no gradient is lost
-    silently."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError('this operator has no gradient: detach its inputs or run under torch.no_grad()')
+    silently. A forward-mode tangent is one too, also under no_grad."""
+    grad = torch.is_grad_enabled()
+    forward = forward_ad._current_level >= 0   # (tensors have tangents inside a level only)
+    if not (grad or forward):
+        return
+    for t in tensors:
+        if t is not None and ((grad and t.requires_grad) or
+                              (forward and forward_ad.unpack_dual(t).tangent is not None)):
+            raise ValueError('this operator has no gradient: detach its inputs or run under torch.no_grad()')
 
 
 def _call_on(device, name, args):

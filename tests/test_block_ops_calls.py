@@ -2,8 +2,9 @@
 and the 4-bit quantizer's range."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from w8a8 import block_norm, linear_w4
+from w8a8 import axial_rope, block_norm, linear_w4
 
 
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
@@ -65,3 +66,29 @@ def test_outputs_that_want_a_gradient_are_refused():
     out = torch.zeros((2, 16), dtype=torch.float16, requires_grad=True)
     with pytest.raises(ValueError, match='no gradient'):
         linear_w4.linear(x, torch.zeros((16, 32), dtype=torch.int32), torch.ones((2, 16), dtype=torch.float16), out=out)
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor has requires_grad False, and no_grad does not stop its tangent."""
+    x = torch.zeros((2, 256), dtype=torch.float16)
+    q = torch.zeros((2, 4, 128), dtype=torch.float16)
+    inv, axis = axial_rope.ladder((16, 16, 16))
+    pos = torch.zeros((2, 3))
+    codes, scales = torch.zeros((16, 32), dtype=torch.int32), torch.ones((2, 16), dtype=torch.float16)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: block_norm.residual_norm(dual(x), x, eps=1e-6),
+                 lambda: block_norm.residual_norm(x, x, eps=1e-6, weight=dual(torch.ones(256))),
+                 lambda: axial_rope.rotate(dual(q), None, pos, inv, axis),
+                 lambda: axial_rope.rotate(q, None, dual(pos), inv, axis),
+                 lambda: axial_rope.freqs(dual(pos), inv, axis),
+                 lambda: linear_w4.linear(dual(x), codes, scales),
+                 lambda: linear_w4.linear(x, codes, dual(scales))]
+        for call in calls:
+            with pytest.raises(ValueError, match='no gradient'):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match='no gradient'):
+                call()
+    with pytest.raises(ValueError, match='HIP device'):
+        block_norm.residual_norm(x, x, eps=1e-6)

@@ -2,9 +2,10 @@
 operator do not make."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from block_refs import assert_close, linear_w4 as exact_w4
-from w8a8 import axial_rope, linear_w4
+from w8a8 import axial_rope, block_norm, linear_w4
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +46,27 @@ def test_subnormal_scales(gpu, m, group, zeros):
     assert float(mod.scales.max()) < 2.0 ** -14
     y = mod(args[0])
     assert_close(y, *exact_w4(args[0], linear_w4.unpack(mod.codes), mod.scales, mod.zeros), 'module')
+
+
+def test_forward_mode_tangents_are_refused(gpu):
+    x = torch.zeros((2, 256), dtype=torch.float16, device=gpu)
+    q = torch.zeros((2, 4, 128), dtype=torch.float16, device=gpu)
+    inv, axis = axial_rope.ladder((16, 16, 16), device=gpu)
+    pos = torch.zeros((2, 3), device=gpu)
+    codes = torch.zeros((16, 32), dtype=torch.int32, device=gpu)
+    scales = torch.ones((2, 16), dtype=torch.float16, device=gpu)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: block_norm.residual_norm(dual(x), x, eps=1e-6),
+                     lambda: block_norm.residual_norm(x, x, eps=1e-6, weight=dual(torch.ones(256, device=gpu))),
+                     lambda: block_norm.residual_norm(x, x, out=dual(x)),
+                     lambda: axial_rope.rotate(dual(q), None, pos, inv, axis),
+                     lambda: axial_rope.freqs(dual(pos), inv, axis),
+                     lambda: linear_w4.linear(dual(x), codes, scales),
+                     lambda: linear_w4.linear(x, codes, scales, bias=dual(scales[0]))):
+            with pytest.raises(ValueError, match='no gradient'):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match='no gradient'):
+                call()
+        block_norm.residual_norm(x, x, eps=1e-6)
