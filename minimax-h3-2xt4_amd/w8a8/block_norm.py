@@ -42,6 +42,8 @@ def update_and_prepare(x, branch, gate, segments, norm, shift, scale, *, post_no
     and post_norm the branch's own RMSNorm (or None). Inference only: the norms'
     weights are taken as constants, any other input that requires a gradient is
     refused."""
+    if gate.ndim != 2 or shift.shape != gate.shape or scale.shape != gate.shape:
+        raise ValueError('gate, shift and scale must be tables [R, hidden] of the same rows')
     weight, eps, labels, shift, scale = _norm_args(norm, x, shift, scale, segments)
     post_weight = post_eps = None
     if post_norm is not None:

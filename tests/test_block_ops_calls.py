@@ -92,3 +92,11 @@ def test_forward_mode_tangents_are_refused():
                 call()
     with pytest.raises(ValueError, match='HIP device'):
         block_norm.residual_norm(x, x, eps=1e-6)
+
+
+def test_modulation_tables_share_their_rows():
+    """The segments name one row of gate, shift and scale alike."""
+    args = _update_args()
+    args[2] = args[2][:1]
+    with pytest.raises(ValueError, match='same rows'):
+        block_norm.update_and_prepare(*args)
