@@ -42,7 +42,7 @@ def update_and_prepare(x, branch, gate, segments, norm, shift, scale, *, post_no
     and post_norm the branch's own RMSNorm (or None). Inference only: the norms'
     weights are taken as constants, any other input that requires a gradient is
     refused."""
-    if gate.ndim != 2 or shift.shape != gate.shape or scale.shape != gate.shape:
+    if any(t is None or t.ndim != 2 or t.shape != gate.shape for t in (gate, shift, scale)):
         raise ValueError('gate, shift and scale must be tables [R, hidden] of the same rows')
     weight, eps, labels, shift, scale = _norm_args(norm, x, shift, scale, segments)
     post_weight = post_eps = None

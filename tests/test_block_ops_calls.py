@@ -96,7 +96,8 @@ def test_forward_mode_tangents_are_refused():
 
 def test_modulation_tables_share_their_rows():
     """The segments name one row of gate, shift and scale alike."""
-    args = _update_args()
-    args[2] = args[2][:1]
-    with pytest.raises(ValueError, match='same rows'):
-        block_norm.update_and_prepare(*args)
+    for which, change in ((2, lambda t: t[:1]), (5, lambda t: t[0]), (6, lambda t: None), (2, lambda t: None)):
+        args = _update_args()
+        args[which] = change(args[which])
+        with pytest.raises(ValueError, match='same rows'):
+            block_norm.update_and_prepare(*args)
