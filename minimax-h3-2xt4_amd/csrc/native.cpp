@@ -577,12 +577,12 @@ PyObject* linear_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if ((group != 32 && group != 64 && group % 128) || (gated && (nn % 2 || residual)) ||
       (zeros && (zeros->scalar_type() != at::kByte || zeros->sizes() != scales->sizes() || !zeros->is_contiguous())) ||
       (bias && (bias->scalar_type() != type || bias->numel() != nn || !bias->is_contiguous())) ||
-      (residual && (residual->scalar_type() != type || residual->numel() != m * nn || residual->size(-1) != nn ||
-                    !residual->is_contiguous())))
+      (residual && (residual->scalar_type() != type || !residual->is_contiguous())))
     Py_RETURN_NONE;
   const auto opt = at::TensorOptions().device(x->device());
   at::DimVector shape(x->sizes().begin(), x->sizes().end());
   shape.back() = width;
+  if (residual && !residual->sizes().equals(shape) && !residual->sizes().equals({m, nn})) Py_RETURN_NONE;
   at::Tensor out = at::empty(shape, opt.dtype(type));
   W8A8LinearW4Args a{};
   at::Tensor workspace;

@@ -818,7 +818,8 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
     codes int32 [N, K / 8] (linear_w4.pack's words), scales [K / group, N] in
     x's dtype, zeros uint8 [K / group, N] (0 to 15) or None for 8:
     W[n, k] = scales[k // group, n] * (code[n, k] - zeros[k // group, n]).
-    bias [N] in x's dtype. residual [.., N] in x's dtype is added. gated: W's
+    bias [N] in x's dtype. residual [.., N] in x's dtype (x's leading sizes, or
+    all rows as [M, N]) is added. gated: W's
     first N / 2 rows are gate, the others up; returns silu(gate) * up
     [.., N / 2]. out: [rows, width] in x's dtype to write into; it may be the
     residual itself.
@@ -854,8 +855,8 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
     zeros = zeros.contiguous() if zeros is not None else None
     bias = bias.reshape(-1).contiguous() if bias is not None else None
     if residual is not None:
-        if residual.dtype != x.dtype or residual.numel() != m * n or residual.shape[-1] != n:
-            raise ValueError('residual must be [.., N] in x\'s dtype')
+        if residual.dtype != x.dtype or tuple(residual.shape) not in ((*lead, n), (m, n)):
+            raise ValueError('residual must be [.., N] in x\'s dtype, with x\'s leading sizes or one row for each of them')
         residual = residual.reshape(m, n)
         if (n > 1 and residual.stride(1) != 1) or (m > 1 and residual.stride(0) < n):
             residual = residual.contiguous()   # (a broadcast one too)

@@ -70,3 +70,20 @@ def test_forward_mode_tangents_are_refused(gpu):
             with torch.no_grad(), pytest.raises(ValueError, match='no gradient'):
                 call()
         block_norm.residual_norm(x, x, eps=1e-6)
+
+
+@pytest.mark.parametrize('out', [False, True])
+def test_residuals_of_other_rows_are_refused(gpu, out):
+    """A residual has x's leading sizes, or is the [rows, N] of all of them."""
+    x = torch.randn((2, 3, 256), device=gpu).half()
+    codes, scales, _ = linear_w4.quantize_weight(torch.randn((16, 256)))
+    codes, scales = codes.to(gpu), scales.to(gpu)
+    r = torch.randn((2, 3, 16), device=gpu).half()
+    kw = dict(out=torch.zeros((6, 16), dtype=torch.float16, device=gpu)) if out else {}
+    want = linear_w4.linear(x, codes, scales, residual=r)
+    assert torch.equal(linear_w4.linear(x, codes, scales, residual=r.view(6, 16), **kw).view(2, 3, 16), want)
+    assert torch.equal(linear_w4.linear(x, codes, scales, residual=r, **kw).view(2, 3, 16), want)
+    assert torch.equal(linear_w4.linear(x[0, 0], codes, scales, residual=r[0, :1]), want[0, 0])
+    for bad in (r.transpose(0, 1).contiguous(), r.view(6, 1, 16), r.view(1, 2, 3, 16)):
+        with pytest.raises(ValueError, match='residual'):
+            linear_w4.linear(x, codes, scales, residual=bad, **kw)
