@@ -682,8 +682,8 @@ int w8a8_axial_freqs(const W8A8AxialFreqsArgs* args);
  *   may, and a captured graph may replay it.
  * Requirements: group 32, 64 or a multiple of 128, k % group == 0; gated:
  *   n even, no residual; x and codes 16-byte aligned, ldx % 8 == 0,
- *   ldw % 4 == 0; m < 2^22; with more than eight rows n < 2^30, ldx and
- *   ldw < 2^22.
+ *   ldw % 4 == 0; m < 2^22; with up to eight rows n < 2^29, with more
+ *   n < 2^30, ldx and ldw < 2^22.
  */
 typedef struct W8A8LinearW4Args {
   uint32_t struct_size;

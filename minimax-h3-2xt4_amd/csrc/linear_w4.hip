@@ -754,6 +754,7 @@ static int launch_w4_tiles(const W4Params& p, void* workspace, hipStream_t strea
 template <int DT, int GB, bool GATED>
 static int launch_w4(const W4Params& p, void* workspace, hipStream_t stream) {
   if (w4_tiled(p.m)) return launch_w4_tiles<DT, GB, GATED>(p, workspace, stream);
+  W8A8_REQUIRE(p.n < (1 << 29), "w8a8_linear_w4: too many outputs for one launch");   // (eight threads an output)
   // Two tiles of weight rows share a wave's x, and four waves of ten or so blocks
   // each cost less to set up than eight of five; but where that leaves CUs idle on
   // long sums, one tile and eight waves (us, two tiles / one; one row of x: 14336 x

@@ -1,10 +1,12 @@
 """Calls of the operators around a block's projections without a GPU: refusals
 and the 4-bit quantizer's range."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from w8a8 import axial_rope, block_norm, linear_w4
+from w8a8 import _abi, axial_rope, block_norm, linear_w4
 
 
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
@@ -101,3 +103,14 @@ def test_modulation_tables_share_their_rows():
         args[which] = change(args[which])
         with pytest.raises(ValueError, match='same rows'):
             block_norm.update_and_prepare(*args)
+
+
+@pytest.mark.parametrize('gated', [0, 1])
+def test_few_rows_of_too_many_outputs_are_refused(gated):
+    """Up to eight rows are one launch of n / 32 workgroups of 256 lanes: below 2^32."""
+    args = _abi.LinearW4Args(dtype=_abi.F16, x=1 << 20, ldx=32, codes=1 << 41, ldw=4, scales=64, m=1, n=1 << 29, k=32,
+                             group=32, gated=gated, out=1 << 40, ldo=1 << 29)
+    args.struct_size = ctypes.sizeof(args)
+    lib = _abi.load()
+    assert lib.w8a8_linear_w4(ctypes.byref(args)) == _abi.ERR_INVALID
+    assert 'too many outputs' in lib.w8a8_last_error().decode()
