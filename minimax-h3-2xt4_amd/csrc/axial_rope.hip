@@ -240,8 +240,27 @@ void axial_freqs_kernel(AxTable t, int64_t rows, int layout, void* freqs) {
 }
 
 // A [rows, heads, dim] view's memory.
-static RowsOf view_of(const void* at, const int64_t (&st)[2], int64_t rows, int64_t heads, int64_t dim, int es) {
-  return {at, st[0] * es, ((heads - 1) * st[1] + dim) * es, ((rows - 1) * st[0] + (heads - 1) * st[1] + dim) * es};
+struct HeadsView {
+  const void* at;
+  int64_t row, head, rows, heads, dim;   // (bytes, numbers of rows and heads, bytes)
+};
+
+static HeadsView view_of(const void* at, const int64_t* st, int64_t rows, int64_t heads, int64_t dim, int es) {
+  return {at, st[0] * es, st[1] * es, rows, heads, dim * es};
+}
+
+// Whether two such views share no byte, as far as spans, rows (or heads, where they
+// are the outer dimension) and heads between each other's tell.
+static bool views_apart(const HeadsView& a, const HeadsView& b) {
+  auto span = [](const HeadsView& v) { return (v.rows - 1) * v.row + (v.heads - 1) * v.head + v.dim; };
+  auto by_rows = [&](const HeadsView& v) { return RowsOf{v.at, v.row, (v.heads - 1) * v.head + v.dim, span(v)}; };
+  auto by_heads = [&](const HeadsView& v) { return RowsOf{v.at, v.head, (v.rows - 1) * v.row + v.dim, span(v)}; };
+  // The inner stride alone, where the outer is a multiple of it; 0 (tells nothing) else.
+  auto inner = [&](const HeadsView& v) {
+    const int64_t s = v.row < v.head ? v.row : v.head;
+    return RowsOf{v.at, s > 0 && v.row % s == 0 && v.head % s == 0 ? s : 0, v.dim, span(v)};
+  };
+  return apart(by_rows(a), by_rows(b)) || apart(by_heads(a), by_heads(b)) || apart(inner(a), inner(b));
 }
 
 }  // namespace w8a8
@@ -283,7 +302,7 @@ extern "C" int w8a8_axial_rope(const W8A8AxialRopeArgs* a) {
   int v = 8;
   while (v > 1 && (a->pairs % v || (a->dim - 2 * a->pairs) % (2 * v))) v >>= 1;
   AxRopeParams p{};
-  RowsOf vin[2] = {}, vout[2] = {};
+  HeadsView vin[2] = {}, vout[2] = {};
   for (int w = 0; w < 2; ++w) {
     if (!heads[w]) continue;
     W8A8_REQUIRE((uintptr_t)in[w] % es == 0 && (uintptr_t)out[w] % es == 0, "w8a8_axial_rope: misaligned tensor");
@@ -305,17 +324,17 @@ extern "C" int w8a8_axial_rope(const W8A8AxialRopeArgs* a) {
     p.out_row[w] = ost[w][0];
     p.out_head[w] = ost[w][1];
     p.heads[w] = heads[w];
-    vin[w] = view_of(in[w], w ? a->k_strides : a->q_strides, a->rows, heads[w], d, es);
-    vout[w] = view_of(out[w], w ? a->k_out_strides : a->q_out_strides, a->rows, heads[w], d, es);
+    vin[w] = view_of(in[w], ist[w], a->rows, heads[w], d, es);
+    vout[w] = view_of(out[w], ost[w], a->rows, heads[w], d, es);
   }
   for (int o = 0; o < 2; ++o) {
     if (!heads[o]) continue;
     for (int i = 0; i < 2; ++i) {
       const bool same = i == o && out[o] == in[i] && ost[o][0] == ist[i][0] && ost[o][1] == ist[i][1];
-      W8A8_REQUIRE(!heads[i] || same || apart(vout[o], vin[i]), "w8a8_axial_rope: an output overlaps an input");
+      W8A8_REQUIRE(!heads[i] || same || views_apart(vout[o], vin[i]), "w8a8_axial_rope: an output overlaps an input");
     }
   }
-  W8A8_REQUIRE(!heads[1] || apart(vout[0], vout[1]), "w8a8_axial_rope: q_out and k_out overlap");
+  W8A8_REQUIRE(!heads[1] || views_apart(vout[0], vout[1]), "w8a8_axial_rope: q_out and k_out overlap");
   p.gain[0] = a->q_gain;
   p.gain[1] = a->k_gain;
   p.table = AxTable{a->positions, a->pos_strides[0], a->pos_strides[1], a->pos_type, a->pairs, a->axes, a->inv_freq, a->axis};

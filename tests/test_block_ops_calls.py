@@ -114,3 +114,18 @@ def test_few_rows_of_too_many_outputs_are_refused(gated):
     lib = _abi.load()
     assert lib.w8a8_linear_w4(ctypes.byref(args)) == _abi.ERR_INVALID
     assert 'too many outputs' in lib.w8a8_last_error().decode()
+
+
+@pytest.mark.parametrize('first,second', [(0, 64), (0, 300), (128, 200)])
+def test_interleaved_heads_that_overlap_are_refused(first, second):
+    # q and k of [rows, heads, 3, dim]: k's channels may not run into q's.
+    st = (3 * 4 * 128, 3 * 128)
+    base = 1 << 20
+    q, k = base + 2 * first, base + 2 * second
+    args = _abi.AxialRopeArgs(dtype=_abi.F16, q=q, k=k, q_out=q, k_out=k, rows=5, q_heads=4, k_heads=4, dim=128,
+                              pairs=64, axes=1, q_strides=st, k_strides=st, q_out_strides=st, k_out_strides=st,
+                              positions=64, pos_strides=(1, 1), inv_freq=128, axis=256, eps=1e-6)
+    args.struct_size = ctypes.sizeof(args)
+    lib = _abi.load()
+    assert lib.w8a8_axial_rope(ctypes.byref(args)) == _abi.ERR_INVALID
+    assert 'overlap' in lib.w8a8_last_error().decode()

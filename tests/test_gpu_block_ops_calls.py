@@ -87,3 +87,24 @@ def test_residuals_of_other_rows_are_refused(gpu, out):
     for bad in (r.transpose(0, 1).contiguous(), r.view(6, 1, 16), r.view(1, 2, 3, 16)):
         with pytest.raises(ValueError, match='residual'):
             linear_w4.linear(x, codes, scales, residual=bad, **kw)
+
+
+@pytest.mark.parametrize('heads_first', [False, True])
+@pytest.mark.parametrize('rows,heads,dim', [(37, 5, 128), (1, 3, 64), (9, 1, 96)])
+def test_interleaved_heads_in_place(gpu, rows, heads, dim, heads_first):
+    """q and k of a buffer [rows, heads, 3, dim] (or [heads, 3, rows, dim]) turn in
+    place: their heads lie between each other and share nothing."""
+    g = torch.Generator().manual_seed(rows)
+    shape = (heads, 3, rows, dim) if heads_first else (rows, heads, 3, dim)
+    buf = torch.randn(shape, generator=g).half().to(gpu)
+
+    def views(t):
+        return tuple(t[:, i].transpose(0, 1) if heads_first else t[:, :, i] for i in range(3))
+    pos = torch.randint(0, 500, (rows, 2), generator=g).to(gpu)
+    inv, axis = axial_rope.ladder((dim // 4, dim // 4), device=gpu)
+    q, k, v = views(buf)
+    keep = v.clone()
+    want = axial_rope.rotate(q.contiguous(), k.contiguous(), pos, inv, axis)
+    got = axial_rope.rotate(q, k, pos, inv, axis, out=(q, k))
+    assert got[0] is q and got[1] is k
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, keep)
