@@ -362,6 +362,12 @@ bool set_item(PyObject* dict, const char* key, at::Tensor t) {
   return ok;
 }
 
+// Counts a write into a caller's tensor, as torch's own in-place operators do:
+// autograd then sees that a tensor it saved has changed.
+void written(const at::Tensor* t) {
+  if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // residual_norm(x, branch, weight, eps, post_weight, post_eps, gate, shift,
 // scale, labels, residual_scale, branch_scale, quantize, convrot,
 // round_rotated, want_normalized, out): kernels.residual_norm without signs.
@@ -452,6 +458,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.stream = stream_of(x->get_device());
   const int rc = call(w8a8_residual_norm, a);
   if (rc != W8A8_OK) return fail("w8a8_residual_norm", rc);
+  written(out);
   PyObject* d = PyDict_New();
   if (!d) return nullptr;
   ok = out ? PyDict_SetItemString(d, "x", args[16]) == 0 : set_item(d, "x", std::move(fresh));
@@ -542,6 +549,8 @@ PyObject* axial_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.stream = stream_of(q->get_device());
   const int rc = call(w8a8_axial_rope, a);
   if (rc != W8A8_OK) return fail("w8a8_axial_rope", rc);
+  written(qo);
+  written(ko);
   PyObject* pq = qo ? Py_NewRef(args[9]) : THPVariable_Wrap(std::move(q_new));
   PyObject* pk = !k ? Py_NewRef(Py_None) : ko ? Py_NewRef(args[10]) : THPVariable_Wrap(std::move(k_new));
   PyObject* r = pq && pk ? PyTuple_Pack(2, pq, pk) : nullptr;

@@ -588,11 +588,16 @@ def _no_gradient(*tensors):
             raise ValueError('this operator has no gradient: detach its inputs or run under torch.no_grad()')
 
 
-def _call_on(device, name, args):
+def _call_on(device, name, args, *given):
     """_abi.call with the tensors' device as the current one: a launch, and its
-    choice by the number of CUs, belong to it."""
+    choice by the number of CUs, belong to it. Writes into the caller's own tensors
+    (given) are counted as torch's in-place operators count theirs: autograd then
+    sees that a tensor it saved has changed."""
     with torch.cuda.device(device):
         _abi.call(name, args)
+    for t in given:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 def _vector(t, name, n):
@@ -673,6 +678,7 @@ def residual_norm(x, branch, *, weight=None, eps=None, post_weight=None, post_ep
     if signs is not None and not (quantize and convrot):
         raise ValueError('signs apply to the ConvRot256 rotation of the quantized output')
     signs = _sign_words(signs, cols, x.device)
+    given = out
     if out is None:
         out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
     elif (out.dtype != x.dtype or out.ndim != 2 or tuple(out.shape) != (rows, cols) or out.stride(1) != 1
@@ -698,7 +704,7 @@ def residual_norm(x, branch, *, weight=None, eps=None, post_weight=None, post_ep
         mod_rows=shift.shape[0] if shift is not None else 0, eps=float(eps or 0.0), y=_abi.ptr(y), ldy=cols,
         convrot=256 if quantize and convrot else 0, round_rotated=1 if round_rotated else 0, q=_abi.ptr(q), ldq=cols,
         q_scale=_abi.ptr(qs), convrot_signs=_abi.ptr(signs), stream=_abi.stream_of(x))
-    _call_on(x.device, 'w8a8_residual_norm', args)
+    _call_on(x.device, 'w8a8_residual_norm', args, given)
     return res
 
 
@@ -784,7 +790,7 @@ def axial_rope(q, k, positions, inv_freq, axis, *, adjacent=False, q_gain=None, 
         positions=positions.data_ptr(), pos_strides=tuple(positions.stride()),
         pos_type=_POSITION_TYPES[positions.dtype], eps=float(eps), inv_freq=inv_freq.data_ptr(),
         axis=axis.data_ptr(), q_gain=_abi.ptr(q_gain), k_gain=_abi.ptr(k_gain), stream=_abi.stream_of(q))
-    _call_on(q.device, 'w8a8_axial_rope', args)
+    _call_on(q.device, 'w8a8_axial_rope', args, *(out or ()))
     return q_out, k_out
 
 
@@ -878,5 +884,5 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
         ldr=residual.stride(0) if residual is not None and m > 1 else n,
         out=y.data_ptr(), ldo=y.stride(0) if m > 1 else width, workspace=_abi.ptr(ws), workspace_bytes=nbytes,
         stream=_abi.stream_of(x))
-    _call_on(x.device, 'w8a8_linear_w4', args)
+    _call_on(x.device, 'w8a8_linear_w4', args, out)
     return y if out is not None else y.reshape(*lead, width)

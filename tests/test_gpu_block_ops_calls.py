@@ -5,7 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 from block_refs import assert_close, linear_w4 as exact_w4
-from w8a8 import axial_rope, block_norm, linear_w4
+from w8a8 import axial_rope, block_norm, kernels, linear_w4
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,36 @@ def test_interleaved_heads_in_place(gpu, rows, heads, dim, heads_first):
     got = axial_rope.rotate(q, k, pos, inv, axis, out=(q, k))
     assert got[0] is q and got[1] is k
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, keep)
+
+
+def test_writes_into_given_outputs_are_counted(gpu):
+    """A tensor that autograd has saved elsewhere and that a call writes into is not
+    taken for unchanged by a later backward pass."""
+    h = torch.randn((4, 256), device=gpu).half()
+    q = torch.randn((4, 2, 64), device=gpu).half()
+    inv, axis = axial_rope.ladder((32,), device=gpu)
+    pos = torch.zeros((4, 1), dtype=torch.int64, device=gpu)
+    codes, scales, _ = linear_w4.quantize_weight(torch.randn((256, 256)))
+    codes, scales = codes.to(gpu), scales.to(gpu)
+    signs = torch.zeros(256, dtype=torch.int32, device=gpu)
+    for call in (lambda t: block_norm.residual_norm(t, h, out=t),
+                 lambda t: block_norm.residual_norm(t, h, eps=1e-6, quantize=True, signs=signs, out=t),
+                 lambda t: linear_w4.linear(h, codes, scales, residual=t, out=t)):
+        x = torch.randn((4, 256), device=gpu).half()
+        weight = torch.ones(256, dtype=torch.float16, device=gpu, requires_grad=True)
+        y = (x * weight).sum()                                  # saves x
+        before = x._version
+        call(x)
+        assert x._version > before
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.backward()
+    for turn in (axial_rope.rotate, kernels.axial_rope):
+        before = q._version, (k := q.clone())._version
+        turn(q, k, pos, inv, axis, out=(q, k))
+        assert q._version > before[0] and k._version > before[1]
+    with torch.inference_mode():
+        t = torch.zeros((4, 256), dtype=torch.float16, device=gpu)
+    block_norm.residual_norm(t, h, out=t)                       # a tensor without a count
+    with torch.inference_mode():
+        block_norm.residual_norm(t, h, out=t)
+        kernels.residual_norm(t, h, out=t)
