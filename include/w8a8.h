@@ -674,7 +674,8 @@ int w8a8_axial_freqs(const W8A8AxialFreqsArgs* args);
  * scales: [k / group, n] of dtype, contiguous; zeros: [k / group, n] uint8
  *   (0..15), contiguous, or NULL: 8.
  * An infinity or NaN in a row of x makes that row's outputs infinite or NaN,
- *   and no other row's.
+ *   and no other row's. So do finite inputs whose sums of (16 + code) * x over
+ *   a block of up to 128 inputs leave fp32's range (BF16 beyond 2^115).
  * workspace: device buffer of at least w8a8_linear_w4_workspace_size() bytes
  *   (16-byte aligned, any contents; NULL where that is 0): sums of x where its
  *   rows are many, and partial outputs of calls too small to fill the GPU,

@@ -7,9 +7,12 @@
 // the type's own MFMA takes them. Their group sum is the codes' plus 16 times
 // the group's sum of x, which an MFMA with a row of ones gives, so that
 //   sum (c - z) x = sum (16 + c) x - (16 + z) sum x
-// in fp32: the two sums are at most some five times the result's size, so the
-// difference keeps all but three of fp32's bits. Scales apply to a group's sum,
-// in fp32.
+// in fp32. The error is fp32's relative to (16 + z) sum |x|, whatever the difference
+// leaves of it: the two sums are some five times the result at the median of normal
+// inputs and random codes (32 times at the ninth decile), 45 and 233 times with inputs
+// of one sign. Times the scale that stays below half a 16-bit step of results of
+// ordinary size, not of those that cancel out. (fp16 tiles take z off the
+// weights and have no such sums.) Scales apply to a group's sum, in fp32.
 //
 // A 16-bit operand fragment of the 16 x 16 x 32 MFMA is eight inputs a lane,
 // one word of codes; a lane's inputs of a block of GB (a group, or 128 inputs of
@@ -361,10 +364,12 @@ __device__ __forceinline__ void store_tile(const W4Params& p, const v16f (&tot)[
 // loads in flight (a load into registers behind a DMA waits for all of them). A
 // step's work is laid out product by product (below), since the compiler's own
 // order reads each operand right before its use and scales and unpacks between the
-// chains of MFMAs. 2048 x 14336 x 4096: bf16 in groups of 64 381 -> 294 us (817
-// TFLOP/s), fp16 in groups of 128 294 -> 258. What bounds it there: every wave
-// reads all of x's tile, 256 KB of LDS a step, as long as its MFMAs take, and the
-// two waves of a SIMD do not fill the rest.
+// chains of MFMAs. 2048 x 14336 x 4096: bf16 in groups of 64 278 to 291 us (381 in
+// the compiler's order; 827 to 865 TFLOP/s), fp16 in groups of 128 254 (294). What
+// bounds it: VALU and MFMA add up to the time (bf16 265 and 287 of 494 thousand cycles
+// a SIMD, the gated fp16 call below 101 and 96 of 196: 7.4 and 8.4 VALU instructions a
+// product), so the two waves of a SIMD hardly overlap; LDS has cycles to spare (144
+// and 55 thousand a CU).
 //
 // fp16 takes the zeros off its weights (packed subtraction, exact). bf16 has no
 // such instruction. Where the rows are many (U = 4) an MFMA puts -(16 + z) sum x
@@ -687,8 +692,8 @@ void linear_w4_join_kernel(W4Params p, const float* parts, int mtiles, int whole
 // How a call of more than eight rows is cut: 32 u rows and 32 w weight rows a tile.
 // With 128 rows a tile a CU holds one workgroup, and the tiles past the last whole
 // round of the GPU take ranges of k, as many as give each CU one and of at least four
-// steps (300 tiles of 353 x 25600 x 5120 gated: 117 to 124 us, 152 to 156 with a second round of
-// 44 tiles). Smaller tiles do so where they are fewer than the CUs. (Two ranges a CU
+// steps (300 tiles of 353 x 25600 x 5120 gated: 111 to 117 us, 152 to 156 with a second
+// round of 44 tiles). Smaller tiles do so where they are fewer than the CUs. (Two ranges a CU
 // cost more to join than they hide: us, one / two, 64 x 4096 x 14336 21.3 / 24.2, 16 x
 // 4096 x 14336 14.6 / 16.9, 64 x 14336 x 4096 20.3 / 21.4; 32 x 14336 x 4096 15.7 /
 // 15.8.)

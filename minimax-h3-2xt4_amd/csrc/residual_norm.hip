@@ -314,10 +314,12 @@ void residual_norm_split_kernel(ResNormParams p) {
 
 // Many rows: a row per wave, all its units in the wave's registers. A row's tables
 // are up to five times its own bytes, and read from L2 for every row they bound the
-// kernel (53504 x 5376 fp16 with all tables: 629 us), so a workgroup of twelve
-// waves (eight where the branch is fp32: its units take twice the registers) stages those of its middle row's label in LDS - the branch's factor, the
-// gain, 1 + mod_scale and mod_shift - and takes `per` rows; a row of another label
-// reads its own from memory.
+// kernel (53504 x 5376 fp16 with all tables: 629 us), so a workgroup of twelve waves
+// (eight where the branch is fp32: its units take twice the registers) stages those of
+// its middle row's label in LDS - the branch's factor, the gain, 1 + mod_scale and
+// mod_shift - and takes `per` rows; a row of another label reads its own from memory.
+// 53504 x 5376 fp16 to rows 504 us (its bytes 476); 6814 x 5376 with an fp32 branch to
+// codes 112 (68): there VALU is 38 % of the time and half of it is waiting for a row.
 constexpr int staged_waves(int bt) { return bt == kF32 ? 8 : 12; }
 
 // A unit's raw words out of the compiler's sight: it would otherwise keep what the
@@ -594,11 +596,11 @@ void residual_norm_wide_kernel(ResNormParams p) {
   }
 }
 
-// Rows that a workgroup per row takes, about three a CU; more go to the staged
-// kernel (us, split / staged: 5120 columns with post norm to rows, 512 rows 7.3 /
-// 9.8, 768 11.0 / 10.9, 1536 21.2 / 16.2; 5376 columns with gate, modulation and
-// rotation to codes, fp32 branch, 512 rows 11.2 / 16.9, 768 15.7 / 19.4, 1024 25.1 /
-// 21.2).
+// Rows that a workgroup per row takes: three for each of 256 CUs (of which a CU holds
+// two at a time where a row has six waves). More go to the staged kernel (us, split /
+// staged: 5120 columns with post norm to rows, 512 rows 7.3 / 9.8, 768 11.0 / 10.9,
+// 1536 21.2 / 16.2; 5376 columns with gate, modulation and rotation to codes, fp32
+// branch, 512 rows 11.2 / 16.9, 768 15.7 / 19.4, 1024 25.1 / 21.2).
 constexpr int64_t kSplitRows = 768;
 
 template <int DT, int BT, int MODE>
