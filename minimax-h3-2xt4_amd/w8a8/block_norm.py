@@ -42,9 +42,11 @@ def update_and_prepare(x, branch, gate, segments, norm, shift, scale, *, post_no
     and post_norm the branch's own RMSNorm (or None). Inference only: the norms'
     weights are taken as constants, any other input that requires a gradient is
     refused."""
-    if any(t is None or t.ndim != 2 or t.shape != gate.shape for t in (gate, shift, scale)):
-        raise ValueError('gate, shift and scale must be tables [R, hidden] of the same rows')
+    if any(t is None or t.ndim != 2 for t in (gate, shift, scale)):
+        raise ValueError('gate, shift and scale must be tables [R, hidden]')
     weight, eps, labels, shift, scale = _norm_args(norm, x, shift, scale, segments)
+    if any(row >= gate.shape[0] for _, _, row in segments):
+        raise ValueError('segments name a row that the gate table has not')
     post_weight = post_eps = None
     if post_norm is not None:
         post_weight, post_eps, _, _, _ = _norm_args(post_norm, x, None, None, None)

@@ -96,12 +96,17 @@ def test_forward_mode_tangents_are_refused():
         block_norm.residual_norm(x, x, eps=1e-6)
 
 
-def test_modulation_tables_share_their_rows():
-    """The segments name one row of gate, shift and scale alike."""
+def test_modulation_tables_have_the_segments_rows():
+    """The segments name one row of gate, shift and scale alike; a table may have others."""
     for which, change in ((2, lambda t: t[:1]), (5, lambda t: t[0]), (6, lambda t: None), (2, lambda t: None)):
         args = _update_args()
         args[which] = change(args[which])
-        with pytest.raises(ValueError, match='same rows'):
+        with pytest.raises(ValueError, match='table'):
+            block_norm.update_and_prepare(*args)
+    for rows in (2, 7):
+        args = _update_args()
+        args[2] = torch.zeros((rows, 256))
+        with pytest.raises(ValueError, match='HIP device'):
             block_norm.update_and_prepare(*args)
 
 
