@@ -825,10 +825,9 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
     x's dtype, zeros uint8 [K / group, N] (0 to 15) or None for 8:
     W[n, k] = scales[k // group, n] * (code[n, k] - zeros[k // group, n]).
     bias [N] in x's dtype. residual [.., N] in x's dtype (x's leading sizes, or
-    all rows as [M, N]) is added. gated: W's
-    first N / 2 rows are gate, the others up; returns silu(gate) * up
-    [.., N / 2]. out: [rows, width] in x's dtype to write into; it may be the
-    residual itself.
+    all rows in one dimension) is added. gated: W's first N / 2 rows are gate,
+    the others up; returns silu(gate) * up [.., N / 2]. out: [rows, width] in
+    x's dtype to write into; it may be the residual itself.
     """
     _no_gradient(x, codes, scales, bias, residual, out)
     _device(x, codes, scales, zeros, bias, residual, out)
@@ -861,8 +860,11 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
     zeros = zeros.contiguous() if zeros is not None else None
     bias = bias.reshape(-1).contiguous() if bias is not None else None
     if residual is not None:
-        if residual.dtype != x.dtype or tuple(residual.shape) not in ((*lead, n), (m, n)):
-            raise ValueError('residual must be [.., N] in x\'s dtype, with x\'s leading sizes or one row for each of them')
+        if residual.dtype != x.dtype or residual.numel() != m * n or residual.shape[-1] != n:
+            raise ValueError('residual must be [.., N] in x\'s dtype')
+        ours, theirs = ([s for s in sizes if s != 1] for sizes in (lead, residual.shape[:-1]))
+        if len(ours) > 1 and len(theirs) > 1 and ours != theirs:
+            raise ValueError('residual must have x\'s leading sizes, or its rows in one dimension')
         residual = residual.reshape(m, n)
         if (n > 1 and residual.stride(1) != 1) or (m > 1 and residual.stride(0) < n):
             residual = residual.contiguous()   # (a broadcast one too)

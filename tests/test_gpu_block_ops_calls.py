@@ -74,7 +74,7 @@ def test_forward_mode_tangents_are_refused(gpu):
 
 @pytest.mark.parametrize('out', [False, True])
 def test_residuals_of_other_rows_are_refused(gpu, out):
-    """A residual has x's leading sizes, or is the [rows, N] of all of them."""
+    """A residual has x's leading sizes, or its rows in one dimension."""
     x = torch.randn((2, 3, 256), device=gpu).half()
     codes, scales, _ = linear_w4.quantize_weight(torch.randn((16, 256)))
     codes, scales = codes.to(gpu), scales.to(gpu)
@@ -84,7 +84,10 @@ def test_residuals_of_other_rows_are_refused(gpu, out):
     assert torch.equal(linear_w4.linear(x, codes, scales, residual=r.view(6, 16), **kw).view(2, 3, 16), want)
     assert torch.equal(linear_w4.linear(x, codes, scales, residual=r, **kw).view(2, 3, 16), want)
     assert torch.equal(linear_w4.linear(x[0, 0], codes, scales, residual=r[0, :1]), want[0, 0])
-    for bad in (r.transpose(0, 1).contiguous(), r.view(6, 1, 16), r.view(1, 2, 3, 16)):
+    for same in (r.view(6, 1, 16), r.view(1, 2, 3, 16)):
+        assert torch.equal(linear_w4.linear(x, codes, scales, residual=same, **kw).view(2, 3, 16), want)
+    assert torch.equal(linear_w4.linear(x.view(6, 256), codes, scales, residual=r, **kw).view(2, 3, 16), want)
+    for bad in (r.transpose(0, 1).contiguous(), r[:1], r[..., :8], r.view(2, 3, 8, 2)):
         with pytest.raises(ValueError, match='residual'):
             linear_w4.linear(x, codes, scales, residual=bad, **kw)
 
