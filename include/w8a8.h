@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define W8A8_ABI_VERSION 15
+#define W8A8_ABI_VERSION 16
 
 typedef enum w8a8_status {
   W8A8_OK = 0,
@@ -715,13 +715,210 @@ int w8a8_linear_w4(const W8A8LinearW4Args* args);
 /* Workspace bytes of w8a8_linear_w4 for these sizes on the current device. */
 int64_t w8a8_linear_w4_workspace_size(int64_t m, int64_t n, int64_t k, int32_t group, int32_t gated);
 
+/*
+ * A paged cache of keys and values. No counterpart in the reference, which
+ * runs its text encoder over whole prompts only.
+ * k, v: [pages, heads, page_size, dim] of dtype, element strides {page, head,
+ *   token} (the same for both), channels contiguous: F16 or BF16 values, or I8
+ *   codes with k_scale and v_scale fp32 [pages, heads, page_size], element
+ *   strides {page, head}, tokens contiguous (NULL for 16-bit caches); a row's
+ *   scale is max(absmax * fp32(1/127), 1e-30), its codes
+ *   clamp(rne(x / scale), -128, 127) (those of w8a8_quantize_rows); a row with
+ *   an infinity or a NaN has the scale NaN.
+ * Key j of sequence b lies in page page_table[b][j / page_size] at token
+ *   j % page_size. An entry of the table outside [0, pages) is a page that is
+ *   not there: nothing is written to it, zeros are read from it, and its keys
+ *   take no part in an attention.
+ * Requirements: page_size a multiple of 16, at most 4096; dim a multiple of 8,
+ *   8 to 256; heads up to 65536; k and v 16-byte aligned, strides multiples of
+ *   8 elements (token stride below 2^26), k_scale and v_scale 16-byte aligned,
+ *   their strides multiples of 4.
+ */
+typedef struct W8A8KvCache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages;
+  int64_t strides[3];
+  int64_t scale_strides[2];
+  int32_t dtype;
+  int32_t page_size;
+  int32_t heads;
+  int32_t dim;
+} W8A8KvCache;
+
+/*
+ * New keys and values of every sequence, written into the cache.
+ * k, v: [rows, cache.heads, cache.dim] of dtype (F16 or BF16; a 16-bit cache's
+ *   own), element strides {row, head}, channels contiguous, rows and heads on
+ *   16-byte boundaries.
+ * page_table: int32 [sequences, table_width], row stride ld_table.
+ * lengths: int32 [sequences], each sequence's keys with the new ones.
+ * starts: int32 [sequences + 1], ascending from 0: sequence b's new rows are
+ *   [starts[b], starts[b + 1]), its last keys in order; NULL: one row each.
+ * Rows from starts[sequences] on, and keys outside of the table, are not
+ *   written. If two rows name the same key (a page that two places of the
+ *   table share), either may remain, or parts of both.
+ */
+typedef struct W8A8CacheWriteArgs {
+  uint32_t struct_size;
+  int32_t dtype;
+  W8A8KvCache cache;
+  const void* k;
+  const void* v;
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  int64_t rows;
+  int64_t sequences;
+  const int32_t* page_table;
+  int64_t ld_table;
+  int64_t table_width;
+  const int32_t* lengths;
+  const int32_t* starts;
+  void* stream;
+} W8A8CacheWriteArgs;
+
+int w8a8_cache_write(const W8A8CacheWriteArgs* args);
+
+/*
+ * The first keys and values of every sequence, read back as packed rows:
+ * k, v [rows, cache.heads, cache.dim] of dtype (F16 or BF16; a 16-bit cache's
+ * own), strides as in W8A8CacheWriteArgs; codes as dtype(code * scale).
+ * starts: int32 [sequences + 1], ascending from 0: rows [starts[b],
+ *   starts[b + 1]) take the keys 0, 1, ... of sequence b (zeros from keys
+ *   outside of its table).
+ * fill: rows from starts[sequences] on are left as they are (0) or set to 0.
+ */
+typedef struct W8A8CacheReadArgs {
+  uint32_t struct_size;
+  int32_t dtype;
+  W8A8KvCache cache;
+  void* k;
+  void* v;
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  int64_t rows;
+  int64_t sequences;
+  const int32_t* page_table;
+  int64_t ld_table;
+  int64_t table_width;
+  const int32_t* starts;
+  int32_t fill;
+  int32_t reserved;
+  void* stream;
+} W8A8CacheReadArgs;
+
+int w8a8_cache_read(const W8A8CacheReadArgs* args);
+
+/*
+ * Attention of one new token of every sequence over its cached keys:
+ *   out[b][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(sm_scale q[b][h] . k_j)
+ * over the keys j < lengths[b] (within the table) of kv head
+ * h / (heads / cache.heads); 0 where there are none.
+ * q, out: [sequences, heads, cache.dim] of dtype (F16 or BF16; a 16-bit
+ *   cache's own), element strides {row, head}, channels contiguous, rows and
+ *   heads on 16-byte boundaries.
+ * Scores, statistics and sums are fp32; p is rounded to dtype (relative to the
+ *   running maximum, with codes times the value's scale relative to the running
+ *   largest scale) for the product with v. The same call gives the same bits
+ *   every time.
+ * workspace: device buffer of at least w8a8_cache_attend_workspace_size()
+ *   bytes (16-byte aligned, any contents; NULL where that is 0): partial sums
+ *   of sequences that several workgroups share. Calls that share one must not
+ *   overlap; calls in sequence may, and a captured graph may replay it.
+ * Requirements: heads a multiple of cache.heads, up to 65536 each; sequences
+ *   below 2^20; table_width * page_size below 2^27; sm_scale positive, finite.
+ */
+typedef struct W8A8CacheAttendArgs {
+  uint32_t struct_size;
+  int32_t dtype;
+  W8A8KvCache cache;
+  const void* q;
+  void* out;
+  int64_t q_strides[2];
+  int64_t out_strides[2];
+  int64_t sequences;
+  int64_t heads;
+  const int32_t* page_table;
+  int64_t ld_table;
+  int64_t table_width;
+  const int32_t* lengths;
+  float sm_scale;
+  int32_t reserved;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} W8A8CacheAttendArgs;
+
+int w8a8_cache_attend(const W8A8CacheAttendArgs* args);
+
+/* Workspace bytes of w8a8_cache_attend for these sizes on the current device. */
+int64_t w8a8_cache_attend_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int32_t dim,
+                                         int64_t max_keys);
+
+/*
+ * Attention of packed sequences of different lengths:
+ *   out[i][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(sm_scale q[i][h] . k_j)
+ * Query rows of sequence b are [starts[b], starts[b + 1]), its keys
+ * [k_starts[b], k_starts[b + 1]); with causal != 0 query i of nq sees keys
+ * j <= i + nk - nq, else all nk. 0 where it sees none. A masked key takes no
+ * part, whatever it and its value hold.
+ * q, out: [rows, heads, dim], k, v: [keys, kv_heads, dim], all of dtype (F16
+ *   or BF16), element strides {row, head}, channels contiguous, rows and heads
+ *   on 16-byte boundaries. Head h reads kv head h / (heads / kv_heads).
+ * starts, k_starts: int32 [sequences + 1], ascending from 0.
+ * fill: out's rows from starts[sequences] on are left as they are (0) or set
+ *   to 0.
+ * Scores, statistics and sums are fp32; p is rounded to dtype relative to the
+ *   running maximum. The same call gives the same bits every time.
+ * Requirements: heads a multiple of kv_heads, up to 65536; dim a multiple of
+ *   8, 8 to 256; rows and keys below 2^27, row strides of k and v below 2^23
+ *   elements; sequences below 2^20; sm_scale positive, finite.
+ */
+typedef struct W8A8PackedAttentionArgs {
+  uint32_t struct_size;
+  int32_t dtype;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_strides[2];
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  int64_t out_strides[2];
+  int64_t rows;
+  int64_t keys;
+  int64_t sequences;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t dim;
+  int32_t causal;
+  const int32_t* starts;
+  const int32_t* k_starts;
+  float sm_scale;
+  int32_t fill;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} W8A8PackedAttentionArgs;
+
+int w8a8_packed_attention(const W8A8PackedAttentionArgs* args);
+
+/* Workspace bytes of w8a8_packed_attention for these sizes on the current device. */
+int64_t w8a8_packed_attention_workspace_size(int64_t rows, int64_t keys, int64_t sequences, int64_t heads,
+                                             int32_t dim);
+
 /* ABI version (W8A8_ABI_VERSION; 14 added w8a8_segment_labels, 15
- * w8a8_residual_norm, w8a8_axial_rope, w8a8_axial_freqs and w8a8_linear_w4). */
+ * w8a8_residual_norm, w8a8_axial_rope, w8a8_axial_freqs and w8a8_linear_w4, 16
+ * w8a8_cache_write, w8a8_cache_read, w8a8_cache_attend and
+ * w8a8_packed_attention). */
 int w8a8_abi_version(void);
 
 /* sizeof of each argument struct, by index: 0 Quant, 1 Swiglu, 2 Gemm,
  * 3 Dequant, 4 Norm, 5 RmsRope, 6 AttnPrepare, 7 Attention, 8 ResidualNorm,
- * 9 AxialRope, 10 AxialFreqs, 11 LinearW4; -1 for an unknown index. Lets bindings verify their layout. */
+ * 9 AxialRope, 10 AxialFreqs, 11 LinearW4, 12 CacheWrite, 13 CacheRead,
+ * 14 CacheAttend, 15 PackedAttention; -1 for an unknown index. Lets bindings verify their layout. */
 int64_t w8a8_struct_size(int32_t which);
 
 /* Message describing the last error returned on the calling thread. */

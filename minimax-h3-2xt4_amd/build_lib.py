@@ -47,9 +47,10 @@ INST_VARIANTS = [(0, 4), (1, 1), (1, 2), (1, 3), (2, 1), (2, 2), (2, 3)]
 
 # Per-file options. attention.hip: MFMA results in VGPRs (its scores feed
 # VALU work every block; in AGPRs each block would copy them over).
-# linear_w4.hip: a block's sums take their scale on the VALU.
-FILE_FLAGS = {'attention.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form'],
-              'linear_w4.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form']}
+# linear_w4.hip: a block's sums take their scale on the VALU. cache_attend.hip,
+# packed_attention.hip: as attention.hip.
+FILE_FLAGS = {name: ['-mllvm', '-amdgpu-mfma-vgpr-form']
+              for name in ('attention.hip', 'linear_w4.hip', 'cache_attend.hip', 'packed_attention.hip')}
 
 
 # Kernels whose MFMAs come from inline assembly: mfma_hazards.py checks the

@@ -30,6 +30,11 @@ static_assert(sizeof(W8A8ResidualNormArgs) == 232, "W8A8ResidualNormArgs layout"
 static_assert(sizeof(W8A8AxialRopeArgs) == 208, "W8A8AxialRopeArgs layout");
 static_assert(sizeof(W8A8AxialFreqsArgs) == 88, "W8A8AxialFreqsArgs layout");
 static_assert(sizeof(W8A8LinearW4Args) == 152, "W8A8LinearW4Args layout");
+static_assert(sizeof(W8A8KvCache) == 96, "W8A8KvCache layout");
+static_assert(sizeof(W8A8CacheWriteArgs) == 216, "W8A8CacheWriteArgs layout");
+static_assert(sizeof(W8A8CacheReadArgs) == 216, "W8A8CacheReadArgs layout");
+static_assert(sizeof(W8A8CacheAttendArgs) == 232, "W8A8CacheAttendArgs layout");
+static_assert(sizeof(W8A8PackedAttentionArgs) == 192, "W8A8PackedAttentionArgs layout");
 
 extern "C" int w8a8_abi_version(void) { return W8A8_ABI_VERSION; }
 
@@ -47,6 +52,10 @@ extern "C" int64_t w8a8_struct_size(int32_t which) {
     case 9: return (int64_t)sizeof(W8A8AxialRopeArgs);
     case 10: return (int64_t)sizeof(W8A8AxialFreqsArgs);
     case 11: return (int64_t)sizeof(W8A8LinearW4Args);
+    case 12: return (int64_t)sizeof(W8A8CacheWriteArgs);
+    case 13: return (int64_t)sizeof(W8A8CacheReadArgs);
+    case 14: return (int64_t)sizeof(W8A8CacheAttendArgs);
+    case 15: return (int64_t)sizeof(W8A8PackedAttentionArgs);
     default: return -1;
   }
 }

@@ -1,0 +1,285 @@
+// Keys and values into a paged cache and back out.
+//
+// A wave takes one row of the packed keys and values and a run of its heads,
+// LPH lanes to a head, eight channels a lane (16 bytes of 16-bit values, 8 of
+// codes). It finds the row's sequence by comparing the starts of 64 sequences
+// at once, and the page is then one scalar load. With codes the row's largest
+// magnitude is a reduction over a head's lanes; scale and codes are those of
+// the activation quantizer (quant1). Bound by HBM.
+#include "paged.h"
+
+namespace w8a8 {
+
+struct CacheMoveParams {
+  CacheView cache;
+  char* k;
+  char* v;
+  int64_t k_row, k_head, v_row, v_head;   // bytes
+  int64_t rows;
+  int sequences, width;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int runs;   // runs of heads of a row
+  int fill;
+};
+
+constexpr int kMoveHeads = 2;   // heads of a lane
+
+// The largest of a head's lanes. Magnitudes are compared as the integers of
+// their bits, among which infinities and then NaNs are the largest.
+template <int LPH>
+__device__ __forceinline__ uint32_t head_max(uint32_t v) {
+#pragma unroll
+  for (int off = LPH / 2; off >= 1; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
+  return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void widen8(uint4 u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint16_t lo = (uint16_t)(w[i] & 0xffffu), hi = (uint16_t)(w[i] >> 16);
+    f[2 * i] = DT == kF16 ? h2f(lo) : bf2f(lo);
+    f[2 * i + 1] = DT == kF16 ? h2f(hi) : bf2f(hi);
+  }
+}
+
+// The wave's row, its run of heads, and the byte offsets of its key's place in
+// the cache; false where the row has none.
+template <int LPH>
+struct Move {
+  int64_t row;
+  int head, chunk;   // this lane's first head (the others follow in steps of 64 / LPH), and its eight channels
+};
+
+template <int LPH>
+__device__ __forceinline__ Move<LPH> move_of(const CacheMoveParams& p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = item / p.runs;
+  const int run = (int)(item - row * p.runs);
+  return {row, run * (kMoveHeads * 64 / LPH) + lane / LPH, lane % LPH};
+}
+
+// The page and token of key pos of sequence b; -1 where it is not there.
+__device__ __forceinline__ int key_place(const CacheMoveParams& p, int b, int pos, int& token) {
+  if (pos < 0) return -1;
+  int entry, first;
+  group_place(p.cache, (uint32_t)pos / kGroupTokens, entry, first);
+  if (entry >= p.width) return -1;
+  token = first + pos % kGroupTokens;
+  const int page = scalar_int(p.table, (int64_t)b * p.ld_table + entry);
+  return page < p.cache.pages ? page : -1;
+}
+
+// codes: the cache holds I8; DT is the rows' type.
+template <int DT, bool CODES, int LPH>
+__global__ __launch_bounds__(256) void cache_write_kernel(CacheMoveParams p) {
+  const Move<LPH> m = move_of<LPH>(p);
+  if (m.row >= p.rows) return;
+  int b, pos;
+  if (p.starts) {
+    b = sequence_of(p.starts, p.sequences, m.row);
+    if (b >= p.sequences) return;
+    pos = scalar_int(p.lengths, b) - (scalar_int(p.starts, b + 1) - (int)m.row);
+  } else {
+    b = __builtin_amdgcn_readfirstlane((int)m.row);
+    pos = scalar_int(p.lengths, b) - 1;
+  }
+  int token;
+  const int page = key_place(p, b, pos, token);
+  if (page < 0) return;
+  const bool mine = 8 * m.chunk < p.cache.dim;   // (lanes beyond the channels stay for the maximum)
+  const int64_t at = (int64_t)page * p.cache.page_b + (int64_t)token * p.cache.token_b;
+  uint4 x[2][kMoveHeads];
+#pragma unroll
+  for (int i = 0; i < kMoveHeads; ++i) {
+    const int h = m.head + i * (64 / LPH);
+    x[0][i] = x[1][i] = make_uint4(0, 0, 0, 0);
+    if (h < p.cache.heads && mine) {
+      x[0][i] = *reinterpret_cast<const uint4*>(p.k + m.row * p.k_row + h * p.k_head + 16 * m.chunk);
+      x[1][i] = *reinterpret_cast<const uint4*>(p.v + m.row * p.v_row + h * p.v_head + 16 * m.chunk);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kMoveHeads; ++i) {
+    const int h = m.head + i * (64 / LPH);
+    if (h >= p.cache.heads) continue;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      char* to = (t ? p.cache.v : p.cache.k) + at + h * p.cache.head_b;
+      if constexpr (!CODES) {
+        if (mine) *reinterpret_cast<uint4*>(to + 16 * m.chunk) = x[t][i];
+      } else {
+        float f[8];
+        uint32_t top = 0;
+        widen8<DT>(x[t][i], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+        top = head_max<LPH>(top);
+        // A row that holds an infinity or a NaN has the scale NaN.
+        const float s = top < 0x7f800000u ? row_scale_of(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
+        const float rcp = 1.0f / s;
+        if (!mine) continue;
+        int q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = quant1(f[j], s, rcp);
+        *reinterpret_cast<uint2*>(to + 8 * m.chunk) = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        if (m.chunk == 0)
+          (t ? p.cache.vs : p.cache.ks)[(int64_t)page * p.cache.s_page + h * p.cache.s_head + token] = s;
+      }
+    }
+  }
+}
+
+template <int DT, bool CODES, int LPH>
+__global__ __launch_bounds__(256) void cache_read_kernel(CacheMoveParams p) {
+  const Move<LPH> m = move_of<LPH>(p);
+  if (m.row >= p.rows) return;
+  const int b = sequence_of(p.starts, p.sequences, m.row);
+  int token = 0, page = -1;
+  if (b < p.sequences) page = key_place(p, b, (int)m.row - scalar_int(p.starts, b), token);
+  else if (!p.fill) return;
+  if (8 * m.chunk >= p.cache.dim) return;
+  const int64_t at = (int64_t)page * p.cache.page_b + (int64_t)token * p.cache.token_b;
+  uint4 x[2][kMoveHeads];
+  uint2 c[2][kMoveHeads];
+  float s[2][kMoveHeads];
+#pragma unroll
+  for (int i = 0; i < kMoveHeads; ++i) {
+    const int h = m.head + i * (64 / LPH);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x[t][i] = make_uint4(0, 0, 0, 0);
+      c[t][i] = make_uint2(0, 0);
+      s[t][i] = 0.0f;
+      if (h >= p.cache.heads || page < 0) continue;
+      const char* from = (t ? p.cache.v : p.cache.k) + at + h * p.cache.head_b;
+      if constexpr (!CODES) {
+        x[t][i] = *reinterpret_cast<const uint4*>(from + 16 * m.chunk);
+      } else {
+        c[t][i] = *reinterpret_cast<const uint2*>(from + 8 * m.chunk);
+        s[t][i] = (t ? p.cache.vs : p.cache.ks)[(int64_t)page * p.cache.s_page + h * p.cache.s_head + token];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kMoveHeads; ++i) {
+    const int h = m.head + i * (64 / LPH);
+    if (h >= p.cache.heads) continue;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if constexpr (CODES) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t q = j < 2 ? c[t][i].x : c[t][i].y;
+          const float lo = (float)(int8_t)(q >> (16 * (j & 1))), hi = (float)(int8_t)(q >> (16 * (j & 1) + 8));
+          float a = lo * s[t][i], d = hi * s[t][i];   // (rounded to fp32 first, as the plain product is)
+          __asm__("" : "+v"(a), "+v"(d));
+          w[j] = pack2<DT>(a, d);
+        }
+        x[t][i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      char* to = t ? p.v + m.row * p.v_row + h * p.v_head : p.k + m.row * p.k_row + h * p.k_head;
+      *reinterpret_cast<uint4*>(to + 16 * m.chunk) = x[t][i];
+    }
+  }
+}
+
+template <bool WRITE, int DT, bool CODES>
+static int launch_move(const char* who, const CacheMoveParams& in, hipStream_t stream) {
+  CacheMoveParams p = in;
+  const int lph = p.cache.dim <= 64 ? 8 : p.cache.dim <= 128 ? 16 : 32;
+  const int per = kMoveHeads * 64 / lph;
+  p.runs = (p.cache.heads + per - 1) / per;
+  const int64_t grid = (p.rows * p.runs + 3) / 4;
+  W8A8_REQUIRE(grid < (1ll << 24), "%s: too many rows and heads for one launch", who);   // (2^32 work-items)
+  const dim3 g((unsigned)grid), t(256);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, t, 0, stream, p); };
+  if constexpr (WRITE) {
+    lph == 8 ? go(cache_write_kernel<DT, CODES, 8>)
+             : lph == 16 ? go(cache_write_kernel<DT, CODES, 16>) : go(cache_write_kernel<DT, CODES, 32>);
+  } else {
+    lph == 8 ? go(cache_read_kernel<DT, CODES, 8>)
+             : lph == 16 ? go(cache_read_kernel<DT, CODES, 16>) : go(cache_read_kernel<DT, CODES, 32>);
+  }
+  return launch_status(who);
+}
+
+template <bool WRITE>
+static int launch_move_type(const char* who, int dtype, int held, const CacheMoveParams& p, hipStream_t stream) {
+  const bool codes = held == W8A8_I8;
+  if (!codes) return launch_move<WRITE, kF16, false>(who, p, stream);   // (16 bits are moved as they are)
+  return dtype == W8A8_F16 ? launch_move<WRITE, kF16, true>(who, p, stream) : launch_move<WRITE, kBF16, true>(who, p, stream);
+}
+
+// The checks that both share; p's fields.
+static int move_params(const char* who, int dtype, const W8A8KvCache& c, const void* k, const void* v,
+                       const int64_t (&kst)[2], const int64_t (&vst)[2], int64_t rows, int64_t sequences,
+                       const int32_t* table, int64_t ld_table, int64_t width, CacheMoveParams& p) {
+  W8A8_REQUIRE(dtype == W8A8_F16 || dtype == W8A8_BF16, "%s: dtype %d not F16/BF16", who, dtype);
+  W8A8_REQUIRE(rows >= 0 && rows < (1ll << 31) && sequences >= 0 && sequences < (1 << 20), "%s: rows or sequences out of range",
+               who);
+  W8A8_PASS(cache_view(who, c, p.cache));
+  W8A8_REQUIRE(c.dtype == W8A8_I8 || c.dtype == dtype, "%s: a 16-bit cache takes rows of its own dtype", who);
+  W8A8_PASS(rows_check(who, "k", k, kst));
+  W8A8_PASS(rows_check(who, "v", v, vst));
+  W8A8_REQUIRE(width >= 0 && width * c.page_size < (1ll << 27) && (width == 0 || sequences == 0 || table) &&
+                   (sequences <= 1 || ld_table >= width),
+               "%s: page table null, its rows overlap, or 2^27 keys and more", who);
+  p.k = reinterpret_cast<char*>(const_cast<void*>(k));
+  p.v = reinterpret_cast<char*>(const_cast<void*>(v));
+  p.k_row = 2 * kst[0]; p.k_head = 2 * kst[1]; p.v_row = 2 * vst[0]; p.v_head = 2 * vst[1];
+  p.rows = rows;
+  p.sequences = (int)sequences;
+  p.width = (int)width;
+  p.table = table;
+  p.ld_table = ld_table;
+  p.lengths = nullptr;
+  p.starts = nullptr;
+  p.fill = 0;
+  return W8A8_OK;
+}
+
+}  // namespace w8a8
+
+extern "C" int w8a8_cache_write(const W8A8CacheWriteArgs* a) {
+  using namespace w8a8;
+  const char* who = "w8a8_cache_write";
+  W8A8_REQUIRE(a != nullptr, "%s: null args", who);
+  W8A8_REQUIRE(a->struct_size == sizeof(W8A8CacheWriteArgs), "%s: struct_size %u != %zu", who, a->struct_size,
+               sizeof(W8A8CacheWriteArgs));
+  if (a->rows == 0) return W8A8_OK;
+  CacheMoveParams p;
+  W8A8_PASS(move_params(who, a->dtype, a->cache, a->k, a->v, a->k_strides, a->v_strides, a->rows, a->sequences,
+                        a->page_table, a->ld_table, a->table_width, p));
+  W8A8_REQUIRE(a->sequences == 0 || a->lengths, "%s: null lengths", who);
+  W8A8_REQUIRE(a->starts || a->rows == a->sequences, "%s: without starts every sequence has one row", who);
+  if (a->sequences == 0) return W8A8_OK;
+  p.lengths = a->lengths;
+  p.starts = a->starts;
+  return launch_move_type<true>(who, a->dtype, a->cache.dtype, p, reinterpret_cast<hipStream_t>(a->stream));
+}
+
+extern "C" int w8a8_cache_read(const W8A8CacheReadArgs* a) {
+  using namespace w8a8;
+  const char* who = "w8a8_cache_read";
+  W8A8_REQUIRE(a != nullptr, "%s: null args", who);
+  W8A8_REQUIRE(a->struct_size == sizeof(W8A8CacheReadArgs), "%s: struct_size %u != %zu", who, a->struct_size,
+               sizeof(W8A8CacheReadArgs));
+  if (a->rows == 0) return W8A8_OK;
+  CacheMoveParams p;
+  W8A8_PASS(move_params(who, a->dtype, a->cache, a->k, a->v, a->k_strides, a->v_strides, a->rows, a->sequences,
+                        a->page_table, a->ld_table, a->table_width, p));
+  W8A8_REQUIRE(a->starts, "%s: null starts", who);
+  W8A8_REQUIRE(rows_apart(a->rows, a->cache.heads, a->cache.dim, a->k_strides) &&
+                   rows_apart(a->rows, a->cache.heads, a->cache.dim, a->v_strides),
+               "%s: output rows overlap", who);
+  p.starts = a->starts;
+  p.fill = a->fill;
+  return launch_move_type<false>(who, a->dtype, a->cache.dtype, p, reinterpret_cast<hipStream_t>(a->stream));
+}

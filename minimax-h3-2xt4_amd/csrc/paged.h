@@ -1,0 +1,140 @@
+// Packed sequences and the paged key-value cache: what the kernels of
+// kv_cache.hip, cache_attend.hip and packed_attention.hip share.
+#pragma once
+
+#include "w8a8_device.h"
+#include "w8a8_host.h"
+
+#include <cmath>
+
+namespace w8a8 {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2eF = 1.44269504088896341f;
+constexpr int kGroupTokens = 16;   // a page holds whole groups of so many tokens
+
+// Tables and lengths are read by scalar loads where a wave agrees on the place
+// (a vector load would wait behind the wave's own tiles).
+typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
+__device__ __forceinline__ int scalar_int(const int32_t* p, int64_t i) { return ((ScalarInts)p)[i]; }
+
+// Two fp32 as a word of two DT values, rounded to nearest even, a in the low half.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == kF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2h));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
+}
+
+// A cache as the kernels take it: strides in bytes (scales': in floats).
+struct CacheView {
+  char* k;
+  char* v;
+  float* ks;
+  float* vs;
+  int64_t page_b, head_b, s_page, s_head;
+  uint32_t token_b;
+  int pages, page_size, heads, dim;
+  uint64_t magic;   // floor(2^36 / groups a page) + 1
+};
+
+// Page of the table and token within it of a sequence's group of 16 tokens
+// (g < 2^23): with d groups a page (d <= 256) magic = 2^36/d + e, 0 < e <= 1,
+// and g * e / 2^36 < 1/d, so the quotient is floor(g / d).
+__device__ __forceinline__ void group_place(const CacheView& c, uint32_t g, int& entry, int& token) {
+  entry = (int)(((uint64_t)g * c.magic) >> 36);
+  token = ((int)g - entry * (c.page_size / kGroupTokens)) * kGroupTokens;
+}
+
+// Sum of a 64-bit value over the wave's 64 lanes, and its inclusive prefix.
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+__device__ __forceinline__ int64_t wave_prefix64(int64_t v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t t = __shfl_up(v, off, 64);
+    if (lane >= off) v += t;
+  }
+  return v;
+}
+
+// The last b in [0, n) with starts[b] <= row, or n when row is at or past
+// starts[n] (a wave works together; the row is the wave's). Sequences without
+// rows are passed over, since the next one starts at the same row.
+__device__ __forceinline__ int sequence_of(const int32_t* starts, int n, int64_t row) {
+  const int lane = threadIdx.x & 63;
+  int count = 0;
+  for (int b = 0; b <= n; b += 64) {
+    const int i = b + lane;
+    const bool below = i <= n && starts[i] <= row;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(below);
+    count += __builtin_popcountll(m);
+    if (m != ~0ull) break;
+  }
+  return __builtin_amdgcn_readfirstlane(count > n ? n : max(count - 1, 0));
+}
+
+inline bool stride8(int64_t s) { return s >= 0 && s % 8 == 0; }
+
+// Checks of a W8A8KvCache and its view.
+inline int cache_view(const char* who, const W8A8KvCache& c, CacheView& v) {
+  const bool codes = c.dtype == W8A8_I8;
+  W8A8_REQUIRE(codes || c.dtype == W8A8_F16 || c.dtype == W8A8_BF16, "%s: cache dtype %d not F16/BF16/I8", who, c.dtype);
+  W8A8_REQUIRE(c.k && c.v && aligned16(c.k) && aligned16(c.v), "%s: cache k or v null or misaligned", who);
+  W8A8_REQUIRE(c.dim >= 8 && c.dim <= 256 && c.dim % 8 == 0, "%s: dim %d not a multiple of 8 up to 256", who, c.dim);
+  W8A8_REQUIRE(c.heads > 0 && c.heads <= 65536 && c.pages > 0 && c.pages < (1ll << 31), "%s: heads or pages out of range",
+               who);
+  W8A8_REQUIRE(c.page_size > 0 && c.page_size <= 4096 && c.page_size % kGroupTokens == 0,
+               "%s: page_size %d not a multiple of 16 up to 4096", who, c.page_size);
+  W8A8_REQUIRE(stride8(c.strides[0]) && stride8(c.strides[1]) && stride8(c.strides[2]) && c.strides[2] >= c.dim &&
+                   c.strides[2] < (1ll << 26),
+               "%s: cache strides must be multiples of 8, the token's from dim to 2^26", who);
+  if (codes)
+    W8A8_REQUIRE(c.k_scale && c.v_scale && aligned16(c.k_scale) && aligned16(c.v_scale) && c.scale_strides[0] >= 0 &&
+                     c.scale_strides[1] >= 0 && c.scale_strides[0] % 4 == 0 && c.scale_strides[1] % 4 == 0,
+                 "%s: codes need k_scale and v_scale, 16-byte aligned, strides multiples of 4", who);
+  const int es = codes ? 1 : 2;
+  v = CacheView{reinterpret_cast<char*>(c.k), reinterpret_cast<char*>(c.v), c.k_scale, c.v_scale,
+                c.strides[0] * es, c.strides[1] * es, c.scale_strides[0], c.scale_strides[1],
+                (uint32_t)(c.strides[2] * es), (int)c.pages, c.page_size, c.heads, c.dim,
+                (1ull << 36) / (uint64_t)(c.page_size / kGroupTokens) + 1};
+  return W8A8_OK;
+}
+
+// Checks of rows [n, heads, dim] of 16-bit elements with strides {row, head}.
+inline int rows_check(const char* who, const char* name, const void* p, const int64_t (&st)[2]) {
+  W8A8_REQUIRE(p && aligned16(p), "%s: %s null or misaligned", who, name);
+  W8A8_REQUIRE(stride8(st[0]) && stride8(st[1]), "%s: %s strides must be multiples of 8 elements", who, name);
+  return W8A8_OK;
+}
+
+// Whether rows [n, heads, dim] with these strides are written once each.
+inline bool rows_apart(int64_t n, int64_t heads, int64_t dim, const int64_t (&st)[2]) {
+  const bool row_in = n <= 1 || heads <= 1 || st[0] >= st[1];   // heads within a row, or rows within a head
+  const int64_t in = row_in ? (heads > 1 ? st[1] : dim) : st[0];
+  const int64_t span = (row_in ? (heads - 1) * (heads > 1 ? st[1] : 0) : (n - 1) * st[0]) + dim;
+  const int64_t out = row_in ? (n > 1 ? st[0] : span) : st[1];
+  return in >= dim && out >= dim && (out >= span || in >= ((row_in ? n : heads) - 1) * out + dim);
+}
+
+// Bytes from the first element of such rows to behind the last.
+inline int64_t rows_span(int64_t n, int64_t heads, int64_t dim, const int64_t (&st)[2]) {
+  return 2 * ((n - 1) * st[0] + (heads - 1) * st[1] + dim);
+}
+
+}  // namespace w8a8
+
+#define W8A8_PASS(expr)                  \
+  do {                                   \
+    const int rc_ = (expr);              \
+    if (rc_ != W8A8_OK) return rc_;      \
+  } while (0)

@@ -13,6 +13,8 @@ Modules mirror the reference's operator API for this path:
   block_norm         - residual update by a block's branch with the norms around it
   axial_rope         - rotary positions with several axes, from the rows' positions
   linear_w4          - projections with 4-bit weights and group scales
+  kv_cache           - paged keys and values, 16-bit or INT8, and one token's attention over them
+  packed_attention   - attention of packed sequences of different lengths, causal or not
   kernels            - typed wrappers of the C ABI
   workloads          - seeded synthetic inputs of the benchmark shapes
 """
@@ -20,4 +22,4 @@ from . import _abi  # noqa: F401
 
 __all__ = ['kernels', 'parallel_int8', 'dit_column_linear', 'swiglu_quant', 'row_quant', 'column_epilogue',
            'h3_operator_policy', 'h3_tensor_flow', 'tp_dit', 'workloads', 'convrot',
-           'block_norm', 'axial_rope', 'linear_w4']
+           'block_norm', 'axial_rope', 'linear_w4', 'kv_cache', 'packed_attention']

@@ -15,7 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / 'libw8a8.so'
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_LAUNCH = 0, 1, 2, 3
 F16, BF16, F32, I32, I8 = 1, 2, 3, 4, 5
 EPI_INT32, EPI_ROW, EPI_COLUMN = 0, 1, 2
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _c = ctypes
 _p = ctypes.c_void_p
@@ -126,6 +126,44 @@ class LinearW4Args(ctypes.Structure):
                 ('workspace_bytes', _c.c_int64), ('stream', _p)]
 
 
+class KvCache(ctypes.Structure):
+    _fields_ = [('k', _p), ('v', _p), ('k_scale', _p), ('v_scale', _p), ('pages', _c.c_int64),
+                ('strides', _c.c_int64 * 3), ('scale_strides', _c.c_int64 * 2), ('dtype', _c.c_int32),
+                ('page_size', _c.c_int32), ('heads', _c.c_int32), ('dim', _c.c_int32)]
+
+
+class CacheWriteArgs(ctypes.Structure):
+    _fields_ = [('struct_size', _c.c_uint32), ('dtype', _c.c_int32), ('cache', KvCache), ('k', _p), ('v', _p),
+                ('k_strides', _c.c_int64 * 2), ('v_strides', _c.c_int64 * 2), ('rows', _c.c_int64),
+                ('sequences', _c.c_int64), ('page_table', _p), ('ld_table', _c.c_int64),
+                ('table_width', _c.c_int64), ('lengths', _p), ('starts', _p), ('stream', _p)]
+
+
+class CacheReadArgs(ctypes.Structure):
+    _fields_ = [('struct_size', _c.c_uint32), ('dtype', _c.c_int32), ('cache', KvCache), ('k', _p), ('v', _p),
+                ('k_strides', _c.c_int64 * 2), ('v_strides', _c.c_int64 * 2), ('rows', _c.c_int64),
+                ('sequences', _c.c_int64), ('page_table', _p), ('ld_table', _c.c_int64),
+                ('table_width', _c.c_int64), ('starts', _p), ('fill', _c.c_int32), ('reserved', _c.c_int32),
+                ('stream', _p)]
+
+
+class CacheAttendArgs(ctypes.Structure):
+    _fields_ = [('struct_size', _c.c_uint32), ('dtype', _c.c_int32), ('cache', KvCache), ('q', _p), ('out', _p),
+                ('q_strides', _c.c_int64 * 2), ('out_strides', _c.c_int64 * 2), ('sequences', _c.c_int64),
+                ('heads', _c.c_int64), ('page_table', _p), ('ld_table', _c.c_int64), ('table_width', _c.c_int64),
+                ('lengths', _p), ('sm_scale', _c.c_float), ('reserved', _c.c_int32), ('workspace', _p),
+                ('workspace_bytes', _c.c_int64), ('stream', _p)]
+
+
+class PackedAttentionArgs(ctypes.Structure):
+    _fields_ = [('struct_size', _c.c_uint32), ('dtype', _c.c_int32), ('q', _p), ('k', _p), ('v', _p), ('out', _p),
+                ('q_strides', _c.c_int64 * 2), ('k_strides', _c.c_int64 * 2), ('v_strides', _c.c_int64 * 2),
+                ('out_strides', _c.c_int64 * 2), ('rows', _c.c_int64), ('keys', _c.c_int64),
+                ('sequences', _c.c_int64), ('heads', _c.c_int32), ('kv_heads', _c.c_int32), ('dim', _c.c_int32),
+                ('causal', _c.c_int32), ('starts', _p), ('k_starts', _p), ('sm_scale', _c.c_float),
+                ('fill', _c.c_int32), ('workspace', _p), ('workspace_bytes', _c.c_int64), ('stream', _p)]
+
+
 # Argument structs in w8a8_struct_size() index order, with their entry points.
 STRUCTS = (QuantArgs, SwigluArgs, GemmArgs, DequantArgs, NormArgs, RmsRopeArgs, AttnPrepareArgs, AttentionArgs)
 STRUCT_ENTRY_POINTS = ('w8a8_quantize_rows', 'w8a8_swiglu_quantize', 'w8a8_gemm', 'w8a8_dequantize',
@@ -133,10 +171,14 @@ STRUCT_ENTRY_POINTS = ('w8a8_quantize_rows', 'w8a8_swiglu_quantize', 'w8a8_gemm'
 # Those of the operators around the projections of a block follow (indices 8 on).
 BLOCK_STRUCTS = (ResidualNormArgs, AxialRopeArgs, AxialFreqsArgs, LinearW4Args)
 BLOCK_ENTRY_POINTS = ('w8a8_residual_norm', 'w8a8_axial_rope', 'w8a8_axial_freqs', 'w8a8_linear_w4')
-ENTRY_POINTS = STRUCT_ENTRY_POINTS + BLOCK_ENTRY_POINTS + ('w8a8_gemm_noalloc', 'w8a8_abi_version', 'w8a8_struct_size',
+# Those of the paged cache and the attention over packed rows (indices 12 on).
+CACHE_STRUCTS = (CacheWriteArgs, CacheReadArgs, CacheAttendArgs, PackedAttentionArgs)
+CACHE_ENTRY_POINTS = ('w8a8_cache_write', 'w8a8_cache_read', 'w8a8_cache_attend', 'w8a8_packed_attention')
+ENTRY_POINTS = STRUCT_ENTRY_POINTS + BLOCK_ENTRY_POINTS + CACHE_ENTRY_POINTS + ('w8a8_gemm_noalloc', 'w8a8_abi_version', 'w8a8_struct_size',
                                       'w8a8_last_error', 'w8a8_gemm_workspace_size',
                                       'w8a8_attention_workspace_size', 'w8a8_segment_labels',
-                                      'w8a8_linear_w4_workspace_size')
+                                      'w8a8_linear_w4_workspace_size', 'w8a8_cache_attend_workspace_size',
+                                      'w8a8_packed_attention_workspace_size')
 GEMM_SCRATCH_BYTES = 64 << 20   # W8A8_GEMM_SCRATCH_BYTES: the no-allocation GEMM's split-K scratch per GPU
 
 _LIB = None
@@ -176,12 +218,16 @@ def load(path=None):
     lib.w8a8_segment_labels.argtypes = [_p, _p, _c.c_int64, _p, _c.c_int64, _p]
     lib.w8a8_linear_w4_workspace_size.restype = _c.c_int64
     lib.w8a8_linear_w4_workspace_size.argtypes = [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int32, _c.c_int32]
-    for name, st in zip(STRUCT_ENTRY_POINTS + BLOCK_ENTRY_POINTS + ('w8a8_gemm_noalloc',),
-                        STRUCTS + BLOCK_STRUCTS + (GemmArgs,)):
+    lib.w8a8_cache_attend_workspace_size.restype = _c.c_int64
+    lib.w8a8_cache_attend_workspace_size.argtypes = [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int32, _c.c_int64]
+    lib.w8a8_packed_attention_workspace_size.restype = _c.c_int64
+    lib.w8a8_packed_attention_workspace_size.argtypes = [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int32]
+    for name, st in zip(STRUCT_ENTRY_POINTS + BLOCK_ENTRY_POINTS + CACHE_ENTRY_POINTS + ('w8a8_gemm_noalloc',),
+                        STRUCTS + BLOCK_STRUCTS + CACHE_STRUCTS + (GemmArgs,)):
         fn = getattr(lib, name)
         fn.restype = _c.c_int
         fn.argtypes = [ctypes.POINTER(st)]
-    for i, st in enumerate(STRUCTS + BLOCK_STRUCTS):
+    for i, st in enumerate(STRUCTS + BLOCK_STRUCTS + CACHE_STRUCTS):
         if lib.w8a8_struct_size(i) != ctypes.sizeof(st):
             raise RuntimeError(f'{st.__name__}: library size {lib.w8a8_struct_size(i)} != '
                                f'binding size {ctypes.sizeof(st)}')

@@ -888,3 +888,220 @@ def linear_w4(x, codes, scales, zeros=None, *, bias=None, residual=None, gated=F
         stream=_abi.stream_of(x))
     _call_on(x.device, 'w8a8_linear_w4', args, out)
     return y if out is not None else y.reshape(*lead, width)
+
+
+def _rows16(t, name):
+    """A [rows, heads, dim] tensor whose channels are contiguous, rows and heads
+    on 16-byte boundaries and apart (a copy if need be), and its strides."""
+    st = _row_head_strides(t)
+    if st is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = _row_head_strides(t)
+    return t, st
+
+
+def _row_head_strides(t):
+    """Element strides {row, head} of a [rows, heads, dim] tensor that the
+    kernels read or write in place (those of sizes of 1 made regular), else None."""
+    rows, heads, dim = t.shape
+    if dim > 1 and t.stride(2) != 1 or t.data_ptr() % 16:
+        return None
+    sr, sh = t.stride(0), t.stride(1)
+    if heads <= 1:
+        sh = dim
+    if rows <= 1:
+        sr = max(heads * dim, (heads - 1) * sh + dim)
+    if sr % 8 or sh % 8 or sr < dim or sh < dim:
+        return None
+    return sr, sh
+
+
+def _out_strides(t, like, name):
+    """The strides of a given output, checked against the rows it takes."""
+    if t.shape != like.shape or t.dtype != like.dtype:
+        raise ValueError(f'{name} must be {like.dtype} {tuple(like.shape)}')
+    st = _row_head_strides(t)
+    if st is None:
+        raise ValueError(f'{name} must have contiguous channels, with rows and heads on 16-byte boundaries')
+    return st
+
+
+def _starts(t, name, sequences=None):
+    """int32 [sequences + 1] contiguous."""
+    if t.ndim != 1 or t.dtype != torch.int32 or t.numel() < 1 or (sequences is not None and t.numel() != sequences + 1):
+        raise ValueError(f'{name} must be int32 [sequences + 1]')
+    return t.contiguous()
+
+
+def _cache_args(cache):
+    """The W8A8KvCache of a kv_cache.KVCache."""
+    k, codes = cache.k, cache.k.dtype == torch.int8
+    return _abi.KvCache(k=k.data_ptr(), v=cache.v.data_ptr(), k_scale=_abi.ptr(cache.k_scale),
+                        v_scale=_abi.ptr(cache.v_scale), pages=k.shape[0], strides=tuple(k.stride())[:3],
+                        scale_strides=tuple(cache.k_scale.stride())[:2] if codes else (0, 0),
+                        dtype=_abi.DTYPE_CODE[k.dtype], page_size=k.shape[2], heads=k.shape[1], dim=k.shape[3])
+
+
+def _page_table(page_table):
+    if page_table.ndim != 2 or page_table.dtype != torch.int32:
+        raise ValueError('page_table must be int32 [sequences, pages of a sequence]')
+    if page_table.shape[1] > 1 and page_table.stride(1) != 1 or (page_table.shape[0] > 1 and
+                                                                  page_table.stride(0) < page_table.shape[1]):
+        page_table = page_table.contiguous()
+    rows, width = page_table.shape
+    return page_table, page_table.stride(0) if rows > 1 else width
+
+
+def _cache_tensors(cache):
+    return cache.k, cache.v, cache.k_scale, cache.v_scale
+
+
+def _cache_rows(cache, t, name):
+    if t.ndim != 3 or tuple(t.shape[1:]) != (cache.heads, cache.dim):
+        raise ValueError(f'{name} must be [rows, {cache.heads}, {cache.dim}]')
+    if t.dtype not in (torch.float16, torch.bfloat16) or (not cache.codes and t.dtype != cache.k.dtype):
+        raise ValueError(f'{name} must be float16 or bfloat16, a 16-bit cache\'s own type')
+
+
+def cache_write(cache, k, v, page_table, lengths, starts=None):
+    """New keys and values [rows, heads, dim] of every sequence into a paged
+    cache (kv_cache.KVCache); see kv_cache.write."""
+    _no_gradient(k, v, *_cache_tensors(cache))
+    _device(k, v, page_table, lengths, starts, *_cache_tensors(cache))
+    _cache_rows(cache, k, 'k')
+    _cache_rows(cache, v, 'v')
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError('k and v must have the same shape and type')
+    page_table, ld = _page_table(page_table)
+    sequences = page_table.shape[0]
+    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (sequences,):
+        raise ValueError('lengths must be int32 [sequences]')
+    if starts is not None:
+        starts = _starts(starts, 'starts', sequences)
+    elif k.shape[0] != sequences:
+        raise ValueError('without starts k and v must have one row for each sequence')
+    if k.shape[0] == 0 or sequences == 0:
+        return
+    lengths = lengths.contiguous()
+    (k, kst), (v, vst) = _rows16(k, 'k'), _rows16(v, 'v')
+    args = _abi.CacheWriteArgs(
+        dtype=_abi.DTYPE_CODE[k.dtype], cache=_cache_args(cache), k=k.data_ptr(), v=v.data_ptr(), k_strides=kst,
+        v_strides=vst, rows=k.shape[0], sequences=sequences, page_table=page_table.data_ptr(), ld_table=ld,
+        table_width=page_table.shape[1], lengths=lengths.data_ptr(), starts=_abi.ptr(starts),
+        stream=_abi.stream_of(k))
+    _call_on(k.device, 'w8a8_cache_write', args, *_cache_tensors(cache))
+
+
+def cache_read(cache, page_table, starts, rows, *, dtype=None, out=None):
+    """The first keys and values of every sequence of a paged cache as packed
+    rows (k, v); see kv_cache.read."""
+    given = () if out is None else tuple(out)
+    _no_gradient(*_cache_tensors(cache), *given)
+    _device(page_table, starts, *_cache_tensors(cache), *given)
+    page_table, ld = _page_table(page_table)
+    starts = _starts(starts, 'starts', page_table.shape[0])
+    if dtype is None:
+        dtype = given[0].dtype if given else torch.float16 if cache.codes else cache.k.dtype
+    if out is None:
+        k, v = (torch.empty((rows, cache.heads, cache.dim), dtype=dtype, device=page_table.device) for _ in range(2))
+    else:
+        k, v = given
+    for t, name in ((k, 'k'), (v, 'v')):
+        _cache_rows(cache, t, name)
+        if t.shape[0] != rows or t.dtype != dtype:
+            raise ValueError(f'out must hold two {dtype} tensors [{rows}, {cache.heads}, {cache.dim}]')
+    if rows == 0:
+        return k, v
+    args = _abi.CacheReadArgs(
+        dtype=_abi.DTYPE_CODE[dtype], cache=_cache_args(cache), k=k.data_ptr(), v=v.data_ptr(),
+        k_strides=_out_strides(k, k, 'k'), v_strides=_out_strides(v, v, 'v'), rows=rows,
+        sequences=page_table.shape[0], page_table=page_table.data_ptr(), ld_table=ld,
+        table_width=page_table.shape[1], starts=starts.data_ptr(), fill=0 if given else 1, stream=_abi.stream_of(k))
+    _call_on(k.device, 'w8a8_cache_read', args, *given)
+    return k, v
+
+
+def _positive(scale, dim):
+    """The softmax scale (1 / sqrt(dim) where none is given)."""
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 1e-38 < scale < 1e38:
+        raise ValueError('scale must be positive and finite')
+    return scale
+
+
+def cache_attend(q, cache, page_table, lengths, *, scale=None, out=None):
+    """Attention of one new token of every sequence over its cached keys; see
+    kv_cache.attend."""
+    _no_gradient(q, out, *_cache_tensors(cache))
+    _device(q, page_table, lengths, out, *_cache_tensors(cache))
+    page_table, ld = _page_table(page_table)
+    sequences = page_table.shape[0]
+    if q.ndim != 3 or q.shape[0] != sequences or q.shape[2] != cache.dim:
+        raise ValueError(f'q must be [sequences, heads, {cache.dim}]')
+    heads = q.shape[1]
+    if heads == 0 or heads % cache.heads:
+        raise ValueError('the query heads must be a positive multiple of the cache\'s')
+    if q.dtype not in (torch.float16, torch.bfloat16) or (not cache.codes and q.dtype != cache.k.dtype):
+        raise ValueError('q must be float16 or bfloat16, a 16-bit cache\'s own type')
+    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (sequences,):
+        raise ValueError('lengths must be int32 [sequences]')
+    scale = _positive(scale, cache.dim)
+    y = torch.empty((sequences, heads, cache.dim), dtype=q.dtype, device=q.device) if out is None else out
+    ost = _out_strides(y, q, 'out')
+    if sequences == 0:
+        return y
+    q, qst = _rows16(q, 'q')
+    lengths = lengths.contiguous()
+    with torch.cuda.device(q.device):
+        nbytes = int(_abi.load().w8a8_cache_attend_workspace_size(sequences, heads, cache.heads, cache.dim,
+                                                                  page_table.shape[1] * cache.page_size))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    args = _abi.CacheAttendArgs(
+        dtype=_abi.DTYPE_CODE[q.dtype], cache=_cache_args(cache), q=q.data_ptr(), out=y.data_ptr(), q_strides=qst,
+        out_strides=ost, sequences=sequences, heads=heads, page_table=page_table.data_ptr(), ld_table=ld,
+        table_width=page_table.shape[1], lengths=lengths.data_ptr(), sm_scale=scale, workspace=_abi.ptr(ws),
+        workspace_bytes=nbytes, stream=_abi.stream_of(q))
+    _call_on(q.device, 'w8a8_cache_attend', args, out)
+    return y
+
+
+def packed_attention(q, k, v, starts, k_starts=None, *, causal=True, scale=None, out=None):
+    """Attention of packed sequences of different lengths; see
+    packed_attention.packed_attention."""
+    _no_gradient(q, k, v, out)
+    _device(q, k, v, starts, k_starts, out)
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError('q, k and v must share float16 or bfloat16')
+    if q.ndim != 3 or k.ndim != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise ValueError('q must be [rows, heads, dim], k and v [keys, kv_heads, dim]')
+    rows, heads, dim = q.shape
+    keys, kv_heads = k.shape[:2]
+    if not 8 <= dim <= 256 or dim % 8:
+        raise ValueError('dim must be a multiple of 8, 8 to 256')
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
+        raise ValueError('the query heads must be a positive multiple of the key heads')
+    starts = _starts(starts, 'starts')
+    sequences = starts.numel() - 1
+    if k_starts is None:
+        if keys != rows:
+            raise ValueError('without k_starts k and v must have q\'s rows')
+        k_starts = starts
+    else:
+        k_starts = _starts(k_starts, 'k_starts', sequences)
+    scale = _positive(scale, dim)
+    y = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device) if out is None else out
+    ost = _out_strides(y, q, 'out')
+    if rows == 0:
+        return y
+    (q, qst), (k, kst), (v, vst) = _rows16(q, 'q'), _rows16(k, 'k'), _rows16(v, 'v')
+    with torch.cuda.device(q.device):
+        nbytes = int(_abi.load().w8a8_packed_attention_workspace_size(rows, keys, sequences, heads, dim))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    args = _abi.PackedAttentionArgs(
+        dtype=_abi.DTYPE_CODE[q.dtype], q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=y.data_ptr(),
+        q_strides=qst, k_strides=kst, v_strides=vst, out_strides=ost, rows=rows, keys=keys, sequences=sequences,
+        heads=heads, kv_heads=kv_heads, dim=dim, causal=1 if causal else 0, starts=starts.data_ptr(),
+        k_starts=k_starts.data_ptr(), sm_scale=scale, fill=1 if out is None else 0, workspace=_abi.ptr(ws),
+        workspace_bytes=nbytes, stream=_abi.stream_of(q))
+    _call_on(q.device, 'w8a8_packed_attention', args, out)
+    return y

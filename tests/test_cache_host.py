@@ -1,0 +1,226 @@
+"""The paged cache and the attention over packed rows without a GPU: argument
+checks of the C entry points (nothing is launched) and of the cache's handle."""
+import ctypes
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from w8a8 import _abi, kv_cache
+from w8a8.kv_cache import KVCache
+from w8a8.packed_attention import packed_attention
+
+
+def _status(name, args):
+    lib = _abi.load()
+    args.struct_size = ctypes.sizeof(args)
+    return getattr(lib, name)(ctypes.byref(args)), lib.w8a8_last_error().decode()
+
+
+def _refused(name, args, fragment):
+    rc, message = _status(name, args)
+    assert rc == _abi.ERR_INVALID and fragment in message, message
+
+
+def test_struct_layouts():
+    lib = _abi.load()
+    assert ctypes.sizeof(_abi.KvCache) == 96
+    assert [ctypes.sizeof(s) for s in _abi.CACHE_STRUCTS] == [216, 216, 232, 192]
+    for i, st in enumerate(_abi.CACHE_STRUCTS):
+        assert lib.w8a8_struct_size(12 + i) == ctypes.sizeof(st)
+    for name, st in zip(_abi.CACHE_ENTRY_POINTS, _abi.CACHE_STRUCTS):
+        a = st(struct_size=8)
+        assert getattr(lib, name)(ctypes.byref(a)) == _abi.ERR_INVALID
+        assert 'struct_size' in lib.w8a8_last_error().decode()
+        assert getattr(lib, name)(None) == _abi.ERR_INVALID
+
+
+CACHE = dict(k=1 << 30, v=2 << 30, pages=10, strides=(2 * 16 * 64, 16 * 64, 64), dtype=_abi.F16, page_size=16, heads=2,
+             dim=64)
+CODES = dict(CACHE, dtype=_abi.I8, k_scale=3 << 30, v_scale=4 << 30, scale_strides=(32, 16))
+
+BAD_CACHES = [
+    (dict(dtype=_abi.F32), 'cache dtype'),
+    (dict(k=None), 'null'),
+    (dict(v=(2 << 30) + 8), 'misaligned'),
+    (dict(dim=60), 'dim'), (dict(dim=0), 'dim'), (dict(dim=264), 'dim'),
+    (dict(heads=0), 'heads'), (dict(pages=0), 'pages'), (dict(pages=1 << 31), 'pages'),
+    (dict(page_size=0), 'page_size'), (dict(page_size=24), 'page_size'), (dict(page_size=4112), 'page_size'),
+    (dict(strides=(2048, 1024, 60)), 'strides'), (dict(strides=(2048, 1024, 56)), 'strides'),
+    (dict(strides=(-2048, 1024, 64)), 'strides'), (dict(strides=(2048, 1024, 1 << 26)), 'strides'),
+]
+BAD_CODES = [(dict(k_scale=None), 'scale'), (dict(v_scale=(4 << 30) + 4), 'scale'), (dict(scale_strides=(30, 16)), 'scale'),
+             (dict(scale_strides=(32, -16)), 'scale')]
+
+WRITE = dict(dtype=_abi.F16, k=5 << 30, v=6 << 30, k_strides=(128, 64), v_strides=(128, 64), rows=7, sequences=3,
+             page_table=7 << 30, ld_table=4, table_width=4, lengths=8 << 30, starts=9 << 30)
+READ = {k: v for k, v in WRITE.items() if k != 'lengths'}
+ATTEND = dict(dtype=_abi.F16, q=5 << 30, out=6 << 30, q_strides=(512, 64), out_strides=(512, 64), sequences=3, heads=8,
+              page_table=7 << 30, ld_table=4, table_width=4, lengths=8 << 30, sm_scale=0.1, workspace=9 << 30,
+              workspace_bytes=1 << 30)
+
+
+def _args(which, change=None, cache=None, codes=False):
+    struct, base = {'write': (_abi.CacheWriteArgs, WRITE), 'read': (_abi.CacheReadArgs, READ),
+                    'attend': (_abi.CacheAttendArgs, ATTEND)}[which]
+    return struct(cache=_abi.KvCache(**{**(CODES if codes else CACHE), **(cache or {})}), **{**base, **(change or {})})
+
+
+@pytest.mark.parametrize('which', ['write', 'read', 'attend'])
+def test_cache_refusals(which):
+    for change, fragment in BAD_CACHES:
+        _refused(f'w8a8_cache_{which}', _args(which, cache=change), fragment)
+    for change, fragment in BAD_CODES:
+        _refused(f'w8a8_cache_{which}', _args(which, cache=change, codes=True), fragment)
+    _refused(f'w8a8_cache_{which}', _args(which, dict(dtype=_abi.F32)), 'dtype')
+    _refused(f'w8a8_cache_{which}', _args(which, dict(dtype=_abi.BF16)), 'own dtype')
+    _refused(f'w8a8_cache_{which}', _args(which, dict(page_table=None)), 'page table')
+    _refused(f'w8a8_cache_{which}', _args(which, dict(ld_table=3)), 'page table')
+    _refused(f'w8a8_cache_{which}', _args(which, dict(table_width=1 << 23, ld_table=1 << 23)), '2^27')
+    _refused(f'w8a8_cache_{which}', _args(which, dict(sequences=-1)), 'sequences')
+    _refused(f'w8a8_cache_{which}', _args(which, dict(sequences=1 << 20)), 'sequences')
+
+
+@pytest.mark.parametrize('change,fragment', [
+    (dict(k=None), 'k null'), (dict(v=(6 << 30) + 8), 'v null or misaligned'), (dict(k_strides=(132, 64)), 'k strides'),
+    (dict(v_strides=(128, -64)), 'v strides'), (dict(rows=-1), 'rows'), (dict(rows=1 << 31), 'rows'),
+])
+def test_row_refusals(change, fragment):
+    _refused('w8a8_cache_write', _args('write', change), fragment)
+    _refused('w8a8_cache_read', _args('read', change), fragment)
+
+
+def test_write_and_read_refusals():
+    _refused('w8a8_cache_write', _args('write', dict(lengths=None)), 'lengths')
+    _refused('w8a8_cache_write', _args('write', dict(starts=None)), 'one row')
+    _refused('w8a8_cache_write', _args('write', dict(rows=(1 << 31) - 1), dict(heads=65536)), 'too many rows')
+    _refused('w8a8_cache_read', _args('read', dict(starts=None)), 'starts')
+    for st in ((64, 64), (0, 64), (128, 0), (128, 56)):
+        _refused('w8a8_cache_read', _args('read', dict(k_strides=st)), 'overlap')
+        _refused('w8a8_cache_read', _args('read', dict(v_strides=st)), 'overlap')
+    for which in ('write', 'read'):
+        assert _status(f'w8a8_cache_{which}', _args(which, dict(rows=0)))[0] == _abi.OK
+
+
+@pytest.mark.parametrize('change,fragment', [
+    (dict(q=None), 'q null'), (dict(out=(6 << 30) + 8), 'out null or misaligned'), (dict(q_strides=(516, 64)), 'q strides'),
+    (dict(out_strides=(512, 0)), 'overlap'), (dict(out_strides=(448, 64)), 'overlap'), (dict(out=5 << 30), 'overlaps q'),
+    (dict(heads=0), 'heads'), (dict(heads=7), 'heads'), (dict(heads=65538), 'heads'), (dict(lengths=None), 'lengths'),
+    (dict(sm_scale=0.0), 'sm_scale'), (dict(sm_scale=-1.0), 'sm_scale'), (dict(sm_scale=float('inf')), 'sm_scale'),
+    (dict(sm_scale=float('nan')), 'sm_scale'), (dict(workspace=None), 'workspace'), (dict(workspace_bytes=64), 'workspace'),
+    (dict(workspace=(9 << 30) + 4), 'workspace'),
+])
+def test_attend_refusals(change, fragment):
+    _refused('w8a8_cache_attend', _args('attend', change), fragment)
+
+
+def test_attend_workspace():
+    lib = _abi.load()
+    assert lib.w8a8_cache_attend_workspace_size(0, 8, 2, 64, 100) == 0
+    assert lib.w8a8_cache_attend_workspace_size(3, 8, 3, 64, 100) == 0
+    small, large = (lib.w8a8_cache_attend_workspace_size(1, 8, 2, 128, n) for n in (100, 1 << 20))
+    assert 0 <= small <= large < 1 << 26
+    assert lib.w8a8_cache_attend_workspace_size(100000, 64, 8, 128, 1 << 26) == large
+    assert _status('w8a8_cache_attend', _args('attend', dict(sequences=0)))[0] == _abi.OK
+
+
+PACKED = dict(dtype=_abi.F16, q=1 << 30, k=2 << 30, v=3 << 30, out=4 << 30, q_strides=(256, 64), k_strides=(128, 64),
+              v_strides=(128, 64), out_strides=(256, 64), rows=100, keys=120, sequences=2, heads=4, kv_heads=2, dim=64,
+              causal=1, starts=5 << 30, k_starts=6 << 30, sm_scale=0.1)
+
+
+@pytest.mark.parametrize('change,fragment', [
+    (dict(dtype=_abi.F32), 'dtype'), (dict(dim=60), 'dim'), (dict(dim=264), 'dim'), (dict(dim=0), 'dim'),
+    (dict(heads=0), 'heads'), (dict(heads=5), 'heads'), (dict(kv_heads=0), 'heads'), (dict(heads=65538), 'heads'),
+    (dict(rows=-1), 'rows'), (dict(rows=1 << 27), 'rows'), (dict(keys=1 << 27), 'keys'), (dict(keys=-1), 'keys'),
+    (dict(sequences=1 << 20), 'sequences'), (dict(sequences=-1), 'sequences'), (dict(sm_scale=0.0), 'sm_scale'),
+    (dict(sm_scale=float('inf')), 'sm_scale'), (dict(causal=2), 'causal'), (dict(q=None), 'q null'),
+    (dict(k=(2 << 30) + 8), 'k null or misaligned'), (dict(v=None), 'v null'), (dict(out=None), 'out null'),
+    (dict(q_strides=(260, 64)), 'q strides'), (dict(k_strides=(128, -8)), 'k strides'), (dict(k_strides=(56, 64)), 'row strides'),
+    (dict(v_strides=(1 << 23, 64)), 'row strides'), (dict(starts=None), 'starts'), (dict(k_starts=None), 'starts'),
+    (dict(out_strides=(192, 64)), 'output rows overlap'), (dict(out_strides=(256, 0)), 'output rows overlap'),
+    (dict(out=1 << 30), 'overlaps an input'), (dict(out=(2 << 30) - 64), 'overlaps an input'),
+    (dict(out=(3 << 30) + 16), 'overlaps an input'), (dict(rows=(1 << 27) - 1, heads=64, kv_heads=64, q_strides=(4096, 64),
+                                                           out_strides=(4096, 64), out=1 << 44), 'too many'),
+])
+def test_packed_attention_refusals(change, fragment):
+    _refused('w8a8_packed_attention', _abi.PackedAttentionArgs(**{**PACKED, **change}), fragment)
+
+
+def test_packed_attention_of_nothing():
+    assert _status('w8a8_packed_attention', _abi.PackedAttentionArgs(**{**PACKED, 'rows': 0}))[0] == _abi.OK
+
+
+# ------------------------------------------------------------- the handle
+def _buffers(shape=(3, 2, 16, 64), dtype=torch.float16):
+    return torch.zeros(shape, dtype=dtype), torch.zeros(shape, dtype=dtype)
+
+
+def test_handle():
+    k, v = _buffers()
+    c = KVCache(k, v)
+    assert (c.heads, c.page_size, c.dim, c.codes) == (2, 16, 64, False)
+    c = KVCache.allocate(3, 48, 2, 72, dtype=torch.int8, device='cpu')
+    assert c.codes and c.k_scale.shape == (3, 2, 48) and c.k.shape == (3, 2, 48, 72)
+
+
+@pytest.mark.parametrize('shape', [(3, 2, 16), (0, 2, 16, 64), (3, 0, 16, 64), (3, 2, 24, 64), (3, 2, 4112, 64), (3, 2, 16, 60),
+                                   (3, 2, 16, 264), (3, 2, 0, 64)])
+def test_handles_are_refused(shape):
+    with pytest.raises(ValueError):
+        KVCache(*_buffers(shape))
+
+
+def test_handles_of_other_tensors_are_refused():
+    k, v = _buffers()
+    for a, b in ((k, v.bfloat16()), (k, v[:2]), (k.float(), v.float()), (k, torch.zeros((3, 16, 2, 64)).half().transpose(1, 2)),
+                 (k.transpose(2, 3).contiguous().transpose(2, 3),) * 2, (torch.zeros((3, 2, 16, 68)).half()[..., :64],) * 2,
+                 (torch.zeros(3 * 2 * 16 * 64 + 4).half()[4:].view(3, 2, 16, 64),) * 2):
+        with pytest.raises(ValueError):
+            KVCache(a, b)
+    s = torch.zeros((3, 2, 16))
+    k8, v8 = _buffers(dtype=torch.int8)
+    for args in ((k, v, s, s), (k8, v8), (k8, v8, s), (k8, v8, s, s.half()), (k8, v8, s, s[:2]),
+                 (k8, v8, s, torch.zeros((3, 16, 2)).transpose(1, 2)), (k8, v8, *(torch.zeros((3, 2, 18))[..., :16],) * 2)):
+        with pytest.raises(ValueError):
+            KVCache(*args)
+
+
+def _calls(grad=None, wrap=lambda t: t):
+    cache = KVCache(*_buffers())
+    table = torch.zeros((1, 1), dtype=torch.int32)
+    n, starts = torch.ones(1, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+    x, q = torch.zeros((1, 2, 64)).half(), torch.zeros((1, 4, 64)).half()
+    return {
+        'write': lambda: kv_cache.write(cache, wrap(x), x, table, n),
+        'write v': lambda: kv_cache.write(cache, x, wrap(x), table, n),
+        'read out': lambda: kv_cache.read(cache, table, starts, 1, out=(wrap(x), x)),
+        'attend': lambda: kv_cache.attend(wrap(q), cache, table, n),
+        'attend out': lambda: kv_cache.attend(q, cache, table, n, out=wrap(q.clone())),
+        'packed': lambda: packed_attention(wrap(q), x, x, starts),
+        'packed k': lambda: packed_attention(q, wrap(x), x, starts),
+        'packed v': lambda: packed_attention(q, x, wrap(x), starts),
+        'packed out': lambda: packed_attention(q, x, x, starts, out=wrap(q.clone())),
+        'a cache': lambda: kv_cache.attend(q, KVCache(wrap(cache.k), cache.v), table, n),
+    }
+
+
+def test_gradients_are_refused_not_lost():
+    for name, call in _calls(wrap=lambda t: t.clone().requires_grad_()).items():
+        with pytest.raises(ValueError, match='no gradient'):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match='HIP device'):
+            call()
+
+
+def test_forward_mode_tangents_are_refused():
+    with forward_ad.dual_level():
+        for name, call in _calls(wrap=lambda t: forward_ad.make_dual(t, torch.ones_like(t))).items():
+            with torch.no_grad(), pytest.raises(ValueError, match='no gradient'):
+                call()
+
+
+def test_cpu_tensors_are_refused():
+    for name, call in _calls().items():
+        with pytest.raises(ValueError, match='HIP device'):
+            call()

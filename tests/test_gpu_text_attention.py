@@ -1,0 +1,165 @@
+"""The cache and both attentions as a text encoder's serving step uses them:
+prompts, their keys and values into pages, a prompt's next part behind its
+cached keys, then tokens one by one. And the calls that are refused."""
+import pytest
+import torch
+
+from attention_refs import attention64, bound, check, check_packed, starts_of, table_of
+from w8a8 import axial_rope, kv_cache
+from w8a8.kv_cache import KVCache
+from w8a8.packed_attention import packed_attention
+
+pytestmark = pytest.mark.gpu
+
+HEADS, KV, DIM = 8, 2, 128
+
+
+def projections(rows, dtype, seed):
+    """Packed Q, K, V rows as one projection gives them."""
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn((rows, HEADS + 2 * KV, DIM), generator=g).to(dtype).cuda()
+
+
+@pytest.mark.parametrize('held,dtype', [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
+                                        (torch.int8, torch.bfloat16), (torch.int8, torch.float16)])
+def test_prompt_parts_and_tokens(gpu, held, dtype):
+    """Every route gives the attention of the whole sequences: a prompt at once, its second part behind the
+    cache's keys, and its last tokens one at a time. The reference runs over the keys and values that the
+    cache holds (16 bits as they are, codes as their values), packed, in 64 bits."""
+    total, part, tokens = [150, 40, 97], [60, 33, 1], 5
+    st, starts = starts_of(total, 'cuda')
+    rows = projections(st[-1], dtype, 3)
+    inv, axis = axial_rope.ladder((DIM // 2,), device=gpu)
+    pos = torch.cat([torch.arange(n) for n in total]).int()[:, None].cuda()
+    q, k = axial_rope.rotate(rows[:, :HEADS], rows[:, HEADS:HEADS + KV], pos, inv, axis)
+    v = rows[:, HEADS + KV:]
+    table, pages = table_of(total, 16, torch.Generator().manual_seed(1), 'cuda')
+    cache = KVCache.allocate(pages, 16, KV, DIM, dtype=held)
+
+    def rows_of(first, last):
+        """The packed rows [first[b], last[b]) of every sequence, and their starts."""
+        ids = torch.cat([torch.arange(st[b] + f, st[b] + n) for b, (f, n) in enumerate(zip(first, last))]).cuda()
+        return ids, starts_of([n - f for f, n in zip(first, last)], 'cuda')[1]
+
+    def lengths(n):
+        return torch.tensor(n, dtype=torch.int32, device='cuda')
+
+    outs = torch.zeros_like(q)
+    # the first part of every prompt, from the rows themselves; its keys go into pages
+    ids, s = rows_of([0] * 3, part)
+    outs[ids] = packed_attention(q[ids], k[ids], v[ids], s)
+    kv_cache.write(cache, k[ids], v[ids], table, lengths(part), s)
+    # the second part, up to the last tokens, over what the cache holds
+    upto = [n - tokens for n in total]
+    ids, s = rows_of(part, upto)
+    kv_cache.write(cache, k[ids], v[ids], table, lengths(upto), s)
+    ks, k_starts = starts_of(upto, 'cuda')
+    ck, cv = kv_cache.read(cache, table, k_starts, ks[-1], dtype=dtype)
+    outs[ids] = packed_attention(q[ids], ck, cv, s, k_starts)
+    # the last tokens, one by one
+    for i in range(tokens):
+        n = [m + i + 1 for m in upto]
+        ids, _ = rows_of([m - 1 for m in n], n)
+        kv_cache.write(cache, k[ids], v[ids], table, lengths(n))
+        outs[ids] = kv_cache.attend(q[ids], cache, table, lengths(n))
+    hk, hv = kv_cache.read(cache, table, starts, st[-1], dtype=dtype)
+    if held != torch.int8:
+        assert torch.equal(hk, k) and torch.equal(hv, v)
+        check_packed(outs, q, hk, hv, st, st, True, DIM ** -0.5)
+        return
+    # with codes the first parts saw the rows themselves, the second what `read` rounds to 16 bits
+    for b in range(3):
+        a, z = st[b] + part[b], st[b + 1] - tokens
+        check_packed(outs[st[b]:a], q[st[b]:a], k[st[b]:a], v[st[b]:a], [0, part[b]], [0, part[b]], True, DIM ** -0.5)
+        check_packed(outs[a:z], q[a:z], hk[st[b]:z], hv[st[b]:z], [0, z - a], [0, z - st[b]], True, DIM ** -0.5)
+    for b in range(3):   # the tokens see the codes' exact values
+        ids = torch.arange(total[b], device='cuda')
+        at, off = table[b].long()[ids // 16], ids % 16
+        for h in range(HEADS):
+            j = h // (HEADS // KV)
+            vs = cache.v_scale[at, j, off].double()[:, None]
+            k64, v64 = cache.k[at, j, off].double() * cache.k_scale[at, j, off].double()[:, None], cache.v[at, j, off].double()
+            first = torch.arange(total[b] - tokens + 1, total[b] + 1, device='cuda')
+            z = slice(st[b + 1] - tokens, st[b + 1])
+            o, parts = attention64(q[z, h].double(), k64, v64 * vs, DIM ** -0.5, first, codes_scale=v64.abs() * vs.max())
+            check(outs[z, h], o, bound(o, parts, dtype), f'tokens of sequence {b} head {h}')
+
+
+def test_refusals(gpu):
+    cache = KVCache.allocate(3, 16, 2, 64)
+    codes = KVCache.allocate(3, 16, 2, 64, dtype=torch.int8)
+    table = torch.zeros((2, 2), dtype=torch.int32, device='cuda')
+    n, starts = (torch.tensor(x, dtype=torch.int32, device='cuda') for x in ([1, 2], [0, 1, 3]))
+    x, q = torch.zeros((3, 2, 64), device='cuda').half(), torch.zeros((2, 4, 64), device='cuda').half()
+    bad = [
+        lambda: kv_cache.write(cache, x.bfloat16(), x.bfloat16(), table, n, starts),
+        lambda: kv_cache.write(codes, x.float(), x.float(), table, n, starts),
+        lambda: kv_cache.write(cache, x, x[:2], table, n, starts),
+        lambda: kv_cache.write(codes, x, x.bfloat16(), table, n, starts),
+        lambda: kv_cache.write(cache, x[:, :1], x[:, :1], table, n, starts),
+        lambda: kv_cache.write(cache, x[..., :32], x[..., :32], table, n, starts),
+        lambda: kv_cache.write(cache, x, x, table, n),
+        lambda: kv_cache.write(cache, x, x, table.long(), n, starts),
+        lambda: kv_cache.write(cache, x, x, table[0], n, starts),
+        lambda: kv_cache.write(cache, x, x, table, n.long(), starts),
+        lambda: kv_cache.write(cache, x, x, table, n[:1], starts),
+        lambda: kv_cache.write(cache, x, x, table, n, starts[:2]),
+        lambda: kv_cache.write(cache, x, x, table, n, starts.long()),
+        lambda: kv_cache.write(cache, x, x, table, n.cpu(), starts),
+        lambda: kv_cache.read(cache, table, starts, 3, dtype=torch.bfloat16),
+        lambda: kv_cache.read(codes, table, starts, 3, dtype=torch.float32),
+        lambda: kv_cache.read(cache, table, starts[:2], 3),
+        lambda: kv_cache.read(cache, table, starts, 3, out=(x, x[:2])),
+        lambda: kv_cache.read(cache, table, starts, 3, out=(x, x.bfloat16())),
+        lambda: kv_cache.read(cache, table, starts, 3, out=(x.transpose(1, 2).contiguous().transpose(1, 2), x)),
+        lambda: kv_cache.read(cache, table, starts, 3, out=(x[:1].expand(3, 2, 64), x)),
+        lambda: kv_cache.attend(q[:1], cache, table, n),
+        lambda: kv_cache.attend(q[:, :3], cache, table, n),
+        lambda: kv_cache.attend(q[:, :0], cache, table, n),
+        lambda: kv_cache.attend(q[..., :32], cache, table, n),
+        lambda: kv_cache.attend(q.bfloat16(), cache, table, n),
+        lambda: kv_cache.attend(q.float(), codes, table, n),
+        lambda: kv_cache.attend(q, cache, table, n.float()),
+        lambda: kv_cache.attend(q, cache, table, n, scale=0.0),
+        lambda: kv_cache.attend(q, cache, table, n, scale=-0.1),
+        lambda: kv_cache.attend(q, cache, table, n, scale=float('nan')),
+        lambda: kv_cache.attend(q, cache, table, n, out=q[:1]),
+        lambda: kv_cache.attend(q, cache, table, n, out=q.bfloat16()),
+        lambda: kv_cache.attend(q, cache, table, n, out=torch.empty((2, 64, 4), device='cuda').half().transpose(1, 2)),
+        lambda: packed_attention(q, x, x, starts),
+        lambda: packed_attention(x, x, x.bfloat16(), starts),
+        lambda: packed_attention(x.float(), x.float(), x.float(), starts),
+        lambda: packed_attention(x, x, x[:2], starts, starts),
+        lambda: packed_attention(x, x[..., :32], x[..., :32], starts),
+        lambda: packed_attention(x[..., :60], x[..., :60], x[..., :60], starts),
+        lambda: packed_attention(x[:, :1], x, x, starts),
+        lambda: packed_attention(x[:, :0], x, x, starts),
+        lambda: packed_attention(x, x, x, starts.long()),
+        lambda: packed_attention(x, x, x, starts, starts[:2]),
+        lambda: packed_attention(x, x, x, starts[:0]),
+        lambda: packed_attention(x, x, x, starts, scale=float('inf')),
+        lambda: packed_attention(x, x, x, starts, out=x[:2]),
+        lambda: packed_attention(x, x, x, starts, out=x[:1].expand(3, 2, 64)),
+        lambda: packed_attention(x[0], x, x, starts),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            print(i)   # (the call that was taken)
+
+
+def test_writes_are_counted(gpu):
+    """Autograd sees that a tensor it saved has changed."""
+    cache = KVCache.allocate(3, 16, 2, 64, dtype=torch.int8)
+    table = torch.zeros((1, 2), dtype=torch.int32, device='cuda')
+    n, starts = (torch.tensor(t, dtype=torch.int32, device='cuda') for t in ([3], [0, 3]))
+    x, q = torch.zeros((3, 2, 64), device='cuda').half(), torch.zeros((1, 4, 64), device='cuda').half()
+    before = [t._version for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    kv_cache.write(cache, x, x, table, n, starts)
+    assert all(t._version > b for t, b in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), before))
+    outs = [torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(q), torch.zeros_like(x)]
+    before = [t._version for t in outs]
+    kv_cache.read(cache, table, starts, 3, out=(outs[0], outs[1]))
+    kv_cache.attend(q, cache, table, n, out=outs[2])
+    packed_attention(x, x, x, starts, out=outs[3])
+    assert all(t._version > b for t, b in zip(outs, before))
