@@ -624,6 +624,254 @@ PyObject* linear_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// --------------------------------------- the paged cache and packed attention
+
+// Element strides {row, head} of a [rows, heads, dim] tensor of 16-bit values
+// that the kernels take as it lies (kernels._row_head_strides).
+bool row_head_strides(const at::Tensor& t, int64_t (&st)[2]) {
+  if (t.dim() != 3 || (t.size(2) > 1 && t.stride(2) != 1) || !aligned(t, 16)) return false;
+  const int64_t rows = t.size(0), heads = t.size(1), dim = t.size(2);
+  st[1] = heads > 1 ? t.stride(1) : dim;
+  st[0] = rows > 1 ? t.stride(0) : std::max(heads * dim, (heads - 1) * st[1] + dim);
+  return st[0] % 8 == 0 && st[1] % 8 == 0 && st[0] >= dim && st[1] >= dim;
+}
+
+bool int_vector(const at::Tensor* t, int64_t n) {
+  return t && t->scalar_type() == at::kInt && t->dim() == 1 && (n < 0 || t->size(0) == n) && t->is_contiguous();
+}
+
+// The cache of four arguments (k, v, k_scale, v_scale), whose handle has
+// checked its layout; its tensors for written().
+struct CacheArg {
+  const at::Tensor* t[4];
+  bool codes;
+};
+bool cache_arg(PyObject* const* args, CacheArg& c, W8A8KvCache& v) {
+  bool ok = true;
+  for (int i = 0; i < 4; ++i) c.t[i] = optional(args[i], ok);
+  if (!ok || !c.t[0] || !c.t[1] || c.t[0]->dim() != 4 || c.t[1]->sizes() != c.t[0]->sizes() ||
+      c.t[1]->strides() != c.t[0]->strides() || c.t[1]->scalar_type() != c.t[0]->scalar_type() ||
+      wants_gradient({c.t[0], c.t[1], c.t[2], c.t[3]}))
+    return false;
+  const at::Tensor& k = *c.t[0];
+  c.codes = k.scalar_type() == at::kChar;
+  v.dtype = c.codes ? W8A8_I8 : dtype_code(k.scalar_type());
+  if (!v.dtype || (c.codes && (!c.t[2] || !c.t[3] || c.t[2]->dim() != 3 || c.t[3]->strides() != c.t[2]->strides() ||
+                               c.t[2]->scalar_type() != at::kFloat || c.t[3]->scalar_type() != at::kFloat)))
+    return false;
+  v.k = k.data_ptr();
+  v.v = c.t[1]->data_ptr();
+  v.pages = k.size(0);
+  for (int i = 0; i < 3; ++i) v.strides[i] = k.stride(i);
+  v.heads = (int32_t)k.size(1);
+  v.page_size = (int32_t)k.size(2);
+  v.dim = (int32_t)k.size(3);
+  if (c.codes) {
+    v.k_scale = ptr<float>(*c.t[2]);
+    v.v_scale = ptr<float>(*c.t[3]);
+    v.scale_strides[0] = c.t[2]->stride(0);
+    v.scale_strides[1] = c.t[2]->stride(1);
+  }
+  return true;
+}
+
+// Rows for a cache: fp16 or bf16, a 16-bit cache's own.
+bool cache_rows(const at::Tensor& t, const W8A8KvCache& c) {
+  return t.dim() == 3 && t.size(2) == c.dim && (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) &&
+         (c.dtype == W8A8_I8 || c.dtype == dtype_code(t.scalar_type()));
+}
+
+template <typename Args>
+bool table_arg(const at::Tensor* t, Args& a) {
+  if (!t || t->dim() != 2 || t->scalar_type() != at::kInt || !t->is_contiguous()) return false;
+  a.sequences = t->size(0);
+  a.page_table = ptr<int32_t>(*t);
+  a.ld_table = a.table_width = t->size(1);
+  return a.sequences > 0;
+}
+
+// cache_write(cache k, v, k_scale, v_scale, k, v, page_table, lengths, starts):
+// kernels.cache_write; True when done.
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || modes_active()) Py_RETURN_NONE;
+  bool ok = true;
+  CacheArg c;
+  W8A8CacheWriteArgs a{};
+  if (!cache_arg(args, c, a.cache)) Py_RETURN_NONE;
+  const at::Tensor* k = plain(args[4]);
+  const at::Tensor* v = plain(args[5]);
+  const at::Tensor* lengths = plain(args[7]);
+  const at::Tensor* starts = optional(args[8], ok);
+  if (!k || !v || !ok || !table_arg(plain(args[6]), a) || !cache_rows(*k, a.cache) || k->size(1) != a.cache.heads ||
+      v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() || k->size(0) == 0 ||
+      !row_head_strides(*k, a.k_strides) || !row_head_strides(*v, a.v_strides) || !int_vector(lengths, a.sequences) ||
+      (starts ? !int_vector(starts, a.sequences + 1) : k->size(0) != a.sequences) || wants_gradient({k, v}))
+    Py_RETURN_NONE;
+  a.dtype = dtype_code(k->scalar_type());
+  a.k = k->data_ptr();
+  a.v = v->data_ptr();
+  a.rows = k->size(0);
+  a.lengths = ptr<int32_t>(*lengths);
+  a.starts = starts ? ptr<int32_t>(*starts) : nullptr;
+  a.stream = stream_of(k->get_device());
+  const int rc = call(w8a8_cache_write, a);
+  if (rc != W8A8_OK) return fail("w8a8_cache_write", rc);
+  for (const at::Tensor* t : c.t) written(t);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_read(cache k, v, k_scale, v_scale, page_table, starts, rows, dtype |
+// None): kernels.cache_read into new outputs; returns (k, v).
+PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || modes_active() || !PyLong_CheckExact(args[6]) || (args[7] != Py_None && !THPDtype_Check(args[7])))
+    Py_RETURN_NONE;
+  CacheArg c;
+  W8A8CacheReadArgs a{};
+  if (!cache_arg(args, c, a.cache)) Py_RETURN_NONE;
+  const at::Tensor* starts = plain(args[5]);
+  int overflow = 0;
+  a.rows = PyLong_AsLongLongAndOverflow(args[6], &overflow);
+  const at::ScalarType type = args[7] != Py_None ? reinterpret_cast<THPDtype*>(args[7])->scalar_type
+                              : c.codes          ? at::kHalf
+                                                 : c.t[0]->scalar_type();
+  if (overflow || a.rows <= 0 || !table_arg(plain(args[4]), a) || !int_vector(starts, a.sequences + 1) ||
+      (type != at::kHalf && type != at::kBFloat16) || (!c.codes && type != c.t[0]->scalar_type()))
+    Py_RETURN_NONE;
+  const auto opt = at::TensorOptions().device(c.t[0]->device()).dtype(type);
+  const int64_t heads = a.cache.heads, dim = a.cache.dim;
+  at::Tensor k = at::empty({a.rows, heads, dim}, opt), v = at::empty({a.rows, heads, dim}, opt);
+  a.dtype = dtype_code(type);
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_strides[0] = a.v_strides[0] = heads * dim;
+  a.k_strides[1] = a.v_strides[1] = dim;
+  a.starts = ptr<int32_t>(*starts);
+  a.fill = 1;
+  a.stream = stream_of(k.get_device());
+  const int rc = call(w8a8_cache_read, a);
+  if (rc != W8A8_OK) return fail("w8a8_cache_read", rc);
+  PyObject* pk = THPVariable_Wrap(std::move(k));
+  PyObject* pv = THPVariable_Wrap(std::move(v));
+  PyObject* r = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
+  Py_XDECREF(pk);
+  Py_XDECREF(pv);
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// The softmax scale: what kernels._positive takes.
+bool scale_arg(PyObject* o, int64_t dim, float& scale) {
+  bool given = false;
+  if (!optional_float(o, scale, given)) return false;
+  if (!given) scale = (float)std::pow((double)dim, -0.5);
+  return scale > 1e-37f && scale < 1e37f;
+}
+
+// cache_attend(cache k, v, k_scale, v_scale, q, page_table, lengths, scale,
+// out): kernels.cache_attend.
+PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || modes_active()) Py_RETURN_NONE;
+  bool ok = true;
+  CacheArg c;
+  W8A8CacheAttendArgs a{};
+  if (!cache_arg(args, c, a.cache)) Py_RETURN_NONE;
+  const at::Tensor* q = plain(args[4]);
+  const at::Tensor* lengths = plain(args[6]);
+  const at::Tensor* out = optional(args[8], ok);
+  if (!q || !ok || !table_arg(plain(args[5]), a) || !cache_rows(*q, a.cache) || q->size(0) != a.sequences ||
+      q->size(1) <= 0 || q->size(1) % a.cache.heads || !row_head_strides(*q, a.q_strides) ||
+      !int_vector(lengths, a.sequences) || !scale_arg(args[7], a.cache.dim, a.sm_scale) || wants_gradient({q, out}) ||
+      (out && (out->sizes() != q->sizes() || out->scalar_type() != q->scalar_type() ||
+               !row_head_strides(*out, a.out_strides))))
+    Py_RETURN_NONE;
+  const auto opt = at::TensorOptions().device(q->device());
+  at::Tensor fresh, workspace;
+  if (!out) {
+    fresh = at::empty(q->sizes(), opt.dtype(q->scalar_type()));
+    row_head_strides(fresh, a.out_strides);
+  }
+  a.heads = q->size(1);
+  a.workspace_bytes = w8a8_cache_attend_workspace_size(a.sequences, a.heads, a.cache.heads, a.cache.dim,
+                                                       a.table_width * a.cache.page_size);
+  if (a.workspace_bytes > 0) {
+    workspace = at::empty({a.workspace_bytes}, opt.dtype(at::kByte));
+    a.workspace = workspace.data_ptr();
+  }
+  a.dtype = dtype_code(q->scalar_type());
+  a.q = q->data_ptr();
+  a.out = out ? out->data_ptr() : fresh.data_ptr();
+  a.lengths = ptr<int32_t>(*lengths);
+  a.stream = stream_of(q->get_device());
+  const int rc = call(w8a8_cache_attend, a);
+  if (rc != W8A8_OK) return fail("w8a8_cache_attend", rc);
+  written(out);
+  return out ? Py_NewRef(args[8]) : THPVariable_Wrap(std::move(fresh));
+  END_HANDLE_TH_ERRORS
+}
+
+// packed_attention(q, k, v, starts, k_starts, causal, scale, out):
+// kernels.packed_attention.
+PyObject* packed_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || modes_active() || !PyBool_Check(args[5])) Py_RETURN_NONE;
+  bool ok = true;
+  const at::Tensor* q = plain(args[0]);
+  const at::Tensor* k = plain(args[1]);
+  const at::Tensor* v = plain(args[2]);
+  const at::Tensor* starts = plain(args[3]);
+  const at::Tensor* k_starts = optional(args[4], ok);
+  const at::Tensor* out = optional(args[7], ok);
+  W8A8PackedAttentionArgs a{};
+  if (!q || !k || !v || !ok || !row_head_strides(*q, a.q_strides) || !row_head_strides(*k, a.k_strides) ||
+      !row_head_strides(*v, a.v_strides))
+    Py_RETURN_NONE;
+  const at::ScalarType type = q->scalar_type();
+  const int64_t heads = q->size(1), dim = q->size(2), kv_heads = k->size(1);
+  a.rows = q->size(0);
+  a.keys = k->size(0);
+  if ((type != at::kHalf && type != at::kBFloat16) || k->scalar_type() != type || v->scalar_type() != type ||
+      v->sizes() != k->sizes() || k->size(2) != dim || dim < 8 || dim > 256 || dim % 8 || heads <= 0 || kv_heads <= 0 ||
+      heads % kv_heads || heads > 65536 || a.rows <= 0 || a.keys <= 0 || !int_vector(starts, -1) || starts->size(0) < 1 ||
+      (k_starts ? !int_vector(k_starts, starts->size(0)) : a.keys != a.rows) || !scale_arg(args[6], dim, a.sm_scale) ||
+      wants_gradient({q, k, v, out}) ||
+      (out && (out->sizes() != q->sizes() || out->scalar_type() != type || !row_head_strides(*out, a.out_strides))))
+    Py_RETURN_NONE;
+  const auto opt = at::TensorOptions().device(q->device());
+  at::Tensor fresh, workspace;
+  if (!out) {
+    fresh = at::empty({a.rows, heads, dim}, opt.dtype(type));
+    row_head_strides(fresh, a.out_strides);
+  }
+  a.sequences = starts->size(0) - 1;
+  a.workspace_bytes = w8a8_packed_attention_workspace_size(a.rows, a.keys, a.sequences, heads, (int32_t)dim);
+  if (a.workspace_bytes > 0) {
+    workspace = at::empty({a.workspace_bytes}, opt.dtype(at::kByte));
+    a.workspace = workspace.data_ptr();
+  }
+  a.dtype = dtype_code(type);
+  a.q = q->data_ptr();
+  a.k = k->data_ptr();
+  a.v = v->data_ptr();
+  a.out = out ? out->data_ptr() : fresh.data_ptr();
+  a.heads = (int32_t)heads;
+  a.kv_heads = (int32_t)kv_heads;
+  a.dim = (int32_t)dim;
+  a.causal = args[5] == Py_True;
+  a.starts = ptr<int32_t>(*starts);
+  a.k_starts = k_starts ? ptr<int32_t>(*k_starts) : a.starts;
+  a.fill = out ? 0 : 1;
+  a.stream = stream_of(q->get_device());
+  const int rc = call(w8a8_packed_attention, a);
+  if (rc != W8A8_OK) return fail("w8a8_packed_attention", rc);
+  written(out);
+  return out ? Py_NewRef(args[7]) : THPVariable_Wrap(std::move(fresh));
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_error_class(PyObject*, PyObject* cls) {
   Py_INCREF(cls);
   Py_XSETREF(g_error_class, cls);
@@ -643,6 +891,10 @@ PyMODINIT_FUNC PyInit__native() {
       {"residual_norm", fast(residual_norm), METH_FASTCALL, nullptr},
       {"axial_rope", fast(axial_rope), METH_FASTCALL, nullptr},
       {"linear_w4", fast(linear_w4), METH_FASTCALL, nullptr},
+      {"cache_write", fast(cache_write), METH_FASTCALL, nullptr},
+      {"cache_read", fast(cache_read), METH_FASTCALL, nullptr},
+      {"cache_attend", fast(cache_attend), METH_FASTCALL, nullptr},
+      {"packed_attention", fast(packed_attention), METH_FASTCALL, nullptr},
       {"set_error_class", set_error_class, METH_O, nullptr},
       {nullptr, nullptr, 0, nullptr},
   };

@@ -16,7 +16,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import kernels
+from . import _abi, kernels
 
 
 @dataclass(frozen=True)
@@ -94,7 +94,8 @@ def write(cache, k, v, page_table, lengths, starts=None):
     one place (a page that is listed twice), either may remain, or a mixture.
     Codes are those of the activation quantizer; a row that holds an infinity
     or a NaN gets the scale NaN."""
-    kernels.cache_write(cache, k, v, page_table, lengths, starts)
+    if not _abi.native().cache_write(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, page_table, lengths, starts):
+        kernels.cache_write(cache, k, v, page_table, lengths, starts)
 
 
 def read(cache, page_table, starts, rows, *, dtype=None, out=None):
@@ -104,6 +105,10 @@ def read(cache, page_table, starts, rows, *, dtype=None, out=None):
     stand for (a 16-bit cache gives its own). out: (k, v) to write into, whose
     rows behind the last sequence stay as they are; new outputs have zeros
     there. What packed_attention takes for a prompt's next part."""
+    if out is None:
+        r = _abi.native().cache_read(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, starts, rows, dtype)
+        if r is not None:
+            return r
     return kernels.cache_read(cache, page_table, starts, rows, dtype=dtype, out=out)
 
 
@@ -113,4 +118,7 @@ def attend(q, cache, page_table, lengths, *, scale=None, out=None):
     once written): softmax(scale q . k) v, query head h with the cache's head
     h // (heads / cache.heads). scale: 1 / sqrt(dim) by default. A sequence
     without keys gives 0. Inference only."""
+    y = _abi.native().cache_attend(cache.k, cache.v, cache.k_scale, cache.v_scale, q, page_table, lengths, scale, out)
+    if y is not None:
+        return y
     return kernels.cache_attend(q, cache, page_table, lengths, scale=scale, out=out)

@@ -5,7 +5,7 @@ tp_qwen3vl mirrors (patches/tp_qwen3vl.py:259 takes its output), and of image
 encoders; the INT8 attention (int8_attention) takes equal lengths without a mask. This one takes the prompts of several requests, or the images
 of an encoder, as they lie one behind the other, in fp16 or bf16.
 """
-from . import kernels
+from . import _abi, kernels
 
 
 def packed_attention(q, k, v, starts, k_starts=None, *, causal=True, scale=None, out=None):
@@ -21,4 +21,7 @@ def packed_attention(q, k, v, starts, k_starts=None, *, causal=True, scale=None,
     included. scale: 1 / sqrt(dim) by default. out: to write into, its rows
     behind the last sequence staying as they are; a new output has zeros there.
     Inference only."""
+    y = _abi.native().packed_attention(q, k, v, starts, k_starts, causal, scale, out)
+    if y is not None:
+        return y
     return kernels.packed_attention(q, k, v, starts, k_starts, causal=causal, scale=scale, out=out)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from attention_refs import attention64, bound, check, check_packed, starts_of, table_of
-from w8a8 import axial_rope, kv_cache
+from w8a8 import _abi, axial_rope, kernels, kv_cache
 from w8a8.kv_cache import KVCache
 from w8a8.packed_attention import packed_attention
 
@@ -163,3 +163,32 @@ def test_writes_are_counted(gpu):
     kv_cache.attend(q, cache, table, n, out=outs[2])
     packed_attention(x, x, x, starts, out=outs[3])
     assert all(t._version > b for t, b in zip(outs, before))
+
+
+def test_host_routes_give_the_same_bits(gpu):
+    """The native calls and the Python route that they fall back to."""
+    g = torch.Generator().manual_seed(2)
+    total = [40, 0, 90]
+    st, starts = starts_of(total, 'cuda')
+    table, pages = table_of(total, 16, g, 'cuda')
+    n = torch.tensor(total, dtype=torch.int32, device='cuda')
+    for held, dtype in ((torch.float16,) * 2, (torch.int8, torch.bfloat16)):
+        rows = projections(st[-1], dtype, 4)
+        q, k, v = rows[:, :HEADS], rows[:, HEADS:HEADS + KV], rows[:, HEADS + KV:]
+        one, two = (KVCache.allocate(pages, 16, KV, DIM, dtype=held) for _ in range(2))
+        args = (one.k, one.v, one.k_scale, one.v_scale)
+        native = _abi.native()
+        assert native.cache_write(*args, k, v, table, n, starts) is True
+        kernels.cache_write(two, k, v, table, n, starts)
+        assert all(a is None or torch.equal(a, b) for a, b in zip(args, (two.k, two.v, two.k_scale, two.v_scale)))
+        for a, b in zip(native.cache_read(*args, table, starts, st[-1], dtype),
+                        kernels.cache_read(two, table, starts, st[-1], dtype=dtype)):
+            assert torch.equal(a, b)
+        x = rows[:3, :HEADS]
+        out = torch.empty_like(x)
+        for scale in (None, 0.2):
+            want = kernels.cache_attend(x, two, table, n, scale=scale)
+            assert torch.equal(native.cache_attend(*args, x, table, n, scale, None), want)
+            assert native.cache_attend(*args, x, table, n, scale, out) is out and torch.equal(out, want)
+            want = kernels.packed_attention(q, k, v, starts, causal=False, scale=scale)
+            assert torch.equal(native.packed_attention(q, k, v, starts, starts, False, scale, None), want)
