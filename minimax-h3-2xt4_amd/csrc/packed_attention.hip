@@ -22,6 +22,7 @@
 #include "paged.h"
 
 #include <type_traits>
+#include <utility>
 
 namespace w8a8 {
 
@@ -52,6 +53,25 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+}
+
+// The reference of p may lie so much below the maximum (as a power of 2): p is
+// at most 2^kSlack, far inside both types, and rescaling the sums is rare.
+constexpr float kSlack = 8.0f;
+
+// l plus the two DT values of a word.
+template <int DT>
+__device__ __forceinline__ float add2(uint32_t w, float l) {
+  if constexpr (DT == kF16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), l, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, w), __builtin_bit_cast(v2b, 0x3f803f80u), l, false);
+}
+
+// Both halves' values of a pair of lanes l, l ^ 32.
+__device__ __forceinline__ std::pair<float, float> lane_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return {__uint_as_float(r[0]), __uint_as_float(r[1])};
 }
 
 // Chunks of 16 bytes: a key row of 2 DP bytes spans all banks (DP 128, 256), half
@@ -108,43 +128,68 @@ __device__ __forceinline__ PackedTile packed_find(const PackedParams& p, int t) 
   return {-1, 0, 0, 0};
 }
 
-// DT: F16 or BF16; DP: dim rounded up to 64, 96, 128 or 256.
+// What a workgroup and its waves work on, DP channels wide, BK keys a block.
+// TID is the thread's index (a copy of it that the compiler takes for another
+// value keeps nothing alive from the one's use to the other's).
 template <int DT, int DP, bool CAUSAL>
-__global__ __launch_bounds__(64 * kPackWaves, 2) void packed_attention_kernel(PackedParams p) {
-  constexpr int BK = DP > 128 ? 32 : 64;      // keys of a block
-  constexpr int CH = DP / 8;                  // chunks of a row
-  constexpr int NS = DP / 16, DF = DP / 32;   // steps of Q K^T, channel tiles of O^T
-  constexpr int TF = BK / 32;                 // score tiles
-  constexpr int kTile = BK * DP * 2;
-  constexpr int kDma = kTile / (1024 * kPackWaves);   // DMA instructions of a wave for a tile
-  __shared__ __attribute__((aligned(1024))) char kt[2][kTile], vt[2][kTile];
-  __shared__ int again;
-  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int item = blockIdx.x / p.kv_heads, kvh = blockIdx.x - item * p.kv_heads;
-  const int head = kvh * p.group + item % p.group;
-  const PackedTile tile = packed_find(p, item / p.group);
-  if (tile.b < 0) return;
-  const int q0 = tile.first + 32 * wave;      // the wave's first query of its sequence
-  const int mine = q0 + col;
-  const bool stored = mine < tile.n;
-  char* to = p.out + (int64_t)(tile.row0 + min(mine, tile.n - 1)) * p.o_row + head * p.o_head;
-  if (tile.b == p.sequences) {
-    if (p.fill && stored)
-      for (int d = 4 * half; d < p.dim; d += 8) *reinterpret_cast<uint2*>(to + 2 * d) = make_uint2(0, 0);
-    return;
-  }
-  const int key0 = clamp_to(scalar_int(p.k_starts, tile.b), 0, p.keys);
-  const int nk = clamp_to(scalar_int(p.k_starts, tile.b + 1), key0, p.keys) - key0;
-  const int shift = nk - tile.n;              // causal: query i sees keys up to i + shift
-  const int seen = CAUSAL ? clamp_to(tile.first + kPackQ + shift, 0, nk) : nk;   // of the workgroup
-  const int blocks = (seen + BK - 1) / BK;
-  const int limit = CAUSAL ? clamp_to(mine + shift + 1, 0, nk) : nk;             // of this query
-  const int wave_clean = CAUSAL ? clamp_to(q0 + shift + 1, 0, nk) : nk;          // keys that all of the wave see
-  const int wave_seen = CAUSAL ? clamp_to(q0 + 32 + shift, 0, nk) : nk;          // keys that some of it see
+struct Packed {
+  static constexpr int BK = DP > 128 ? 32 : 64;      // keys of a block
+  static constexpr int CH = DP / 8;                  // chunks of a row
+  static constexpr int NS = DP / 16, DF = DP / 32;   // steps of Q K^T, channel tiles of O^T
+  static constexpr int TF = BK / 32;                 // score tiles
+  static constexpr int kTile = BK * DP * 2;
+  static constexpr int kDma = kTile / (1024 * kPackWaves);   // DMA instructions of a wave for a tile
 
-  v4u qf[NS];
-  {
+  const PackedParams& p;
+  char* tiles;
+  int lane, wave, col, half;
+  PackedTile tile;
+  int head, mine, key0, nk;
+  bool stored;
+  int blocks, limit, wave_clean, wave_blocks;
+  const char* kbase;
+  const char* vbase;
+  uint32_t ksrc[kDma], vsrc[kDma];
+
+  __device__ __forceinline__ Packed(const PackedParams& p_, char* tiles_, int tid) : p(p_), tiles(tiles_) {
+    lane = tid & 63;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    col = lane & 31;
+    half = lane >> 5;
+    const int item = blockIdx.x / p.kv_heads, kvh = blockIdx.x - item * p.kv_heads;
+    head = kvh * p.group + item % p.group;
+    tile = packed_find(p, item / p.group);
+    if (tile.b < 0) return;
+    const int q0 = tile.first + 32 * wave;      // the wave's first query of its sequence
+    mine = q0 + col;
+    stored = mine < tile.n;
+    if (tile.b == p.sequences) return;
+    key0 = clamp_to(scalar_int(p.k_starts, tile.b), 0, p.keys);
+    nk = clamp_to(scalar_int(p.k_starts, tile.b + 1), key0, p.keys) - key0;
+    const int shift = nk - tile.n;              // causal: query i sees keys up to i + shift
+    const int seen = CAUSAL ? clamp_to(tile.first + kPackQ + shift, 0, nk) : nk;   // keys that the workgroup sees,
+    limit = CAUSAL ? clamp_to(mine + shift + 1, 0, nk) : nk;                       // this query,
+    wave_clean = CAUSAL ? clamp_to(q0 + shift + 1, 0, nk) : nk;                    // all of the wave's,
+    wave_blocks = ((CAUSAL ? clamp_to(q0 + 32 + shift, 0, nk) : nk) + BK - 1) / BK;   // and some of them (in blocks)
+    blocks = (seen + BK - 1) / BK;
+    kbase = p.k + (int64_t)key0 * p.k_row + kvh * p.k_head;
+    vbase = p.v + (int64_t)key0 * p.v_row + kvh * p.v_head;
+    // Copies of a tile: lane l of instruction u of wave w brings what lies at
+    // chunk (4 u + w) * 64 + l of the tile.
+#pragma unroll
+    for (int u = 0; u < kDma; ++u) {
+      const int at = (u * kPackWaves + wave) * 64 + lane, r = at / CH, c = at - r * CH;
+      const int ck = c ^ k_swizzle<DP>(r), cv = c ^ v_swizzle<DP>(r);
+      ksrc[u] = 8 * ck < p.dim ? r * p.k_row + 16 * ck : 0x7fffff00u;
+      vsrc[u] = 8 * cv < p.dim ? r * p.v_row + 16 * cv : 0x7fffff00u;
+    }
+  }
+
+  __device__ __forceinline__ char* to() const {
+    return p.out + (int64_t)(tile.row0 + min(mine, tile.n - 1)) * p.o_row + head * p.o_head;
+  }
+
+  __device__ __forceinline__ void queries(v4u (&qf)[NS]) const {
     const char* from = p.q + (int64_t)(tile.row0 + min(mine, tile.n - 1)) * p.q_row + head * p.q_head;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -154,19 +199,10 @@ __global__ __launch_bounds__(64 * kPackWaves, 2) void packed_attention_kernel(Pa
     }
   }
 
-  // Copies of a tile: lane l of instruction u of wave w brings what lies at
-  // chunk (4 u + w) * 64 + l of the tile.
-  uint32_t ksrc[kDma], vsrc[kDma];
-#pragma unroll
-  for (int u = 0; u < kDma; ++u) {
-    const int at = (u * kPackWaves + wave) * 64 + lane, r = at / CH, c = at - r * CH;
-    const int ck = c ^ k_swizzle<DP>(r), cv = c ^ v_swizzle<DP>(r);
-    ksrc[u] = 8 * ck < p.dim ? r * p.k_row + 16 * ck : 0x7fffff00u;
-    vsrc[u] = 8 * cv < p.dim ? r * p.v_row + 16 * cv : 0x7fffff00u;
-  }
-  const char* kbase = p.k + (int64_t)key0 * p.k_row + kvh * p.k_head;
-  const char* vbase = p.v + (int64_t)key0 * p.v_row + kvh * p.v_head;
-  auto copy = [&](const char* base, uint32_t row_b, const uint32_t (&src)[kDma], int block, char* dst) {
+  __device__ __forceinline__ char* kt(int i) const { return tiles + i * kTile; }
+  __device__ __forceinline__ char* vt(int i) const { return tiles + (2 + i) * kTile; }
+  __device__ __forceinline__ void copy(const char* base, uint32_t row_b, const uint32_t (&src)[kDma], int block,
+                                       char* dst) const {
     const int rows = min(nk - block * BK, BK);
     const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + (int64_t)block * BK * row_b), 0,
                                                      (int)((rows - 1) * row_b) + 2 * p.dim, 0x00027000);
@@ -174,177 +210,346 @@ __global__ __launch_bounds__(64 * kPackWaves, 2) void packed_attention_kernel(Pa
     for (int u = 0; u < kDma; ++u)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           r, (__attribute__((address_space(3))) void*)(dst + (u * kPackWaves + wave) * 1024), 16, (int)src[u], 0, 0, 0);
-  };
-  auto copy_block = [&](int block, int buf) {
-    copy(kbase, p.k_row, ksrc, block, kt[buf]);
-    copy(vbase, p.v_row, vsrc, block, vt[buf]);
-  };
+  }
+  __device__ __forceinline__ void copy_k(int block, char* dst) const { copy(kbase, p.k_row, ksrc, block, dst); }
+  __device__ __forceinline__ void copy_v(int block, char* dst) const { copy(vbase, p.v_row, vsrc, block, dst); }
+
   // Operands: key row col of score tile t, channels 16 s + 8 half; channel tile
   // f's column col of keys 16 s + 4 half + {0..3, 8..11}.
-  auto k_frag = [&](const char* tile_at, int t, int s) {
+  __device__ __forceinline__ v4u k_frag(const char* from, int t, int s) const {
     const int r = 32 * t + col;
-    return *reinterpret_cast<const v4u*>(tile_at + r * (2 * DP) + (((2 * s + half) ^ k_swizzle<DP>(r)) << 4));
-  };
-  auto v_frag = [&](const char* tile_at, int f, int s) {
+    return *reinterpret_cast<const v4u*>(from + r * (2 * DP) + (((2 * s + half) ^ k_swizzle<DP>(r)) << 4));
+  }
+  __device__ __forceinline__ v4u v_frag(const char* from, int f, int s) const {
     v4u a;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = 16 * s + 8 * e + 4 * half + ((lane & 15) >> 2);
       const int d = 32 * f + (lane & 16) + 4 * (lane & 3);
-      const char* at = tile_at + r * (2 * DP) + (((d >> 3) ^ v_swizzle<DP>(r)) << 4) + 2 * (d & 7);
+      const char* at = from + r * (2 * DP) + (((d >> 3) ^ v_swizzle<DP>(r)) << 4) + 2 * (d & 7);
       const v2u w = __builtin_bit_cast(
           v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(at)));
       a[2 * e] = w.x;
       a[2 * e + 1] = w.y;
     }
     return a;
-  };
-  auto other_half = [](float x) {   // the larger or the sum over lanes l and l ^ 32 needs the other's value
-    return __shfl_xor(x, 32, 64);
-  };
+  }
+  // Product n of a block's scores is step n / TF of score tile n % TF, product n
+  // of its values step n / DF of channel tile n % DF: neighbours are independent.
+  __device__ __forceinline__ v4u k_of(const char* from, int n) const { return k_frag(from, n % TF, n / TF); }
+  __device__ __forceinline__ v4u v_of(const char* from, int n) const { return v_frag(from, n % DF, n / DF); }
 
+  // The largest of a block's scores; those behind a query's last key set to -inf.
+  static __device__ __forceinline__ float largest(const v16f (&x)[TF]) {
+    float mx = x[0][0];
+#pragma unroll
+    for (int t = 0; t < TF; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
+    return mx;
+  }
+  __device__ __forceinline__ void mask(int j, v16f (&x)[TF]) const {
+    __asm__ volatile("");   // (not to be done without the branch)
+#pragma unroll
+    for (int t = 0; t < TF; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (j * BK + 32 * t + 8 * (e / 4) + 4 * half + e % 4 >= limit) x[t][e] = -INFINITY;
+  }
+
+  __device__ __forceinline__ void store(const v16f (&o)[DF], float l) const {
+    const auto both = lane_halves(l);
+    l = both.first + both.second;
+    const float rcp = l == 0.0f ? 0.0f : 1.0f / l;
+    if (!stored) return;
+    char* at = to();
+#pragma unroll
+    for (int f = 0; f < DF; ++f)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * f + 8 * g + 4 * half;
+        if (d >= p.dim) continue;
+        *reinterpret_cast<uint2*>(at + 2 * d) = make_uint2(pack2<DT>(o[f][4 * g] * rcp, o[f][4 * g + 1] * rcp),
+                                                            pack2<DT>(o[f][4 * g + 2] * rcp, o[f][4 * g + 3] * rcp));
+      }
+  }
+};
+
+// The sums, the exponent that p is relative to and this half's sum of p. The
+// reference follows the maximum only once that lies more than kSlack above it.
+template <int DF>
+struct PackedState {
   v16f o[DF];
-  float m = -INFINITY, l = 0.0f;
-
-  // One walk over the keys. CAREFUL: a masked key's value may be infinite or
-  // NaN, and its product with P = 0 would not be 0. Such values are set to 0
-  // for the product, and a count of the visible ones brings them back.
-  auto walk = [&](auto careful_tag) {
-    constexpr bool CAREFUL = decltype(careful_tag)::value;
+  float ref, l;
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int f = 0; f < DF; ++f) o[f] = v16f{};
-    m = -INFINITY;
+    ref = -INFINITY;
     l = 0.0f;
-    if (blocks > 0) copy_block(0, 0);
-    for (int j = 0; j < blocks; ++j) {
-      const int buf = j & 1;
-      __builtin_amdgcn_s_waitcnt(0x0F70);   // this wave's copies of block j have landed,
-      __syncthreads();                      // and everyone's; block j - 1 has been read
-      if (j + 1 < blocks) copy_block(j + 1, buf ^ 1);
-      const int first = j * BK;
-      if (first >= wave_seen) continue;
-      v16f s[TF];
+  }
+  __device__ __forceinline__ void follow(float mx) {
+    if (__builtin_amdgcn_ballot_w64(mx > ref + kSlack) == 0) return;
+    const auto both = lane_halves(mx);
+    const float to = fmaxf(ref, fmaxf(both.first, both.second));
+    const float fade = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+    ref = to;
+    l = l * fade;
 #pragma unroll
-      for (int t = 0; t < TF; ++t) {
-        s[t] = v16f{};
+    for (int f = 0; f < DF; ++f)
 #pragma unroll
-        for (int i = 0; i < NS; ++i) s[t] = mfma32<DT>(k_frag(kt[buf], t, i), qf[i], s[t]);
-      }
-      const bool masked = first + BK > wave_clean;
-      if (masked) {
-#pragma unroll
-        for (int t = 0; t < TF; ++t)
-#pragma unroll
-          for (int x = 0; x < 16; ++x)
-            if (first + 32 * t + 8 * (x / 4) + 4 * half + x % 4 >= limit) s[t][x] = -INFINITY;
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int t = 0; t < TF; ++t)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[t][x]);
-      mx = fmaxf(mx, other_half(mx));
-      mx = fmaxf(m, mx);
-      const float ref = mx == -INFINITY ? 0.0f : mx * p.c;
-      const float fade = __builtin_amdgcn_exp2f(__builtin_fmaf(m, p.c, -ref));
-      m = mx;
-      float sum = 0.0f;
-#pragma unroll
-      for (int t = 0; t < TF; ++t)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          s[t][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], p.c, -ref));
-          sum += s[t][x];
-        }
-      l = __builtin_fmaf(l, fade, sum);
-      if (__builtin_amdgcn_ballot_w64(fade != 1.0f)) {
-#pragma unroll
-        for (int f = 0; f < DF; ++f)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[f][x] = o[f][x] * fade;
-      }
-      v4u pf[BK / 16];
-#pragma unroll
-      for (int i = 0; i < BK / 16; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          pf[i][x] = pack2<DT>(s[i / 2][8 * (i % 2) + 2 * x], s[i / 2][8 * (i % 2) + 2 * x + 1]);
-      if (!CAREFUL || !masked) {
-#pragma unroll
-        for (int i = 0; i < BK / 16; ++i)
-#pragma unroll
-          for (int f = 0; f < DF; ++f) o[f] = mfma32<DT>(v_frag(vt[buf], f, i), pf[i], o[f]);
-      } else {
-        constexpr uint32_t kInf = DT == kF16 ? 0x7c00u : 0x7f80u, kOne = DT == kF16 ? 0x3c00u : 0x3f80u;
+      for (int x = 0; x < 16; ++x) o[f][x] = o[f][x] * fade;
+  }
+  __device__ __forceinline__ float at() const { return ref == -INFINITY ? 0.0f : ref; }
+};
+
+// The walk again for a workgroup with sums that are not finite, causal only: a
+// masked key's value may be infinite or NaN, and its product with P = 0 is not 0.
+// In blocks with masked keys such values are set to 0 for the product, and a
+// count of those that a query sees brings them back. One block at a time.
+template <int DT, int DP>
+__device__ __forceinline__ void packed_careful(const PackedParams& p, char* tiles) {
+  int tid = threadIdx.x;
+  __asm__ volatile("" : "+v"(tid));
+  using W = Packed<DT, DP, true>;
+  const W w(p, tiles, tid);
+  v4u qf[W::NS];
+  w.queries(qf);
+  PackedState<W::DF> st;
+  st.clear();
 #pragma unroll 1
-        for (int f = 0; f < DF; ++f) {
-          v16f up{}, down{}, add{};
+  for (int j = 0; j < w.blocks; ++j) {
+    __syncthreads();   // the last block has been read
+    w.copy_k(j, w.kt(0));
+    w.copy_v(j, w.vt(0));
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    if (j >= w.wave_blocks) continue;
+    v16f s[W::TF];
 #pragma unroll
-          for (int i = 0; i < BK / 16; ++i) {
-            const v4u a = v_frag(vt[buf], f, i);
-            v4u fin, pos, neg, vis;
+    for (int t = 0; t < W::TF; ++t) s[t] = v16f{};
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint32_t wf = 0, wp = 0, wn = 0, wv = 0;
+    for (int n = 0; n < W::TF * W::NS; ++n) s[n % W::TF] = mfma32<DT>(w.k_of(w.kt(0), n), qf[n / W::TF], s[n % W::TF]);
+    w.mask(j, s);
+    st.follow(W::largest(s) * p.c);
+    v4u pf[W::BK / 16];
+    const float at = st.at();
 #pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                const uint32_t u = (a[x] >> (16 * y)) & 0xffffu, mag = u & 0x7fffu;
-                const int key = first + 16 * i + 8 * (x / 2) + 4 * half + 2 * (x % 2) + y;
-                wf |= (mag < kInf ? u : 0u) << (16 * y);
-                wp |= (mag > kInf || u == kInf ? kOne : 0u) << (16 * y);
-                wn |= (mag > kInf || u == (kInf | 0x8000u) ? kOne : 0u) << (16 * y);
-                wv |= (key < limit ? kOne : 0u) << (16 * y);
-              }
-              fin[x] = wf; pos[x] = wp; neg[x] = wn; vis[x] = wv;
-            }
-            add = mfma32<DT>(fin, pf[i], add);
-            up = mfma32<DT>(pos, vis, up);
-            down = mfma32<DT>(neg, vis, down);
+    for (int i = 0; i < 8 * W::TF; ++i) {
+      const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 8][2 * (i % 8)], p.c, -at));
+      const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 8][2 * (i % 8) + 1], p.c, -at));
+      pf[i / 4][i % 4] = pack2<DT>(a, b);
+      st.l = add2<DT>(pf[i / 4][i % 4], st.l);
+    }
+    const int sees = (j + 1) * W::BK > w.wave_clean ? w.limit : INT32_MAX;
+    constexpr uint32_t kInf = DT == kF16 ? 0x7c00u : 0x7f80u, kOne = DT == kF16 ? 0x3c00u : 0x3f80u;
+#pragma unroll
+    for (int f = 0; f < W::DF; ++f) {
+      v16f up{}, down{};
+#pragma unroll
+      for (int i = 0; i < W::BK / 16; ++i) {
+        const v4u a = w.v_frag(w.vt(0), f, i);
+        v4u fin, pos, neg, vis;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t wf = 0, wp = 0, wn = 0, wv = 0;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t u = (a[x] >> (16 * y)) & 0xffffu, mag = u & 0x7fffu;
+            const int key = j * W::BK + 16 * i + 8 * (x / 2) + 4 * w.half + 2 * (x % 2) + y;
+            wf |= (mag < kInf ? u : 0u) << (16 * y);
+            wp |= (mag > kInf || u == kInf ? kOne : 0u) << (16 * y);
+            wn |= (mag > kInf || u == (kInf | 0x8000u) ? kOne : 0u) << (16 * y);
+            wv |= (key < sees ? kOne : 0u) << (16 * y);
           }
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            float y = add[x];
-            if (up[x] > 0.0f) y += INFINITY;
-            if (down[x] > 0.0f) y -= INFINITY;
-            add[x] = y;
-          }
-#pragma unroll
-          for (int g = 0; g < DF; ++g)
-            if (g == f) {
-#pragma unroll
-              for (int x = 0; x < 16; ++x) o[g][x] = o[g][x] + add[x];
-            }
+          fin[x] = wf; pos[x] = wp; neg[x] = wn; vis[x] = wv;
         }
+        st.o[f] = mfma32<DT>(fin, pf[i], st.o[f]);
+        up = mfma32<DT>(pos, vis, up);
+        down = mfma32<DT>(neg, vis, down);
+      }
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        float y = st.o[f][x];
+        if (up[x] > 0.0f) y += INFINITY;
+        if (down[x] > 0.0f) y -= INFINITY;
+        st.o[f][x] = y;
       }
     }
+  }
+  w.store(st.o, st.l);
+}
+
+// DT: F16 or BF16; DP: dim rounded up to 64, 96, 128 or 256.
+//
+// Step j forms block j's probabilities between the MFMAs that score block j + 1
+// and, the last of them, between the first that add block j's values; between
+// the others it takes block j + 1's maximum. K of block j + 1 and V of block j are read in a step,
+// so K's copies run a step ahead of V's. The order is laid out product by
+// product (left to the compiler, all fragments are read at once, which spills,
+// and the VALU's work follows the MFMAs').
+template <int DT, int DP, bool CAUSAL>
+__global__ __launch_bounds__(64 * kPackWaves, DP > 128 ? 1 : 2) void packed_attention_kernel(PackedParams p) {
+  using W = Packed<DT, DP, CAUSAL>;
+  constexpr int BK = W::BK, NS = W::NS, DF = W::DF, TF = W::TF;
+  constexpr int QK = TF * NS, PV = BK / 16 * DF, AHEAD = 3;
+  __shared__ __attribute__((aligned(1024))) char tiles[4 * W::kTile];   // two of K, two of V
+  const W w(p, tiles, threadIdx.x);
+  if (w.tile.b < 0) return;
+  if (w.tile.b == p.sequences) {
+    if (p.fill && w.stored)
+      for (int d = 4 * w.half; d < p.dim; d += 8) *reinterpret_cast<uint2*>(w.to() + 2 * d) = make_uint2(0, 0);
+    return;
+  }
+  v4u qf[NS];
+  w.queries(qf);
+  PackedState<DF> st;
+  st.clear();
+
+  // Step j with block j's scores in s and K of block j + 1 and V of block j in
+  // the tiles of these numbers; block j + 1's scores go to next.
+  auto step = [&](int j, const v16f (&s)[TF], v16f (&next)[TF], auto ktile_tag, auto last_tag) {
+    constexpr bool LAST = decltype(last_tag)::value;   // the wave's last block
+    const char* kn = w.kt(decltype(ktile_tag)::value);
+    const char* vc = w.vt(1 - decltype(ktile_tag)::value);
+    v4u pf[BK / 16], vf[AHEAD + 1];
+    const float at = st.at();
+    float ea = 0.0f, eb = 0.0f;   // a pair of probabilities on its way
+    auto form = [&](int pair) {
+      ea = __builtin_amdgcn_exp2f(__builtin_fmaf(s[pair / 8][2 * (pair % 8)], p.c, -at));
+      eb = __builtin_amdgcn_exp2f(__builtin_fmaf(s[pair / 8][2 * (pair % 8) + 1], p.c, -at));
+    };
+    auto keep = [&](int pair) {
+      const uint32_t x = pack2<DT>(ea, eb);
+      pf[pair / 4][pair % 4] = x;
+      st.l = add2<DT>(x, st.l);
+      __asm__ volatile("" : "+v"(st.l));   // (not to be put off behind the products)
+    };
+    // A quarter of the pairs while the first fragments are on their way, a
+    // quarter with the first half of the values (which need them last).
+    constexpr int PAIRS = 8 * TF, EARLY = PAIRS / 4, LATE = PAIRS / 4;
+    if constexpr (LAST) {
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) vf[n] = w.v_of(vc, n);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        form(i);
+        keep(i);
+      }
+    } else {
+      v4u kf[AHEAD + 1];
+#pragma unroll
+      for (int t = 0; t < TF; ++t) next[t] = v16f{};
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) kf[n] = w.k_of(kn, n);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < EARLY; ++i) {
+        if (i > 0) keep(i - 1);
+        form(i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < QK; ++n) {
+        if (n + AHEAD < QK) kf[(n + AHEAD) % (AHEAD + 1)] = w.k_of(kn, n + AHEAD);
+        else vf[n + AHEAD - QK] = w.v_of(vc, n + AHEAD - QK);
+        next[n % TF] = mfma32<DT>(kf[n % (AHEAD + 1)], qf[n / TF], next[n % TF]);
+#pragma unroll
+        for (int i = EARLY + (PAIRS - EARLY - LATE) * n / QK; i < EARLY + (PAIRS - EARLY - LATE) * (n + 1) / QK; ++i) {
+          keep(i - 1);
+          form(i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    float mx = LAST ? 0.0f : next[0][0];
+#pragma unroll
+    for (int n = 0; n < PV; ++n) {
+      if (n + AHEAD < PV) vf[(n + AHEAD) % (AHEAD + 1)] = w.v_of(vc, n + AHEAD);
+      st.o[n % DF] = mfma32<DT>(vf[n % (AHEAD + 1)], pf[n / DF], st.o[n % DF]);
+      if constexpr (!LAST) {
+#pragma unroll
+        for (int i = PAIRS - LATE + 2 * LATE * n / PV; i < PAIRS - LATE + 2 * LATE * (n + 1) / PV && i < PAIRS; ++i) {
+          keep(i - 1);
+          form(i);
+          if (i == PAIRS - 1) keep(i);
+        }
+#pragma unroll
+        for (int e = max(16 * TF * (2 * n - PV) / PV, 0); e < 16 * TF * (2 * n + 2 - PV) / PV; ++e)
+          mx = fmaxf(mx, next[e / 16][e % 16]);
+        __asm__ volatile("" : "+v"(mx));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (!LAST) {
+      if ((j + 2) * BK > w.wave_clean) {
+        w.mask(j + 1, next);
+        mx = W::largest(next);
+      }
+      st.follow(mx * p.c);
+    }
   };
-  walk(std::false_type{});
+  auto sync = [&](int j) {
+    if (j > 0) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);   // this wave's copies of K j + 1 and V j have landed,
+      __syncthreads();                      // and everyone's; K j and V j - 1 have been read
+    }
+    if (j + 2 < w.blocks) w.copy_k(j + 2, w.kt(j & 1));
+    if (j + 1 < w.blocks) w.copy_v(j + 1, w.vt((j + 1) & 1));
+  };
+  using Tile0 = std::integral_constant<int, 0>;
+  using Tile1 = std::integral_constant<int, 1>;
+  if (w.blocks > 0) {
+    w.copy_k(0, w.kt(0));
+    if (w.blocks > 1) w.copy_k(1, w.kt(1));
+    w.copy_v(0, w.vt(0));
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+  }
+  int j = 0;
+  if (w.wave_blocks > 0) {
+    v16f sa[TF], sb[TF];
+#pragma unroll
+    for (int t = 0; t < TF; ++t) sa[t] = v16f{};
+#pragma unroll
+    for (int n = 0; n < QK; ++n) sa[n % TF] = mfma32<DT>(w.k_of(w.kt(0), n), qf[n / TF], sa[n % TF]);
+    if (BK > w.wave_clean) w.mask(0, sa);
+    st.follow(W::largest(sa) * p.c);
+    for (; j + 2 < w.wave_blocks; j += 2) {
+      sync(j);
+      step(j, sa, sb, Tile1{}, std::false_type{});
+      sync(j + 1);
+      step(j + 1, sb, sa, Tile0{}, std::false_type{});
+    }
+    if (j + 2 == w.wave_blocks) {
+      sync(j);
+      step(j, sa, sb, Tile1{}, std::false_type{});
+      sync(++j);
+      step(j, sb, sa, Tile0{}, std::true_type{});
+    } else {
+      sync(j);
+      step(j, sa, sb, Tile1{}, std::true_type{});
+    }
+    ++j;
+  }
+  for (; j < w.blocks; ++j) sync(j);   // the rest is the other waves'
+
   if constexpr (CAUSAL) {
     // Finite sums times 0 are 0: only where they are not can a masked value have come in.
     float z = 0.0f;
 #pragma unroll
     for (int f = 0; f < DF; ++f)
 #pragma unroll
-      for (int x = 0; x < 16; ++x) z = __builtin_fmaf(o[f][x], 0.0f, z);
-    if (threadIdx.x == 0) again = 0;
+      for (int x = 0; x < 16; ++x) z = __builtin_fmaf(st.o[f][x], 0.0f, z);
+    w.store(st.o, st.l);
+    const bool odd = __builtin_amdgcn_ballot_w64(z != 0.0f) != 0;
+    __syncthreads();   // the tiles have been read
+    int* again = reinterpret_cast<int*>(tiles);
+    if (w.lane == 0) again[w.wave] = odd;
     __syncthreads();
-    if (z != 0.0f) again = 1;
-    __syncthreads();
-    if (again) walk(std::true_type{});
+    if (again[0] | again[1] | again[2] | again[3]) packed_careful<DT, DP>(p, tiles);
+  } else {
+    w.store(st.o, st.l);
   }
-
-  l = l + other_half(l);
-  const float rcp = l == 0.0f ? 0.0f : 1.0f / l;
-  if (!stored) return;
-#pragma unroll
-  for (int f = 0; f < DF; ++f)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * f + 8 * g + 4 * half;
-      if (d >= p.dim) continue;
-      *reinterpret_cast<uint2*>(to + 2 * d) = make_uint2(pack2<DT>(o[f][4 * g] * rcp, o[f][4 * g + 1] * rcp),
-                                                          pack2<DT>(o[f][4 * g + 2] * rcp, o[f][4 * g + 3] * rcp));
-    }
 }
 
 template <int DT, int DP>

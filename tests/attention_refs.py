@@ -4,7 +4,10 @@ The kernels hold scores, maxima, sums and products in fp32 and round twice to
 the operands' type T (half a step, u = eps / 2 relative): p, relative to the
 running maximum, before its product with v, and the output. With
 A = sum p |v| / sum p:
-  * p's rounding:            u A; in fp16 what lies below 2^-24 is lost, by
+  * p's rounding:            u (A + |o|) if the sum in the denominator takes
+                             the rounded p, as packed attention does
+                             (sum of p d_j (v_j - o) / sum p with |d_j| <= u),
+                             u A if it does not; in fp16 what lies below 2^-24 is lost, by
                              half of that at most: 2^-25 sum |v| / sum p,
                              where sum p >= 1 relative to the maximum
   * the score's sum of D products and its scaling: (D + 4) 2^-24 of the sum of
@@ -54,7 +57,7 @@ def bound(o, parts, dtype):
         return torch.zeros_like(o)
     a, lost, d, nk = parts
     u = _u(dtype)
-    tol = u * o.abs() + a * (u + 2 * d + 2 * (nk + nk / 32 + 8) * 2.0 ** -24)
+    tol = 2 * u * o.abs() + a * (u + 2 * d + 2 * (nk + nk / 32 + 8) * 2.0 ** -24)
     if dtype == torch.float16:
         tol = tol + 2.0 ** -25 * lost + 2.0 ** -25
     return tol * 1.01 + 1e-37   # (the bound's own products of small terms)
