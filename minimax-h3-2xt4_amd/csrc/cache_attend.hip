@@ -26,12 +26,22 @@
 // descriptor of their group: their loads return zeros, whatever memory holds.
 #include "paged.h"
 
+#include <algorithm>
+
 namespace w8a8 {
 
 constexpr int kAttendWaves = 4;
-constexpr int kWaveKeys = 32;
-constexpr int kBlockKeys = kAttendWaves * kWaveKeys;
 constexpr int kHeadTile = 16;
+constexpr int kWaveKeys = 32;   // keys of a wave at a time: two groups
+constexpr int kBlockKeys = kAttendWaves * kWaveKeys;
+// dim rounded up to the channels that a kernel works on.
+constexpr int attend_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+// Workgroups of a CU, by the registers of 128 and of 256 channels.
+constexpr int attend_per_cu(int dp) { return 2; }
+// The reference of p may lie so much below the maximum (as a power of 2), and
+// the reference of the values' scales 2^kScaleSlack: p times the scale is then
+// at most 2^12, far inside fp16, and rescaling the sums is rare.
+constexpr float kSlack = 8.0f, kScaleSlack = 16.0f;
 
 struct AttendParams {
   CacheView cache;
@@ -40,59 +50,77 @@ struct AttendParams {
   int64_t q_row, q_head, o_row, o_head;   // bytes
   int sequences, heads, group, tiles;     // tiles: of 16 query heads of a kv head
   int width;
+  int whole;    // a workgroup for each pair
   const int32_t* table;
   int64_t ld_table;
   const int32_t* lengths;
   float c;   // log2(e) * scale
   float* part;       // [workgroups][2][kHeadTile][dim padded]
-  float* part_ml;    // [workgroups][2][2][kHeadTile]: maximum, sum
+  float* part_ml;    // [workgroups][2][2][kHeadTile]: reference, sum
+  int4* shared;      // [workgroups]: sequence, pair and last range of a pair that begins in a range and goes on, or -1
 };
 
 __device__ __forceinline__ int attend_length(const AttendParams& p, int len) {
   return min(max(len, 0), p.width * p.cache.page_size);
 }
+// Blocks of a pair of this length; an empty sequence has a block of no keys.
 __device__ __forceinline__ int attend_blocks(const AttendParams& p, int len) {
-  return max((attend_length(p, len) + kBlockKeys - 1) / kBlockKeys, 1);   // (an empty sequence has a block of no keys)
+  return max((attend_length(p, len) + kBlockKeys - 1) / kBlockKeys, 1);
 }
 
-// Blocks of all pairs.
-__device__ __forceinline__ int64_t attend_total(const AttendParams& p) {
-  int64_t n = 0;
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// The line of all pairs' blocks, cut into ranges that differ by one block at
+// most: the first `extra` have per + 1.
+struct Ranges {
+  int per, extra, used;
+  __device__ __forceinline__ Ranges(int total, int workgroups) {
+    used = min(total, workgroups);
+    per = total / used;
+    extra = total - per * used;
+  }
+  __device__ __forceinline__ int begin(int g) const { return per * g + min(g, extra); }
+  static __device__ __forceinline__ int of(int n, int per, int extra) {   // the range that block n lies in
+    const int big = extra * (per + 1);
+    return n < big ? n / (per + 1) : extra + (n - big) / per;
+  }
+};
+
+// Blocks of all sequences' first pairs.
+__device__ __forceinline__ int attend_total(const AttendParams& p) {
+  int n = 0;
   for (int b = threadIdx.x & 63; b < p.sequences; b += 64) n += attend_blocks(p, p.lengths[b]);
-  return wave_sum64(n) * (p.cache.heads * p.tiles);
+  return wave_sum(n) * (p.cache.heads * p.tiles);
 }
 
 // The sequence that block n of the line belongs to, and the blocks before it.
-__device__ __forceinline__ int attend_find(const AttendParams& p, int64_t n, int64_t& before) {
-  const int lane = threadIdx.x & 63;
-  const int64_t pairs = p.cache.heads * p.tiles;
-  int64_t sum = 0;
+__device__ __forceinline__ int attend_find(const AttendParams& p, int n, int& before) {
+  const int lane = threadIdx.x & 63, pairs = p.cache.heads * p.tiles;
+  int sum = 0;
   for (int b0 = 0; b0 < p.sequences; b0 += 64) {
-    const int64_t mine = b0 + lane < p.sequences ? attend_blocks(p, p.lengths[b0 + lane]) * pairs : 0;
-    const int64_t upto = sum + wave_prefix64(mine);
+    const int mine = b0 + lane < p.sequences ? attend_blocks(p, p.lengths[b0 + lane]) * pairs : 0;
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int t = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += t;
+    }
+    upto += sum;
     const uint64_t past = __builtin_amdgcn_ballot_w64(upto > n);
     if (past) {
       const int at = __builtin_ctzll(past);
-      before = __shfl(upto - mine, at, 64);
-      return __builtin_amdgcn_readfirstlane(b0 + at);
+      before = __builtin_amdgcn_readlane(upto - mine, at);
+      return b0 + at;
     }
-    sum = __shfl(upto, 63, 64);
+    sum = __builtin_amdgcn_readlane(upto, 63);
   }
   before = sum;
   return p.sequences;
 }
-
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
-  return (int64_t)(((uint64_t)hi << 32) | lo);
-}
-
-// Ranges that hold a block, of so many workgroups: none in between is empty.
-__device__ __forceinline__ int attend_used(int64_t total, int ranges) { return (int)min(total, (int64_t)ranges); }
-
-// Where range g of n blocks begins.
-__device__ __forceinline__ int64_t range_at(int64_t n, int g, int ranges) { return n / ranges * g + n % ranges * g / ranges; }
 
 template <int DT>
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
@@ -141,8 +169,9 @@ constexpr uint32_t kNowhere = 0x7fffff00u;   // an offset behind every descripto
 
 // DT: type of q and out; CODES: the cache holds I8; DP: dim rounded up to 64, 128 or 256.
 template <int DT, bool CODES, int DP>
-__global__ __launch_bounds__(64 * kAttendWaves, 2) void cache_attend_kernel(AttendParams p) {
+__global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_attend_kernel(AttendParams p) {
   constexpr int ES = CODES ? 1 : 2;
+  constexpr int G = kWaveKeys / kGroupTokens;
   constexpr int NS = DP / 32;          // products of a key tile
   constexpr int VL = DP / 16;          // channels a lane reads of a value row
   constexpr int KW = CODES ? 2 : 4;    // words of eight channels
@@ -154,17 +183,26 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void cache_attend_kernel(Atte
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int dim = p.cache.dim;
 
-  const int64_t total = uniform64(attend_total(p));
-  const int ranges = attend_used(total, gridDim.x);
-  if ((int)blockIdx.x >= ranges) return;
-  int64_t at = uniform64(range_at(total, blockIdx.x, ranges));
-  const int64_t end = uniform64(range_at(total, blockIdx.x + 1, ranges));
-  int64_t before;
-  int b = attend_find(p, at, before);
-  before = uniform64(before);
-  int nblk = attend_blocks(p, scalar_int(p.lengths, b));
-  int64_t rest = at - before;
-  int pair = (int)(rest / nblk), blk = (int)(rest - (int64_t)pair * nblk);
+  int b, pair, blk = 0, nblk, at = 0, end, ranges_per = 0, ranges_extra = 0;
+  if (p.whole) {
+    const int pairs = p.cache.heads * p.tiles;
+    b = blockIdx.x / pairs;
+    pair = blockIdx.x - b * pairs;
+    end = nblk = attend_blocks(p, scalar_int(p.lengths, b));
+  } else {
+    const Ranges r(attend_total(p), gridDim.x);
+    if (threadIdx.x == 0) p.shared[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if ((int)blockIdx.x >= r.used) return;
+    ranges_per = r.per;
+    ranges_extra = r.extra;
+    at = r.begin(blockIdx.x);
+    end = r.begin(blockIdx.x + 1);
+    int before;
+    b = attend_find(p, at, before);
+    nblk = attend_blocks(p, scalar_int(p.lengths, b));
+    pair = (at - before) / nblk;
+    blk = at - before - pair * nblk;
+  }
 
   // Byte offsets within a group of 16 tokens.
   uint32_t koff[NS], voff[4];
@@ -177,184 +215,215 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void cache_attend_kernel(Atte
   for (int i = 0; i < 4; ++i)
     voff[i] = VL * col < dim ? (4 * quad + i) * p.cache.token_b + VL * col * ES : kNowhere;
 
-  while (true) {
-    const int len = attend_length(p, scalar_int(p.lengths, b));
-    const int kvh = pair / p.tiles, tile = pair - kvh * p.tiles;
-    const int take = (int)min((int64_t)(nblk - blk), end - at);
-    const int nh = min(p.group - kHeadTile * tile, kHeadTile);
-    const int head0 = kvh * p.group + kHeadTile * tile;
-    const char* kb = p.cache.k + kvh * p.cache.head_b;
-    const char* vb = p.cache.v + kvh * p.cache.head_b;
-    v4u qf[NS];
+  // What is loaded runs ahead of what is computed, over the pairs' ends too: the
+  // place of this wave's two groups of 16 keys in the next block, and how many
+  // keys of each count.
+  struct Keys {
+    int page[G], token[G], n[G], kvh;
+  };
+  struct {
+    int b, pair, blk, nblk, len, left;
+  } ahead = {b, pair, blk, nblk, attend_length(p, scalar_int(p.lengths, b)), end - at};
+  const int pairs = p.cache.heads * p.tiles;
+  auto next_keys = [&]() {
+    Keys k;
+    const int k0 = (ahead.blk * kAttendWaves + wave) * kWaveKeys;
+    k.kvh = ahead.pair / p.tiles;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int first = k0 + i * kGroupTokens;
+      int n = ahead.left > 0 ? min(max(ahead.len - first, 0), kGroupTokens) : 0, entry, page = 0;
+      group_place(p.cache, (uint32_t)first / kGroupTokens, entry, k.token[i]);
+      if (n > 0) page = scalar_int(p.table, (int64_t)ahead.b * p.ld_table + entry);
+      if (page < 0 || page >= p.cache.pages) page = n = 0;
+      k.page[i] = page;
+      k.n[i] = n;
+    }
+    if (--ahead.left > 0 && ++ahead.blk == ahead.nblk) {
+      ahead.blk = 0;
+      if (++ahead.pair == pairs) {
+        ahead.pair = 0;
+        const int len = scalar_int(p.lengths, ++ahead.b);
+        ahead.len = attend_length(p, len);
+        ahead.nblk = attend_blocks(p, len);
+      }
+    }
+    return k;
+  };
+  auto group_rsrc = [&](const char* base, const Keys& k, int i) {
+    const char* t = base + (int64_t)k.page[i] * p.cache.page_b + k.kvh * p.cache.head_b +
+                    (int64_t)k.token[i] * p.cache.token_b;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(t), 0,
+                                             k.n[i] ? (int)((k.n[i] - 1) * p.cache.token_b) + dim * ES : 0, 0x00027000);
+  };
+  uint32_t kr[G][NS][KW], vr[4 * G][VW];
+  auto load_k = [&](const Keys& k) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const auto r = group_rsrc(p.cache.k, k, i);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) group_load<KW>(r, koff[s], kr[i][s]);
+    }
+  };
+  auto load_v = [&](const Keys& k) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const auto r = group_rsrc(p.cache.v, k, i);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) group_load<VW>(r, voff[t], vr[4 * i + t]);
+    }
+  };
+  struct Scales {
+    v4f k[G], v[G];
+  };
+  auto load_scales = [&](const Keys& k) {
+    Scales sc{};
+    if constexpr (!CODES) return sc;
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int64_t s = (int64_t)k.page[i] * p.cache.s_page + k.kvh * p.cache.s_head + k.token[i] + 4 * quad;
+      sc.k[i] = *reinterpret_cast<const v4f*>(p.cache.ks + s);
+      sc.v[i] = *reinterpret_cast<const v4f*>(p.cache.vs + s);
+    }
+    return sc;
+  };
+  Keys now = next_keys();
+  load_k(now);
+  load_v(now);
+  Scales sc = load_scales(now);
+  Keys next = next_keys();
+
+  v4u qf[NS];
+  auto load_q = [&](int seq, int pr) {
+    const int kvh = pr / p.tiles, first = kHeadTile * (pr - kvh * p.tiles) + col;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const int d = 8 * quad + 32 * s;
       qf[s] = v4u{0, 0, 0, 0};
-      if (col < nh && d < dim)
-        qf[s] = *reinterpret_cast<const v4u*>(p.q + (int64_t)b * p.q_row + (head0 + col) * p.q_head + 2 * d);
+      if (first < p.group && d < dim)
+        qf[s] = *reinterpret_cast<const v4u*>(p.q + (int64_t)seq * p.q_row + (kvh * p.group + first) * p.q_head + 2 * d);
     }
+  };
+  load_q(b, pair);
+
+  while (true) {
+    const int kvh = pair / p.tiles, tile = pair - kvh * p.tiles;
+    const int take = min(nblk - blk, end - at);
+    const int nh = min(p.group - kHeadTile * tile, kHeadTile);
+    const int head0 = kvh * p.group + kHeadTile * tile;
     v4f o[VL];
 #pragma unroll
     for (int j = 0; j < VL; ++j) o[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f, top = 0.0f;   // top: the largest value scale so far (codes)
-
-    // Two groups of 16 keys, their places and how many keys of each count.
-    struct Keys {
-      int page[2], token[2], n[2];
-    };
-    auto place = [&](int block) {
-      Keys k;
-      const int k0 = (block * kAttendWaves + wave) * kWaveKeys;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int first = k0 + i * kGroupTokens;
-        int n = min(max(len - first, 0), kGroupTokens), entry, page = 0;
-        group_place(p.cache, (uint32_t)first / kGroupTokens, entry, k.token[i]);
-        if (n > 0) page = scalar_int(p.table, (int64_t)b * p.ld_table + entry);
-        if (page < 0 || page >= p.cache.pages) page = n = 0;
-        k.page[i] = page;
-        k.n[i] = n;
-      }
-      return k;
-    };
-    auto group_rsrc = [&](const char* base, const Keys& k, int i) {
-      const char* t = base + (int64_t)k.page[i] * p.cache.page_b + (int64_t)k.token[i] * p.cache.token_b;
-      return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(t), 0, 
-                                               k.n[i] ? (int)((k.n[i] - 1) * p.cache.token_b) + dim * ES : 0, 0x00027000);
-    };
-    uint32_t kr[2][NS][KW], vr[8][VW];
-    auto load_k = [&](const Keys& k) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const auto r = group_rsrc(kb, k, i);
-#pragma unroll
-        for (int s = 0; s < NS; ++s) group_load<KW>(r, koff[s], kr[i][s]);
-      }
-    };
-    auto load_v = [&](const Keys& k) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const auto r = group_rsrc(vb, k, i);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) group_load<VW>(r, voff[t], vr[4 * i + t]);
-      }
-    };
-    struct Scales {
-      v4f k[2], v[2];
-    };
-    auto load_scales = [&](const Keys& k) {
-      Scales sc{};
-      if constexpr (!CODES) return sc;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int64_t s = (int64_t)k.page[i] * p.cache.s_page + kvh * p.cache.s_head + k.token[i] + 4 * quad;
-        sc.k[i] = *reinterpret_cast<const v4f*>(p.cache.ks + s);
-        sc.v[i] = *reinterpret_cast<const v4f*>(p.cache.vs + s);
-      }
-      return sc;
-    };
+    float ref = -INFINITY, l = 0.0f, top = 0.0f;   // top: the value scale that P's are relative to (codes)
 
     auto spread_max = [&](float x) {   // over the four quads: the keys of a column
       x = fmaxf(x, __shfl_xor(x, 16, 64));
       return fmaxf(x, __shfl_xor(x, 32, 64));
     };
-    const int last = blk + take;
-    Keys now = place(blk);
-    load_k(now);
-    load_v(now);
-    Scales sc = load_scales(now);
-    for (int block = blk; block < last; ++block) {
-      v4f s[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+    for (int block = 0; block < take; ++block) {
+      float t[4 * G];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < G; ++i) {
+        v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < NS; ++t) {
+        for (int x = 0; x < NS; ++x) {
           v4u a;
           if constexpr (CODES) {
-            const v2u lo = codes4<DT>(kr[i][t][0]), hi = codes4<DT>(kr[i][t][1]);
+            const v2u lo = codes4<DT>(kr[i][x][0]), hi = codes4<DT>(kr[i][x][1]);
             a = v4u{lo.x, lo.y, hi.x, hi.y};
           } else {
-            a = v4u{kr[i][t][0], kr[i][t][1], kr[i][t][2], kr[i][t][3]};
+            a = v4u{kr[i][x][0], kr[i][x][1], kr[i][x][2], kr[i][x][3]};
           }
-          s[i] = mfma16<DT>(a, qf[t], s[i]);
+          s = mfma16<DT>(a, qf[x], s);
         }
-      float t[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        t[i] = s[i / 4][i % 4] * p.c;
-        if constexpr (CODES) t[i] = t[i] * sc.k[i / 4][i % 4];
+        for (int x = 0; x < 4; ++x) {
+          t[4 * i + x] = s[x] * p.c;
+          if constexpr (CODES) t[4 * i + x] = t[4 * i + x] * sc.k[i][x];
+        }
       }
-      const Keys next = block + 1 < last ? place(block + 1) : Keys{{0, 0}, {0, 0}, {0, 0}};
       load_k(next);
       const Scales sn = load_scales(next);
-      if (now.n[0] < kGroupTokens || now.n[1] < kGroupTokens) {
+      int fewest = now.n[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (4 * quad + i % 4 >= now.n[i / 4]) t[i] = -INFINITY;
+      for (int i = 1; i < G; ++i) fewest = min(fewest, now.n[i]);
+      if (fewest < kGroupTokens) {
+#pragma unroll
+        for (int i = 0; i < 4 * G; ++i)
+          if (4 * quad + i % 4 >= now.n[i / 4]) {
+            t[i] = -INFINITY;
+            if constexpr (CODES) sc.v[i / 4][i % 4] = 0.0f;
+          }
       }
-      float mx = t[0];
+      // The references follow the maxima only once those lie far enough above.
+      float mx = t[0], u = 0.0f;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, t[i]);
-      mx = fmaxf(m, spread_max(mx));
-      const float ref = mx == -INFINITY ? 0.0f : mx;
-      float w[8], fade = __builtin_amdgcn_exp2f(m - ref);
-      m = mx;
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(t[i] - ref);
-        sum += w[i];
-      }
-      l = __builtin_fmaf(l, fade, sum);
+      for (int i = 1; i < 4 * G; ++i) mx = fmaxf(mx, t[i]);
       if constexpr (CODES) {
-        // P carries the values' scales, relative to the largest so far, so
-        // that it keeps the type's precision whatever their size.
-        float u = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (4 * quad + i % 4 < now.n[i / 4]) u = fmaxf(u, sc.v[i / 4][i % 4]);
-        u = fmaxf(fmaxf(top, spread_max(u)), 0x1p-126f);
-        const float inv = 1.0f / u;
-        fade = fade * (top * inv);
-        top = u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          w[i] = 4 * quad + i % 4 < now.n[i / 4] ? w[i] * (sc.v[i / 4][i % 4] * inv) : 0.0f;
+        for (int i = 0; i < 4 * G; ++i) u = fmaxf(u, sc.v[i / 4][i % 4]);
       }
-      if (__builtin_amdgcn_ballot_w64(fade != 1.0f)) {
+      if (__builtin_amdgcn_ballot_w64(mx > ref + kSlack || (CODES && u > top * kScaleSlack))) {
+        const float to = fmaxf(ref, spread_max(mx));
+        float fade = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+        ref = to;
+        l = l * fade;
+        if constexpr (CODES) {
+          u = fmaxf(fmaxf(top, spread_max(u)), 0x1p-126f);
+          fade = fade * (top / u);
+          top = u;
+        }
 #pragma unroll
         for (int j = 0; j < VL; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[j][i] = o[j][i] * fade;
       }
-      const v4u pf = {pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7])};
-      uint32_t x[8][VL / 2];
+      const float base = ref == -INFINITY ? 0.0f : ref;
+      float inv = 0.0f;
+      if constexpr (CODES) inv = 1.0f / fmaxf(top, 0x1p-126f);   // (top 0: no key so far)
+      float w[4 * G];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 4 * G; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(t[i] - base);
+        l += w[i];
+        // P carries the values' scales, relative to about the largest so far,
+        // so that it keeps the type's precision whatever their size.
+        if constexpr (CODES) w[i] = w[i] * (sc.v[i / 4][i % 4] * inv);
+      }
 #pragma unroll
-        for (int j = 0; j < VL / 2; j += 2) {
-          if constexpr (CODES) {
-            const v2u c = codes4<DT>(vr[i][j / 2]);
-            x[i][j] = c.x;
-            x[i][j + 1] = c.y;
-          } else {
-            x[i][j] = vr[i][j];
-            x[i][j + 1] = vr[i][j + 1];
+      for (int g = 0; g < G; g += 2) {
+        const v4u pf = {pack2<DT>(w[4 * g], w[4 * g + 1]), pack2<DT>(w[4 * g + 2], w[4 * g + 3]),
+                        pack2<DT>(w[4 * g + 4], w[4 * g + 5]), pack2<DT>(w[4 * g + 6], w[4 * g + 7])};
+        uint32_t x[8][VL / 2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < VL / 2; j += 2) {
+            if constexpr (CODES) {
+              const v2u c = codes4<DT>(vr[4 * g + i][j / 2]);
+              x[i][j] = c.x;
+              x[i][j + 1] = c.y;
+            } else {
+              x[i][j] = vr[4 * g + i][j];
+              x[i][j + 1] = vr[4 * g + i][j + 1];
+            }
           }
+#pragma unroll
+        for (int j = 0; j < VL; ++j) {
+          const uint32_t pick = j % 2 ? 0x07060302u : 0x05040100u;
+          v4u a;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(x[2 * i + 1][j / 2], x[2 * i][j / 2], pick);
+          o[j] = mfma16<DT>(a, pf, o[j]);
         }
-#pragma unroll
-      for (int j = 0; j < VL; ++j) {
-        const uint32_t pick = j % 2 ? 0x07060302u : 0x05040100u;
-        v4u a;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(x[2 * i + 1][j / 2], x[2 * i][j / 2], pick);
-        o[j] = mfma16<DT>(a, pf, o[j]);
       }
       load_v(next);
       now = next;
       sc = sn;
+      next = next_keys();
     }
 
+    if (at + take < end) load_q(pair + 1 == pairs ? b + 1 : b, pair + 1 == pairs ? 0 : pair + 1);
     // The waves' sums meet: O's lane (col, quad) holds head col, channels
     // VL (4 quad + r) + j.
     l = l + __shfl_xor(l, 16, 64);
@@ -365,13 +434,13 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void cache_attend_kernel(Atte
       for (int j = 0; j < VL; j += 4)
         *reinterpret_cast<v4f*>(&sums[wave][col][VL * (4 * quad + r) + j]) = v4f{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
     if (quad == 0) {
-      stat[wave][0][col] = m;
+      stat[wave][0][col] = ref;
       stat[wave][1][col] = l;
       stat[wave][2][col] = top;
     }
     __syncthreads();
     const bool whole = blk == 0 && take == nblk;
-    const int64_t slot = (int64_t)blockIdx.x * 2 + (blk == 0 ? 1 : 0);   // the pair begins in this range, or before it
+    const int slot = blockIdx.x * 2 + (blk == 0 ? 1 : 0);   // the pair begins in this range, or before it
     for (int i = threadIdx.x; i < nh * (DP / 4); i += 64 * kAttendWaves) {
       const int h = i / (DP / 4), d = 4 * (i - h * (DP / 4));
       float mx = stat[0][0][h], sum = 0.0f;
@@ -395,13 +464,15 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void cache_attend_kernel(Atte
               make_uint2(pack2<DT>(y[0] * rcp, y[1] * rcp), pack2<DT>(y[2] * rcp, y[3] * rcp));
         }
       } else {
-        *reinterpret_cast<v4f*>(p.part + (slot * kHeadTile + h) * DP + d) = y;
+        *reinterpret_cast<v4f*>(p.part + ((int64_t)slot * kHeadTile + h) * DP + d) = y;
         if (d == 0) {
           p.part_ml[(slot * 2) * kHeadTile + h] = mx;
           p.part_ml[(slot * 2 + 1) * kHeadTile + h] = sum;
         }
       }
     }
+    if (blk == 0 && take < nblk && threadIdx.x == 0)
+      p.shared[blockIdx.x] = make_int4(b, pair, Ranges::of(at + nblk - 1, ranges_per, ranges_extra), 0);
     at += take;
     if (at >= end) return;
     __syncthreads();   // the sums have been read
@@ -413,63 +484,91 @@ __global__ __launch_bounds__(64 * kAttendWaves, 2) void cache_attend_kernel(Atte
   }
 }
 
-// The partial sums of a pair that several ranges share, in order: a workgroup
-// of one wave takes a query head, four channels a lane (DP 64: 16 lanes work).
+// The partial sums of the pair that begins in a range and goes on behind it: a
+// workgroup for each range and some of its heads. A wave takes 256 / DP heads
+// (four channels a lane), `parts` waves share their ranges, eight at a time, and
+// meet in LDS. The order is the ranges', whatever ends when.
+constexpr int kJoinWaves = 8, kJoinBatch = 8;
+constexpr int join_heads(int dp) { return 256 / dp; }
 template <int DT, int DP>
-__global__ __launch_bounds__(64) void cache_attend_join_kernel(AttendParams p, int workgroups) {
-  const int head = blockIdx.x, b = blockIdx.y + gridDim.y * blockIdx.z;
-  if (b >= p.sequences) return;
-  const int kvh = head / p.group, in = head - kvh * p.group, tile = in / kHeadTile, h = in - tile * kHeadTile;
-  const int64_t pairs = p.cache.heads * p.tiles;
-  int64_t before = 0, total = 0;
-  for (int i = threadIdx.x; i < p.sequences; i += 64) {
-    const int64_t n = attend_blocks(p, p.lengths[i]);
-    total += n;
-    if (i < b) before += n;
-  }
-  total = uniform64(wave_sum64(total) * pairs);
-  const int ranges = attend_used(total, workgroups);
-  const int nblk = attend_blocks(p, scalar_int(p.lengths, b));
-  const int64_t first = uniform64(wave_sum64(before)) * pairs + (int64_t)(kvh * p.tiles + tile) * nblk;
-  // The ranges that hold its first and its last block.
-  auto range_of = [&](int64_t n) {
-    int g = (int)(n * ranges / total);
-    while (g > 0 && range_at(total, g, ranges) > n) --g;
-    while (range_at(total, g + 1, ranges) <= n) ++g;
-    return g;
-  };
-  const int g0 = range_of(first), g1 = range_of(first + nblk - 1);
-  if (g0 == g1) return;
-  const int d = 4 * threadIdx.x;
-  float mx = -INFINITY;
-  for (int g = g0 + (int)threadIdx.x; g <= g1; g += 64)
-    mx = fmaxf(mx, p.part_ml[((int64_t)(2 * g + (g == g0)) * 2) * kHeadTile + h]);
-  mx = wave_max(mx);
-  const float ref = mx == -INFINITY ? 0.0f : mx;
+__global__ __launch_bounds__(64 * kJoinWaves) void cache_attend_join_kernel(AttendParams p, int parts) {
+  constexpr int LANES = DP / 4;
+  __shared__ v4f sums[kJoinWaves][64];
+  __shared__ float refs[kJoinWaves][64], totals[kJoinWaves][64];
+  const int g0 = blockIdx.x;
+  const int4 info = p.shared[g0];
+  if (info.x < 0) return;
+  const int b = info.x, pair = info.y, g1 = info.z;
+  const int kvh = pair / p.tiles, tile = pair - kvh * p.tiles;
+  const int heads = min(p.group - kHeadTile * tile, kHeadTile);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % parts;
+  const int h = (blockIdx.y * kJoinWaves + wave) / parts * join_heads(DP) + lane / LANES, d = 4 * (lane % LANES);
+  const bool mine = h < heads;
+  auto slot = [&](int g) { return 2 * g + (g == g0); };
   v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
-  float sum = 0.0f;
-#pragma unroll 8
-  for (int g = g0; g <= g1; ++g) {
-    const int64_t slot = 2 * (int64_t)g + (g == g0);
-    const float f = __builtin_amdgcn_exp2f(p.part_ml[(slot * 2) * kHeadTile + h] - ref);
-    sum = __builtin_fmaf(p.part_ml[(slot * 2 + 1) * kHeadTile + h], f, sum);
-    const v4f part = *reinterpret_cast<const v4f*>(p.part + (slot * kHeadTile + h) * DP + (d < DP ? d : 0));
+  float sum = 0.0f, ref = -INFINITY;
+  if (mine) {
+    for (int g = g0 + part; g <= g1; g += kJoinBatch * parts) {
+      float m[kJoinBatch], l[kJoinBatch];
+      v4f x[kJoinBatch];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(part[e], f, y[e]);
+      for (int i = 0; i < kJoinBatch; ++i) {
+        const int at = slot(min(g + i * parts, g1));
+        m[i] = p.part_ml[(2 * at) * kHeadTile + h];
+        l[i] = p.part_ml[(2 * at + 1) * kHeadTile + h];
+        x[i] = *reinterpret_cast<const v4f*>(p.part + ((int64_t)at * kHeadTile + h) * DP + d);
+      }
+      float to = ref;
+#pragma unroll
+      for (int i = 0; i < kJoinBatch; ++i) to = fmaxf(to, m[i]);
+      const float base = to == -INFINITY ? 0.0f : to, fade = __builtin_amdgcn_exp2f(ref - base);
+      ref = to;
+      sum = sum * fade;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = y[e] * fade;
+#pragma unroll
+      for (int i = 0; i < kJoinBatch; ++i) {
+        if (g + i * parts > g1) continue;
+        const float f = __builtin_amdgcn_exp2f(m[i] - base);
+        sum = __builtin_fmaf(l[i], f, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(x[i][e], f, y[e]);
+      }
+    }
   }
-  if (d >= p.cache.dim) return;
-  const float rcp = mx == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
-  *reinterpret_cast<uint2*>(p.out + (int64_t)b * p.o_row + head * p.o_head + 2 * d) =
+  sums[wave][lane] = y;
+  refs[wave][lane] = ref;
+  totals[wave][lane] = sum;
+  __syncthreads();
+  if (part > 0 || !mine || d >= p.cache.dim) return;
+  for (int i = 1; i < parts; ++i) ref = fmaxf(ref, refs[wave + i][lane]);
+  const float base = ref == -INFINITY ? 0.0f : ref;
+  sum = 0.0f;
+  y = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < parts; ++i) {
+    const float f = __builtin_amdgcn_exp2f(refs[wave + i][lane] - base);
+    sum = __builtin_fmaf(totals[wave + i][lane], f, sum);
+    const v4f x = sums[wave + i][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(x[e], f, y[e]);
+  }
+  const float rcp = ref == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(p.out + (int64_t)b * p.o_row + (kvh * p.group + kHeadTile * tile + h) * p.o_head + 2 * d) =
       make_uint2(pack2<DT>(y[0] * rcp, y[1] * rcp), pack2<DT>(y[2] * rcp, y[3] * rcp));
 }
 
-static int attend_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-
-// Ranges of a call: two workgroups a CU, unless all keys that the table can
-// hold are fewer blocks.
-static int64_t attend_ranges(int64_t pairs, int64_t max_keys) {
-  const int64_t most = pairs * std::max<int64_t>((max_keys + kBlockKeys - 1) / kBlockKeys, 1);
-  return std::min<int64_t>(most, 2 * current_device_cus());
+// Workgroups of a call: what the GPU holds, each with a range of the blocks of
+// all pairs; or one for each pair, if no pair can have more than kWholeBlocks
+// blocks (then nothing has to be joined).
+constexpr int64_t kWholeBlocks = 8;
+struct AttendPlan {
+  int64_t workgroups;
+  bool whole;
+};
+static AttendPlan attend_plan(int64_t pairs, int64_t max_keys, int dim) {
+  const int64_t blocks = std::max<int64_t>((max_keys + kBlockKeys - 1) / kBlockKeys, 1);
+  if (blocks <= kWholeBlocks) return {pairs, true};
+  return {std::min<int64_t>(pairs * blocks, attend_per_cu(attend_dp(dim)) * current_device_cus()), false};
 }
 
 static int64_t attend_tiles(int64_t heads, int64_t kv_heads) {
@@ -477,20 +576,27 @@ static int64_t attend_tiles(int64_t heads, int64_t kv_heads) {
 }
 
 template <int DT, bool CODES, int DP>
-static int launch_attend(const AttendParams& p, int64_t ranges, hipStream_t s) {
-  hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP>), dim3((unsigned)ranges), dim3(64 * kAttendWaves), 0, s, p);
-  const unsigned y = (unsigned)std::min(p.sequences, 32768);
-  hipLaunchKernelGGL((cache_attend_join_kernel<DT, DP>), dim3((unsigned)p.heads, y, (unsigned)((p.sequences + y - 1) / y)),
-                     dim3(64), 0, s, p, (int)ranges);
+static int launch_attend(const AttendParams& p, int64_t workgroups, hipStream_t s) {
+  hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP>), dim3((unsigned)workgroups), dim3(64 * kAttendWaves), 0, s, p);
+  if (!p.whole) {
+    // Waves for the ranges of a pair, where it can have many of them, or for its
+    // heads (64 pairs of 64 sequences, two or three ranges each: 5.0 us that way,
+    // 7.0 this way; one sequence's 8 pairs of 64 ranges 9.8 and 6.8).
+    const int64_t each = workgroups / ((int64_t)p.sequences * p.cache.heads * p.tiles);
+    const int parts = each >= 32 ? 8 : each >= 8 ? 4 : 1, per = kJoinWaves / parts * join_heads(DP);
+    hipLaunchKernelGGL((cache_attend_join_kernel<DT, DP>),
+                       dim3((unsigned)workgroups, (std::min(p.group, kHeadTile) + per - 1) / per), dim3(64 * kJoinWaves), 0,
+                       s, p, parts);
+  }
   return launch_status("w8a8_cache_attend");
 }
 
 template <int DT, bool CODES>
-static int launch_attend_dim(const AttendParams& p, int64_t ranges, hipStream_t s) {
+static int launch_attend_dim(const AttendParams& p, int64_t workgroups, hipStream_t s) {
   switch (attend_dp(p.cache.dim)) {
-    case 64: return launch_attend<DT, CODES, 64>(p, ranges, s);
-    case 128: return launch_attend<DT, CODES, 128>(p, ranges, s);
-    default: return launch_attend<DT, CODES, 256>(p, ranges, s);
+    case 64: return launch_attend<DT, CODES, 64>(p, workgroups, s);
+    case 128: return launch_attend<DT, CODES, 128>(p, workgroups, s);
+    default: return launch_attend<DT, CODES, 256>(p, workgroups, s);
   }
 }
 
@@ -500,8 +606,8 @@ extern "C" int64_t w8a8_cache_attend_workspace_size(int64_t sequences, int64_t h
                                                     int64_t max_keys) {
   using namespace w8a8;
   if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim > 256) return 0;
-  const int64_t ranges = attend_ranges(sequences * attend_tiles(heads, kv_heads), max_keys);
-  return ranges * 2 * kHeadTile * (attend_dp(dim) + 2) * (int64_t)sizeof(float);
+  const AttendPlan plan = attend_plan(sequences * attend_tiles(heads, kv_heads), max_keys, dim);
+  return plan.whole ? 0 : plan.workgroups * (2 * kHeadTile * (attend_dp(dim) + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(int4));
 }
 
 extern "C" int w8a8_cache_attend(const W8A8CacheAttendArgs* a) {
@@ -547,12 +653,15 @@ extern "C" int w8a8_cache_attend(const W8A8CacheAttendArgs* a) {
   p.lengths = a->lengths;
   p.c = a->sm_scale * kLog2eF;
   const int64_t pairs = a->sequences * p.cache.heads * p.tiles;
-  W8A8_REQUIRE(pairs * ((keys + kBlockKeys - 1) / kBlockKeys + 1) < (1ll << 48), "%s: too many keys in all", who);
-  const int64_t ranges = attend_ranges(pairs, keys);
-  p.part = reinterpret_cast<float*>(a->workspace);
-  p.part_ml = p.part + ranges * 2 * kHeadTile * attend_dp(p.cache.dim);
-  hipStream_t s = reinterpret_cast<hipStream_t>(a->stream);
   const bool codes = a->cache.dtype == W8A8_I8;
-  if (a->dtype == W8A8_F16) return codes ? launch_attend_dim<kF16, true>(p, ranges, s) : launch_attend_dim<kF16, false>(p, ranges, s);
-  return codes ? launch_attend_dim<kBF16, true>(p, ranges, s) : launch_attend_dim<kBF16, false>(p, ranges, s);
+  const AttendPlan plan = attend_plan(pairs, keys, p.cache.dim);
+  W8A8_REQUIRE(pairs * (keys / kBlockKeys + 1) < (1ll << 31) && plan.workgroups < (1 << 23),
+               "%s: too many sequences, heads and keys for one launch", who);   // (2^32 work-items)
+  p.whole = plan.whole;
+  p.part = reinterpret_cast<float*>(a->workspace);
+  p.part_ml = p.part + plan.workgroups * 2 * kHeadTile * attend_dp(p.cache.dim);
+  p.shared = reinterpret_cast<int4*>(p.part_ml + plan.workgroups * 4 * kHeadTile);
+  hipStream_t s = reinterpret_cast<hipStream_t>(a->stream);
+  if (a->dtype == W8A8_F16) return codes ? launch_attend_dim<kF16, true>(p, plan.workgroups, s) : launch_attend_dim<kF16, false>(p, plan.workgroups, s);
+  return codes ? launch_attend_dim<kBF16, true>(p, plan.workgroups, s) : launch_attend_dim<kBF16, false>(p, plan.workgroups, s);
 }
