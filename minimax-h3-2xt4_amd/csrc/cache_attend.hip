@@ -51,6 +51,7 @@ struct AttendParams {
   int sequences, heads, group, tiles;     // tiles: of 16 query heads of a kv head
   int width;
   int whole;    // a workgroup for each pair
+  int stream;   // more keys and values than the last cache holds
   const int32_t* table;
   int64_t ld_table;
   const int32_t* lengths;
@@ -148,18 +149,19 @@ __device__ __forceinline__ v2u codes4(uint32_t w) {
   }
 }
 
-// A lane's loads of a group of 16 tokens: W words from byte offset off of its descriptor.
-template <int W>
+// A lane's loads of a group of 16 tokens: W words from byte offset off of its
+// descriptor. AUX 2: non-temporal.
+template <int W, int AUX>
 __device__ __forceinline__ void group_load(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t (&w)[W]) {
   if constexpr (W == 1) {
-    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0);
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, AUX);
   } else if constexpr (W == 2) {
-    const v2u t = __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0);
+    const v2u t = __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, AUX);
     w[0] = t.x; w[1] = t.y;
   } else {
 #pragma unroll
     for (int i = 0; i < W / 4; ++i) {
-      const v4u t = __builtin_amdgcn_raw_buffer_load_b128(r, (int)off + 16 * i, 0, 0);
+      const v4u t = __builtin_amdgcn_raw_buffer_load_b128(r, (int)off + 16 * i, 0, AUX);
       w[4 * i] = t.x; w[4 * i + 1] = t.y; w[4 * i + 2] = t.z; w[4 * i + 3] = t.w;
     }
   }
@@ -167,14 +169,18 @@ __device__ __forceinline__ void group_load(__amdgpu_buffer_rsrc_t r, uint32_t of
 
 constexpr uint32_t kNowhere = 0x7fffff00u;   // an offset behind every descriptor's end
 
-// DT: type of q and out; CODES: the cache holds I8; DP: dim rounded up to 64, 128 or 256.
-template <int DT, bool CODES, int DP>
+// DT: type of q and out; CODES: the cache holds I8; DP: dim rounded up to 64, 128
+// or 256; STREAM: the keys and values pass through the caches without staying.
+template <int DT, bool CODES, int DP, bool STREAM>
 __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_attend_kernel(AttendParams p) {
-  constexpr int ES = CODES ? 1 : 2;
+  constexpr int ES = CODES ? 1 : 2, AUX = STREAM ? 2 : 0;
   constexpr int G = kWaveKeys / kGroupTokens;
   constexpr int NS = DP / 32;          // products of a key tile
   constexpr int VL = DP / 16;          // channels a lane reads of a value row
-  constexpr int KW = CODES ? 2 : 4;    // words of eight channels
+  // Channel of lane quad in step s of K Q^T, any order being as good as another:
+  // loads are 16 bytes a lane, eight channels of a step, or with codes of two.
+  constexpr int KS = CODES ? 2 : 1;
+  auto channel = [](int quad, int s) { return CODES ? 64 * (s / 2) + 16 * quad + 8 * (s % 2) : 32 * s + 8 * quad; };
   constexpr int VW = VL * ES / 4;      // words of VL channels
   constexpr int kRow = DP + 4;         // a head's sums in LDS, padded
   __shared__ __attribute__((aligned(16))) float sums[kAttendWaves][kHeadTile][kRow];
@@ -205,10 +211,10 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
   }
 
   // Byte offsets within a group of 16 tokens.
-  uint32_t koff[NS], voff[4];
+  uint32_t koff[NS / KS], voff[4];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const int d = 8 * quad + 32 * s;
+  for (int s = 0; s < NS / KS; ++s) {
+    const int d = channel(quad, KS * s);
     koff[s] = d < dim ? col * p.cache.token_b + d * ES : kNowhere;
   }
 #pragma unroll
@@ -256,13 +262,13 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(t), 0,
                                              k.n[i] ? (int)((k.n[i] - 1) * p.cache.token_b) + dim * ES : 0, 0x00027000);
   };
-  uint32_t kr[G][NS][KW], vr[4 * G][VW];
+  uint32_t kr[G][NS / KS][4], vr[4 * G][VW];
   auto load_k = [&](const Keys& k) {
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const auto r = group_rsrc(p.cache.k, k, i);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) group_load<KW>(r, koff[s], kr[i][s]);
+      for (int s = 0; s < NS / KS; ++s) group_load<4, AUX>(r, koff[s], kr[i][s]);
     }
   };
   auto load_v = [&](const Keys& k) {
@@ -270,7 +276,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
     for (int i = 0; i < G; ++i) {
       const auto r = group_rsrc(p.cache.v, k, i);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) group_load<VW>(r, voff[t], vr[4 * i + t]);
+      for (int t = 0; t < 4; ++t) group_load<VW, AUX>(r, voff[t], vr[4 * i + t]);
     }
   };
   struct Scales {
@@ -298,7 +304,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
     const int kvh = pr / p.tiles, first = kHeadTile * (pr - kvh * p.tiles) + col;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      const int d = 8 * quad + 32 * s;
+      const int d = channel(quad, s);
       qf[s] = v4u{0, 0, 0, 0};
       if (first < p.group && d < dim)
         qf[s] = *reinterpret_cast<const v4u*>(p.q + (int64_t)seq * p.q_row + (kvh * p.group + first) * p.q_head + 2 * d);
@@ -329,7 +335,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
         for (int x = 0; x < NS; ++x) {
           v4u a;
           if constexpr (CODES) {
-            const v2u lo = codes4<DT>(kr[i][x][0]), hi = codes4<DT>(kr[i][x][1]);
+            const v2u lo = codes4<DT>(kr[i][x / 2][2 * (x % 2)]), hi = codes4<DT>(kr[i][x / 2][2 * (x % 2) + 1]);
             a = v4u{lo.x, lo.y, hi.x, hi.y};
           } else {
             a = v4u{kr[i][x][0], kr[i][x][1], kr[i][x][2], kr[i][x][3]};
@@ -577,7 +583,9 @@ static int64_t attend_tiles(int64_t heads, int64_t kv_heads) {
 
 template <int DT, bool CODES, int DP>
 static int launch_attend(const AttendParams& p, int64_t workgroups, hipStream_t s) {
-  hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP>), dim3((unsigned)workgroups), dim3(64 * kAttendWaves), 0, s, p);
+  const dim3 g((unsigned)workgroups), t(64 * kAttendWaves);
+  if (p.stream) hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP, true>), g, t, 0, s, p);
+  else hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP, false>), g, t, 0, s, p);
   if (!p.whole) {
     // Waves for the ranges of a pair, where it can have many of them, or for its
     // heads (64 pairs of 64 sequences, two or three ranges each: 5.0 us that way,
@@ -658,6 +666,11 @@ extern "C" int w8a8_cache_attend(const W8A8CacheAttendArgs* a) {
   W8A8_REQUIRE(pairs * (keys / kBlockKeys + 1) < (1ll << 31) && plan.workgroups < (1 << 23),
                "%s: too many sequences, heads and keys for one launch", who);   // (2^32 work-items)
   p.whole = plan.whole;
+  // What the table can name, against the last cache's 256 MB: read once and never
+  // again, so let it pass (512 MB: 102 -> 89 us; 94 MB that the last call left
+  // there: 23.3 -> 26.2 that way).
+  const int64_t row = codes ? a->cache.dim + 4 : 2 * a->cache.dim;
+  p.stream = 2 * row * a->cache.heads * keys * a->sequences > (256ll << 20);
   p.part = reinterpret_cast<float*>(a->workspace);
   p.part_ml = p.part + plan.workgroups * 2 * kHeadTile * attend_dp(p.cache.dim);
   p.shared = reinterpret_cast<int4*>(p.part_ml + plan.workgroups * 4 * kHeadTile);

@@ -21,6 +21,7 @@
 // that the rows of one read fall on different banks.
 #include "paged.h"
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -45,6 +46,9 @@ struct PackedParams {
   const int32_t* k_starts;
   float c;
   int fill;
+  int splits;       // ranges of a tile's keys, each a workgroup's
+  float* part;      // [splits][rows][heads][DP]
+  float* part_ml;   // [splits][rows][heads][2]: reference, sum
 };
 
 template <int DT>
@@ -87,51 +91,57 @@ __device__ __forceinline__ int v_swizzle(int r) {
 
 __device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// The wave's sequence and tile of queries of tile t, the tiles of a sequence
-// taken from the last (of causal ones the longest) to the first. Behind the
-// sequences come the tiles of the rows behind them, as a sequence of its own.
+// The sequence and the tile of queries of tile t. Of up to 64 sequences those
+// with the most keys come first, and the tiles of a sequence from its last (of
+// causal ones the longest) to its first, so that what is left at the end is
+// short. (More sequences are taken 64 at a time.) Behind the sequences come the
+// tiles of the rows behind them, as a sequence of its own without keys.
 struct PackedTile {
-  int b, first, n;   // first row of the tile in its sequence, the sequence's rows
-  int row0;          // the sequence's first row
+  int b, first, n;     // first row of the tile in its sequence, the sequence's rows
+  int row0, key0, nk;  // the sequence's first row, first key and keys
 };
 
 __device__ __forceinline__ PackedTile packed_find(const PackedParams& p, int t) {
   const int lane = threadIdx.x & 63;
   int sum = 0;
   for (int b0 = 0; b0 <= p.sequences; b0 += 64) {
-    const int b = b0 + lane;
-    int lo = 0, n = 0;
+    const int b = b0 + lane, count = min(p.sequences + 1 - b0, 64);
+    int lo = 0, n = 0, key0 = 0, nk = -1;
     if (b <= p.sequences) {
       lo = clamp_to(p.starts[b], 0, p.rows);
       n = clamp_to(b < p.sequences ? p.starts[b + 1] : p.rows, lo, p.rows) - lo;
+      if (b < p.sequences) {
+        key0 = clamp_to(p.k_starts[b], 0, p.keys);
+        nk = clamp_to(p.k_starts[b + 1], key0, p.keys) - key0;
+      }
     }
     const int tiles = (n + kPackQ - 1) / kPackQ;
-    int upto = tiles;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int u = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += u;
+    int before = sum;   // tiles of the sequences that come first
+    for (int j = 0; j < count; ++j) {
+      const int other = __builtin_amdgcn_readlane(nk, j);
+      if (other > nk || (other == nk && j < lane)) before += __builtin_amdgcn_readlane(tiles, j);
+      sum += __builtin_amdgcn_readlane(tiles, j);
     }
-    upto += sum;
-    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > t);
-    if (past) {
-      const int at = __builtin_ctzll(past);
+    const uint64_t here = __builtin_amdgcn_ballot_w64(lane < count && before <= t && t < before + tiles);
+    if (here) {
+      const int at = __builtin_ctzll(here);
       PackedTile r;
       r.b = b0 + at;
       r.row0 = __builtin_amdgcn_readlane(lo, at);
       r.n = __builtin_amdgcn_readlane(n, at);
-      r.first = (__builtin_amdgcn_readlane(upto, at) - 1 - t) * kPackQ;
+      r.key0 = __builtin_amdgcn_readlane(key0, at);
+      r.nk = max(__builtin_amdgcn_readlane(nk, at), 0);
+      r.first = (__builtin_amdgcn_readlane(before + tiles, at) - 1 - t) * kPackQ;
       return r;
     }
-    sum = __builtin_amdgcn_readlane(upto, 63);
   }
-  return {-1, 0, 0, 0};
+  return {-1, 0, 0, 0, 0, 0};
 }
 
 // What a workgroup and its waves work on, DP channels wide, BK keys a block.
 // TID is the thread's index (a copy of it that the compiler takes for another
 // value keeps nothing alive from the one's use to the other's).
-template <int DT, int DP, bool CAUSAL>
+template <int DT, int DP, bool CAUSAL, bool SPLIT>
 struct Packed {
   static constexpr int BK = DP > 128 ? 32 : 64;      // keys of a block
   static constexpr int CH = DP / 8;                  // chunks of a row
@@ -144,7 +154,7 @@ struct Packed {
   char* tiles;
   int lane, wave, col, half;
   PackedTile tile;
-  int head, mine, key0, nk;
+  int head, mine, nk, split;
   bool stored;
   int blocks, limit, wave_clean, wave_blocks;
   const char* kbase;
@@ -156,7 +166,15 @@ struct Packed {
     wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     col = lane & 31;
     half = lane >> 5;
-    const int item = blockIdx.x / p.kv_heads, kvh = blockIdx.x - item * p.kv_heads;
+    // Neighbours are the key heads: workgroups go round the XCDs in turn, so with
+    // a multiple of eight of them a key head's stay with one XCD's cache.
+    int item = blockIdx.x / p.kv_heads;
+    const int kvh = blockIdx.x - item * p.kv_heads;
+    split = 0;
+    if constexpr (SPLIT) {
+      split = item % p.splits;
+      item /= p.splits;
+    }
     head = kvh * p.group + item % p.group;
     tile = packed_find(p, item / p.group);
     if (tile.b < 0) return;
@@ -164,16 +182,26 @@ struct Packed {
     mine = q0 + col;
     stored = mine < tile.n;
     if (tile.b == p.sequences) return;
-    key0 = clamp_to(scalar_int(p.k_starts, tile.b), 0, p.keys);
-    nk = clamp_to(scalar_int(p.k_starts, tile.b + 1), key0, p.keys) - key0;
+    nk = tile.nk;
     const int shift = nk - tile.n;              // causal: query i sees keys up to i + shift
     const int seen = CAUSAL ? clamp_to(tile.first + kPackQ + shift, 0, nk) : nk;   // keys that the workgroup sees,
     limit = CAUSAL ? clamp_to(mine + shift + 1, 0, nk) : nk;                       // this query,
     wave_clean = CAUSAL ? clamp_to(q0 + shift + 1, 0, nk) : nk;                    // all of the wave's,
-    wave_blocks = ((CAUSAL ? clamp_to(q0 + 32 + shift, 0, nk) : nk) + BK - 1) / BK;   // and some of them (in blocks)
+    const int some = q0 >= tile.n ? 0 : CAUSAL ? clamp_to(q0 + 32 + shift, 0, nk) : nk;   // some of them
+    wave_blocks = (some + BK - 1) / BK;
     blocks = (seen + BK - 1) / BK;
-    kbase = p.k + (int64_t)key0 * p.k_row + kvh * p.k_head;
-    vbase = p.v + (int64_t)key0 * p.v_row + kvh * p.v_head;
+    int64_t from = tile.key0;
+    if constexpr (SPLIT) {   // the keys before this range's first are another's: count from there
+      const int begin = blocks * split / p.splits, end = blocks * (split + 1) / p.splits, off = begin * BK;
+      blocks = end - begin;
+      wave_blocks = clamp_to(wave_blocks - begin, 0, blocks);
+      nk -= off;
+      limit -= off;
+      wave_clean -= off;
+      from += off;
+    }
+    kbase = p.k + from * p.k_row + kvh * p.k_head;
+    vbase = p.v + from * p.v_row + kvh * p.v_head;
     // Copies of a tile: lane l of instruction u of wave w brings what lies at
     // chunk (4 u + w) * 64 + l of the tile.
 #pragma unroll
@@ -257,9 +285,21 @@ struct Packed {
         if (j * BK + 32 * t + 8 * (e / 4) + 4 * half + e % 4 >= limit) x[t][e] = -INFINITY;
   }
 
-  __device__ __forceinline__ void store(const v16f (&o)[DF], float l) const {
+  __device__ __forceinline__ void store(const v16f (&o)[DF], float ref, float l) const {
     const auto both = lane_halves(l);
     l = both.first + both.second;
+    if constexpr (SPLIT) {
+      if (!stored) return;
+      const int64_t at = ((int64_t)split * p.rows + tile.row0 + mine) * (p.group * p.kv_heads) + head;
+#pragma unroll
+      for (int f = 0; f < DF; ++f)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<v4f*>(p.part + at * DP + 32 * f + 8 * g + 4 * half) =
+              v4f{o[f][4 * g], o[f][4 * g + 1], o[f][4 * g + 2], o[f][4 * g + 3]};
+      if (half == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(ref, l);
+      return;
+    }
     const float rcp = l == 0.0f ? 0.0f : 1.0f / l;
     if (!stored) return;
     char* at = to();
@@ -306,11 +346,11 @@ struct PackedState {
 // masked key's value may be infinite or NaN, and its product with P = 0 is not 0.
 // In blocks with masked keys such values are set to 0 for the product, and a
 // count of those that a query sees brings them back. One block at a time.
-template <int DT, int DP>
+template <int DT, int DP, bool SPLIT>
 __device__ __forceinline__ void packed_careful(const PackedParams& p, char* tiles) {
   int tid = threadIdx.x;
   __asm__ volatile("" : "+v"(tid));
-  using W = Packed<DT, DP, true>;
+  using W = Packed<DT, DP, true, SPLIT>;
   const W w(p, tiles, tid);
   v4u qf[W::NS];
   w.queries(qf);
@@ -376,7 +416,7 @@ __device__ __forceinline__ void packed_careful(const PackedParams& p, char* tile
       }
     }
   }
-  w.store(st.o, st.l);
+  w.store(st.o, st.ref, st.l);
 }
 
 // DT: F16 or BF16; DP: dim rounded up to 64, 96, 128 or 256.
@@ -387,16 +427,16 @@ __device__ __forceinline__ void packed_careful(const PackedParams& p, char* tile
 // so K's copies run a step ahead of V's. The order is laid out product by
 // product (left to the compiler, all fragments are read at once, which spills,
 // and the VALU's work follows the MFMAs').
-template <int DT, int DP, bool CAUSAL>
+template <int DT, int DP, bool CAUSAL, bool SPLIT>
 __global__ __launch_bounds__(64 * kPackWaves, DP > 128 ? 1 : 2) void packed_attention_kernel(PackedParams p) {
-  using W = Packed<DT, DP, CAUSAL>;
+  using W = Packed<DT, DP, CAUSAL, SPLIT>;
   constexpr int BK = W::BK, NS = W::NS, DF = W::DF, TF = W::TF;
   constexpr int QK = TF * NS, PV = BK / 16 * DF, AHEAD = 3;
   __shared__ __attribute__((aligned(1024))) char tiles[4 * W::kTile];   // two of K, two of V
   const W w(p, tiles, threadIdx.x);
   if (w.tile.b < 0) return;
   if (w.tile.b == p.sequences) {
-    if (p.fill && w.stored)
+    if (p.fill && w.stored && w.split == 0)
       for (int d = 4 * w.half; d < p.dim; d += 8) *reinterpret_cast<uint2*>(w.to() + 2 * d) = make_uint2(0, 0);
     return;
   }
@@ -489,10 +529,8 @@ __global__ __launch_bounds__(64 * kPackWaves, DP > 128 ? 1 : 2) void packed_atte
     }
   };
   auto sync = [&](int j) {
-    if (j > 0) {
-      __builtin_amdgcn_s_waitcnt(0x0F70);   // this wave's copies of K j + 1 and V j have landed,
-      __syncthreads();                      // and everyone's; K j and V j - 1 have been read
-    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // this wave's copies of K j + 1 and V j have landed,
+    __syncthreads();                      // and everyone's; K j and V j - 1 have been read
     if (j + 2 < w.blocks) w.copy_k(j + 2, w.kt(j & 1));
     if (j + 1 < w.blocks) w.copy_v(j + 1, w.vt((j + 1) & 1));
   };
@@ -540,37 +578,111 @@ __global__ __launch_bounds__(64 * kPackWaves, DP > 128 ? 1 : 2) void packed_atte
     for (int f = 0; f < DF; ++f)
 #pragma unroll
       for (int x = 0; x < 16; ++x) z = __builtin_fmaf(st.o[f][x], 0.0f, z);
-    w.store(st.o, st.l);
+    w.store(st.o, st.ref, st.l);
     const bool odd = __builtin_amdgcn_ballot_w64(z != 0.0f) != 0;
     __syncthreads();   // the tiles have been read
     int* again = reinterpret_cast<int*>(tiles);
     if (w.lane == 0) again[w.wave] = odd;
     __syncthreads();
-    if (again[0] | again[1] | again[2] | again[3]) packed_careful<DT, DP>(p, tiles);
+    if (again[0] | again[1] | again[2] | again[3]) packed_careful<DT, DP, SPLIT>(p, tiles);
   } else {
-    w.store(st.o, st.l);
+    w.store(st.o, st.ref, st.l);
   }
+}
+
+// The ranges' sums of a row and head, joined in order: DP / 4 lanes each.
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
+  constexpr int LANES = DP == 96 ? 32 : DP / 4;
+  const int heads = p.group * p.kv_heads;
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
+  const int d = 4 * (threadIdx.x % LANES);
+  const int64_t row = item / heads;
+  const int head = (int)(item - row * heads);
+  if (row >= p.rows || row >= scalar_int(p.starts, p.sequences) || d >= p.dim) return;
+  float ref = -INFINITY, sum = 0.0f;
+  v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int BATCH = 8;
+  for (int s = 0; s < p.splits; s += BATCH) {
+    float2 ml[BATCH];
+    v4f x[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int64_t at = ((int64_t)min(s + i, p.splits - 1) * p.rows + row) * heads + head;
+      ml[i] = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+      x[i] = *reinterpret_cast<const v4f*>(p.part + at * DP + d);
+    }
+    float to = ref;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) to = fmaxf(to, ml[i].x);
+    const float base = to == -INFINITY ? 0.0f : to, fade = __builtin_amdgcn_exp2f(ref - base);
+    ref = to;
+    sum = sum * fade;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = y[e] * fade;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      if (s + i >= p.splits) continue;
+      const float f = __builtin_amdgcn_exp2f(ml[i].x - base);
+      sum = __builtin_fmaf(ml[i].y, f, sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(x[i][e], f, y[e]);
+    }
+  }
+  const float rcp = sum == 0.0f ? 0.0f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(p.out + row * p.o_row + head * p.o_head + 2 * d) =
+      make_uint2(pack2<DT>(y[0] * rcp, y[1] * rcp), pack2<DT>(y[2] * rcp, y[3] * rcp));
+}
+
+static int packed_dp(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
+
+// Ranges of a tile's keys: where the tiles of all heads are fewer than half of
+// what the GPU holds, as many as fill it, if each has four blocks or more of a
+// sequence's average keys.
+static int packed_splits(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int dim) {
+  if (rows <= 0 || keys <= 0 || sequences <= 0 || heads <= 0 || dim <= 0) return 1;
+  const int64_t filled = std::min(rows, sequences), tiles = (rows + (kPackQ - 1) * filled) / kPackQ;
+  const int64_t slots = (dim > 128 ? 1 : 2) * current_device_cus(), block = dim > 128 ? 32 : 64;
+  const int64_t splits = std::min(slots / (tiles * heads), keys / sequences / (4 * block));
+  return splits >= 2 ? (int)splits : 1;
+}
+
+template <int DT, int DP, bool CAUSAL>
+static int launch_packed(const PackedParams& p, int64_t grid, hipStream_t s) {
+  const dim3 g((unsigned)(grid * p.splits)), t(64 * kPackWaves);
+  if (p.splits == 1) {
+    hipLaunchKernelGGL((packed_attention_kernel<DT, DP, CAUSAL, false>), g, t, 0, s, p);
+  } else {
+    hipLaunchKernelGGL((packed_attention_kernel<DT, DP, CAUSAL, true>), g, t, 0, s, p);
+    const int64_t per = 256 / (DP == 96 ? 32 : DP / 4), items = (int64_t)p.rows * p.group * p.kv_heads;
+    hipLaunchKernelGGL((packed_join_kernel<DT, DP>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, s, p);
+  }
+  return launch_status("w8a8_packed_attention");
 }
 
 template <int DT, int DP>
 static int launch_packed(const PackedParams& p, bool causal, int64_t grid, hipStream_t s) {
-  const dim3 g((unsigned)grid), t(64 * kPackWaves);
-  if (causal) hipLaunchKernelGGL((packed_attention_kernel<DT, DP, true>), g, t, 0, s, p);
-  else hipLaunchKernelGGL((packed_attention_kernel<DT, DP, false>), g, t, 0, s, p);
-  return launch_status("w8a8_packed_attention");
+  return causal ? launch_packed<DT, DP, true>(p, grid, s) : launch_packed<DT, DP, false>(p, grid, s);
 }
 
 template <int DT>
 static int launch_packed_dim(const PackedParams& p, bool causal, int64_t grid, hipStream_t s) {
-  if (p.dim <= 64) return launch_packed<DT, 64>(p, causal, grid, s);
-  if (p.dim <= 96) return launch_packed<DT, 96>(p, causal, grid, s);
-  if (p.dim <= 128) return launch_packed<DT, 128>(p, causal, grid, s);
-  return launch_packed<DT, 256>(p, causal, grid, s);
+  switch (packed_dp(p.dim)) {
+    case 64: return launch_packed<DT, 64>(p, causal, grid, s);
+    case 96: return launch_packed<DT, 96>(p, causal, grid, s);
+    case 128: return launch_packed<DT, 128>(p, causal, grid, s);
+    default: return launch_packed<DT, 256>(p, causal, grid, s);
+  }
 }
 
 }  // namespace w8a8
 
-extern "C" int64_t w8a8_packed_attention_workspace_size(int64_t, int64_t, int64_t, int64_t, int32_t) { return 0; }
+extern "C" int64_t w8a8_packed_attention_workspace_size(int64_t rows, int64_t keys, int64_t sequences, int64_t heads,
+                                                        int32_t dim) {
+  using namespace w8a8;
+  const int splits = packed_splits(rows, keys, sequences, heads, dim);
+  return splits == 1 ? 0 : splits * rows * heads * (packed_dp(dim) + 2) * (int64_t)sizeof(float);
+}
 
 extern "C" int w8a8_packed_attention(const W8A8PackedAttentionArgs* a) {
   using namespace w8a8;
@@ -605,15 +717,21 @@ extern "C" int w8a8_packed_attention(const W8A8PackedAttentionArgs* a) {
                     (!spans_overlap(a->k, rows_span(a->keys, a->kv_heads, a->dim, a->k_strides), a->out, osize) &&
                      !spans_overlap(a->v, rows_span(a->keys, a->kv_heads, a->dim, a->v_strides), a->out, osize))),
                "%s: out overlaps an input", who);
+  const int splits = packed_splits(a->rows, a->keys, a->sequences, a->heads, a->dim);
+  const int64_t need = w8a8_packed_attention_workspace_size(a->rows, a->keys, a->sequences, a->heads, a->dim);
+  W8A8_REQUIRE(need == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= need),
+               "%s: workspace of %lld bytes needed", who, (long long)need);
   const int64_t grid = (a->rows / kPackQ + a->sequences + 1) * a->heads;
-  W8A8_REQUIRE(grid < (1 << 24), "%s: too many rows, sequences and heads for one launch", who);   // (2^32 work-items)
+  W8A8_REQUIRE(grid * splits < (1 << 24), "%s: too many rows, sequences and heads for one launch", who);   // (2^32 work-items)
   const PackedParams p{reinterpret_cast<const char*>(a->q), reinterpret_cast<const char*>(a->k),
                        reinterpret_cast<const char*>(a->v), reinterpret_cast<char*>(a->out),
                        2 * a->q_strides[0], 2 * a->q_strides[1], 2 * a->k_strides[1], 2 * a->v_strides[1],
                        2 * a->out_strides[0], 2 * a->out_strides[1],
                        (uint32_t)(2 * a->k_strides[0]), (uint32_t)(2 * a->v_strides[0]),
                        (int)a->rows, (int)a->keys, (int)a->sequences, a->heads / a->kv_heads, a->kv_heads, a->dim,
-                       a->starts, a->k_starts, a->sm_scale * kLog2eF, a->fill};
+                       a->starts, a->k_starts, a->sm_scale * kLog2eF, a->fill, splits,
+                       reinterpret_cast<float*>(a->workspace),
+                       reinterpret_cast<float*>(a->workspace) + splits * a->rows * a->heads * packed_dp(a->dim)};
   hipStream_t s = reinterpret_cast<hipStream_t>(a->stream);
   return a->dtype == W8A8_F16 ? launch_packed_dim<kF16>(p, a->causal != 0, grid, s)
                               : launch_packed_dim<kBF16>(p, a->causal != 0, grid, s);

@@ -51,36 +51,28 @@ __device__ __forceinline__ void group_place(const CacheView& c, uint32_t g, int&
   token = ((int)g - entry * (c.page_size / kGroupTokens)) * kGroupTokens;
 }
 
-// Sum of a 64-bit value over the wave's 64 lanes, and its inclusive prefix.
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
-}
-__device__ __forceinline__ int64_t wave_prefix64(int64_t v) {
+// The sequence b in [0, n) with starts[b] <= row < starts[b + 1], or n, with its
+// two starts and its length, if lengths are given (a wave works together; the
+// row is the wave's). The lanes look at 64 sequences at once.
+struct SequenceRow {
+  int b, first, last, length;
+};
+__device__ __forceinline__ SequenceRow sequence_of(const int32_t* starts, int n, int64_t row, const int32_t* lengths) {
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t t = __shfl_up(v, off, 64);
-    if (lane >= off) v += t;
+  SequenceRow r{n, 0, 0, 0};
+  for (int b0 = 0; b0 < n; b0 += 64) {
+    const int i = min(b0 + lane, n - 1);
+    const int first = starts[i], last = starts[i + 1], length = lengths ? lengths[i] : 0;
+    const uint64_t in = __builtin_amdgcn_ballot_w64(b0 + lane < n && first <= row && row < last);
+    if (in == 0) continue;
+    const int at = __builtin_ctzll(in);
+    r.b = b0 + at;
+    r.first = __builtin_amdgcn_readlane(first, at);
+    r.last = __builtin_amdgcn_readlane(last, at);
+    r.length = __builtin_amdgcn_readlane(length, at);
+    break;
   }
-  return v;
-}
-
-// The last b in [0, n) with starts[b] <= row, or n when row is at or past
-// starts[n] (a wave works together; the row is the wave's). Sequences without
-// rows are passed over, since the next one starts at the same row.
-__device__ __forceinline__ int sequence_of(const int32_t* starts, int n, int64_t row) {
-  const int lane = threadIdx.x & 63;
-  int count = 0;
-  for (int b = 0; b <= n; b += 64) {
-    const int i = b + lane;
-    const bool below = i <= n && starts[i] <= row;
-    const uint64_t m = __builtin_amdgcn_ballot_w64(below);
-    count += __builtin_popcountll(m);
-    if (m != ~0ull) break;
-  }
-  return __builtin_amdgcn_readfirstlane(count > n ? n : max(count - 1, 0));
+  return r;
 }
 
 inline bool stride8(int64_t s) { return s >= 0 && s % 8 == 0; }

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from attention_refs import attention64, bound, check, check_packed, starts_of
+from w8a8 import _abi
 from w8a8.packed_attention import packed_attention
 
 pytestmark = pytest.mark.gpu
@@ -45,6 +46,40 @@ LENGTHS = [([1], [1]), ([1], [300]), ([31], [31]), ([32, 33], [32, 33]), ([127, 
 def test_lengths(gpu, new, keys, causal):
     run(torch.bfloat16, 2, 1, 128, new, keys, causal)
     run(torch.float16, 2, 2, 64, new, keys, causal)
+
+
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('dtype,dim', [(torch.bfloat16, 128), (torch.float16, 72), (torch.bfloat16, 64), (torch.float16, 200)])
+@pytest.mark.parametrize('new,keys', [([16], [4000]), ([1, 1, 1], [3000, 1, 2900]), ([130], [3001]), ([300, 2], [40, 5000]),
+                                      ([0, 7, 33], [900, 2500, 2600])])
+def test_few_rows_behind_many_keys(gpu, new, keys, dtype, dim, causal):
+    """Workgroups share a tile's keys and join their sums."""
+    assert _abi.load().w8a8_packed_attention_workspace_size(sum(new), sum(keys), len(new), 4, dim) > 0
+    run(dtype, 4, 2, dim, new, keys, causal, seed=dim)
+
+
+def test_shared_keys_that_are_masked_have_no_effect(gpu):
+    st, starts = starts_of([40], 'cuda')
+    ks, k_starts = starts_of([3000], 'cuda')
+    q, k, v = make(torch.bfloat16, 40, 3000, 2, 1, 128, seed=9)
+    vv, kk = v.clone(), k.clone()
+    vv[2980, :, ::3], kk[2980, :, 1::4] = math.nan, math.inf
+    y = packed_attention(q, kk, vv, starts, k_starts)
+    check_packed(y[:20], q[:20], k[:2980], v[:2980], [0, 20], [0, 2980], True, 128 ** -0.5)
+    assert bool(torch.isnan(y[20:, :, ::3]).all())
+    out = torch.full((50, 2, 128), 5.0, dtype=torch.bfloat16, device='cuda')
+    q = torch.cat([q, q[:10]])
+    packed_attention(q, k, v, starts, k_starts, out=out)
+    check_packed(out, q, k, v, st, ks, True, 128 ** -0.5)
+    assert bool((out[40:] == 5.0).all())
+    fresh = packed_attention(q, k, v, starts, k_starts)
+    assert torch.equal(fresh[:40], out[:40]) and not bool(fresh[40:].any())
+
+
+def test_more_sequences_than_lanes(gpu):
+    """Tiles are found 64 sequences at a time."""
+    new = [(7 * i) % 150 for i in range(131)]
+    run(torch.float16, 1, 1, 64, new, [n + 3 * (i % 40) for i, n in enumerate(new)], True)
 
 
 @pytest.mark.parametrize('heads,kv', [(1, 1), (6, 2), (8, 1), (20, 1), (7, 7), (64, 8)])
