@@ -131,22 +131,13 @@ __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
 }
 
-// Four codes of a word as two words of DT values (exact in both types).
-template <int DT>
+// Four codes of a word as two words of fp16 values: 0x6400 | (code + 128) is 1152 + code.
 __device__ __forceinline__ v2u codes4(uint32_t w) {
-  if constexpr (DT == kF16) {
-    // 0x6400 | (code + 128) is the fp16 value 1152 + code.
-    const uint32_t u = w ^ 0x80808080u;
-    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u), hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
-    return v2u{__builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, lo) - off),
-               __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, hi) - off)};
-  } else {
-    uint32_t f[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = __float_as_uint((float)(int8_t)(w >> (8 * i)));
-    return v2u{__builtin_amdgcn_perm(f[1], f[0], 0x07060302u), __builtin_amdgcn_perm(f[3], f[2], 0x07060302u)};
-  }
+  const uint32_t u = w ^ 0x80808080u;
+  const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u), hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+  const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
+  return v2u{__builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, lo) - off),
+             __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, hi) - off)};
 }
 
 // A lane's loads of a group of 16 tokens: W words from byte offset off of its
@@ -174,6 +165,10 @@ constexpr uint32_t kNowhere = 0x7fffff00u;   // an offset behind every descripto
 template <int DT, bool CODES, int DP, bool STREAM>
 __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_attend_kernel(AttendParams p) {
   constexpr int ES = CODES ? 1 : 2, AUX = STREAM ? 2 : 0;
+  // Codes are multiplied as fp16, whatever q's type: cheaper to make than bf16,
+  // and P keeps eleven bits. q of bf16 is scaled by a power of 2 for it, so that a
+  // head's largest is from 1 to 2: exact but for what lies 2^-14 below that.
+  constexpr int MT = CODES ? kF16 : DT;
   constexpr int G = kWaveKeys / kGroupTokens;
   constexpr int NS = DP / 32;          // products of a key tile
   constexpr int VL = DP / 16;          // channels a lane reads of a value row
@@ -310,6 +305,28 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
         qf[s] = *reinterpret_cast<const v4u*>(p.q + (int64_t)seq * p.q_row + (kvh * p.group + first) * p.q_head + 2 * d);
     }
   };
+  // bf16 queries as fp16 ones, and the scores' factor for them.
+  float factor = p.c;
+  auto convert_q = [&]() {
+    if constexpr (CODES && DT == kBF16) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, max(qf[s][i] & 0x7fffu, (qf[s][i] >> 16) & 0x7fffu));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+      const int e = (int)(top >> 7) - 127;
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = qf[s][i];
+          qf[s][i] = pack2<kF16>(ldexpf(__uint_as_float(w << 16), -e), ldexpf(__uint_as_float(w & 0xffff0000u), -e));
+        }
+      factor = ldexpf(p.c, e);
+    }
+  };
   load_q(b, pair);
 
   while (true) {
@@ -317,6 +334,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
     const int take = min(nblk - blk, end - at);
     const int nh = min(p.group - kHeadTile * tile, kHeadTile);
     const int head0 = kvh * p.group + kHeadTile * tile;
+    convert_q();
     v4f o[VL];
 #pragma unroll
     for (int j = 0; j < VL; ++j) o[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -335,16 +353,16 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
         for (int x = 0; x < NS; ++x) {
           v4u a;
           if constexpr (CODES) {
-            const v2u lo = codes4<DT>(kr[i][x / 2][2 * (x % 2)]), hi = codes4<DT>(kr[i][x / 2][2 * (x % 2) + 1]);
+            const v2u lo = codes4(kr[i][x / 2][2 * (x % 2)]), hi = codes4(kr[i][x / 2][2 * (x % 2) + 1]);
             a = v4u{lo.x, lo.y, hi.x, hi.y};
           } else {
             a = v4u{kr[i][x][0], kr[i][x][1], kr[i][x][2], kr[i][x][3]};
           }
-          s = mfma16<DT>(a, qf[x], s);
+          s = mfma16<MT>(a, qf[x], s);
         }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          t[4 * i + x] = s[x] * p.c;
+          t[4 * i + x] = s[x] * factor;
           if constexpr (CODES) t[4 * i + x] = t[4 * i + x] * sc.k[i][x];
         }
       }
@@ -391,22 +409,26 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
 #pragma unroll
       for (int i = 0; i < 4 * G; ++i) {
         w[i] = __builtin_amdgcn_exp2f(t[i] - base);
-        l += w[i];
+        if constexpr (CODES) l += w[i];
         // P carries the values' scales, relative to about the largest so far,
         // so that it keeps the type's precision whatever their size.
         if constexpr (CODES) w[i] = w[i] * (sc.v[i / 4][i % 4] * inv);
       }
 #pragma unroll
       for (int g = 0; g < G; g += 2) {
-        const v4u pf = {pack2<DT>(w[4 * g], w[4 * g + 1]), pack2<DT>(w[4 * g + 2], w[4 * g + 3]),
-                        pack2<DT>(w[4 * g + 4], w[4 * g + 5]), pack2<DT>(w[4 * g + 6], w[4 * g + 7])};
+        const v4u pf = {pack2<MT>(w[4 * g], w[4 * g + 1]), pack2<MT>(w[4 * g + 2], w[4 * g + 3]),
+                        pack2<MT>(w[4 * g + 4], w[4 * g + 5]), pack2<MT>(w[4 * g + 6], w[4 * g + 7])};
+        if constexpr (!CODES) {   // the sum of what the values are weighted with
+#pragma unroll
+          for (int x = 0; x < 4; ++x) l = add2<DT>(pf[x], l);
+        }
         uint32_t x[8][VL / 2];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int j = 0; j < VL / 2; j += 2) {
             if constexpr (CODES) {
-              const v2u c = codes4<DT>(vr[4 * g + i][j / 2]);
+              const v2u c = codes4(vr[4 * g + i][j / 2]);
               x[i][j] = c.x;
               x[i][j + 1] = c.y;
             } else {
@@ -420,7 +442,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_at
           v4u a;
 #pragma unroll
           for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(x[2 * i + 1][j / 2], x[2 * i][j / 2], pick);
-          o[j] = mfma16<DT>(a, pf, o[j]);
+          o[j] = mfma16<MT>(a, pf, o[j]);
         }
       }
       load_v(next);

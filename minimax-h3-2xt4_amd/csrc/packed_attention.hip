@@ -63,15 +63,6 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
 // at most 2^kSlack, far inside both types, and rescaling the sums is rare.
 constexpr float kSlack = 8.0f;
 
-// l plus the two DT values of a word.
-template <int DT>
-__device__ __forceinline__ float add2(uint32_t w, float l) {
-  if constexpr (DT == kF16)
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), l, false);
-  else
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, w), __builtin_bit_cast(v2b, 0x3f803f80u), l, false);
-}
-
 // Both halves' values of a pair of lanes l, l ^ 32.
 __device__ __forceinline__ std::pair<float, float> lane_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

@@ -31,6 +31,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
 }
 
+// l plus the two DT values of a word.
+template <int DT>
+__device__ __forceinline__ float add2(uint32_t w, float l) {
+  if constexpr (DT == kF16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), __builtin_bit_cast(v2h, 0x3c003c00u), l, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, w), __builtin_bit_cast(v2b, 0x3f803f80u), l, false);
+}
+
 // A cache as the kernels take it: strides in bytes (scales': in floats).
 struct CacheView {
   char* k;

@@ -5,7 +5,7 @@ the operands' type T (half a step, u = eps / 2 relative): p, relative to the
 running maximum, before its product with v, and the output. With
 A = sum p |v| / sum p:
   * p's rounding:            u (A + |o|) if the sum in the denominator takes
-                             the rounded p, as packed attention does
+                             the rounded p, as with 16-bit values
                              (sum of p d_j (v_j - o) / sum p with |d_j| <= u),
                              u A if it does not; in fp16 what lies below 2^-24 is lost, by
                              half of that at most: 2^-25 sum |v| / sum p,
@@ -17,8 +17,10 @@ A = sum p |v| / sum p:
     (n + n / 32 + 8) 2^-24 A, twice
   * the output:              u |o| (in fp16 2^-25 where it is subnormal)
 A cache of codes adds two fp32 products before p's rounding (in (n + 8)
-above) and p's fp16 loss counts relative to the largest scale of v:
-2^-25 sum max(s) |code|.
+above). Codes are multiplied as fp16 whatever T is, so that p's fp16 loss counts
+for both, relative to the largest scale of v: 2^-25 sum max(s) |code|; and q of
+bf16, scaled by a power of 2 to a largest from 1 to 2, loses 2^-25 of that at
+most in a small element: d has |c| D 2^-25 2 max|q| max|k| more.
 """
 import math
 
@@ -48,18 +50,22 @@ def attention64(q, k, v, scale, first=None, codes_scale=None):
     a = (p @ v.abs()) / total
     lost = torch.where(seen, 1.0, 0.0).double() @ (v.abs() if codes_scale is None else codes_scale)
     d = (q.shape[1] + 4) * 2.0 ** -24 * ((q.abs() @ k.abs().t()) * scale * seen).amax(1, keepdim=True) + 2.0 ** -22
-    return o, (a, lost, d, nk)
+    if codes_scale is not None:
+        d = d + scale * q.shape[1] * 2.0 ** -24 * q.abs().amax(1, keepdim=True) * k.abs().max()
+    return o, (a, lost, d, nk, codes_scale is not None)
 
 
 def bound(o, parts, dtype):
     """The largest difference that attention64's comment allows."""
     if not isinstance(parts, tuple):
         return torch.zeros_like(o)
-    a, lost, d, nk = parts
+    a, lost, d, nk, codes = parts
     u = _u(dtype)
     tol = 2 * u * o.abs() + a * (u + 2 * d + 2 * (nk + nk / 32 + 8) * 2.0 ** -24)
+    if dtype == torch.float16 or codes:
+        tol = tol + 2.0 ** -25 * lost
     if dtype == torch.float16:
-        tol = tol + 2.0 ** -25 * lost + 2.0 ** -25
+        tol = tol + 2.0 ** -25
     return tol * 1.01 + 1e-37   # (the bound's own products of small terms)
 
 
