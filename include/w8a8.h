@@ -907,7 +907,7 @@ int w8a8_packed_attention(const W8A8PackedAttentionArgs* args);
 
 /* Workspace bytes of w8a8_packed_attention for these sizes on the current device. */
 int64_t w8a8_packed_attention_workspace_size(int64_t rows, int64_t keys, int64_t sequences, int64_t heads,
-                                             int32_t dim);
+                                             int64_t kv_heads, int32_t dim);
 
 /* ABI version (W8A8_ABI_VERSION; 14 added w8a8_segment_labels, 15
  * w8a8_residual_norm, w8a8_axial_rope, w8a8_axial_freqs and w8a8_linear_w4, 16

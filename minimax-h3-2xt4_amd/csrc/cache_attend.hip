@@ -36,8 +36,9 @@ constexpr int kWaveKeys = 32;   // keys of a wave at a time: two groups
 constexpr int kBlockKeys = kAttendWaves * kWaveKeys;
 // dim rounded up to the channels that a kernel works on.
 constexpr int attend_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-// Workgroups of a CU, by the registers of 128 and of 256 channels.
-constexpr int attend_per_cu(int dp) { return 2; }
+// Workgroups of a CU: with one of eight waves, the ends of pairs leave it idle
+// (64 contexts of codes 115 -> 124 us), three have no more bytes under way.
+constexpr int kAttendPerCu = 2;
 // The reference of p may lie so much below the maximum (as a power of 2), and
 // the reference of the values' scales 2^kScaleSlack: p times the scale is then
 // at most 2^12, far inside fp16, and rescaling the sums is rare.
@@ -163,7 +164,7 @@ constexpr uint32_t kNowhere = 0x7fffff00u;   // an offset behind every descripto
 // DT: type of q and out; CODES: the cache holds I8; DP: dim rounded up to 64, 128
 // or 256; STREAM: the keys and values pass through the caches without staying.
 template <int DT, bool CODES, int DP, bool STREAM>
-__global__ __launch_bounds__(64 * kAttendWaves, attend_per_cu(DP)) void cache_attend_kernel(AttendParams p) {
+__global__ __launch_bounds__(64 * kAttendWaves, kAttendPerCu) void cache_attend_kernel(AttendParams p) {
   constexpr int ES = CODES ? 1 : 2, AUX = STREAM ? 2 : 0;
   // Codes are multiplied as fp16, whatever q's type: cheaper to make than bf16,
   // and P keeps eleven bits. q of bf16 is scaled by a power of 2 for it, so that a
@@ -586,17 +587,17 @@ __global__ __launch_bounds__(64 * kJoinWaves) void cache_attend_join_kernel(Atte
 }
 
 // Workgroups of a call: what the GPU holds, each with a range of the blocks of
-// all pairs; or one for each pair, if no pair can have more than kWholeBlocks
-// blocks (then nothing has to be joined).
-constexpr int64_t kWholeBlocks = 8;
+// all pairs; or one for each pair (then nothing has to be joined), if none can
+// have more than four blocks, or eight where the pairs are half as many as the
+// CUs: 256 pairs of up to six blocks 17.7 -> 12.9 us, 16 of seven 10.8 -> 13.0.
 struct AttendPlan {
   int64_t workgroups;
   bool whole;
 };
 static AttendPlan attend_plan(int64_t pairs, int64_t max_keys, int dim) {
-  const int64_t blocks = std::max<int64_t>((max_keys + kBlockKeys - 1) / kBlockKeys, 1);
-  if (blocks <= kWholeBlocks) return {pairs, true};
-  return {std::min<int64_t>(pairs * blocks, attend_per_cu(attend_dp(dim)) * current_device_cus()), false};
+  const int64_t blocks = std::max<int64_t>((max_keys + kBlockKeys - 1) / kBlockKeys, 1), cus = current_device_cus();
+  if (blocks <= 4 || (blocks <= 8 && 2 * pairs >= cus)) return {pairs, true};
+  return {std::min<int64_t>(pairs * blocks, kAttendPerCu * cus), false};
 }
 
 static int64_t attend_tiles(int64_t heads, int64_t kv_heads) {

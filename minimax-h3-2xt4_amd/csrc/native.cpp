@@ -847,7 +847,7 @@ PyObject* packed_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     row_head_strides(fresh, a.out_strides);
   }
   a.sequences = starts->size(0) - 1;
-  a.workspace_bytes = w8a8_packed_attention_workspace_size(a.rows, a.keys, a.sequences, heads, (int32_t)dim);
+  a.workspace_bytes = w8a8_packed_attention_workspace_size(a.rows, a.keys, a.sequences, heads, kv_heads, (int32_t)dim);
   if (a.workspace_bytes > 0) {
     workspace = at::empty({a.workspace_bytes}, opt.dtype(at::kByte));
     a.workspace = workspace.data_ptr();

@@ -4,8 +4,8 @@
 //   o_i = sum_j 2^(c s_ij - m_i) v_j / sum_j 2^(c s_ij - m_i),
 //   s_ij = q_i . k_j, c = log2(e) sm_scale, m_i the running maximum of c s_ij
 //
-// A workgroup takes 128 queries of one head, a wave 32 of them, and walks the
-// keys in blocks that all four waves read from LDS. Scores are computed
+// A workgroup takes 128 rows of a key head (a query with one of the group's query
+// heads each), a wave 32 of them, and walks the keys in blocks that all four waves read from LDS. Scores are computed
 // transposed, S^T = K Q^T on the 32 x 32 x 16 MFMA, so that a lane holds one
 // query (l % 32) and sixteen of 32 keys, 8 a + 4 (l / 32) + b (a, b < 4): the
 // softmax's maximum and sum are then a lane's own but for one exchange with
@@ -42,6 +42,7 @@ struct PackedParams {
   uint32_t k_row, v_row;
   int rows, keys, sequences;
   int group, kv_heads, dim;
+  uint64_t group_magic;   // floor((2^64 - 1) / group) + 1
   const int32_t* starts;
   const int32_t* k_starts;
   float c;
@@ -82,14 +83,16 @@ __device__ __forceinline__ int v_swizzle(int r) {
 
 __device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// The sequence and the tile of queries of tile t. Of up to 64 sequences those
+// The sequence and the tile of key head's tile t. A tile's rows are a sequence's
+// queries with the heads of the group, query by query: short sequences fill it,
+// and a causal one's tile spans few queries. Of up to 64 sequences those
 // with the most keys come first, and the tiles of a sequence from its last (of
 // causal ones the longest) to its first, so that what is left at the end is
 // short. (More sequences are taken 64 at a time.) Behind the sequences come the
 // tiles of the rows behind them, as a sequence of its own without keys.
 struct PackedTile {
   int b, first, n;     // first row of the tile in its sequence, the sequence's rows
-  int row0, key0, nk;  // the sequence's first row, first key and keys
+  int row0, key0, nk;  // the sequence's first query, first key and keys
 };
 
 __device__ __forceinline__ PackedTile packed_find(const PackedParams& p, int t) {
@@ -100,7 +103,7 @@ __device__ __forceinline__ PackedTile packed_find(const PackedParams& p, int t) 
     int lo = 0, n = 0, key0 = 0, nk = -1;
     if (b <= p.sequences) {
       lo = clamp_to(p.starts[b], 0, p.rows);
-      n = clamp_to(b < p.sequences ? p.starts[b + 1] : p.rows, lo, p.rows) - lo;
+      n = (clamp_to(b < p.sequences ? p.starts[b + 1] : p.rows, lo, p.rows) - lo) * p.group;
       if (b < p.sequences) {
         key0 = clamp_to(p.k_starts[b], 0, p.keys);
         nk = clamp_to(p.k_starts[b + 1], key0, p.keys) - key0;
@@ -129,6 +132,12 @@ __device__ __forceinline__ PackedTile packed_find(const PackedParams& p, int t) 
   return {-1, 0, 0, 0, 0, 0};
 }
 
+// r / group (r >= 0): the high half of r * (2^64 / group + e), 0 < e <= 1, where
+// r e < 2^32 leaves the quotient's floor.
+__device__ __forceinline__ int by_group(const PackedParams& p, int r) {
+  return p.group == 1 ? r : (int)__umul64hi((uint64_t)(uint32_t)r, p.group_magic);
+}
+
 // What a workgroup and its waves work on, DP channels wide, BK keys a block.
 // TID is the thread's index (a copy of it that the compiler takes for another
 // value keeps nothing alive from the one's use to the other's). Tiles are PITCH
@@ -147,7 +156,7 @@ struct Packed {
   char* tiles;
   int lane, wave, col, half;
   PackedTile tile;
-  int head, mine, nk, split;
+  int query, head, nk, split;   // of this lane's row
   bool stored;
   int blocks, limit, wave_clean, wave_blocks;
   const char* kbase;
@@ -168,20 +177,20 @@ struct Packed {
       split = item % p.splits;
       item /= p.splits;
     }
-    head = kvh * p.group + item % p.group;
-    tile = packed_find(p, item / p.group);
+    tile = packed_find(p, item);
     if (tile.b < 0) return;
-    const int q0 = tile.first + 32 * wave;      // the wave's first query of its sequence
-    mine = q0 + col;
-    stored = mine < tile.n;
+    const int r0 = tile.first + 32 * wave, row = min(r0 + col, tile.n - 1);   // the wave's first row, and this lane's
+    stored = r0 + col < tile.n;
+    query = by_group(p, row);
+    head = kvh * p.group + row - query * p.group;
     if (tile.b == p.sequences) return;
     nk = tile.nk;
-    const int shift = nk - tile.n;              // causal: query i sees keys up to i + shift
-    const int seen = CAUSAL ? clamp_to(tile.first + kPackQ + shift, 0, nk) : nk;   // keys that the workgroup sees,
-    limit = CAUSAL ? clamp_to(mine + shift + 1, 0, nk) : nk;                       // this query,
-    wave_clean = CAUSAL ? clamp_to(q0 + shift + 1, 0, nk) : nk;                    // all of the wave's,
-    const int some = q0 >= tile.n ? 0 : CAUSAL ? clamp_to(q0 + 32 + shift, 0, nk) : nk;   // some of them
-    wave_blocks = (some + BK - 1) / BK;
+    const int shift = nk - by_group(p, tile.n);    // causal: query i sees keys up to i + shift
+    auto sees = [&](int r) { return CAUSAL ? clamp_to(by_group(p, min(r, tile.n - 1)) + shift + 1, 0, nk) : nk; };
+    const int seen = sees(tile.first + kPackQ - 1);                 // keys that the workgroup sees,
+    limit = CAUSAL ? clamp_to(query + shift + 1, 0, nk) : nk;       // this query,
+    wave_clean = sees(r0);                                          // all of the wave's,
+    wave_blocks = ((r0 < tile.n ? sees(r0 + 31) : 0) + BK - 1) / BK;   // and some of them (in blocks)
     blocks = (seen + BK - 1) / BK;
     int64_t from = tile.key0;
     if constexpr (SPLIT) {   // the keys before this range's first are another's: count from there
@@ -207,11 +216,11 @@ struct Packed {
   }
 
   __device__ __forceinline__ char* to() const {
-    return p.out + (int64_t)(tile.row0 + min(mine, tile.n - 1)) * p.o_row + head * p.o_head;
+    return p.out + (int64_t)(tile.row0 + query) * p.o_row + head * p.o_head;
   }
 
   __device__ __forceinline__ void queries(v4u (&qf)[NS]) const {
-    const char* from = p.q + (int64_t)(tile.row0 + min(mine, tile.n - 1)) * p.q_row + head * p.q_head;
+    const char* from = p.q + (int64_t)(tile.row0 + query) * p.q_row + head * p.q_head;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const int d = 16 * s + 8 * half;
@@ -283,7 +292,7 @@ struct Packed {
     l = both.first + both.second;
     if constexpr (SPLIT) {
       if (!stored) return;
-      const int64_t at = ((int64_t)split * p.rows + tile.row0 + mine) * (p.group * p.kv_heads) + head;
+      const int64_t at = ((int64_t)split * p.rows + tile.row0 + query) * (p.group * p.kv_heads) + head;
 #pragma unroll
       for (int f = 0; f < DF; ++f)
 #pragma unroll
@@ -638,9 +647,9 @@ static int packed_pitch(int dim) { return (packed_dp(dim) + 31) / 32 * 32; }
 // sums' way through memory (3.6 MB a step): one row behind 8000 keys 130 -> 25
 // us, but 512 rows of a prompt 17 -> 29. (The halves of a workgroup of eight waves
 // sharing the keys and meeting in LDS: 353 rows 13.0 -> 14.7.)
-static int packed_splits(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int dim) {
-  if (rows <= 0 || keys <= 0 || sequences <= 0 || heads <= 0 || dim <= 0) return 1;
-  const int64_t filled = std::min(rows, sequences), tiles = (rows + (kPackQ - 1) * filled) / kPackQ * heads;
+static int packed_splits(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads, int dim) {
+  if (rows <= 0 || keys <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 1;
+  const int64_t filled = std::min(rows, sequences), tiles = (rows * (heads / kv_heads) + (kPackQ - 1) * filled) / kPackQ * kv_heads;
   const int64_t slots = (dim > 128 ? 1 : 2) * current_device_cus(), block = dim > 128 ? 32 : 64;
   const int64_t steps = (keys / sequences + block - 1) / block, splits = std::min(slots / tiles, steps / 4);
   return splits >= 2 && steps - steps / splits >= 8 + rows * heads * splits * packed_pitch(dim) * 8 / 3600000 ? (int)splits : 1;
@@ -678,9 +687,9 @@ static int launch_packed_dim(const PackedParams& p, bool causal, int64_t grid, h
 }  // namespace w8a8
 
 extern "C" int64_t w8a8_packed_attention_workspace_size(int64_t rows, int64_t keys, int64_t sequences, int64_t heads,
-                                                        int32_t dim) {
+                                                        int64_t kv_heads, int32_t dim) {
   using namespace w8a8;
-  const int splits = packed_splits(rows, keys, sequences, heads, dim);
+  const int splits = packed_splits(rows, keys, sequences, heads, kv_heads, dim);
   return splits == 1 ? 0 : splits * rows * heads * (packed_pitch(dim) + 2) * (int64_t)sizeof(float);
 }
 
@@ -717,18 +726,19 @@ extern "C" int w8a8_packed_attention(const W8A8PackedAttentionArgs* a) {
                     (!spans_overlap(a->k, rows_span(a->keys, a->kv_heads, a->dim, a->k_strides), a->out, osize) &&
                      !spans_overlap(a->v, rows_span(a->keys, a->kv_heads, a->dim, a->v_strides), a->out, osize))),
                "%s: out overlaps an input", who);
-  const int splits = packed_splits(a->rows, a->keys, a->sequences, a->heads, a->dim);
-  const int64_t need = w8a8_packed_attention_workspace_size(a->rows, a->keys, a->sequences, a->heads, a->dim);
+  const int splits = packed_splits(a->rows, a->keys, a->sequences, a->heads, a->kv_heads, a->dim);
+  const int64_t need = w8a8_packed_attention_workspace_size(a->rows, a->keys, a->sequences, a->heads, a->kv_heads, a->dim);
   W8A8_REQUIRE(need == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= need),
                "%s: workspace of %lld bytes needed", who, (long long)need);
-  const int64_t grid = (a->rows / kPackQ + a->sequences + 1) * a->heads;
-  W8A8_REQUIRE(grid * splits < (1 << 24), "%s: too many rows, sequences and heads for one launch", who);   // (2^32 work-items)
+  const int64_t packed = a->rows * (a->heads / a->kv_heads), grid = (packed / kPackQ + a->sequences + 1) * a->kv_heads;
+  W8A8_REQUIRE(packed < (1ll << 31) - kPackQ && grid * splits < (1 << 24), "%s: too many rows, sequences and heads for one launch", who);   // (2^32 work-items)
   const PackedParams p{reinterpret_cast<const char*>(a->q), reinterpret_cast<const char*>(a->k),
                        reinterpret_cast<const char*>(a->v), reinterpret_cast<char*>(a->out),
                        2 * a->q_strides[0], 2 * a->q_strides[1], 2 * a->k_strides[1], 2 * a->v_strides[1],
                        2 * a->out_strides[0], 2 * a->out_strides[1],
                        (uint32_t)(2 * a->k_strides[0]), (uint32_t)(2 * a->v_strides[0]),
                        (int)a->rows, (int)a->keys, (int)a->sequences, a->heads / a->kv_heads, a->kv_heads, a->dim,
+                       ~0ull / (uint64_t)(a->heads / a->kv_heads) + 1,
                        a->starts, a->k_starts, a->sm_scale * kLog2eF, a->fill, splits,
                        reinterpret_cast<float*>(a->workspace),
                        reinterpret_cast<float*>(a->workspace) + splits * a->rows * a->heads * packed_pitch(a->dim)};

@@ -221,7 +221,7 @@ def load(path=None):
     lib.w8a8_cache_attend_workspace_size.restype = _c.c_int64
     lib.w8a8_cache_attend_workspace_size.argtypes = [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int32, _c.c_int64]
     lib.w8a8_packed_attention_workspace_size.restype = _c.c_int64
-    lib.w8a8_packed_attention_workspace_size.argtypes = [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int32]
+    lib.w8a8_packed_attention_workspace_size.argtypes = [_c.c_int64] * 5 + [_c.c_int32]
     for name, st in zip(STRUCT_ENTRY_POINTS + BLOCK_ENTRY_POINTS + CACHE_ENTRY_POINTS + ('w8a8_gemm_noalloc',),
                         STRUCTS + BLOCK_STRUCTS + CACHE_STRUCTS + (GemmArgs,)):
         fn = getattr(lib, name)

@@ -1095,7 +1095,7 @@ def packed_attention(q, k, v, starts, k_starts=None, *, causal=True, scale=None,
         return y
     (q, qst), (k, kst), (v, vst) = _rows16(q, 'q'), _rows16(k, 'k'), _rows16(v, 'v')
     with torch.cuda.device(q.device):
-        nbytes = int(_abi.load().w8a8_packed_attention_workspace_size(rows, keys, sequences, heads, dim))
+        nbytes = int(_abi.load().w8a8_packed_attention_workspace_size(rows, keys, sequences, heads, kv_heads, dim))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     args = _abi.PackedAttentionArgs(
         dtype=_abi.DTYPE_CODE[q.dtype], q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=y.data_ptr(),

@@ -59,6 +59,8 @@ ATTEND = dict(dtype=_abi.F16, q=5 << 30, out=6 << 30, q_strides=(512, 64), out_s
               page_table=7 << 30, ld_table=4, table_width=4, lengths=8 << 30, sm_scale=0.1, workspace=9 << 30,
               workspace_bytes=1 << 30)
 
+LONG = dict(ld_table=1000, table_width=1000)   # keys that several workgroups share
+
 
 def _args(which, change=None, cache=None, codes=False):
     struct, base = {'write': (_abi.CacheWriteArgs, WRITE), 'read': (_abi.CacheReadArgs, READ),
@@ -107,8 +109,8 @@ def test_write_and_read_refusals():
     (dict(out_strides=(512, 0)), 'overlap'), (dict(out_strides=(448, 64)), 'overlap'), (dict(out=5 << 30), 'overlaps q'),
     (dict(heads=0), 'heads'), (dict(heads=7), 'heads'), (dict(heads=65538), 'heads'), (dict(lengths=None), 'lengths'),
     (dict(sm_scale=0.0), 'sm_scale'), (dict(sm_scale=-1.0), 'sm_scale'), (dict(sm_scale=float('inf')), 'sm_scale'),
-    (dict(sm_scale=float('nan')), 'sm_scale'), (dict(workspace=None), 'workspace'), (dict(workspace_bytes=64), 'workspace'),
-    (dict(workspace=(9 << 30) + 4), 'workspace'),
+    (dict(sm_scale=float('nan')), 'sm_scale'), (dict(workspace=None, **LONG), 'workspace'), (dict(workspace_bytes=64, **LONG), 'workspace'),
+    (dict(workspace=(9 << 30) + 4, **LONG), 'workspace'),
 ])
 def test_attend_refusals(change, fragment):
     _refused('w8a8_cache_attend', _args('attend', change), fragment)

@@ -54,7 +54,7 @@ def test_lengths(gpu, new, keys, causal):
                                       ([0, 7, 33], [900, 2500, 2600])])
 def test_few_rows_behind_many_keys(gpu, new, keys, dtype, dim, causal):
     """Workgroups share a tile's keys and join their sums."""
-    shared = _abi.load().w8a8_packed_attention_workspace_size(sum(new), sum(keys), len(new), 4, dim) > 0
+    shared = _abi.load().w8a8_packed_attention_workspace_size(sum(new), sum(keys), len(new), 4, 2, dim) > 0
     assert shared or len(new) > 1
     run(dtype, 4, 2, dim, new, keys, causal, seed=dim)
 
