@@ -758,7 +758,7 @@ typedef struct W8A8KvCache {
  * starts: int32 [sequences + 1], ascending from 0: sequence b's new rows are
  *   [starts[b], starts[b + 1]), its last keys in order; NULL: one row each.
  * Rows from starts[sequences] on, and keys outside of the table, are not
- *   written. If two rows name the same key (a page that two places of the
+ *   written. k and v may not overlap the cache. If two rows name the same key (a page that two places of the
  *   table share), either may remain, or parts of both.
  */
 typedef struct W8A8CacheWriteArgs {
@@ -789,6 +789,8 @@ int w8a8_cache_write(const W8A8CacheWriteArgs* args);
  *   starts[b + 1]) take the keys 0, 1, ... of sequence b (zeros from keys
  *   outside of its table).
  * fill: rows from starts[sequences] on are left as they are (0) or set to 0.
+ * k and v may overlap neither each other nor the cache, but for columns of one
+ *   buffer's rows.
  */
 typedef struct W8A8CacheReadArgs {
   uint32_t struct_size;
@@ -819,14 +821,15 @@ int w8a8_cache_read(const W8A8CacheReadArgs* args);
  * q, out: [sequences, heads, cache.dim] of dtype (F16 or BF16; a 16-bit
  *   cache's own), element strides {row, head}, channels contiguous, rows and
  *   heads on 16-byte boundaries.
- * Scores, statistics and sums are fp32; p is rounded to dtype (relative to the
- *   running maximum, with codes times the value's scale relative to the running
- *   largest scale) for the product with v. The same call gives the same bits
- *   every time.
+ * Scores, statistics and sums are fp32; p is rounded for the product with v,
+ *   relative to 2^r with r at most 8 below the running maximum of its exponent: to
+ *   dtype, or with codes, times the value's scale relative to one of the largest
+ *   scales, to F16. The same call gives the same bits every time.
  * workspace: device buffer of at least w8a8_cache_attend_workspace_size()
  *   bytes (16-byte aligned, any contents; NULL where that is 0): partial sums
  *   of sequences that several workgroups share. Calls that share one must not
  *   overlap; calls in sequence may, and a captured graph may replay it.
+ * out may overlap neither q nor the cache, but for columns of one buffer's rows.
  * Requirements: heads a multiple of cache.heads, up to 65536 each; sequences
  *   below 2^20; table_width * page_size below 2^27; sm_scale positive, finite.
  */
@@ -870,11 +873,18 @@ int64_t w8a8_cache_attend_workspace_size(int64_t sequences, int64_t heads, int64
  * starts, k_starts: int32 [sequences + 1], ascending from 0.
  * fill: out's rows from starts[sequences] on are left as they are (0) or set
  *   to 0.
- * Scores, statistics and sums are fp32; p is rounded to dtype relative to the
- *   running maximum. The same call gives the same bits every time.
+ * Scores, statistics and sums are fp32; p is rounded to dtype, relative to 2^r
+ *   with r at most 8 below the running maximum of its exponent. The same call
+ *   gives the same bits every time.
+ * out may not overlap an input, but for columns of one buffer's rows.
+ * workspace: device buffer of at least w8a8_packed_attention_workspace_size()
+ *   bytes (16-byte aligned, any contents; NULL where that is 0): partial sums of
+ *   calls of few rows and many keys. Calls that share one must not overlap;
+ *   calls in sequence may, and a captured graph may replay it.
  * Requirements: heads a multiple of kv_heads, up to 65536; dim a multiple of
- *   8, 8 to 256; rows and keys below 2^27, row strides of k and v below 2^23
- *   elements; sequences below 2^20; sm_scale positive, finite.
+ *   8, 8 to 256; rows and keys below 2^27, rows * (heads / kv_heads) below 2^31;
+ *   row strides of k and v from dim to 2^23 elements; sequences below 2^20;
+ *   sm_scale positive, finite.
  */
 typedef struct W8A8PackedAttentionArgs {
   uint32_t struct_size;

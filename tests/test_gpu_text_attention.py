@@ -192,3 +192,31 @@ def test_host_routes_give_the_same_bits(gpu):
             assert native.cache_attend(*args, x, table, n, scale, out) is out and torch.equal(out, want)
             want = kernels.packed_attention(q, k, v, starts, causal=False, scale=scale)
             assert torch.equal(native.packed_attention(q, k, v, starts, starts, False, scale, None), want)
+
+
+def test_outputs_between_the_inputs(gpu):
+    """Outputs may be columns of the buffer whose other columns are read or written."""
+    total = [33, 70]
+    st, starts = starts_of(total, 'cuda')
+    table, pages = table_of(total, 16, torch.Generator().manual_seed(8), 'cuda')
+    n = torch.tensor(total, dtype=torch.int32, device='cuda')
+    rows = torch.cat([projections(st[-1], torch.bfloat16, 5), torch.zeros((st[-1], HEADS, DIM)).bfloat16().cuda()], 1)
+    q, k, v = rows[:, :HEADS], rows[:, HEADS:HEADS + KV], rows[:, HEADS + KV:HEADS + 2 * KV]
+    out = rows[:, HEADS + 2 * KV:]
+    want = packed_attention(q.clone(), k.clone(), v.clone(), starts)
+    packed_attention(q, k, v, starts, out=out)
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match='overlaps an input'):
+        packed_attention(q, k, v, starts, out=rows[:, 1:HEADS + 1])
+    cache = KVCache.allocate(pages, 16, KV, DIM, dtype=torch.int8)
+    kv_cache.write(cache, k, v, table, n, starts)
+    both = torch.zeros((st[-1], 2 * KV, DIM), dtype=torch.bfloat16, device='cuda')
+    kv_cache.read(cache, table, starts, st[-1], out=(both[:, :KV], both[:, KV:]))
+    for got, x in zip((both[:, :KV], both[:, KV:]), kv_cache.read(cache, table, starts, st[-1], dtype=torch.bfloat16)):
+        assert torch.equal(got, x)
+    with pytest.raises(RuntimeError, match='overlap'):
+        kv_cache.read(cache, table, starts, st[-1], out=(both[:, :KV], both[:, KV - 1:2 * KV - 1]))
+    buf = torch.zeros((2, 2 * HEADS, DIM), dtype=torch.bfloat16, device='cuda')
+    buf[:, :HEADS] = q[:2]
+    kv_cache.attend(buf[:, :HEADS], cache, table, n, out=buf[:, HEADS:])
+    assert torch.equal(buf[:, HEADS:], kv_cache.attend(q[:2], cache, table, n))
