@@ -758,8 +758,11 @@ typedef struct W8A8KvCache {
  * starts: int32 [sequences + 1], ascending from 0: sequence b's new rows are
  *   [starts[b], starts[b + 1]), its last keys in order; NULL: one row each.
  * Rows from starts[sequences] on, and keys outside of the table, are not
- *   written. k and v may not overlap the cache. If two rows name the same key (a page that two places of the
- *   table share), either may remain, or parts of both.
+ *   written. If two rows name the same key (a page that two places of the table
+ *   share), either may remain, or parts of both.
+ * k and v may not overlap the cache, nor places of the cache each other: its
+ *   strides nest (each is at least what the smaller ones reach), and k and v, and
+ *   their scales, lie apart or are columns of one buffer.
  */
 typedef struct W8A8CacheWriteArgs {
   uint32_t struct_size;
@@ -831,7 +834,7 @@ int w8a8_cache_read(const W8A8CacheReadArgs* args);
  *   overlap; calls in sequence may, and a captured graph may replay it.
  * out may overlap neither q nor the cache, but for columns of one buffer's rows.
  * Requirements: heads a multiple of cache.heads, up to 65536 each; sequences
- *   below 2^20; table_width * page_size below 2^27; sm_scale positive, finite.
+ *   below 2^20; table_width * page_size below 2^27; sm_scale positive, finite (times log2(e) too).
  */
 typedef struct W8A8CacheAttendArgs {
   uint32_t struct_size;
@@ -928,7 +931,8 @@ int w8a8_abi_version(void);
 /* sizeof of each argument struct, by index: 0 Quant, 1 Swiglu, 2 Gemm,
  * 3 Dequant, 4 Norm, 5 RmsRope, 6 AttnPrepare, 7 Attention, 8 ResidualNorm,
  * 9 AxialRope, 10 AxialFreqs, 11 LinearW4, 12 CacheWrite, 13 CacheRead,
- * 14 CacheAttend, 15 PackedAttention; -1 for an unknown index. Lets bindings verify their layout. */
+ * 14 CacheAttend, 15 PackedAttention; -1 for an unknown index. Lets bindings
+ * verify their layout. */
 int64_t w8a8_struct_size(int32_t which);
 
 /* Message describing the last error returned on the calling thread. */

@@ -672,7 +672,7 @@ extern "C" int w8a8_cache_attend(const W8A8CacheAttendArgs* a) {
   W8A8_REQUIRE(a->table_width >= 0 && a->table_width * a->cache.page_size < (1ll << 27) &&
                    (a->table_width == 0 || a->page_table) && (a->sequences == 1 || a->ld_table >= a->table_width) && a->lengths,
                "%s: page table or lengths null, table rows overlap, or 2^27 keys and more", who);
-  W8A8_REQUIRE(a->sm_scale > 0.0f && std::isfinite(a->sm_scale), "%s: sm_scale must be positive and finite", who);
+  W8A8_REQUIRE(a->sm_scale > 0.0f && std::isfinite(a->sm_scale * kLog2eF), "%s: sm_scale must be positive and finite", who);
   const int64_t keys = a->table_width * a->cache.page_size;
   const int64_t need = w8a8_cache_attend_workspace_size(a->sequences, a->heads, a->cache.heads, a->cache.dim, keys);
   W8A8_REQUIRE(need == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= need),

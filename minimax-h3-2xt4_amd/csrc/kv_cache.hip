@@ -219,16 +219,14 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheMoveParams p) {
   }
 }
 
+static int head_lanes(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+
 template <bool WRITE, int DT, bool CODES>
 static int launch_move(const char* who, const CacheMoveParams& in, hipStream_t stream) {
   CacheMoveParams p = in;
-  const int lph = p.cache.dim <= 64 ? 8 : p.cache.dim <= 128 ? 16 : 32;
-  const int per = kMoveHeads * 64 / lph;
-  p.runs = (p.cache.heads + per - 1) / per;
+  const int lph = head_lanes(p.cache.dim);
   p.stream = p.rows * p.cache.heads * p.cache.dim * 4 > (64ll << 20);   // (k and v; 69277 rows of codes read: 80 -> 68 us)
-  const int64_t grid = (p.rows * p.runs + 3) / 4;
-  W8A8_REQUIRE(grid < (1ll << 24), "%s: too many rows and heads for one launch", who);   // (2^32 work-items)
-  const dim3 g((unsigned)grid), t(256);
+  const dim3 g((unsigned)((p.rows * p.runs + 3) / 4)), t(256);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, t, 0, stream, p); };
   if constexpr (WRITE) {
     lph == 8 ? go(cache_write_kernel<DT, CODES, 8>)
@@ -267,6 +265,9 @@ static int move_params(const char* who, int dtype, const W8A8KvCache& c, const v
   p.v = reinterpret_cast<char*>(const_cast<void*>(v));
   p.k_row = 2 * kst[0]; p.k_head = 2 * kst[1]; p.v_row = 2 * vst[0]; p.v_head = 2 * vst[1];
   p.rows = rows;
+  const int per = kMoveHeads * 64 / head_lanes(c.dim);
+  p.runs = (c.heads + per - 1) / per;
+  W8A8_REQUIRE((rows * p.runs + 3) / 4 < (1ll << 24), "%s: too many rows and heads for one launch", who);   // (2^32 work-items)
   p.sequences = (int)sequences;
   p.width = (int)width;
   p.table = table;
@@ -291,6 +292,7 @@ extern "C" int w8a8_cache_write(const W8A8CacheWriteArgs* a) {
                         a->page_table, a->ld_table, a->table_width, p));
   W8A8_REQUIRE(a->sequences == 0 || a->lengths, "%s: null lengths", who);
   W8A8_REQUIRE(a->starts || a->rows == a->sequences, "%s: without starts every sequence has one row", who);
+  W8A8_REQUIRE(places_apart(a->cache), "%s: keys or values of the cache share memory", who);
   if (a->sequences == 0) return W8A8_OK;
   p.lengths = a->lengths;
   p.starts = a->starts;

@@ -6,6 +6,7 @@
 #include "w8a8_host.h"
 
 #include <cmath>
+#include <utility>
 
 namespace w8a8 {
 
@@ -60,28 +61,36 @@ __device__ __forceinline__ void group_place(const CacheView& c, uint32_t g, int&
   token = ((int)g - entry * (c.page_size / kGroupTokens)) * kGroupTokens;
 }
 
+// The last of the lanes with x (0 if there is none).
+__device__ __forceinline__ int last_lane(bool x) {
+  const uint64_t m = __builtin_amdgcn_ballot_w64(x);
+  return m ? 63 - __builtin_clzll(m) : 0;
+}
+
 // The sequence b in [0, n) with starts[b] <= row < starts[b + 1], or n, with its
 // two starts and its length, if lengths are given (a wave works together; the
-// row is the wave's). The lanes look at 64 sequences at once.
+// row is the wave's). The lanes look at 64 sequences at once, where there are more
+// first at the starts of 64 ranges of them (16384 rows of 4096 sequences written
+// as codes 42.7 -> 25.7 us, against all in turn; 20000 of one row 162 -> 34).
 struct SequenceRow {
   int b, first, last, length;
 };
 __device__ __forceinline__ SequenceRow sequence_of(const int32_t* starts, int n, int64_t row, const int32_t* lengths) {
   const int lane = threadIdx.x & 63;
-  SequenceRow r{n, 0, 0, 0};
-  for (int b0 = 0; b0 < n; b0 += 64) {
-    const int i = min(b0 + lane, n - 1);
-    const int first = starts[i], last = starts[i + 1], length = lengths ? lengths[i] : 0;
-    const uint64_t in = __builtin_amdgcn_ballot_w64(b0 + lane < n && first <= row && row < last);
-    if (in == 0) continue;
-    const int at = __builtin_ctzll(in);
-    r.b = b0 + at;
-    r.first = __builtin_amdgcn_readlane(first, at);
-    r.last = __builtin_amdgcn_readlane(last, at);
-    r.length = __builtin_amdgcn_readlane(length, at);
-    break;
+  int b = 0, size = n;
+  while (size > 64) {
+    const int step = (size + 63) / 64, at = lane * step;
+    const int skip = last_lane(at < size && starts[b + min(at, size - 1)] <= row) * step;
+    b += skip;
+    size = min(step, size - skip);
   }
-  return r;
+  const int i = min(b + lane, n - 1);
+  const int first = starts[i], last = starts[i + 1], length = lengths ? lengths[i] : 0;
+  const uint64_t in = __builtin_amdgcn_ballot_w64(lane < size && first <= row && row < last);
+  if (in == 0) return {n, 0, 0, 0};
+  const int at = __builtin_ctzll(in);
+  return {b + at, __builtin_amdgcn_readlane(first, at), __builtin_amdgcn_readlane(last, at),
+          __builtin_amdgcn_readlane(length, at)};
 }
 
 inline bool stride8(int64_t s) { return s >= 0 && s % 8 == 0; }
@@ -135,6 +144,50 @@ inline RowsOf cache_memory(const W8A8KvCache& c, const void* p) {
   const int es = c.dtype == W8A8_I8 ? 1 : 2;
   const int64_t page = (c.heads - 1) * c.strides[1] + (c.page_size - 1) * c.strides[2] + c.dim;
   return rows_of(p, c.strides[0], c.pages, page, es);
+}
+
+// Runs of `extent` bytes, one at each place of a nest of steps.
+struct Places {
+  int64_t step[3], count[3], extent;   // the larger steps first
+};
+// Sorted by their steps; false where steps are less than what they step over.
+inline bool places_nest(Places& p) {
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 3; ++j)
+      if (p.count[i] <= 1 || (p.count[j] > 1 && p.step[j] > p.step[i])) {
+        std::swap(p.step[i], p.step[j]);
+        std::swap(p.count[i], p.count[j]);
+      }
+  int64_t span = p.extent;
+  for (int i = 2; i >= 0; --i) {
+    if (p.count[i] <= 1) continue;
+    if (p.step[i] < span) return false;
+    span += (p.count[i] - 1) * p.step[i];
+  }
+  return true;
+}
+// Whether two such nests, `off` bytes apart, share a byte. Places differ by sums
+// c_i step_i, |c_i| < count_i, and what the inner steps reach is less than a step,
+// so that c_i is one of two.
+inline bool places_meet(const Places& p, int64_t off, int i = 0) {
+  if (i == 3) return -p.extent < off && off < p.extent;
+  if (p.count[i] <= 1) return places_meet(p, off, i + 1);
+  const int64_t c = off / p.step[i] - (off % p.step[i] < 0);
+  for (int64_t at : {c, c + 1})
+    if (-p.count[i] < at && at < p.count[i] && places_meet(p, off - at * p.step[i], i + 1)) return true;
+  return false;
+}
+// Whether every key, value and scale of a cache has memory of its own.
+inline bool places_apart(const W8A8KvCache& c) {
+  const int es = c.dtype == W8A8_I8 ? 1 : 2;
+  auto own = [](Places p, const void* a, const void* b) {
+    return places_nest(p) && !places_meet(p, (int64_t)((uintptr_t)b - (uintptr_t)a));
+  };
+  return own({{c.strides[0] * es, c.strides[1] * es, c.strides[2] * es}, {c.pages, c.heads, c.page_size}, (int64_t)c.dim * es},
+             c.k, c.v) &&
+         (c.dtype != W8A8_I8 ||
+          own({{c.scale_strides[0] * 4, c.scale_strides[1] * 4, 0}, {c.pages, c.heads, 1}, 4ll * c.page_size}, c.k_scale,
+              c.v_scale));
 }
 
 }  // namespace w8a8

@@ -25,7 +25,7 @@ class KVCache:
     with k_scale and v_scale fp32 [pages, heads, page_size]. k and v may be views
     of larger buffers, both with the same strides (channels contiguous, the
     others multiples of 8 elements); so may the scales (tokens contiguous, the
-    others multiples of 4)."""
+    others multiples of 4). To be written to, no two places may share memory."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor = None

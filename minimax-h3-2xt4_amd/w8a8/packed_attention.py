@@ -1,9 +1,10 @@
 """Attention of packed sequences of different lengths, causal or not.
 
-The attention of the text encoder's block, whose projections
-tp_qwen3vl mirrors (patches/tp_qwen3vl.py:259 takes its output), and of image
-encoders; the INT8 attention (int8_attention) takes equal lengths without a mask. This one takes the prompts of several requests, or the images
-of an encoder, as they lie one behind the other, in fp16 or bf16.
+The attention of the text encoder's block, whose projections tp_qwen3vl mirrors
+(patches/tp_qwen3vl.py:259 takes its output), and of image encoders. The INT8
+attention (int8_attention) takes equal lengths without a mask; this one the
+prompts of several requests, or the images of an encoder, as they lie one behind
+the other, in fp16 or bf16.
 """
 from . import _abi, kernels
 

@@ -109,6 +109,42 @@ def test_write_and_read_refusals():
         assert _status(f'w8a8_cache_{which}', _args(which, dict(rows=0)))[0] == _abi.OK
 
 
+@pytest.mark.parametrize('change,codes,ok', [
+    ({}, False, True),
+    (dict(v=1 << 30), False, False),                                                    # k's own memory
+    (dict(v=(1 << 30) + 128, strides=(4096, 2048, 128)), False, True),                  # columns of a token's row
+    (dict(v=(1 << 30) + 112, strides=(4096, 2048, 128)), False, False),
+    (dict(v=(1 << 30) + 2048, strides=(4096, 2048, 64)), False, True),                  # behind k's tokens of a head
+    (dict(v=(1 << 30) + 2032, strides=(4096, 2048, 64)), False, False),
+    (dict(v=(1 << 30) + 4096, strides=(4096, 1024, 64)), False, True),                  # behind k's heads of a page
+    (dict(v=(1 << 30) + 4096, strides=(2048, 1024, 64)), False, False),
+    (dict(v=(1 << 30) + 9 * 4096, strides=(2048, 1024, 64)), False, False),             # k's last page
+    (dict(v=(1 << 30) + 10 * 4096, strides=(2048, 1024, 64)), False, True),
+    (dict(v=(1 << 30) - 10 * 4096, strides=(2048, 1024, 64)), False, True),
+    (dict(v=(1 << 30) - 10 * 4096 + 16, strides=(2048, 1024, 64)), False, False),
+    (dict(strides=(2048, 64, 128)), False, True),                                       # tokens before heads
+    (dict(strides=(1024, 10240, 64)), False, True),                                     # heads before pages
+    (dict(strides=(0, 1024, 64)), False, False),                                        # one page, many times
+    (dict(strides=(2048, 0, 64)), False, False),
+    (dict(strides=(1024, 1024, 64)), False, False),
+    (dict(strides=(2048, 1016, 64)), False, False),
+    (dict(strides=(0, 1024, 64), pages=1), False, True),                                # (steps that are not taken)
+    (dict(strides=(1024, 0, 64), heads=1, dim=64), False, True),
+    ({}, True, True),
+    (dict(v_scale=3 << 30), True, False),
+    (dict(v_scale=(3 << 30) + 64, scale_strides=(64, 32)), True, True),
+    (dict(v_scale=(3 << 30) + 48, scale_strides=(64, 32)), True, False),
+    (dict(scale_strides=(16, 16)), True, False),
+])
+def test_places_that_share_memory_are_not_written(change, codes, ok):
+    """(Of no sequences, so that what is not refused launches nothing.)"""
+    args = _args('write', dict(sequences=0), change, codes)
+    if 'heads' in change:
+        args.k_strides = args.v_strides = (64, 64)
+    rc, message = _status('w8a8_cache_write', args)
+    assert rc == (_abi.OK if ok else _abi.ERR_INVALID) and (ok or 'share memory' in message), message
+
+
 @pytest.mark.parametrize('change,fragment', [
     (dict(q=None), 'q null'), (dict(out=(6 << 30) + 8), 'out null or misaligned'), (dict(q_strides=(516, 64)), 'q strides'),
     (dict(out_strides=(512, 0)), 'overlap'), (dict(out_strides=(448, 64)), 'overlap'), (dict(out=5 << 30), 'overlaps q'),

@@ -90,6 +90,33 @@ def test_one_row_a_sequence(gpu, held):
     same(cache, want)
 
 
+@pytest.mark.parametrize('sequences', [63, 64, 65, 130, 5000])
+def test_many_sequences(gpu, sequences):
+    """Empty ones among them, and rows behind the last."""
+    g = torch.Generator().manual_seed(sequences)
+    new = torch.randint(0, 6, (sequences,), generator=g)
+    new[0] = new[sequences // 2] = new[-1] = 0
+    before = torch.randint(0, 20, (sequences,), generator=g)
+    total = new + before
+    table, pages = table_of(total.tolist(), 16, g, 'cuda')
+    cache, want = twin(pages, 16, 2, 64, torch.float16)
+    st, starts = starts_of(new.tolist(), 'cuda')
+    k, v = kv_rows(torch.float16, st[-1] + 70, 2, 64, seed=sequences)
+    kv_cache.write(cache, k, v, table, total.int().cuda(), starts)
+    b = torch.repeat_interleave(torch.arange(sequences), new)
+    key = (before[b] + torch.arange(st[-1]) - torch.tensor(st)[b]).cuda()
+    page = table[b.cuda(), key // 16].long()
+    want.k[page, :, key % 16], want.v[page, :, key % 16] = k[:st[-1]], v[:st[-1]]
+    same(cache, want)
+    ks, k_starts = starts_of(total.tolist(), 'cuda')
+    rk, rv = kv_cache.read(cache, table, k_starts, ks[-1] + 70)
+    b = torch.repeat_interleave(torch.arange(sequences), total)
+    key = (torch.arange(ks[-1]) - torch.tensor(ks)[b]).cuda()
+    page = table[b.cuda(), key // 16].long()
+    assert torch.equal(rk[:ks[-1]], cache.k[page, :, key % 16]) and torch.equal(rv[:ks[-1]], cache.v[page, :, key % 16])
+    assert not bool(rk[ks[-1]:].any()) and not bool(rv[ks[-1]:].any())
+
+
 def test_places_that_are_not_there(gpu):
     """Keys outside of the table, absent pages and pages outside of the cache are not written."""
     cache, want = twin(4, 16, 2, 64, torch.float16)

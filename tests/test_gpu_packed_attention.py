@@ -102,6 +102,26 @@ def test_more_sequences_than_lanes(gpu):
     run(torch.float16, 1, 1, 64, new, [n + 3 * (i % 40) for i, n in enumerate(new)], True)
 
 
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('sequences', [7, 8, 9, 63, 64, 65, 700, 4200])
+def test_many_sequences(gpu, sequences, causal):
+    """Empty ones among them, and rows behind the last."""
+    g = torch.Generator().manual_seed(sequences)
+    new = (torch.randint(0, 90, (sequences,), generator=g) if sequences < 100 else
+           torch.randint(0, 7, (sequences,), generator=g)).tolist()
+    new[1] = new[sequences // 2] = new[-1] = 0
+    keys = [n + i % 3 for i, n in enumerate(new)]
+    st, starts = starts_of(new, 'cuda')
+    ks, k_starts = starts_of(keys, 'cuda')
+    q, k, v = make(torch.bfloat16, st[-1] + 200, ks[-1], 3, 1, 16, seed=sequences)
+    out = torch.full_like(q, 5.0)
+    packed_attention(q, k, v, starts, k_starts, causal=causal, out=out)
+    check_packed(out, q, k, v, st, ks, causal, 0.25)
+    assert bool((out[st[-1]:] == 5.0).all())
+    fresh = packed_attention(q, k, v, starts, k_starts, causal=causal)
+    assert torch.equal(fresh[:st[-1]], out[:st[-1]]) and not bool(fresh[st[-1]:].any())
+
+
 @pytest.mark.parametrize('heads,kv', [(1, 1), (6, 2), (8, 1), (20, 1), (7, 7), (64, 8)])
 def test_grouped_heads(gpu, heads, kv):
     run(torch.float16, heads, kv, 128, [40, 100], [40, 120], True)
