@@ -220,3 +220,42 @@ def test_outputs_between_the_inputs(gpu):
     buf[:, :HEADS] = q[:2]
     kv_cache.attend(buf[:, :HEADS], cache, table, n, out=buf[:, HEADS:])
     assert torch.equal(buf[:, HEADS:], kv_cache.attend(q[:2], cache, table, n))
+
+
+@pytest.mark.parametrize('held,dtype', [(torch.float16, torch.float16), (torch.int8, torch.bfloat16)])
+def test_calls_at_once(gpu, held, dtype):
+    """Two streams whose calls share keys between workgroups, each with workspaces of its own: the bits of
+    calls one after the other."""
+    def setup(seed, total):
+        rows = projections(sum(total), dtype, seed)
+        st, starts = starts_of(total, 'cuda')
+        table, pages = table_of(total, 32, torch.Generator().manual_seed(seed), 'cuda')
+        cache = KVCache.allocate(pages, 32, KV, DIM, dtype=held)
+        lengths = torch.tensor(total, dtype=torch.int32, device='cuda')
+        few = [min(n, 20) for n in total]
+        return dict(k=rows[:, HEADS:HEADS + KV], v=rows[:, HEADS + KV:], q=rows[:sum(few), :HEADS], cache=cache,
+                    table=table, lengths=lengths, starts=starts, rows=sum(total), few=starts_of(few, 'cuda')[1])
+
+    def run(s):
+        kv_cache.write(s['cache'], s['k'], s['v'], s['table'], s['lengths'], s['starts'])
+        k, v = kv_cache.read(s['cache'], s['table'], s['starts'], s['rows'], dtype=dtype)
+        n = s['lengths'].shape[0]
+        return k, v, packed_attention(s['q'], k, v, s['few'], s['starts']), \
+            kv_cache.attend(s['q'][:n], s['cache'], s['table'], s['lengths'])
+
+    sets = [setup(1, [3000, 17, 1200]), setup(2, [5000, 900])]
+    for s in sets:
+        lib = _abi.load()
+        assert lib.w8a8_packed_attention_workspace_size(s['q'].shape[0], s['rows'], s['few'].numel() - 1, HEADS, KV, DIM) > 0
+        assert lib.w8a8_cache_attend_workspace_size(s['lengths'].numel(), HEADS, KV, DIM, s['table'].shape[1] * 32) > 0
+    want = [run(s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(run(s))
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(outs, want[i % 2])), i
