@@ -11,8 +11,8 @@
 // that several ranges share leaves partial sums, which a second kernel joins in
 // order. Loads run a block ahead, over the pairs' ends too.
 //
-// 131072 keys of 8 heads of 128 in bf16, 64 query heads (537 MB): 82 us and 7 for
-// the join, 6.0 TB/s in all; 64 contexts of 261850 keys as codes (555 MB): 93 to
+// 131072 keys of 8 heads of 128 in bf16, 64 query heads (537 MB): 82 us and 5 for
+// the join, 6.2 TB/s in all; 64 contexts of 261850 keys as codes (555 MB): 93 to
 // 99 us and 5; 354 keys: 7 us, the launch and one pass of latencies. Four waves a
 // workgroup and two of them a CU keep 8 KB and more a wave under way.
 //
@@ -98,10 +98,20 @@ struct Ranges {
   }
 };
 
-// Blocks of all sequences' first pairs.
+// Blocks of all pairs, and of those of the sequences before one.
 __device__ __forceinline__ int attend_total(const AttendParams& p) {
   int n = 0;
   for (int b = threadIdx.x & 63; b < p.sequences; b += 64) n += attend_blocks(p, p.lengths[b]);
+  return wave_sum(n) * (p.cache.heads * p.tiles);
+}
+__device__ __forceinline__ int attend_total(const AttendParams& p, int sequence, int& before) {
+  int n = 0, first = 0;
+  for (int b = threadIdx.x & 63; b < p.sequences; b += 64) {
+    const int mine = attend_blocks(p, p.lengths[b]);
+    n += mine;
+    if (b < sequence) first += mine;
+  }
+  before = wave_sum(first) * (p.cache.heads * p.tiles);
   return wave_sum(n) * (p.cache.heads * p.tiles);
 }
 
@@ -519,21 +529,37 @@ __global__ __launch_bounds__(64 * kAttendWaves, kAttendPerCu) void cache_attend_
   }
 }
 
-// The partial sums of the pair that begins in a range and goes on behind it: a
-// workgroup for each range and some of its heads. A wave takes 256 / DP heads
-// (four channels a lane), `parts` waves share their ranges, eight at a time, and
-// meet in LDS. The order is the ranges', whatever ends when.
+// The partial sums of a pair that several ranges share: a workgroup for some of its
+// heads, of the pair that begins in range blockIdx.x and goes on behind it, or with
+// `ranges` given of pair blockIdx.x, whose ranges it finds from the lengths. A wave
+// takes 256 / DP heads (four channels a lane), `parts` waves share their ranges,
+// eight at a time, and meet in LDS. The order is the ranges', whatever ends when.
 constexpr int kJoinWaves = 8, kJoinBatch = 8;
 constexpr int join_heads(int dp) { return 256 / dp; }
 template <int DT, int DP>
-__global__ __launch_bounds__(64 * kJoinWaves) void cache_attend_join_kernel(AttendParams p, int parts) {
+__global__ __launch_bounds__(64 * kJoinWaves) void cache_attend_join_kernel(AttendParams p, int parts, int ranges) {
   constexpr int LANES = DP / 4;
   __shared__ v4f sums[kJoinWaves][64];
   __shared__ float refs[kJoinWaves][64], totals[kJoinWaves][64];
-  const int g0 = blockIdx.x;
-  const int4 info = p.shared[g0];
-  if (info.x < 0) return;
-  const int b = info.x, pair = info.y, g1 = info.z;
+  int b, pair, g0, g1;
+  if (ranges > 0) {   // a workgroup for each pair
+    const int pairs = p.cache.heads * p.tiles;
+    b = blockIdx.x / pairs;
+    pair = blockIdx.x - b * pairs;
+    int before;
+    const Ranges r(attend_total(p, b, before), ranges);
+    const int n = attend_blocks(p, scalar_int(p.lengths, b)), at = before + pair * n;
+    g0 = Ranges::of(at, r.per, r.extra);
+    g1 = Ranges::of(at + n - 1, r.per, r.extra);
+    if (g0 == g1) return;
+  } else {
+    const int4 info = p.shared[blockIdx.x];
+    if (info.x < 0) return;
+    b = info.x;
+    pair = info.y;
+    g0 = blockIdx.x;
+    g1 = info.z;
+  }
   const int kvh = pair / p.tiles, tile = pair - kvh * p.tiles;
   const int heads = min(p.group - kHeadTile * tile, kHeadTile);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % parts;
@@ -616,14 +642,15 @@ static int launch_attend(const AttendParams& p, int64_t workgroups, hipStream_t 
   if (p.stream) hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP, true>), g, t, 0, s, p);
   else hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP, false>), g, t, 0, s, p);
   if (!p.whole) {
-    // Waves for the ranges of a pair, where it can have many of them, or for its
-    // heads (64 pairs of 64 sequences, two or three ranges each: 5.0 us that way,
+    // Waves for the ranges of a pair, where it can have many of them (and a workgroup
+    // for each pair: 131072 keys of 8 heads 88.6 -> 86.6 us, but 196 pairs of two or
+    // three ranges 22.6 -> 23.2), or for its heads (64 pairs of 64 sequences, two or three ranges each: 5.0 us that way,
     // 7.0 this way; one sequence's 8 pairs of 64 ranges 9.8 and 6.8).
-    const int64_t each = workgroups / ((int64_t)p.sequences * p.cache.heads * p.tiles);
+    const int64_t pairs = (int64_t)p.sequences * p.cache.heads * p.tiles, each = workgroups / pairs;
     const int parts = each >= 32 ? 8 : each >= 8 ? 4 : 1, per = kJoinWaves / parts * join_heads(DP);
     hipLaunchKernelGGL((cache_attend_join_kernel<DT, DP>),
-                       dim3((unsigned)workgroups, (std::min(p.group, kHeadTile) + per - 1) / per), dim3(64 * kJoinWaves), 0,
-                       s, p, parts);
+                       dim3((unsigned)(each >= 8 ? pairs : workgroups), (std::min(p.group, kHeadTile) + per - 1) / per),
+                       dim3(64 * kJoinWaves), 0, s, p, parts, each >= 8 ? (int)workgroups : 0);
   }
   return launch_status("w8a8_cache_attend");
 }
