@@ -642,10 +642,11 @@ static int launch_attend(const AttendParams& p, int64_t workgroups, hipStream_t 
   if (p.stream) hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP, true>), g, t, 0, s, p);
   else hipLaunchKernelGGL((cache_attend_kernel<DT, CODES, DP, false>), g, t, 0, s, p);
   if (!p.whole) {
-    // Waves for the ranges of a pair, where it can have many of them (and a workgroup
-    // for each pair: 131072 keys of 8 heads 88.6 -> 86.6 us, but 196 pairs of two or
-    // three ranges 22.6 -> 23.2), or for its heads (64 pairs of 64 sequences, two or three ranges each: 5.0 us that way,
-    // 7.0 this way; one sequence's 8 pairs of 64 ranges 9.8 and 6.8).
+    // Waves for the ranges of a pair, where it can have many of them, or for its
+    // heads (64 pairs of 64 sequences, two or three ranges each: 5.0 us that way,
+    // 7.0 this way; one sequence's 8 pairs of 64 ranges 9.8 and 6.8). With many, a
+    // workgroup for each pair and not each range: 131072 keys of 8 heads 88.6 -> 86.6
+    // us in all, but 196 pairs of two or three ranges 22.6 -> 23.2.
     const int64_t pairs = (int64_t)p.sequences * p.cache.heads * p.tiles, each = workgroups / pairs;
     const int parts = each >= 32 ? 8 : each >= 8 ? 4 : 1, per = kJoinWaves / parts * join_heads(DP);
     hipLaunchKernelGGL((cache_attend_join_kernel<DT, DP>),

@@ -22,7 +22,8 @@ struct CacheMoveParams {
   int64_t ld_table;
   const int32_t* lengths;
   const int32_t* starts;
-  int runs;   // runs of heads of a row
+  int runs;   // runs of heads of a row,
+  int pack;   // or rows of a wave, of fewer heads than it takes
   int fill;
   int stream;
 };
@@ -78,68 +79,127 @@ __device__ __forceinline__ uint2 codes8(const float (&f)[8], float s, bool tiny)
   return make_uint2(w[0] ^ 0x80808080u, w[1] ^ 0x80808080u);
 }
 
-// The wave's row, its run of heads, and the byte offsets of its key's place in
-// the cache; false where the row has none.
-template <int LPH>
-struct Move {
-  int64_t row;
-  int head, chunk;   // this lane's first head (the others follow in steps of 64 / LPH), and its eight channels
-};
-
-template <int LPH>
-__device__ __forceinline__ Move<LPH> move_of(const CacheMoveParams& p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = item / p.runs;
-  const int run = (int)(item - row * p.runs);
-  return {row, run * (kMoveHeads * 64 / LPH) + lane / LPH, lane % LPH};
-}
-
 // The page and token of key pos of sequence b; -1 where it is not there.
+template <bool SCALAR>
 __device__ __forceinline__ int key_place(const CacheMoveParams& p, int b, int pos, int& token) {
   if (pos < 0) return -1;
   int entry, first;
   group_place(p.cache, (uint32_t)pos / kGroupTokens, entry, first);
   if (entry >= p.width) return -1;
   token = first + pos % kGroupTokens;
-  const int page = scalar_int(p.table, (int64_t)b * p.ld_table + entry);
+  const int64_t i = (int64_t)b * p.ld_table + entry;
+  const int page = SCALAR ? scalar_int(p.table, i) : p.table[i];
   return page < p.cache.pages ? page : -1;
 }
 
+// What a lane moves: eight channels of kMoveHeads heads, each of a row. A row has
+// heads for a wave, or runs of them for several. Where a wave takes three times
+// the heads and more, and rows are more than the GPU holds waves for at once,
+// it takes p.pack rows (PACK): 50000 rows of one head of 128 written as codes 26.1 -> 12.4
+// us and read 17.6 -> 9.7; but 353 rows of two heads 3.9 -> 4.8, and 40000 of four,
+// two to a wave, 28.8 -> 30.5.
+template <int LPH, bool PACK>
+struct Move {
+  int chunk;
+  int64_t row[kMoveHeads];
+  int head[kMoveHeads];   // p.cache.heads where there is nothing to move
+  int64_t first;          // the wave's first row
+  int off[kMoveHeads];    // rows behind it
+  __device__ __forceinline__ explicit Move(const CacheMoveParams& p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    chunk = lane % LPH;
+    first = PACK ? item * p.pack : item / p.runs;
+#pragma unroll
+    for (int i = 0; i < kMoveHeads; ++i) {
+      const int slot = i * (64 / LPH) + lane / LPH;
+      off[i] = PACK ? slot / p.cache.heads : 0;
+      row[i] = first + off[i];
+      head[i] = PACK ? slot - off[i] * p.cache.heads : (int)(item - first * p.runs) * (kMoveHeads * 64 / LPH) + slot;
+      if (PACK && (row[i] >= p.rows || off[i] >= p.pack)) head[i] = p.cache.heads;
+    }
+  }
+};
+
+// The sequences of the rows (p.sequences: none), with starts and, if given, lengths.
+template <int LPH, bool PACK>
+__device__ __forceinline__ void sequences_of(const CacheMoveParams& p, const Move<LPH, PACK>& m, const int32_t* lengths,
+                                             SequenceRow (&s)[kMoveHeads]) {
+  if constexpr (!PACK) {
+    s[0] = sequence_of(p.starts, p.sequences, m.first, lengths);
+#pragma unroll
+    for (int i = 1; i < kMoveHeads; ++i) s[i] = s[0];
+  } else {
+    const int lane = threadIdx.x & 63, rows = (int)min((int64_t)p.pack, p.rows - m.first);
+    int b0 = sequence_window(p.starts, p.sequences, m.first);
+    int found = 0;
+#pragma unroll
+    for (int i = 0; i < kMoveHeads; ++i) s[i] = {p.sequences, 0, 0, 0};
+    for (; b0 < p.sequences && found < rows; b0 += 64) {
+      const int at = min(b0 + lane, p.sequences - 1);
+      const int first = p.starts[at], last = p.starts[at + 1], length = lengths ? lengths[at] : 0;
+      int mine[kMoveHeads];
+#pragma unroll
+      for (int i = 0; i < kMoveHeads; ++i) mine[i] = -1;
+      for (int r = 0; r < rows; ++r) {
+        const int64_t row = m.first + r;
+        const uint64_t in = __builtin_amdgcn_ballot_w64(b0 + lane < p.sequences && first <= row && row < last);
+        if (in == 0) continue;
+        ++found;
+#pragma unroll
+        for (int i = 0; i < kMoveHeads; ++i) mine[i] = r == m.off[i] ? __builtin_ctzll(in) : mine[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kMoveHeads; ++i) {
+        const int from = max(mine[i], 0);
+        const SequenceRow t{b0 + from, __shfl(first, from, 64), __shfl(last, from, 64), __shfl(length, from, 64)};
+        if (mine[i] >= 0 && s[i].b == p.sequences) s[i] = t;
+      }
+      if (__builtin_amdgcn_readlane(last, 63) > m.first + rows - 1) break;   // ascending: the rest lies behind the rows
+    }
+  }
+}
+
 // codes: the cache holds I8; DT is the rows' type.
-template <int DT, bool CODES, int LPH>
+template <int DT, bool CODES, int LPH, bool PACK>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheMoveParams p) {
-  const Move<LPH> m = move_of<LPH>(p);
-  if (m.row >= p.rows) return;
+  const Move<LPH, PACK> m(p);
+  if (m.first >= p.rows) return;
   const bool mine = 8 * m.chunk < p.cache.dim;   // (lanes beyond the channels stay for the maximum)
   uint4 x[2][kMoveHeads];
 #pragma unroll
   for (int i = 0; i < kMoveHeads; ++i) {
-    const int h = m.head + i * (64 / LPH);
     x[0][i] = x[1][i] = make_uint4(0, 0, 0, 0);
-    if (h < p.cache.heads && mine) {
-      x[0][i] = take16(p.k + m.row * p.k_row + h * p.k_head + 16 * m.chunk);
-      x[1][i] = take16(p.v + m.row * p.v_row + h * p.v_head + 16 * m.chunk);
+    if (m.head[i] < p.cache.heads && mine) {
+      x[0][i] = take16(p.k + m.row[i] * p.k_row + m.head[i] * p.k_head + 16 * m.chunk);
+      x[1][i] = take16(p.v + m.row[i] * p.v_row + m.head[i] * p.v_head + 16 * m.chunk);
     }
   }
-  int b, pos;
+  SequenceRow s[kMoveHeads];
   if (p.starts) {
-    const SequenceRow s = sequence_of(p.starts, p.sequences, m.row, p.lengths);
-    if (s.b >= p.sequences) return;
-    b = s.b;
-    pos = s.length - (s.last - (int)m.row);
+    sequences_of(p, m, p.lengths, s);
   } else {
-    b = __builtin_amdgcn_readfirstlane((int)m.row);
-    pos = scalar_int(p.lengths, b) - 1;
+#pragma unroll
+    for (int i = 0; i < kMoveHeads; ++i) {
+      const int b = (int)min(m.row[i], p.rows - 1);
+      s[i] = {b, b, b + 1, PACK ? p.lengths[b] : scalar_int(p.lengths, b)};
+    }
   }
-  int token;
-  const int page = key_place(p, b, pos, token);
-  if (page < 0) return;
-  const int64_t at = (int64_t)page * p.cache.page_b + (int64_t)token * p.cache.token_b;
+  int one_token = 0, one = -1;   // the place of the wave's only row
+  if constexpr (!PACK) {
+    if (s[0].b < p.sequences) one = key_place<true>(p, s[0].b, s[0].length - (s[0].last - (int)m.first), one_token);
+    if (one < 0) return;
+  }
 #pragma unroll
   for (int i = 0; i < kMoveHeads; ++i) {
-    const int h = m.head + i * (64 / LPH);
-    if (h >= p.cache.heads) continue;
+    const int h = m.head[i];
+    int token = one_token, page = one;
+    if (h >= p.cache.heads) continue;   // (a head's lanes together)
+    if constexpr (PACK) {
+      if (s[i].b < p.sequences) page = key_place<false>(p, s[i].b, s[i].length - (s[i].last - (int)m.row[i]), token);
+      if (page < 0) continue;
+    }
+    const int64_t at = (int64_t)page * p.cache.page_b + (int64_t)token * p.cache.token_b;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       char* to = (t ? p.cache.v : p.cache.k) + at + h * p.cache.head_b;
@@ -153,33 +213,36 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheMoveParams p) {
         for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
         top = head_max<LPH>(top);
         // A row that holds an infinity or a NaN has the scale NaN.
-        const float s = top < 0x7f800000u ? row_scale_of(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
+        const float scale = top < 0x7f800000u ? row_scale_of(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
         if (!mine) continue;
-        const bool tiny = __builtin_amdgcn_ballot_w64(s < 0x1p-60f) != 0;
-        *reinterpret_cast<uint2*>(to + 8 * m.chunk) = tiny ? codes8(f, s, true) : codes8(f, s, false);
+        const bool tiny = __builtin_amdgcn_ballot_w64(scale < 0x1p-60f) != 0;
+        *reinterpret_cast<uint2*>(to + 8 * m.chunk) = tiny ? codes8(f, scale, true) : codes8(f, scale, false);
         if (m.chunk == 0)
-          (t ? p.cache.vs : p.cache.ks)[(int64_t)page * p.cache.s_page + h * p.cache.s_head + token] = s;
+          (t ? p.cache.vs : p.cache.ks)[(int64_t)page * p.cache.s_page + h * p.cache.s_head + token] = scale;
       }
     }
   }
 }
 
-template <int DT, bool CODES, int LPH>
+template <int DT, bool CODES, int LPH, bool PACK>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheMoveParams p) {
-  const Move<LPH> m = move_of<LPH>(p);
-  if (m.row >= p.rows) return;
-  const SequenceRow s0 = sequence_of(p.starts, p.sequences, m.row, nullptr);
-  int token = 0, page = -1;
-  if (s0.b < p.sequences) page = key_place(p, s0.b, (int)m.row - s0.first, token);
-  else if (!p.fill) return;
+  const Move<LPH, PACK> m(p);
+  if (m.first >= p.rows) return;
+  SequenceRow s0[kMoveHeads];
+  sequences_of(p, m, nullptr, s0);
+  int one_token = 0, one = -1;   // the place of the wave's only row
+  if (!PACK && s0[0].b < p.sequences) one = key_place<true>(p, s0[0].b, (int)m.first - s0[0].first, one_token);
   if (8 * m.chunk >= p.cache.dim) return;
-  const int64_t at = (int64_t)page * p.cache.page_b + (int64_t)token * p.cache.token_b;
   uint4 x[2][kMoveHeads];
   uint2 c[2][kMoveHeads];
   float s[2][kMoveHeads];
 #pragma unroll
   for (int i = 0; i < kMoveHeads; ++i) {
-    const int h = m.head + i * (64 / LPH);
+    const int h = m.head[i];
+    int token = one_token, page = one;
+    if (PACK && h < p.cache.heads && s0[i].b < p.sequences)
+      page = key_place<false>(p, s0[i].b, (int)m.row[i] - s0[i].first, token);
+    const int64_t at = (int64_t)page * p.cache.page_b + (int64_t)token * p.cache.token_b;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       x[t][i] = make_uint4(0, 0, 0, 0);
@@ -197,8 +260,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheMoveParams p) {
   }
 #pragma unroll
   for (int i = 0; i < kMoveHeads; ++i) {
-    const int h = m.head + i * (64 / LPH);
-    if (h >= p.cache.heads) continue;
+    const int h = m.head[i];
+    if (h >= p.cache.heads || (s0[i].b == p.sequences && !p.fill)) continue;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if constexpr (CODES) {
@@ -213,29 +276,35 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheMoveParams p) {
         }
         x[t][i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      char* to = t ? p.v + m.row * p.v_row + h * p.v_head : p.k + m.row * p.k_row + h * p.k_head;
+      char* to = t ? p.v + m.row[i] * p.v_row + h * p.v_head : p.k + m.row[i] * p.k_row + h * p.k_head;
       put16(to + 16 * m.chunk, x[t][i], p.stream);
     }
   }
 }
 
 static int head_lanes(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+static int64_t move_waves(const CacheMoveParams& p) { return p.pack > 1 ? (p.rows + p.pack - 1) / p.pack : p.rows * p.runs; }
 
-template <bool WRITE, int DT, bool CODES>
+template <bool WRITE, int DT, bool CODES, bool PACK>
 static int launch_move(const char* who, const CacheMoveParams& in, hipStream_t stream) {
   CacheMoveParams p = in;
   const int lph = head_lanes(p.cache.dim);
   p.stream = p.rows * p.cache.heads * p.cache.dim * 4 > (64ll << 20);   // (k and v; 69277 rows of codes read: 80 -> 68 us)
-  const dim3 g((unsigned)((p.rows * p.runs + 3) / 4)), t(256);
+  const dim3 g((unsigned)((move_waves(p) + 3) / 4)), t(256);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, t, 0, stream, p); };
   if constexpr (WRITE) {
-    lph == 8 ? go(cache_write_kernel<DT, CODES, 8>)
-             : lph == 16 ? go(cache_write_kernel<DT, CODES, 16>) : go(cache_write_kernel<DT, CODES, 32>);
+    lph == 8 ? go(cache_write_kernel<DT, CODES, 8, PACK>)
+             : lph == 16 ? go(cache_write_kernel<DT, CODES, 16, PACK>) : go(cache_write_kernel<DT, CODES, 32, PACK>);
   } else {
-    lph == 8 ? go(cache_read_kernel<DT, CODES, 8>)
-             : lph == 16 ? go(cache_read_kernel<DT, CODES, 16>) : go(cache_read_kernel<DT, CODES, 32>);
+    lph == 8 ? go(cache_read_kernel<DT, CODES, 8, PACK>)
+             : lph == 16 ? go(cache_read_kernel<DT, CODES, 16, PACK>) : go(cache_read_kernel<DT, CODES, 32, PACK>);
   }
   return launch_status(who);
+}
+
+template <bool WRITE, int DT, bool CODES>
+static int launch_move(const char* who, const CacheMoveParams& p, hipStream_t stream) {
+  return p.pack > 1 ? launch_move<WRITE, DT, CODES, true>(who, p, stream) : launch_move<WRITE, DT, CODES, false>(who, p, stream);
 }
 
 template <bool WRITE>
@@ -267,7 +336,8 @@ static int move_params(const char* who, int dtype, const W8A8KvCache& c, const v
   p.rows = rows;
   const int per = kMoveHeads * 64 / head_lanes(c.dim);
   p.runs = (c.heads + per - 1) / per;
-  W8A8_REQUIRE((rows * p.runs + 3) / 4 < (1ll << 24), "%s: too many rows and heads for one launch", who);   // (2^32 work-items)
+  p.pack = rows > 4096 && per / c.heads > 2 ? per / c.heads : 1;
+  W8A8_REQUIRE((move_waves(p) + 3) / 4 < (1ll << 24), "%s: too many rows and heads for one launch", who);   // (2^32 work-items)
   p.sequences = (int)sequences;
   p.width = (int)width;
   p.table = table;

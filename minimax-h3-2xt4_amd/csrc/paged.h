@@ -75,7 +75,8 @@ __device__ __forceinline__ int last_lane(bool x) {
 struct SequenceRow {
   int b, first, last, length;
 };
-__device__ __forceinline__ SequenceRow sequence_of(const int32_t* starts, int n, int64_t row, const int32_t* lengths) {
+// The first of 64 sequences or fewer among which the row's lies, if there is one.
+__device__ __forceinline__ int sequence_window(const int32_t* starts, int n, int64_t row) {
   const int lane = threadIdx.x & 63;
   int b = 0, size = n;
   while (size > 64) {
@@ -84,9 +85,13 @@ __device__ __forceinline__ SequenceRow sequence_of(const int32_t* starts, int n,
     b += skip;
     size = min(step, size - skip);
   }
+  return b;
+}
+__device__ __forceinline__ SequenceRow sequence_of(const int32_t* starts, int n, int64_t row, const int32_t* lengths) {
+  const int lane = threadIdx.x & 63, b = sequence_window(starts, n, row);
   const int i = min(b + lane, n - 1);
   const int first = starts[i], last = starts[i + 1], length = lengths ? lengths[i] : 0;
-  const uint64_t in = __builtin_amdgcn_ballot_w64(lane < size && first <= row && row < last);
+  const uint64_t in = __builtin_amdgcn_ballot_w64(b + lane < n && first <= row && row < last);
   if (in == 0) return {n, 0, 0, 0};
   const int at = __builtin_ctzll(in);
   return {b + at, __builtin_amdgcn_readlane(first, at), __builtin_amdgcn_readlane(last, at),

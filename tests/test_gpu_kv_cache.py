@@ -117,6 +117,51 @@ def test_many_sequences(gpu, sequences):
     assert not bool(rk[ks[-1]:].any()) and not bool(rv[ks[-1]:].any())
 
 
+@pytest.mark.parametrize('single', [False, True])
+@pytest.mark.parametrize('held,heads,dim', [(torch.float16, 1, 128), (torch.int8, 1, 72), (torch.int8, 5, 64),
+                                            (torch.bfloat16, 3, 40), (torch.int8, 2, 128), (torch.int8, 1, 256)])
+def test_many_rows_of_few_heads(gpu, held, heads, dim, single):
+    """A wave has several rows: of a sequence or of many, empty ones and absent pages among them."""
+    dtype = torch.bfloat16 if held == torch.int8 else held
+    g = torch.Generator().manual_seed(dim)
+    new = torch.ones(4500, dtype=torch.int64) if single else torch.cat(
+        [torch.randint(0, 4, (200,), generator=g), torch.tensor([4000, 0, 0, 33]), torch.randint(0, 40, (70,), generator=g)])
+    n = len(new)
+    before = torch.randint(0, 40, (n,), generator=g)
+    total = new + before
+    table, pages = table_of(total.tolist(), 32, g, 'cuda')
+    table[::7, 0] = -1
+    cache, want = twin(pages, 32, heads, dim, held)
+    st, starts = starts_of(new.tolist(), 'cuda')
+    k, v = kv_rows(dtype, st[-1] if single else st[-1] + 77, heads, dim, seed=dim)
+    kv_cache.write(cache, k, v, table, total.int().cuda(), None if single else starts)
+    b = torch.repeat_interleave(torch.arange(n), new)
+    key = (before[b] + torch.arange(st[-1]) - torch.tensor(st)[b]).cuda()
+    page = table[b.cuda(), key // 32].long()
+    there, at, off = page >= 0, page[page >= 0], key[page >= 0] % 32
+    for name, x in (('k', k), ('v', v)):
+        x = x[:st[-1]][there]
+        if cache.codes:
+            getattr(want, name)[at, :, off], getattr(want, name + '_scale')[at, :, off] = quantize64(x)
+        else:
+            getattr(want, name)[at, :, off] = x
+    same(cache, want)
+    ks, k_starts = starts_of(total.tolist(), 'cuda')
+    rk, rv = kv_cache.read(cache, table, k_starts, ks[-1] + 77, dtype=dtype)
+    b = torch.repeat_interleave(torch.arange(n), total)
+    key = (torch.arange(ks[-1]) - torch.tensor(ks)[b]).cuda()
+    page = table[b.cuda(), key // 32].long()
+    for got, name in ((rk, 'k'), (rv, 'v')):
+        x = getattr(cache, name)[page.clamp_min(0), :, key % 32]
+        if cache.codes:
+            x = (x.float() * getattr(cache, name + '_scale')[page.clamp_min(0), :, key % 32][..., None]).to(dtype)
+        assert torch.equal(got[:ks[-1]], torch.where((page >= 0)[:, None, None], x, torch.zeros_like(x))), name
+        assert not bool(got[ks[-1]:].any())
+    out = tuple(torch.full_like(rk, 3.0) for _ in range(2))
+    kv_cache.read(cache, table, k_starts, ks[-1] + 77, out=out)
+    assert all(torch.equal(o[:ks[-1]], r[:ks[-1]]) and bool((o[ks[-1]:] == 3.0).all()) for o, r in zip(out, (rk, rv)))
+
+
 def test_places_that_are_not_there(gpu):
     """Keys outside of the table, absent pages and pages outside of the cache are not written."""
     cache, want = twin(4, 16, 2, 64, torch.float16)
