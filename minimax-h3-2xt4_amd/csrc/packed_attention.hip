@@ -699,17 +699,20 @@ static int packed_pitch(int dim) { return (packed_dp(dim) + 31) / 32 * 32; }
 
 // Ranges of a tile's keys. A step along the keys takes a wave about 1 us however
 // few workgroups there are. Where the tiles of all heads are fewer than half of
-// what the GPU holds, several workgroups take a tile's keys, four blocks each or
-// more, if the steps saved are more than the second kernel (8 steps) and the
-// sums' way through memory (3.6 MB a step): one row behind 8000 keys 130 -> 25
-// us, but 512 rows of a prompt 17 -> 29. (The halves of a workgroup of eight waves
-// sharing the keys and meeting in LDS: 353 rows 13.0 -> 14.7.)
+// what the GPU holds, several workgroups take a tile's keys: four blocks each or
+// more (one row behind 8000 keys 130 us alone, 16.7 so, 19.5 by two blocks), or two
+// for up to eight workgroups, which the second kernel joins in one go (one behind
+// 1000 keys 11.4 -> 9.5, 23 of 28 heads behind 587 16.1 -> 12.5). That is, if the steps
+// saved are more than the second kernel (5 steps; 23 rows behind 300 keys save four
+// and lose, 11.5 -> 12.2) and the sums' way through memory (3.6 MB a step): 512
+// rows of a prompt 17 -> 29. (The halves of a workgroup of eight waves sharing the
+// keys and meeting in LDS: 353 rows 13.0 -> 14.7.)
 static int packed_splits(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads, int dim) {
   if (rows <= 0 || keys <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 1;
   const int64_t filled = std::min(rows, sequences), tiles = (rows * (heads / kv_heads) + (kPackQ - 1) * filled) / kPackQ * kv_heads;
   const int64_t slots = (dim > 128 ? 1 : 2) * current_device_cus(), block = dim > 128 ? 32 : 64;
-  const int64_t steps = (keys / sequences + block - 1) / block, splits = std::min(slots / tiles, steps / 4);
-  return splits >= 2 && steps - steps / splits >= 8 + rows * heads * splits * packed_pitch(dim) * 8 / 3600000 ? (int)splits : 1;
+  const int64_t steps = (keys / sequences + block - 1) / block, splits = std::min(slots / tiles, std::max(steps / 4, std::min<int64_t>(steps / 2, 8)));
+  return splits >= 2 && steps - steps / splits >= 5 + rows * heads * splits * packed_pitch(dim) * 8 / 3600000 ? (int)splits : 1;
 }
 
 template <int DT, int DP, bool CAUSAL>
