@@ -42,9 +42,14 @@ constexpr int kWaveKeys = 32;   // keys of a wave at a time: two groups
 constexpr int kBlockKeys = kAttendWaves * kWaveKeys;
 // dim rounded up to the channels that a kernel works on.
 constexpr int attend_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-// Workgroups of a CU: with one of eight waves, the ends of pairs leave it idle
-// (64 contexts of codes 115 -> 124 us), three have no more bytes under way.
-constexpr int kAttendPerCu = 2;
+// Workgroups that a CU's ranges are cut for: with one of eight waves, the ends of
+// pairs leave it idle (64 contexts of codes 115 -> 124 us), with three there are more
+// ends (94.5 -> 104). Registers are for three, which calls of a workgroup for each
+// pair fill (1024 contexts of 200 keys as codes 131 -> 110 us). 256 channels are one
+// workgroup's, all registers: with two that spill, 64 contexts of 4096 keys took
+// 394 us instead of 349.
+constexpr int attend_per_cu(int dim) { return dim > 128 ? 1 : 2; }
+constexpr int attend_fit(int dim) { return dim > 128 ? 1 : 3; }
 // The reference of p may lie so much below the maximum (as a power of 2), and
 // the reference of the values' scales 2^kScaleSlack: p times the scale is then
 // at most 2^12, far inside fp16, and rescaling the sums is rare.
@@ -180,7 +185,7 @@ constexpr uint32_t kNowhere = 0x7fffff00u;   // an offset behind every descripto
 // DT: type of q and out; CODES: the cache holds I8; DP: dim rounded up to 64, 128
 // or 256; STREAM: the keys and values pass through the caches without staying.
 template <int DT, bool CODES, int DP, bool STREAM>
-__global__ __launch_bounds__(64 * kAttendWaves, kAttendPerCu) void cache_attend_kernel(AttendParams p) {
+__global__ __launch_bounds__(64 * kAttendWaves, attend_fit(DP)) void cache_attend_kernel(AttendParams p) {
   constexpr int ES = CODES ? 1 : 2, AUX = STREAM ? 2 : 0;
   // Codes are multiplied as fp16, whatever q's type: cheaper to make than bf16,
   // and P keeps eleven bits. q of bf16 is scaled by a power of 2 for it, so that a
@@ -629,7 +634,7 @@ struct AttendPlan {
 static AttendPlan attend_plan(int64_t pairs, int64_t max_keys, int dim) {
   const int64_t blocks = std::max<int64_t>((max_keys + kBlockKeys - 1) / kBlockKeys, 1), cus = current_device_cus();
   if (blocks <= 4 || (blocks <= 8 && 2 * pairs >= cus)) return {pairs, true};
-  return {std::min<int64_t>(pairs * blocks, kAttendPerCu * cus), false};
+  return {std::min<int64_t>(pairs * blocks, attend_per_cu(dim) * cus), false};
 }
 
 static int64_t attend_tiles(int64_t heads, int64_t kv_heads) {
