@@ -17,8 +17,9 @@
 //
 // Bound by the board's power where it is long: 16384 causal rows of 64 heads of
 // 128 in bf16 take 3.83 ms, 1148 TFLOP/s, with the MFMAs busy 62 % of the cycles at
-// 1.77 GHz (a loop of nothing but MFMAs and these LDS reads reaches 1530 TFLOP/s on
-// random operands, the library's 8192^3 product 1185 to 1440). Moving work between
+// 1.77 GHz. A loop of nothing but MFMAs and these LDS reads reaches 1540 TFLOP/s on
+// random operands, and 1170 with the softmax's instructions between them (1180 on
+// 16 x 16 x 32 MFMAs); the library's 8192^3 product 1185 to 1440. Moving work between
 // the MFMAs, reading further ahead or raising waves' priorities changes it by less
 // than 1 %. Fewer instructions do: a lazy reference, a row sum by dot products of
 // the packed words. Two workgroups a CU, so that the two waves of a SIMD wait at
