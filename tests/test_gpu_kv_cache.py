@@ -183,6 +183,26 @@ def test_places_that_are_not_there(gpu):
     assert not bool(rk[40:56].any()) and torch.equal(rv[56:60], cache.v[1, :, :4].transpose(0, 1))
 
 
+@pytest.mark.parametrize('heads', [1, 8])
+def test_starts_and_lengths_out_of_range_stay_in_bounds(gpu, heads):
+    """Whatever starts and lengths hold, only the cache's pages and the rows are touched."""
+    big = torch.full((2, 12, heads, 16, 64), 7.0, dtype=torch.float16, device='cuda')
+    cache = KVCache(big[0, 4:8], big[1, 4:8])
+    rows = torch.full((2, 7000, heads, 64), 7.0, dtype=torch.float16, device='cuda')
+    k, v = rows[0, 1000:6000], rows[1, 1000:6000]
+    low, high = -2 ** 31, 2 ** 31 - 1
+    table = torch.tensor([[0, 3], [1, 4], [high, 2], [low, -1]], dtype=torch.int32, device='cuda')
+    for starts in ([0, 9000, 9000, 9000, 9000], [0, -5, 3, 2, 4900], [high, low, 0, high, low], [5, 4, 3, 2, 1],
+                   [low, high, high, high, high], [0, 10, 20, 30, 40]):
+        for lengths in ([20, 40, 30, 5], [high] * 4, [low] * 4, [0, -1, 33, 1000]):
+            s, n = (torch.tensor(t, dtype=torch.int32, device='cuda') for t in (starts, lengths))
+            kv_cache.write(cache, torch.zeros_like(k), torch.zeros_like(v), table, n, s)
+            kv_cache.read(cache, table, s, 5000, out=(k, v))
+            kv_cache.attend(torch.zeros((4, heads, 64), dtype=torch.float16, device='cuda'), cache, table, n)
+    assert bool((big[:, :4] == 7.0).all()) and bool((big[:, 8:] == 7.0).all())
+    assert bool((rows[:, :1000] == 7.0).all()) and bool((rows[:, 6000:] == 7.0).all())
+
+
 def test_rows_that_are_not_finite(gpu):
     cache, _ = twin(1, 16, 2, 64, torch.int8)
     k, v = kv_rows(torch.bfloat16, 4, 2, 64)

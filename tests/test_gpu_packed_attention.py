@@ -194,6 +194,36 @@ def test_masked_keys_have_no_effect(gpu, dim, bad):
             assert bool(torch.isnan(y[at:100]).any())
 
 
+@pytest.mark.parametrize('bad', [math.inf, math.nan])
+@pytest.mark.parametrize('dim,shared', [(72, False), (72, True), (80, False), (80, True), (96, False), (40, True)])
+def test_masked_keys_of_other_widths_have_no_effect(gpu, dim, shared, bad):
+    """Whatever takes the sums of P, and whether or not workgroups share the keys."""
+    nk = 1500 if shared else 90
+    starts, k_starts = starts_of([90], 'cuda')[1], starts_of([nk], 'cuda')[1]
+    assert (_abi.load().w8a8_packed_attention_workspace_size(90, nk, 1, 2, 2, dim) > 0) == shared
+    for dtype in DTYPES:
+        q, k, v = make(dtype, 90, nk, 2, 2, dim, seed=dim)
+        at = nk - 30
+        k[at, :, 1::4], v[at, :, ::3] = bad, bad
+        y = packed_attention(q, k, v, starts, k_starts)
+        check_packed(y[:60], q[:60], k[:at], v[:at], [0, 60], [0, at], True, dim ** -0.5)
+        assert bool(torch.isnan(y[60:, :, ::3]).all())
+
+
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('dtype,dim', [(torch.bfloat16, 128), (torch.float16, 80), (torch.bfloat16, 256)])
+@pytest.mark.parametrize('sequences', [8, 40, 70])
+def test_few_rows_of_many_sequences(gpu, sequences, dtype, dim, causal):
+    """Sequences are searched for, and workgroups share their keys."""
+    g = torch.Generator().manual_seed(sequences)
+    new = torch.randint(0, 4, (sequences,), generator=g).tolist()
+    keys = (torch.randint(500, 900, (sequences,), generator=g) if sequences < 70 else
+            torch.randint(0, 1800, (sequences,), generator=g)).tolist()
+    new[0], keys[-1], new[-1] = 0, 0, 2
+    assert _abi.load().w8a8_packed_attention_workspace_size(sum(new), sum(keys), sequences, 2, 1, dim) > 0
+    run(dtype, 2, 1, dim, new, keys, causal, seed=dim)
+
+
 def test_visible_infinities(gpu):
     _, starts = starts_of([70], 'cuda')
     q, k, v = make(torch.bfloat16, 70, 70, 1, 1, 64)
