@@ -824,10 +824,11 @@ int w8a8_cache_read(const W8A8CacheReadArgs* args);
  * q, out: [sequences, heads, cache.dim] of dtype (F16 or BF16; a 16-bit
  *   cache's own), element strides {row, head}, channels contiguous, rows and
  *   heads on 16-byte boundaries.
- * Scores, statistics and sums are fp32; p is rounded for the product with v,
- *   relative to 2^r with r at most 8 below the running maximum of its exponent: to
- *   dtype, or with codes, times the value's scale relative to one of the largest
- *   scales, to F16. The same call gives the same bits every time.
+ * Scores, statistics and sums are fp32; p is rounded for the product with v:
+ *   to dtype, relative to 2^r with r at most 8 below the running maximum of its
+ *   exponent; or with codes, times the value's scale, to F16, where what is lost
+ *   lies below 2^-32 of the largest such product so far. The same call gives the
+ *   same bits every time.
  * workspace: device buffer of at least w8a8_cache_attend_workspace_size()
  *   bytes (16-byte aligned, any contents; NULL where that is 0): partial sums
  *   of sequences that several workgroups share. Calls that share one must not

@@ -50,10 +50,20 @@ constexpr int attend_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 25
 // 394 us instead of 349.
 constexpr int attend_per_cu(int dim) { return dim > 128 ? 1 : 2; }
 constexpr int attend_fit(int dim) { return dim > 128 ? 1 : 3; }
-// The reference of p may lie so much below the maximum (as a power of 2), and
-// the reference of the values' scales 2^kScaleSlack: p times the scale is then
-// at most 2^12, far inside fp16, and rescaling the sums is rare.
-constexpr float kSlack = 8.0f, kScaleSlack = 16.0f;
+// The reference of p may lie so much below the maximum (as a power of 2): rescaling
+// the sums is rare.
+constexpr float kSlack = 8.0f;
+// Codes: P is p times the value's scale, and relative to a reference of its own, of
+// what keys contribute, so that no key's scale takes precision from keys of more
+// weight (relative to the largest scale, a row 2^18 times the others' with a weight
+// of 2^-46 left the output 4 % off). That reference is a power of 2, the largest
+// product so far at most kPartSlack times it, and P relative to 1 / kPartLift of it:
+// at most 2^15, of fp16's 2^16, and what is lost lies below 2^-32 of the largest. p
+// is at most 1, so that its product with the largest scale of bf16 rows, 2^121, is finite.
+constexpr float kPartSlack = 256.0f, kPartLift = 128.0f, kLeastPart = 0x1p-119f;
+// kPartLift / x of a power of 2 from kLeastPart on (of 0 some finite value).
+__device__ __forceinline__ float part_inv(float x) { return __uint_as_float((261u << 23) - __float_as_uint(x)); }
+__device__ __forceinline__ float power_of_2(float x) { return __uint_as_float(__float_as_uint(x) & 0x7f800000u); }
 
 struct AttendParams {
   CacheView cache;
@@ -360,7 +370,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_fit(DP)) void cache_atten
     v4f o[VL];
 #pragma unroll
     for (int j = 0; j < VL; ++j) o[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float ref = -INFINITY, l = 0.0f, top = 0.0f;   // top: the value scale that P's are relative to (codes)
+    float ref = -INFINITY, l = 0.0f, top = 0.0f;   // top: codes' reference of P
 
     auto spread_max = [&](float x) {   // over the four quads: the keys of a column
       x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -402,39 +412,50 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_fit(DP)) void cache_atten
           }
       }
       // The references follow the maxima only once those lie far enough above.
-      float mx = t[0], u = 0.0f;
-#pragma unroll
-      for (int i = 1; i < 4 * G; ++i) mx = fmaxf(mx, t[i]);
-      if constexpr (CODES) {
-#pragma unroll
-        for (int i = 0; i < 4 * G; ++i) u = fmaxf(u, sc.v[i / 4][i % 4]);
-      }
-      if (__builtin_amdgcn_ballot_w64(mx > ref + kSlack || (CODES && u > top * kScaleSlack))) {
-        const float to = fmaxf(ref, spread_max(mx));
-        float fade = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
-        ref = to;
-        l = l * fade;
-        if constexpr (CODES) {
-          u = fmaxf(fmaxf(top, spread_max(u)), 0x1p-126f);
-          fade = fade * (top / u);
-          top = u;
-        }
+      auto fade_sums = [&](float fade) {
 #pragma unroll
         for (int j = 0; j < VL; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[j][i] = o[j][i] * fade;
+      };
+      float mx = t[0];
+#pragma unroll
+      for (int i = 1; i < 4 * G; ++i) mx = fmaxf(mx, t[i]);
+      if (__builtin_amdgcn_ballot_w64(mx > ref + kSlack)) {
+        float to = spread_max(mx);
+        if constexpr (CODES) to = floorf(to);   // (the other reference fades by powers of 2)
+        to = fmaxf(ref, to);
+        const float fade = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
+        l = l * fade;
+        if constexpr (CODES) {   // O stays as it is, but for what the least reference does not hold
+          const float faded = ldexpf(top, (int)fmaxf(ref - to, -300.0f));
+          if (to != -INFINITY) top = fmaxf(faded, kLeastPart);
+          if (__builtin_amdgcn_ballot_w64(faded != top)) fade_sums(top > 0.0f ? faded / top : 0.0f);
+        } else {
+          fade_sums(fade);
+        }
+        ref = to;
       }
-      const float base = ref == -INFINITY ? 0.0f : ref;
-      float inv = 0.0f;
-      if constexpr (CODES) inv = 1.0f / fmaxf(top, 0x1p-126f);   // (top 0: no key so far)
+      const float base = ref == -INFINITY ? 0.0f : CODES ? ref + kSlack : ref;
       float w[4 * G];
 #pragma unroll
-      for (int i = 0; i < 4 * G; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(t[i] - base);
-        if constexpr (CODES) l += w[i];
-        // P carries the values' scales, relative to about the largest so far,
-        // so that it keeps the type's precision whatever their size.
-        if constexpr (CODES) w[i] = w[i] * (sc.v[i / 4][i % 4] * inv);
+      for (int i = 0; i < 4 * G; ++i) w[i] = __builtin_amdgcn_exp2f(t[i] - base);
+      if constexpr (CODES) {
+        float u = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4 * G; ++i) {
+          l += w[i];
+          w[i] = w[i] * sc.v[i / 4][i % 4];
+          u = fmaxf(u, fabsf(w[i]));
+        }
+        if (__builtin_amdgcn_ballot_w64(u > top * kPartSlack)) {
+          const float to = power_of_2(fmaxf(top, spread_max(u)));
+          fade_sums(to > 0.0f ? top / to : 0.0f);
+          top = to;
+        }
+        const float inv = part_inv(top);
+#pragma unroll
+        for (int i = 0; i < 4 * G; ++i) w[i] = w[i] * inv;
       }
 #pragma unroll
       for (int g = 0; g < G; g += 2) {
@@ -502,7 +523,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_fit(DP)) void cache_atten
       for (int w = 0; w < kAttendWaves; ++w) {
         const float f = __builtin_amdgcn_exp2f(stat[w][0][h] - ref);
         const v4f part = *reinterpret_cast<const v4f*>(&sums[w][h][d]);
-        const float g = CODES ? f * stat[w][2][h] : f;
+        const float g = CODES ? f * (stat[w][2][h] * (1.0f / kPartLift)) : f;
         sum = __builtin_fmaf(stat[w][1][h], f, sum);
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(part[e], g, y[e]);

@@ -1,0 +1,107 @@
+"""Attention where weights, values and scores lie far apart, against 64 bits
+(tolerances: attention_refs, but for what is said here)."""
+import math
+
+import pytest
+import torch
+
+from attention_refs import attention64, bound, check, quantize64
+from w8a8 import kv_cache
+from w8a8.kv_cache import KVCache
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16]
+TABLE_PAGE = 64
+
+
+def paged(k, v, held):
+    """A cache of one sequence's keys and values [keys, heads, dim], and its table and length."""
+    n, heads, dim = k.shape
+    pages = -(-n // TABLE_PAGE)
+    cache = KVCache.allocate(pages, TABLE_PAGE, heads, dim, dtype=held)
+    for name, x in (('k', k), ('v', v)):
+        full = torch.zeros((pages * TABLE_PAGE, heads, dim), dtype=x.dtype, device='cuda')
+        full[:n] = x
+        full = full.view(pages, TABLE_PAGE, heads, dim).transpose(1, 2)
+        if held == torch.int8:
+            c, s = quantize64(full)
+            getattr(cache, name).copy_(c)
+            getattr(cache, name + '_scale').copy_(s)
+        else:
+            getattr(cache, name).copy_(full)
+    table = torch.arange(pages, dtype=torch.int32, device='cuda')[None]
+    return cache, table, torch.tensor([n], dtype=torch.int32, device='cuda')
+
+
+def rows_of(x, n):
+    """A cache's [pages, heads, page, ...] as [keys, heads, ...]."""
+    return x.transpose(1, 2).flatten(0, 1)[:n]
+
+
+def keys_with_scores(q0, t, dim, dtype):
+    """Keys [keys, 1, dim] whose scores with q0 (one value in every channel), times
+    1 / sqrt(dim), are about t (in powers of 2)."""
+    return (t[:, None, None] * math.log(2.0) / (q0 * math.sqrt(dim))).expand(-1, 1, dim).contiguous().to(dtype)
+
+
+def attend_codes(k, v, v_times, dtype, q):
+    """Codes whose scales of v are taken times v_times [keys]; o against 64 bits. What
+    the kernel loses of P lies below 2^-32 of the largest product of a weight and a
+    value's scale, whatever the scales of keys without weight."""
+    n, dim = k.shape[0], k.shape[2]
+    cache, table, length = paged(k, v, torch.int8)
+    flat = torch.ones(table.shape[1] * TABLE_PAGE, device='cuda')
+    flat[:n] = v_times
+    cache.v_scale.mul_(flat.view(-1, 1, TABLE_PAGE))
+    y = kv_cache.attend(q, cache, table, length)
+    ks, vs = rows_of(cache.k_scale, n).double(), rows_of(cache.v_scale, n).double()
+    k64, codes = rows_of(cache.k, n)[:, 0].double() * ks, rows_of(cache.v, n)[:, 0].double()
+    for h in range(q.shape[1]):
+        t = (k64 @ q[0, h].double()) * dim ** -0.5
+        most = (torch.exp(t - t.max()) * vs[:, 0]).max()
+        lost = codes.abs() * most * 2.0 ** -7   # (the bound takes 2^-25 of it)
+        o, parts = attention64(q[0, h][None].double(), k64, codes * vs, dim ** -0.5, codes_scale=lost)
+        check(y[0, h][None], o, bound(o, parts, dtype), f'head {h}')
+
+
+@pytest.mark.parametrize('n', [200, 3000])
+@pytest.mark.parametrize('dim', [64, 80, 128, 256])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_codes_beside_a_row_of_large_values(gpu, dtype, dim, n):
+    """A value row far larger than the others, of a key of little weight."""
+    g = torch.Generator().manual_seed(dim)
+    q = (1.0 + 0.01 * torch.randn((1, 3, dim), generator=g)).to(dtype).cuda()
+    for at in (0, 37, n - 1):
+        for size in (0, 10, 18, 26, 40, 46) if dtype == torch.float16 else (0, 18, 26, 46, 60, 90):
+            t = torch.randn(n, generator=g)
+            t[at] = -46.0
+            k = keys_with_scores(1.0, t.cuda(), dim, dtype)
+            v = (torch.randn((n, 1, dim), generator=g) * 2.0 ** -10).to(dtype).cuda()
+            times = torch.ones(n, device='cuda')
+            times[at] = 2.0 ** size
+            attend_codes(k, v, times, dtype, q)
+
+
+@pytest.mark.parametrize('n', [200, 3000])
+@pytest.mark.parametrize('order', ['up', 'down', 'any'])
+@pytest.mark.parametrize('dim', [64, 128, 256])
+def test_codes_whose_scales_undo_their_weights(gpu, dim, order, n):
+    """Weights over a range of 2^80, the scales of values over its inverse: all keys contribute alike."""
+    g = torch.Generator().manual_seed(dim)
+    q = (1.0 + 0.01 * torch.randn((1, 2, dim), generator=g)).bfloat16().cuda()
+    t = torch.linspace(-40.0, 40.0, n)
+    t = t.flip(0) if order == 'down' else t[torch.randperm(n, generator=g)] if order == 'any' else t
+    k = keys_with_scores(1.0, t.cuda(), dim, torch.bfloat16)
+    v = torch.randn((n, 1, dim), generator=g).bfloat16().cuda()
+    attend_codes(k, v, torch.exp2(-t).cuda(), torch.bfloat16, q)
+
+
+def test_codes_of_the_largest_values(gpu):
+    """The largest finite rows beside rows of zeros and of the smallest scale."""
+    g = torch.Generator().manual_seed(5)
+    k = torch.randn((150, 1, 64), generator=g).bfloat16().cuda()
+    v = torch.randn((150, 1, 64), generator=g).bfloat16().cuda()
+    v[::3], v[1::3] = 0.0, torch.finfo(torch.bfloat16).max / 4
+    q = torch.randn((1, 4, 64), generator=g).bfloat16().cuda()
+    attend_codes(k, v, torch.ones(150, device='cuda'), torch.bfloat16, q)
