@@ -825,9 +825,9 @@ int w8a8_cache_read(const W8A8CacheReadArgs* args);
  *   cache's own), element strides {row, head}, channels contiguous, rows and
  *   heads on 16-byte boundaries.
  * Scores, statistics and sums are fp32; p is rounded for the product with v:
- *   to dtype, relative to 2^r with r at most 8 below the running maximum of its
- *   exponent; or with codes, times the value's scale, to F16, where what is lost
- *   lies below 2^-32 of the largest such product so far. The same call gives the
+ *   to dtype (F16: what is lost lies below 2^-32 of the largest so far); or with
+ *   codes, times the value's scale, to F16, where what is lost lies below 2^-32 of
+ *   the largest such product so far. The same call gives the
  *   same bits every time.
  * workspace: device buffer of at least w8a8_cache_attend_workspace_size()
  *   bytes (16-byte aligned, any contents; NULL where that is 0): partial sums
@@ -877,9 +877,9 @@ int64_t w8a8_cache_attend_workspace_size(int64_t sequences, int64_t heads, int64
  * starts, k_starts: int32 [sequences + 1], ascending from 0.
  * fill: out's rows from starts[sequences] on are left as they are (0) or set
  *   to 0.
- * Scores, statistics and sums are fp32; p is rounded to dtype, relative to 2^r
- *   with r at most 8 below the running maximum of its exponent. The same call
- *   gives the same bits every time.
+ * Scores, statistics and sums are fp32; p is rounded to dtype (F16: what is lost
+ *   lies below 2^-32 of the largest so far). The same call gives the same bits
+ *   every time.
  * out may not overlap an input, but for columns of one buffer's rows.
  * workspace: device buffer of at least w8a8_packed_attention_workspace_size()
  *   bytes (16-byte aligned, any contents; NULL where that is 0): partial sums of

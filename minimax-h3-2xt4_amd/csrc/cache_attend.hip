@@ -50,9 +50,6 @@ constexpr int attend_dp(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 25
 // 394 us instead of 349.
 constexpr int attend_per_cu(int dim) { return dim > 128 ? 1 : 2; }
 constexpr int attend_fit(int dim) { return dim > 128 ? 1 : 3; }
-// The reference of p may lie so much below the maximum (as a power of 2): rescaling
-// the sums is rare.
-constexpr float kSlack = 8.0f;
 // Codes: P is p times the value's scale, and relative to a reference of its own, of
 // what keys contribute, so that no key's scale takes precision from keys of more
 // weight (relative to the largest scale, a row 2^18 times the others' with a weight
@@ -436,7 +433,7 @@ __global__ __launch_bounds__(64 * kAttendWaves, attend_fit(DP)) void cache_atten
         }
         ref = to;
       }
-      const float base = ref == -INFINITY ? 0.0f : CODES ? ref + kSlack : ref;
+      const float base = ref == -INFINITY ? 0.0f : CODES ? ref + kSlack : ref - kLift<DT>;
       float w[4 * G];
 #pragma unroll
       for (int i = 0; i < 4 * G; ++i) w[i] = __builtin_amdgcn_exp2f(t[i] - base);

@@ -72,10 +72,6 @@ __device__ __forceinline__ v16f mfma32(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
 }
 
-// The reference of p may lie so much below the maximum (as a power of 2): p is
-// at most 2^kSlack, far inside both types, and rescaling the sums is rare.
-constexpr float kSlack = 8.0f;
-
 // Both halves' values of a pair of lanes l, l ^ 32.
 __device__ __forceinline__ std::pair<float, float> lane_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -374,7 +370,7 @@ struct Packed {
 
 // The sums, the exponent that p is relative to and this half's sum of p. The
 // reference follows the maximum only once that lies more than kSlack above it.
-template <int DF>
+template <int DT, int DF>
 struct PackedState {
   v16f o[DF];
   float ref, l;
@@ -396,7 +392,7 @@ struct PackedState {
 #pragma unroll
       for (int x = 0; x < 16; ++x) o[f][x] = o[f][x] * fade;
   }
-  __device__ __forceinline__ float at() const { return ref == -INFINITY ? 0.0f : ref; }
+  __device__ __forceinline__ float at() const { return ref == -INFINITY ? 0.0f : ref - kLift<DT>; }
 };
 
 // The walk again for a workgroup with sums that are not finite, causal only: a
@@ -411,7 +407,7 @@ __device__ __forceinline__ void packed_careful(const PackedParams& p, char* tile
   const W w(p, tiles, tid);
   v4u qf[W::NS];
   w.queries(qf);
-  PackedState<W::DF> st;
+  PackedState<DT, W::DF> st;
   st.clear();
 #pragma unroll 1
   for (int j = 0; j < w.blocks; ++j) {
@@ -499,7 +495,7 @@ __global__ __launch_bounds__(64 * kPackWaves, DP > 128 ? 1 : 2) void packed_atte
   }
   v4u qf[NS];
   w.queries(qf);
-  PackedState<DF> st;
+  PackedState<DT, DF> st;
   st.clear();
 
   // Step j with block j's scores in s and K of block j + 1 and V of block j in

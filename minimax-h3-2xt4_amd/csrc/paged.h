@@ -33,6 +33,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
 }
 
+// The reference of p may lie so much below the maximum of its exponent (as a power
+// of 2): rescaling the sums is rare.
+constexpr float kSlack = 8.0f;
+// P is p times 2^kLift, so that it ends at 2^15 in fp16, of its 2^16, and what is lost
+// there lies below 2^-32 of the largest p: relative to the reference itself, 2^-25,
+// thousands of keys that share a part of the weight were 0 beside one key.
+template <int DT>
+constexpr float kLift = DT == kF16 ? 7.0f : 0.0f;
+
 // l plus the two DT values of a word.
 template <int DT>
 __device__ __forceinline__ float add2(uint32_t w, float l) {

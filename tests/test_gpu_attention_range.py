@@ -8,6 +8,7 @@ import torch
 from attention_refs import attention64, bound, check, quantize64
 from w8a8 import kv_cache
 from w8a8.kv_cache import KVCache
+from w8a8.packed_attention import packed_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +106,42 @@ def test_codes_of_the_largest_values(gpu):
     v[::3], v[1::3] = 0.0, torch.finfo(torch.bfloat16).max / 4
     q = torch.randn((1, 4, 64), generator=g).bfloat16().cuda()
     attend_codes(k, v, torch.ones(150, device='cuda'), torch.bfloat16, q)
+
+
+def held_of(dtype, n, dim, t, v):
+    """(q, k, v) of one head: scores of about t (powers of 2) with every query."""
+    return keys_with_scores(1.0, t.cuda(), dim, dtype), v.to(dtype).cuda()
+
+
+def check_tail(y, q, k, v, nq_first, what):
+    """y [nq, heads, dim]; query i sees the keys before nq_first[i]. What fp16 loses of P
+    lies below 2^-32 of the largest."""
+    dim = q.shape[2]
+    for h in range(q.shape[1]):
+        o, parts = attention64(q[:, h].double(), k[:, 0].double(), v[:, 0].double(), dim ** -0.5, nq_first)
+        a, lost, d, nk, codes = parts
+        check(y[:, h], o, bound(o, (a, lost * 2.0 ** -7, d, nk, codes), q.dtype), f'{what} head {h}')
+
+
+@pytest.mark.parametrize('dim', [64, 80, 128, 256])
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n', [500, 5000])
+def test_many_keys_of_little_weight(gpu, dtype, dim, n):
+    """One key of nearly all the weight whose value is 0: the others, of weights from
+    2^-24 to 2^-30, are what is left."""
+    g = torch.Generator().manual_seed(dim)
+    q = (1.0 + 0.01 * torch.randn((40, 2, dim), generator=g)).to(dtype).cuda()
+    for at in (0, 70, n - 41):
+        t = -24.0 - 6.0 * torch.rand(n, generator=g)
+        t[at] = 0.0
+        v = 100.0 + torch.randn((n, 1, dim), generator=g)
+        v[at] = 0.0
+        k, v = held_of(dtype, n, dim, t, v)
+        cache, table, length = paged(k, v, dtype)
+        check_tail(kv_cache.attend(q[:1], cache, table, length), q[:1], k, v, None, 'one token')
+        for nq in (1, 40):
+            starts, k_starts = (torch.tensor([0, m], dtype=torch.int32, device='cuda') for m in (nq, n))
+            for causal in (False, True):
+                first = torch.arange(nq, device='cuda') + n - nq + 1 if causal else None
+                y = packed_attention(q[:nq], k, v, starts, k_starts, causal=causal)
+                check_tail(y, q[:nq], k, v, first, f'{nq} rows, causal {causal}')
