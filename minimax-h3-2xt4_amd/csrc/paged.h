@@ -38,9 +38,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 constexpr float kSlack = 8.0f;
 // P is p times 2^kLift, so that it ends at 2^15 in fp16, of its 2^16, and what is lost
 // there lies below 2^-32 of the largest p: relative to the reference itself, 2^-25,
-// thousands of keys that share a part of the weight were 0 beside one key.
+// thousands of keys that share a part of the weight were 0 beside one key. In bf16,
+// whose values reach 2^128 as fp32 sums do, it is at most 1: finite values weigh in
+// as finite products.
 template <int DT>
-constexpr float kLift = DT == kF16 ? 7.0f : 0.0f;
+constexpr float kLift = DT == kF16 ? 7.0f : -kSlack;
 
 // l plus the two DT values of a word.
 template <int DT>

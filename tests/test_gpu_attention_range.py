@@ -145,3 +145,24 @@ def test_many_keys_of_little_weight(gpu, dtype, dim, n):
                 first = torch.arange(nq, device='cuda') + n - nq + 1 if causal else None
                 y = packed_attention(q[:nq], k, v, starts, k_starts, causal=causal)
                 check_tail(y, q[:nq], k, v, first, f'{nq} rows, causal {causal}')
+
+
+@pytest.mark.parametrize('dim', [64, 80, 128, 256])
+@pytest.mark.parametrize('n', [300, 5000])
+def test_values_near_the_largest(gpu, dim, n):
+    """Finite bf16 values whose weighted sum is finite, behind keys of less weight."""
+    g = torch.Generator().manual_seed(dim)
+    q = (1.0 + 0.01 * torch.randn((40, 2, dim), generator=g)).bfloat16().cuda()
+    t = torch.full((n,), -7.5)
+    t[n - 45] = 0.0
+    v = torch.randn((n, 1, dim), generator=g)
+    v[n - 45] = 3e38
+    k, v = held_of(torch.bfloat16, n, dim, t, v)
+    cache, table, length = paged(k, v, torch.bfloat16)
+    check_tail(kv_cache.attend(q[:1], cache, table, length), q[:1], k, v, None, 'one token')
+    for nq in (1, 40):
+        starts, k_starts = (torch.tensor([0, m], dtype=torch.int32, device='cuda') for m in (nq, n))
+        for causal in (False, True):
+            first = torch.arange(nq, device='cuda') + n - nq + 1 if causal else None
+            y = packed_attention(q[:nq], k, v, starts, k_starts, causal=causal)
+            check_tail(y, q[:nq], k, v, first, f'{nq} rows, causal {causal}')
