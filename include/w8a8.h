@@ -820,7 +820,8 @@ int w8a8_cache_read(const W8A8CacheReadArgs* args);
  * Attention of one new token of every sequence over its cached keys:
  *   out[b][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(sm_scale q[b][h] . k_j)
  * over the keys j < lengths[b] (within the table) of kv head
- * h / (heads / cache.heads); 0 where there are none.
+ * h / (heads / cache.heads); 0 where there are none, NaN where all scores are -inf.
+ * An infinite value gives an infinity, or NaN where its p is rounded to 0.
  * q, out: [sequences, heads, cache.dim] of dtype (F16 or BF16; a 16-bit
  *   cache's own), element strides {row, head}, channels contiguous, rows and
  *   heads on 16-byte boundaries.
@@ -869,8 +870,9 @@ int64_t w8a8_cache_attend_workspace_size(int64_t sequences, int64_t heads, int64
  *   out[i][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(sm_scale q[i][h] . k_j)
  * Query rows of sequence b are [starts[b], starts[b + 1]), its keys
  * [k_starts[b], k_starts[b + 1]); with causal != 0 query i of nq sees keys
- * j <= i + nk - nq, else all nk. 0 where it sees none. A masked key takes no
- * part, whatever it and its value hold.
+ * j <= i + nk - nq, else all nk. 0 where it sees none, NaN where all its scores are
+ * -inf. A masked key takes no part, whatever it and its value hold; an infinite
+ * value that is seen gives an infinity, or NaN where its p is rounded to 0.
  * q, out: [rows, heads, dim], k, v: [keys, kv_heads, dim], all of dtype (F16
  *   or BF16), element strides {row, head}, channels contiguous, rows and heads
  *   on 16-byte boundaries. Head h reads kv head h / (heads / kv_heads).

@@ -341,6 +341,7 @@ struct Packed {
   __device__ __forceinline__ void store(const v16f (&o)[DF], float ref, float l) const {
     const auto both = lane_halves(l);
     l = both.first + both.second;
+    ref = with_keys(ref, limit > 0);   // (of a range: whether the row sees keys from its first on)
     if constexpr (SPLIT) {
       if (!stored) return;
       const int64_t at = ((int64_t)split * p.rows + tile.row0 + query) * (p.group * p.kv_heads) + head;
@@ -353,7 +354,7 @@ struct Packed {
       if (half == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(ref, l);
       return;
     }
-    const float rcp = l == 0.0f ? 0.0f : 1.0f / l;
+    const float rcp = ref == -INFINITY ? 0.0f : 1.0f / l;
     if (!stored) return;
     char* at = to();
 #pragma unroll
@@ -686,7 +687,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackedParams p) {
       for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(x[i][e], f, y[e]);
     }
   }
-  const float rcp = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float rcp = ref == -INFINITY ? 0.0f : 1.0f / sum;
   *reinterpret_cast<uint2*>(p.out + row * p.o_row + head * p.o_head + 2 * d) =
       make_uint2(pack2<DT>(y[0] * rcp, y[1] * rcp), pack2<DT>(y[2] * rcp, y[3] * rcp));
 }

@@ -6,6 +6,7 @@
 #include "w8a8_host.h"
 #include "sequence_search.h"
 
+#include <cfloat>
 #include <cmath>
 #include <utility>
 
@@ -43,6 +44,10 @@ constexpr float kSlack = 8.0f;
 // as finite products.
 template <int DT>
 constexpr float kLift = DT == kF16 ? 7.0f : -kSlack;
+
+// The reference of a row with keys, whose scores are all -inf: 0 / 0 is its output,
+// and 0 that of a row without keys, whose reference is -inf.
+__device__ __forceinline__ float with_keys(float ref, bool any) { return any ? fmaxf(ref, -FLT_MAX) : ref; }
 
 // l plus the two DT values of a word.
 template <int DT>

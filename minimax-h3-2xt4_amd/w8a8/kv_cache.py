@@ -117,7 +117,8 @@ def attend(q, cache, page_table, lengths, *, scale=None, out=None):
     over the first lengths[b] keys of its pages (the new token's own included,
     once written): softmax(scale q . k) v, query head h with the cache's head
     h // (heads / cache.heads). scale: 1 / sqrt(dim) by default. A sequence
-    without keys gives 0. Inference only."""
+    without keys gives 0, one whose scores are all -inf NaN, an infinite value
+    an infinity or, where its weight is rounded to 0, NaN. Inference only."""
     y = _abi.native().cache_attend(cache.k, cache.v, cache.k_scale, cache.v_scale, q, page_table, lengths, scale, out)
     if y is not None:
         return y

@@ -19,7 +19,8 @@ def packed_attention(q, k, v, starts, k_starts=None, *, causal=True, scale=None,
     default). causal: of nq queries and nk keys, query i sees the keys up to
     i + nk - nq (a prompt's next part behind its cached keys); a query that sees
     none gives 0, and what it does not see has no effect, infinities and NaNs
-    included. scale: 1 / sqrt(dim) by default. out: to write into, its rows
+    included. A query whose scores are all -inf gives NaN; an infinite value that
+    it sees gives an infinity or, where its weight is rounded to 0, NaN. scale: 1 / sqrt(dim) by default. out: to write into, its rows
     behind the last sequence staying as they are; a new output has zeros there.
     Inference only."""
     y = _abi.native().packed_attention(q, k, v, starts, k_starts, causal, scale, out)

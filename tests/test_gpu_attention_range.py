@@ -166,3 +166,52 @@ def test_values_near_the_largest(gpu, dim, n):
             first = torch.arange(nq, device='cuda') + n - nq + 1 if causal else None
             y = packed_attention(q[:nq], k, v, starts, k_starts, causal=causal)
             check_tail(y, q[:nq], k, v, first, f'{nq} rows, causal {causal}')
+
+
+@pytest.mark.parametrize('dim', [64, 80, 128, 256])
+@pytest.mark.parametrize('n', [300, 5000])
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_scores_of_minus_infinity(gpu, dtype, dim, n):
+    """Keys with the score -inf have no weight; if a query sees no others it is 0 / 0, and if it sees no key 0."""
+    g = torch.Generator().manual_seed(dim)
+    q = (1.0 + 0.01 * torch.randn((40, 2, dim), generator=g)).to(dtype).cuda()
+    k, v = (torch.randn((n, 1, dim), generator=g).to(dtype).cuda() for _ in range(2))
+    k[:, :, 3] = -math.inf
+    nq = 40
+    starts = torch.tensor([0, nq], dtype=torch.int32, device='cuda')
+    k_starts = torch.tensor([0, n], dtype=torch.int32, device='cuda')
+    cache, table, length = paged(k, v, dtype)
+    assert bool(torch.isnan(kv_cache.attend(q[:1], cache, table, length)).all())
+    assert not bool(kv_cache.attend(q[:1], cache, table, length * 0).any())
+    assert not bool(kv_cache.attend(q[:1], cache, table * 0 - 1, length).any())
+    for causal in (False, True):
+        assert bool(torch.isnan(packed_attention(q, k, v, starts, k_starts, causal=causal)).all())
+    few = 30   # of 40 queries the first 10 see no key
+    y = packed_attention(q, k[:few], v[:few], starts, torch.tensor([0, few], dtype=torch.int32, device='cuda'))
+    assert not bool(y[:10].any()) and bool(torch.isnan(y[10:]).all())
+    # some keys with a score: those alone count
+    seen = torch.zeros(n, dtype=torch.bool)
+    seen[torch.tensor([60, n // 2, n - 60])] = True
+    k[seen] = torch.randn((3, 1, dim), generator=g).to(dtype).cuda()
+    cache, table, length = paged(k, v, dtype)
+    o, parts = zip(*(attention64(q[:, h].double(), k[seen][:, 0].double(), v[seen][:, 0].double(), dim ** -0.5) for h in range(2)))
+    for h in range(2):
+        check(kv_cache.attend(q[:1], cache, table, length)[:, h], o[h][:1],
+              bound(o[h], parts[h], dtype)[:1], 'one token')
+        for causal in (False, True):
+            y = packed_attention(q, k, v, starts, k_starts, causal=causal)
+            check(y[:, h], o[h], bound(o[h], parts[h], dtype), f'causal {causal}')
+
+
+def test_codes_with_scores_of_minus_infinity(gpu):
+    """The same of codes, by scales of k that are infinite."""
+    q = torch.ones((1, 2, 64), dtype=torch.float16, device='cuda')
+    k, v = -torch.ones((300, 1, 64), dtype=torch.float16, device='cuda'), torch.ones((300, 1, 64), dtype=torch.float16, device='cuda')
+    for n in (300, 5000):
+        cache, table, length = paged(k.repeat(17, 1, 1)[:n], v.repeat(17, 1, 1)[:n], torch.int8)
+        cache.k_scale.fill_(math.inf)
+        assert bool(torch.isnan(kv_cache.attend(q, cache, table, length)).all())
+        assert not bool(kv_cache.attend(q, cache, table, length * 0).any())
+        cache.k_scale[0, 0, 7] = 1.0
+        check(kv_cache.attend(q, cache, table, length)[0], torch.ones((2, 64), dtype=torch.float64, device='cuda'),
+              torch.full((2, 64), 2.0 ** -10, dtype=torch.float64, device='cuda'))
