@@ -762,7 +762,8 @@ typedef struct W8A8KvCache {
  *   share), either may remain, or parts of both.
  * k and v may not overlap the cache, nor places of the cache each other: its
  *   strides nest (each is at least what the smaller ones reach), and k and v, and
- *   their scales, lie apart or are columns of one buffer.
+ *   their scales, lie apart or are columns of one buffer; so do codes and scales,
+ *   a page's or a head's side by side.
  */
 typedef struct W8A8CacheWriteArgs {
   uint32_t struct_size;

@@ -733,8 +733,7 @@ extern "C" int w8a8_cache_attend(const W8A8CacheAttendArgs* a) {
   W8A8_REQUIRE(rows_apart(a->sequences, a->heads, a->cache.dim, a->out_strides), "%s: output rows overlap", who);
   const RowsOf om = rows_memory(a->out, a->sequences, a->heads, a->cache.dim, a->out_strides);
   W8A8_REQUIRE(apart(om, rows_memory(a->q, a->sequences, a->heads, a->cache.dim, a->q_strides)), "%s: out overlaps q", who);
-  W8A8_REQUIRE(apart(om, cache_memory(a->cache, a->cache.k)) && apart(om, cache_memory(a->cache, a->cache.v)),
-               "%s: out overlaps the cache", who);
+  W8A8_REQUIRE(apart_from_cache(om, a->cache), "%s: out overlaps the cache", who);
   W8A8_REQUIRE(a->table_width >= 0 && a->table_width * a->cache.page_size < (1ll << 27) &&
                    (a->table_width == 0 || a->page_table) && (a->sequences == 1 || a->ld_table >= a->table_width) && a->lengths,
                "%s: page table or lengths null, table rows overlap, or 2^27 keys and more", who);

@@ -329,7 +329,7 @@ static int move_params(const char* who, int dtype, const W8A8KvCache& c, const v
                    (sequences <= 1 || ld_table >= width),
                "%s: page table null, its rows overlap, or 2^27 keys and more", who);
   for (const RowsOf& r : {rows_memory(k, rows, c.heads, c.dim, kst), rows_memory(v, rows, c.heads, c.dim, vst)})
-    W8A8_REQUIRE(apart(r, cache_memory(c, c.k)) && apart(r, cache_memory(c, c.v)), "%s: rows overlap the cache", who);
+    W8A8_REQUIRE(apart_from_cache(r, c), "%s: rows overlap the cache", who);
   p.k = reinterpret_cast<char*>(const_cast<void*>(k));
   p.v = reinterpret_cast<char*>(const_cast<void*>(v));
   p.k_row = 2 * kst[0]; p.k_head = 2 * kst[1]; p.v_row = 2 * vst[0]; p.v_head = 2 * vst[1];

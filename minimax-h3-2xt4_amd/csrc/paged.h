@@ -6,6 +6,7 @@
 #include "w8a8_host.h"
 #include "sequence_search.h"
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <utility>
@@ -130,10 +131,19 @@ inline RowsOf cache_memory(const W8A8KvCache& c, const void* p) {
   const int64_t page = (c.heads - 1) * c.strides[1] + (c.page_size - 1) * c.strides[2] + c.dim;
   return rows_of(p, c.strides[0], c.pages, page, es);
 }
+inline RowsOf scale_memory(const W8A8KvCache& c, const float* p) {
+  return rows_of(p, c.scale_strides[0], c.pages, (c.heads - 1) * c.scale_strides[1] + c.page_size, 4);
+}
+// Whether rows share no byte with a cache's keys, values and scales.
+inline bool apart_from_cache(const RowsOf& r, const W8A8KvCache& c) {
+  return apart(r, cache_memory(c, c.k)) && apart(r, cache_memory(c, c.v)) &&
+         (c.dtype != W8A8_I8 || (apart(r, scale_memory(c, c.k_scale)) && apart(r, scale_memory(c, c.v_scale))));
+}
 
-// Runs of `extent` bytes, one at each place of a nest of steps.
+// Runs of `extent` bytes, or of another such nest of `other` bytes, one at each
+// place of a nest of steps.
 struct Places {
-  int64_t step[3], count[3], extent;   // the larger steps first
+  int64_t step[3], count[3], extent, other;   // the larger steps first
 };
 // Sorted by their steps; false where steps are less than what they step over.
 inline bool places_nest(Places& p) {
@@ -143,7 +153,7 @@ inline bool places_nest(Places& p) {
         std::swap(p.step[i], p.step[j]);
         std::swap(p.count[i], p.count[j]);
       }
-  int64_t span = p.extent;
+  int64_t span = std::max(p.extent, p.other);
   for (int i = 2; i >= 0; --i) {
     if (p.count[i] <= 1) continue;
     if (p.step[i] < span) return false;
@@ -151,28 +161,36 @@ inline bool places_nest(Places& p) {
   }
   return true;
 }
-// Whether two such nests, `off` bytes apart, share a byte. Places differ by sums
+// Whether two such nests, the other `off` bytes behind the one, share a byte. Places differ by sums
 // c_i step_i, |c_i| < count_i, and what the inner steps reach is less than a step,
 // so that c_i is one of two.
 inline bool places_meet(const Places& p, int64_t off, int i = 0) {
-  if (i == 3) return -p.extent < off && off < p.extent;
+  if (i == 3) return -p.other < off && off < p.extent;
   if (p.count[i] <= 1) return places_meet(p, off, i + 1);
   const int64_t c = off / p.step[i] - (off % p.step[i] < 0);
   for (int64_t at : {c, c + 1})
     if (-p.count[i] < at && at < p.count[i] && places_meet(p, off - at * p.step[i], i + 1)) return true;
   return false;
 }
-// Whether every key, value and scale of a cache has memory of its own.
+// Whether every key, value and scale of a cache has memory of its own. Codes and
+// scales have it where all of a page's lie apart, or all of a head's in steps that
+// both take.
 inline bool places_apart(const W8A8KvCache& c) {
-  const int es = c.dtype == W8A8_I8 ? 1 : 2;
+  const bool codes = c.dtype == W8A8_I8;
+  const int64_t es = codes ? 1 : 2, row = c.dim * es, scales = 4ll * c.page_size;
+  const int64_t page = c.strides[0] * es, head = c.strides[1] * es, token = c.strides[2] * es;
+  const int64_t s_page = c.scale_strides[0] * 4, s_head = c.scale_strides[1] * 4;
   auto own = [](Places p, const void* a, const void* b) {
     return places_nest(p) && !places_meet(p, (int64_t)((uintptr_t)b - (uintptr_t)a));
   };
-  return own({{c.strides[0] * es, c.strides[1] * es, c.strides[2] * es}, {c.pages, c.heads, c.page_size}, (int64_t)c.dim * es},
-             c.k, c.v) &&
-         (c.dtype != W8A8_I8 ||
-          own({{c.scale_strides[0] * 4, c.scale_strides[1] * 4, 0}, {c.pages, c.heads, 1}, 4ll * c.page_size}, c.k_scale,
-              c.v_scale));
+  auto beside = [&](const void* x, const float* s) {
+    return apart(cache_memory(c, x), scale_memory(c, s)) ||
+           ((c.pages == 1 || page == s_page) && (c.heads == 1 || head == s_head) &&
+            own({{page, head, 0}, {c.pages, c.heads, 1}, (c.page_size - 1) * token + row, scales}, x, s));
+  };
+  return own({{page, head, token}, {c.pages, c.heads, c.page_size}, row, row}, c.k, c.v) &&
+         (!codes || (own({{s_page, s_head, 0}, {c.pages, c.heads, 1}, scales, scales}, c.k_scale, c.v_scale) &&
+                     beside(c.k, c.k_scale) && beside(c.k, c.v_scale) && beside(c.v, c.k_scale) && beside(c.v, c.v_scale)));
 }
 
 }  // namespace w8a8

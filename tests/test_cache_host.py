@@ -145,6 +145,65 @@ def test_places_that_share_memory_are_not_written(change, codes, ok):
     assert rc == (_abi.OK if ok else _abi.ERR_INVALID) and (ok or 'share memory' in message), message
 
 
+@pytest.mark.parametrize('change,ok', [
+    # codes of 2 heads, 16 tokens of 64 (2048 bytes a page), scales of 64 bytes a head
+    (dict(k_scale=1 << 30), False),                                                     # in k's own pages
+    (dict(v_scale=(1 << 30) + 1024), False),
+    (dict(k_scale=(2 << 30) + 9 * 2048 + 2032), False),                                 # v's last codes
+    (dict(k_scale=(2 << 30) + 10 * 2048), True),                                        # behind them
+    (dict(k_scale=(2 << 30) - (9 * 128 + 128)), True),                                  # before the first
+    (dict(k_scale=(2 << 30) - (9 * 128 + 112)), False),
+    # a page's codes, then its scales
+    (dict(strides=(2048 + 128, 1024, 64), k_scale=(1 << 30) + 2048, scale_strides=(544, 16),
+          v_scale=(2 << 30) + 2048), True),
+    (dict(strides=(2048 + 128, 1024, 64), k_scale=(1 << 30) + 2032, scale_strides=(544, 16),
+          v_scale=(2 << 30) + 2048), False),
+    (dict(strides=(2048 + 128, 1024, 64), k_scale=(1 << 30) + 2048, scale_strides=(544, 16),
+          v_scale=(2 << 30) + 2064), False),                                            # the next page's codes
+    (dict(strides=(2048 + 128, 1024, 64), k_scale=(1 << 30) + 2048, scale_strides=(548, 16),
+          v_scale=(2 << 30) + 2048), False),                                            # steps of another length
+    # a head's codes, then its scales
+    (dict(strides=(2 * 1088, 1088, 64), k_scale=(1 << 30) + 1024, scale_strides=(544, 272),
+          v_scale=(2 << 30) + 1024), True),
+    (dict(strides=(2 * 1088, 1088, 64), k_scale=(1 << 30) + 1008, scale_strides=(544, 272),
+          v_scale=(2 << 30) + 1024), False),
+    (dict(strides=(2 * 1088, 1088, 64), k_scale=(1 << 30) + 1024, scale_strides=(544, 272),
+          v_scale=(2 << 30) + 1040), False),
+    # heads before pages
+    (dict(strides=(1088, 10 * 1088, 64), k_scale=(1 << 30) + 1024, scale_strides=(272, 2720),
+          v_scale=(2 << 30) + 1024), True),
+    (dict(strides=(1088, 10 * 1088, 64), k_scale=(1 << 30) + 1024, scale_strides=(272, 2720),
+          v_scale=(2 << 30) + 1040), False),
+    # tokens before heads, a page's scales behind its codes
+    (dict(strides=(2176, 64, 128), k_scale=(1 << 30) + 2048, scale_strides=(544, 16), v_scale=(2 << 30) + 2048), True),
+    (dict(strides=(2176, 64, 128), k_scale=(1 << 30) + 2016, scale_strides=(544, 16), v_scale=(2 << 30) + 2048), False),
+    # one page, whose step is not taken
+    (dict(pages=1, strides=(0, 1088, 64), k_scale=(1 << 30) + 1024, scale_strides=(4, 272), v_scale=(2 << 30) + 1024), True),
+    # k, v and both scales in one page
+    (dict(v=(1 << 30) + 2048, strides=(4352, 1024, 64), k_scale=(1 << 30) + 4096, scale_strides=(1088, 16),
+          v_scale=(1 << 30) + 4224), True),
+    (dict(v=(1 << 30) + 2048, strides=(4352, 1024, 64), k_scale=(1 << 30) + 4096, scale_strides=(1088, 16),
+          v_scale=(1 << 30) + 4352), False),
+])
+def test_codes_and_scales_that_share_memory_are_not_written(change, ok):
+    rc, message = _status('w8a8_cache_write', _args('write', dict(sequences=0), change, True))
+    assert rc == (_abi.OK if ok else _abi.ERR_INVALID) and (ok or 'share memory' in message), message
+
+
+@pytest.mark.parametrize('scale', [3 << 30, 4 << 30])
+def test_rows_over_scales_are_refused(scale):
+    """10 pages of 2 heads of 16 scales: 1280 bytes."""
+    for at in (scale, scale + 1264, scale - 512):
+        for which in ('write', 'read'):
+            for name in ('k', 'v'):
+                _refused(f'w8a8_cache_{which}', _args(which, {name: at}, codes=True), 'overlap the cache')
+        _refused('w8a8_cache_attend', _args('attend', dict(out=at), codes=True), 'out overlaps the cache')
+    for which in ('write', 'read'):   # behind them (the next refusal is another)
+        missing, fragment = (dict(lengths=None), 'lengths') if which == 'write' else (dict(starts=None), 'starts')
+        _refused(f'w8a8_cache_{which}', _args(which, {'k': scale + 1280, **missing}, codes=True), fragment)
+    _refused('w8a8_cache_attend', _args('attend', dict(out=scale + 1280, lengths=None), codes=True), 'lengths')
+
+
 @pytest.mark.parametrize('change,fragment', [
     (dict(q=None), 'q null'), (dict(out=(6 << 30) + 8), 'out null or misaligned'), (dict(q_strides=(516, 64)), 'q strides'),
     (dict(out_strides=(512, 0)), 'overlap'), (dict(out_strides=(448, 64)), 'overlap'), (dict(out=5 << 30), 'overlaps q'),
