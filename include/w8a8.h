@@ -763,7 +763,7 @@ typedef struct W8A8KvCache {
  * k and v may not overlap the cache, nor places of the cache each other: its
  *   strides nest (each is at least what the smaller ones reach), and k and v, and
  *   their scales, lie apart or are columns of one buffer; so do codes and scales,
- *   a page's or a head's side by side.
+ *   a page's or a head's side by side. The integers may not lie in the cache.
  */
 typedef struct W8A8CacheWriteArgs {
   uint32_t struct_size;
@@ -794,7 +794,7 @@ int w8a8_cache_write(const W8A8CacheWriteArgs* args);
  *   outside of its table).
  * fill: rows from starts[sequences] on are left as they are (0) or set to 0.
  * k and v may overlap neither each other nor the cache, but for columns of one
- *   buffer's rows.
+ *   buffer's rows, nor the integers.
  */
 typedef struct W8A8CacheReadArgs {
   uint32_t struct_size;
@@ -835,7 +835,8 @@ int w8a8_cache_read(const W8A8CacheReadArgs* args);
  *   bytes (16-byte aligned, any contents; NULL where that is 0): partial sums
  *   of sequences that several workgroups share. Calls that share one must not
  *   overlap; calls in sequence may, and a captured graph may replay it.
- * out may overlap neither q nor the cache, but for columns of one buffer's rows.
+ * out may overlap neither q nor the cache, but for columns of one buffer's rows,
+ *   nor the integers or the workspace.
  * Requirements: heads a multiple of cache.heads, up to 65536 each; sequences
  *   below 2^20; table_width * page_size below 2^27; sm_scale positive, finite (times log2(e) too).
  */
@@ -883,7 +884,8 @@ int64_t w8a8_cache_attend_workspace_size(int64_t sequences, int64_t heads, int64
  * Scores, statistics and sums are fp32; p is rounded to dtype (F16: what is lost
  *   lies below 2^-32 of the largest so far). The same call gives the same bits
  *   every time.
- * out may not overlap an input, but for columns of one buffer's rows.
+ * out may not overlap an input, but for columns of one buffer's rows, nor the
+ *   integers or the workspace.
  * workspace: device buffer of at least w8a8_packed_attention_workspace_size()
  *   bytes (16-byte aligned, any contents; NULL where that is 0): partial sums of
  *   calls of few rows and many keys. Calls that share one must not overlap;

@@ -742,6 +742,9 @@ extern "C" int w8a8_cache_attend(const W8A8CacheAttendArgs* a) {
   const int64_t need = w8a8_cache_attend_workspace_size(a->sequences, a->heads, a->cache.heads, a->cache.dim, keys);
   W8A8_REQUIRE(need == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= need),
                "%s: workspace of %lld bytes needed", who, (long long)need);
+  W8A8_REQUIRE(apart_from(om, a->page_table, table_bytes(a->sequences, a->ld_table, a->table_width)) &&
+                   apart_from(om, a->lengths, 4 * a->sequences) && apart_from(om, a->workspace, need),
+               "%s: page table, lengths or workspace lie in the output", who);
   p.q = reinterpret_cast<const char*>(a->q);
   p.out = reinterpret_cast<char*>(a->out);
   p.q_row = 2 * a->q_strides[0]; p.q_head = 2 * a->q_strides[1];

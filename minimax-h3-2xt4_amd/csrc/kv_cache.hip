@@ -363,6 +363,10 @@ extern "C" int w8a8_cache_write(const W8A8CacheWriteArgs* a) {
   W8A8_REQUIRE(a->sequences == 0 || a->lengths, "%s: null lengths", who);
   W8A8_REQUIRE(a->starts || a->rows == a->sequences, "%s: without starts every sequence has one row", who);
   W8A8_REQUIRE(places_apart(a->cache), "%s: keys or values of the cache share memory", who);
+  W8A8_REQUIRE(cache_apart_from(a->cache, a->page_table, table_bytes(a->sequences, a->ld_table, a->table_width)) &&
+                   cache_apart_from(a->cache, a->lengths, 4 * a->sequences) &&
+                   cache_apart_from(a->cache, a->starts, 4 * (a->sequences + 1)),
+               "%s: page table, lengths or starts lie in the cache", who);
   if (a->sequences == 0) return W8A8_OK;
   p.lengths = a->lengths;
   p.starts = a->starts;
@@ -385,6 +389,11 @@ extern "C" int w8a8_cache_read(const W8A8CacheReadArgs* a) {
                    apart(rows_memory(a->k, a->rows, a->cache.heads, a->cache.dim, a->k_strides),
                          rows_memory(a->v, a->rows, a->cache.heads, a->cache.dim, a->v_strides)),
                "%s: output rows overlap", who);
+  for (const RowsOf& r : {rows_memory(a->k, a->rows, a->cache.heads, a->cache.dim, a->k_strides),
+                          rows_memory(a->v, a->rows, a->cache.heads, a->cache.dim, a->v_strides)})
+    W8A8_REQUIRE(apart_from(r, a->page_table, table_bytes(a->sequences, a->ld_table, a->table_width)) &&
+                     apart_from(r, a->starts, 4 * (a->sequences + 1)),
+                 "%s: page table or starts lie in an output", who);
   p.starts = a->starts;
   p.fill = a->fill;
   return launch_move_type<false>(who, a->dtype, a->cache.dtype, p, reinterpret_cast<hipStream_t>(a->stream));

@@ -787,6 +787,9 @@ extern "C" int w8a8_packed_attention(const W8A8PackedAttentionArgs* a) {
   const int64_t need = w8a8_packed_attention_workspace_size(a->rows, a->keys, a->sequences, a->heads, a->kv_heads, a->dim);
   W8A8_REQUIRE(need == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= need),
                "%s: workspace of %lld bytes needed", who, (long long)need);
+  W8A8_REQUIRE(apart_from(om, a->starts, 4 * (a->sequences + 1)) && apart_from(om, a->k_starts, 4 * (a->sequences + 1)) &&
+                   apart_from(om, a->workspace, need),
+               "%s: starts or workspace lie in the output", who);
   const int64_t packed = a->rows * (a->heads / a->kv_heads), grid = (packed / kPackQ + a->sequences + 1) * a->kv_heads;
   W8A8_REQUIRE(packed < (1ll << 31) - kPackQ && grid * splits < (1 << 24), "%s: too many rows, sequences and heads for one launch", who);   // (2^32 work-items)
   const PackedParams p{reinterpret_cast<const char*>(a->q), reinterpret_cast<const char*>(a->k),

@@ -140,6 +140,20 @@ inline bool apart_from_cache(const RowsOf& r, const W8A8KvCache& c) {
          (c.dtype != W8A8_I8 || (apart(r, scale_memory(c, c.k_scale)) && apart(r, scale_memory(c, c.v_scale))));
 }
 
+// Whether rows, or a cache, share no byte with a run of them: the integers that a
+// kernel reads while it writes there, a workspace.
+inline bool apart_from(const RowsOf& r, const void* p, int64_t bytes) {
+  return !p || bytes <= 0 || apart(r, RowsOf{p, r.row, bytes, bytes});
+}
+inline bool cache_apart_from(const W8A8KvCache& c, const void* p, int64_t bytes) {
+  return apart_from(cache_memory(c, c.k), p, bytes) && apart_from(cache_memory(c, c.v), p, bytes) &&
+         (c.dtype != W8A8_I8 ||
+          (apart_from(scale_memory(c, c.k_scale), p, bytes) && apart_from(scale_memory(c, c.v_scale), p, bytes)));
+}
+inline int64_t table_bytes(int64_t sequences, int64_t ld, int64_t width) {
+  return sequences > 0 && width > 0 ? 4 * ((sequences - 1) * ld + width) : 0;
+}
+
 // Runs of `extent` bytes, or of another such nest of `other` bytes, one at each
 // place of a nest of steps.
 struct Places {

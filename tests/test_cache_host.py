@@ -204,6 +204,32 @@ def test_rows_over_scales_are_refused(scale):
     _refused('w8a8_cache_attend', _args('attend', dict(out=scale + 1280, lengths=None), codes=True), 'lengths')
 
 
+def test_integers_in_what_is_written_are_refused():
+    """Tables, lengths and starts that a kernel would write over while it reads them, and workspaces."""
+    none = dict(sequences=0)   # (launches nothing where it is not refused)
+    for codes, at in ((False, 1 << 30), (False, (2 << 30) + 40000), (True, (1 << 30) + 640), (True, 3 << 30), (True, (4 << 30) + 1276)):
+        for name in ('page_table', 'lengths', 'starts'):
+            _refused('w8a8_cache_write', _args('write', {name: at}, codes=codes), 'lie in the cache')
+    assert _status('w8a8_cache_write', _args('write', dict(none, starts=(2 << 30) + 40960)))[0] == _abi.OK
+    assert _status('w8a8_cache_write', _args('write', dict(none, starts=(1 << 30) - 4)))[0] == _abi.OK
+    # in the gaps between the pages' rows, and across them
+    gaps = dict(strides=(4096, 1024, 64))
+    assert _status('w8a8_cache_write', _args('write', dict(none, starts=(1 << 30) + 4096), gaps))[0] == _abi.OK
+    _refused('w8a8_cache_write', _args('write', dict(none, starts=(1 << 30) + 4092), gaps), 'lie in the cache')
+    for at in (5 << 30, (6 << 30) + 7 * 256 - 4):
+        for name in ('page_table', 'starts'):
+            _refused('w8a8_cache_read', _args('read', {name: at}), 'lie in an output')
+    for name in ('page_table', 'lengths'):
+        for at in (6 << 30, (6 << 30) + 3 * 1024 - 4, (6 << 30) - 8):
+            _refused('w8a8_cache_attend', _args('attend', {name: at}), 'lie in the output')
+    _refused('w8a8_cache_attend', _args('attend', dict(workspace=(6 << 30) - 16, **LONG)), 'lie in the output')
+    for change in (dict(starts=4 << 30), dict(k_starts=(4 << 30) - 8), dict(starts=(4 << 30) + 100 * 512 - 4)):
+        _refused('w8a8_packed_attention', _abi.PackedAttentionArgs(**{**PACKED, **change}), 'lie in the output')
+    few = dict(rows=16, keys=4000, sequences=1, workspace_bytes=1 << 30)
+    assert _abi.load().w8a8_packed_attention_workspace_size(16, 4000, 1, 4, 2, 64) > 0
+    _refused('w8a8_packed_attention', _abi.PackedAttentionArgs(**{**PACKED, **few, 'workspace': (4 << 30) - 16}), 'lie in the output')
+
+
 @pytest.mark.parametrize('change,fragment', [
     (dict(q=None), 'q null'), (dict(out=(6 << 30) + 8), 'out null or misaligned'), (dict(q_strides=(516, 64)), 'q strides'),
     (dict(out_strides=(512, 0)), 'overlap'), (dict(out_strides=(448, 64)), 'overlap'), (dict(out=5 << 30), 'overlaps q'),
