@@ -1,70 +1,21 @@
-// csrc/sequence_search.h on the CPU: 64 threads are a wave's lanes, which meet
-// at each ballot. A line "SEQUENCES ROW LENGTHS SIDE" on stdin asks for the
+// csrc/sequence_search.h on the CPU. A line "SEQUENCES ROW LENGTHS SIDE" on stdin asks for the
 // sequence that a row lies in, among the starts 0, 3, 3, 6, 6, 9, ... (LENGTHS 1:
 // with lengths, 100 + b). The starts and lengths lie at the beginning (SIDE 0) or the
 // end (SIDE 1) of memory that nothing around may be read of.
-#include <pthread.h>
-#include <stdint.h>
-#include <sys/mman.h>
-#include <unistd.h>
-
-#include <algorithm>
-#include <cstdio>
-#include <cstdlib>
-#include <thread>
-#include <vector>
-
-#define __device__
-#define __forceinline__ inline
-using std::min;
-
-static thread_local struct { unsigned x; } threadIdx;
-static pthread_barrier_t meet;
-static bool voted[64];
-static int held[64];
-
-static uint64_t __builtin_amdgcn_ballot_w64(bool x) {
-  voted[threadIdx.x] = x;
-  pthread_barrier_wait(&meet);
-  uint64_t m = 0;
-  for (int i = 0; i < 64; ++i) m |= (uint64_t)voted[i] << i;
-  pthread_barrier_wait(&meet);
-  return m;
-}
-static int __builtin_amdgcn_readlane(int v, int lane) {
-  held[threadIdx.x] = v;
-  pthread_barrier_wait(&meet);
-  const int r = held[lane];
-  pthread_barrier_wait(&meet);
-  return r;
-}
+#include "wave_shim.h"
 
 #include "sequence_search.h"
-
-static int32_t* guarded(int n, int side) {
-  const size_t page = (size_t)sysconf(_SC_PAGESIZE), bytes = 4 * (size_t)n, whole = (bytes + page - 1) / page * page;
-  char* at = static_cast<char*>(mmap(nullptr, whole + 2 * page, PROT_NONE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0));
-  if (at == MAP_FAILED || mprotect(at + page, whole, PROT_READ | PROT_WRITE)) std::abort();
-  return reinterpret_cast<int32_t*>(at + page + (side ? whole - bytes : 0));
-}
 
 int main() {
   int n, with_lengths, side;
   long long row;
-  pthread_barrier_init(&meet, nullptr, 64);
   while (std::scanf("%d %lld %d %d", &n, &row, &with_lengths, &side) == 4) {
     int32_t* starts = guarded(n + 1, side);
     int32_t* lengths = with_lengths ? guarded(std::max(n, 1), side) : nullptr;
     for (int b = 0; b <= n; ++b) starts[b] = (b + 1) / 2 * 3;
     for (int b = 0; with_lengths && b < n; ++b) lengths[b] = 100 + b;
     w8a8::SequenceRow r[64];
-    std::vector<std::thread> lanes;
-    for (unsigned lane = 0; lane < 64; ++lane)
-      lanes.emplace_back([&, lane] {
-        threadIdx.x = lane;
-        r[lane] = w8a8::sequence_of(starts, n, row, lengths);
-      });
-    for (std::thread& t : lanes) t.join();
+    wave([&](int lane) { r[lane] = w8a8::sequence_of(starts, n, row, lengths); });
     for (int i = 1; i < 64; ++i)
       if (r[i].b != r[0].b || r[i].first != r[0].first || r[i].last != r[0].last || r[i].length != r[0].length) return 2;
     std::printf("%d %d %d %d\n", r[0].b, r[0].first, r[0].last, r[0].length);

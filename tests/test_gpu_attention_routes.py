@@ -9,6 +9,7 @@ from test_gpu_kv_cache import TYPES, attend_case, check_attend, filled, kv_rows
 from test_gpu_packed_attention import run
 from w8a8 import _abi, kv_cache
 from w8a8.kv_cache import KVCache
+from w8a8.packed_attention import packed_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +111,24 @@ def test_moves_of_more_than_the_last_cache_holds(gpu, held, dim, heads):
 def test_keys_shared_by_workgroups(gpu, new, keys, dtype, dim, causal):
     assert _abi.load().w8a8_packed_attention_workspace_size(sum(new), sum(keys), len(new), 4, 2, dim) > 0
     run(dtype, 4, 2, dim, new, keys, causal, seed=dim)
+
+
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('sequences,rows,keys', [(4, 1500, 1700), (9, 1500, 1700), (4, 40, 6000), (9, 40, 6000)])
+def test_packed_starts_out_of_range_stay_in_bounds(gpu, sequences, rows, keys, causal):
+    """Whatever starts hold, only the output's rows are written; few sequences, a search, and keys
+    that workgroups share. (That the inputs are read within their rows is seen on the CPU: test_packed_tiles.)"""
+    heads, dim = 4, 64
+    assert (_abi.load().w8a8_packed_attention_workspace_size(rows, keys, sequences, heads, 2, dim) > 0) == (rows == 40)
+    big = torch.full((rows + 400, heads, dim), 7.0, dtype=torch.float16, device='cuda')
+    q = torch.zeros((rows, heads, dim), dtype=torch.float16, device='cuda')
+    k = torch.zeros((keys, 2, dim), dtype=torch.float16, device='cuda')
+    low, high = -2 ** 31, 2 ** 31 - 1
+    g = torch.Generator().manual_seed(sequences + rows)
+    pool = torch.tensor([low, high, -1, 0, 1, rows - 1, rows, rows + 1, keys, keys + 1, 90000, rows // 2])
+    for _ in range(8):
+        st, ks = (pool[torch.randint(0, len(pool), (sequences + 1,), generator=g)].int().cuda() for _ in range(2))
+        for starts, k_starts in ((st, ks), (st.sort().values, ks.sort().values)):
+            packed_attention(q, k, k, starts, k_starts, causal=causal, out=big[200:200 + rows])
+            packed_attention(q, k, k, starts, k_starts, causal=causal)
+    assert bool((big[:200] == 7.0).all()) and bool((big[200 + rows:] == 7.0).all())

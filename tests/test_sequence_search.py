@@ -17,7 +17,8 @@ def search(tmp_path_factory):
                     '-o', str(exe)], check=True)
 
     def run(cases):
-        res = subprocess.run([str(exe)], input=''.join('%d %d %d %d\n' % c for c in cases), text=True, capture_output=True)
+        res = subprocess.run([str(exe)], input=''.join('%d %d %d %d\n' % c for c in cases), text=True, capture_output=True,
+                             timeout=60)
         assert res.returncode == 0, f'status {res.returncode} after {len(res.stdout.splitlines())} of {len(cases)} cases'
         return [tuple(map(int, line.split())) for line in res.stdout.splitlines()]
     return run
