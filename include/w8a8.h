@@ -863,7 +863,8 @@ typedef struct W8A8CacheAttendArgs {
 
 int w8a8_cache_attend(const W8A8CacheAttendArgs* args);
 
-/* Workspace bytes of w8a8_cache_attend for these sizes on the current device. */
+/* Workspace bytes of w8a8_cache_attend for these sizes on the current device; 0
+ * for sizes that it refuses. */
 int64_t w8a8_cache_attend_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int32_t dim,
                                          int64_t max_keys);
 
@@ -924,7 +925,8 @@ typedef struct W8A8PackedAttentionArgs {
 
 int w8a8_packed_attention(const W8A8PackedAttentionArgs* args);
 
-/* Workspace bytes of w8a8_packed_attention for these sizes on the current device. */
+/* Workspace bytes of w8a8_packed_attention for these sizes on the current device;
+ * 0 for sizes that it refuses. */
 int64_t w8a8_packed_attention_workspace_size(int64_t rows, int64_t keys, int64_t sequences, int64_t heads,
                                              int64_t kv_heads, int32_t dim);
 

@@ -708,7 +708,9 @@ static int launch_attend_dim(const AttendParams& p, int64_t workgroups, hipStrea
 extern "C" int64_t w8a8_cache_attend_workspace_size(int64_t sequences, int64_t heads, int64_t kv_heads, int32_t dim,
                                                     int64_t max_keys) {
   using namespace w8a8;
-  if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim > 256) return 0;
+  if (sequences <= 0 || sequences >= (1 << 20) || heads <= 0 || heads > 65536 || kv_heads <= 0 || heads % kv_heads ||
+      dim <= 0 || dim > 256 || max_keys < 0 || max_keys >= (1 << 27))
+    return 0;
   const AttendPlan plan = attend_plan(sequences * attend_tiles(heads, kv_heads), max_keys, dim);
   return plan.whole ? 0 : plan.workgroups * (2 * kHeadTile * (attend_dp(dim) + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(int4));
 }

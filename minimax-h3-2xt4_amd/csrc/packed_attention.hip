@@ -629,7 +629,8 @@ static int packed_pitch(int dim) { return (packed_dp(dim) + 31) / 32 * 32; }
 // rows of a prompt 17 -> 29. (The halves of a workgroup of eight waves sharing the
 // keys and meeting in LDS: 353 rows 13.0 -> 14.7.)
 static int packed_splits(int64_t rows, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads, int dim) {
-  if (rows <= 0 || keys <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0) return 1;
+  if (rows <= 0 || rows >= (1 << 27) || keys <= 0 || keys >= (1 << 27) || sequences <= 0 || sequences >= (1 << 20)) return 1;
+  if (heads <= 0 || heads > 65536 || kv_heads <= 0 || heads % kv_heads || dim < 8 || dim > 256 || dim % 8) return 1;
   const int64_t filled = std::min(rows, sequences), tiles = (rows * (heads / kv_heads) + (kPackQ - 1) * filled) / kPackQ * kv_heads;
   const int64_t slots = (dim > 128 ? 1 : 2) * current_device_cus(), block = dim > 128 ? 32 : 64;
   const int64_t steps = (keys / sequences + block - 1) / block, splits = std::min(slots / tiles, std::max(steps / 4, std::min<int64_t>(steps / 2, 8)));

@@ -276,6 +276,22 @@ def test_packed_attention_refusals(change, fragment):
     _refused('w8a8_packed_attention', _abi.PackedAttentionArgs(**{**PACKED, **change}), fragment)
 
 
+def test_workspaces_of_sizes_that_are_refused():
+    lib = _abi.load()
+    good = (1, 4000, 1, 4, 2, 64)
+    assert lib.w8a8_packed_attention_workspace_size(*good) > 0
+    for i, values in enumerate([(0, -1, 1 << 27, (1 << 63) - 1), (0, -1, 1 << 27, (1 << 63) - 1), (0, -1, 1 << 20, (1 << 63) - 1),
+                                (0, -4, 1, 3, 65538, 1 << 62), (0, -2, 3, 8, 1 << 62), (0, -8, 4, 60, 264, (1 << 31) - 1)]):
+        for value in values:
+            assert lib.w8a8_packed_attention_workspace_size(*good[:i], value, *good[i + 1:]) == 0, (i, value)
+    good = (1, 8, 2, 128, 100000)
+    assert lib.w8a8_cache_attend_workspace_size(*good) > 0
+    for i, values in enumerate([(0, -1, 1 << 20, (1 << 63) - 1), (0, -2, 7, 65538, 1 << 62), (0, -2, 3, 16, 1 << 62),
+                                (0, -8, 264, (1 << 31) - 1), (-1, 1 << 27, (1 << 63) - 1)]):
+        for value in values:
+            assert lib.w8a8_cache_attend_workspace_size(*good[:i], value, *good[i + 1:]) == 0, (i, value)
+
+
 def test_packed_attention_of_nothing():
     assert _status('w8a8_packed_attention', _abi.PackedAttentionArgs(**{**PACKED, 'rows': 0}))[0] == _abi.OK
 
