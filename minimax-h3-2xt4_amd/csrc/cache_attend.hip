@@ -12,8 +12,8 @@
 // order. Loads run a block ahead, over the pairs' ends too.
 //
 // 131072 keys of 8 heads of 128 in bf16, 64 query heads (537 MB): 82 us and 5 for
-// the join, 6.2 TB/s in all; 64 contexts of 261850 keys as codes (555 MB): 93 to
-// 99 us and 5; 354 keys: 7 us, the launch and one pass of latencies. Four waves a
+// the join, 6.2 TB/s in all; 64 contexts of 261850 keys as codes (555 MB): 95 us
+// and 5; 354 keys: 7 us, the launch and one pass of latencies. Four waves a
 // workgroup and two of them a CU keep 8 KB and more a wave under way.
 //
 // A wave takes 32 keys of a block (two groups of 16, each within a page), and

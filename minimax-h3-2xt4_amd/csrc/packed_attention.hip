@@ -16,10 +16,11 @@
 // hands each lane four keys of one channel.
 //
 // Bound by the board's power where it is long: 16384 causal rows of 64 heads of
-// 128 in bf16 take 3.83 ms, 1148 TFLOP/s, with the MFMAs busy 62 % of the cycles at
-// 1.77 GHz. A loop of nothing but MFMAs and these LDS reads reaches 1540 TFLOP/s on
-// random operands, and 1170 with the softmax's instructions between them (1180 on
-// 16 x 16 x 32 MFMAs); the library's 8192^3 product 1185 to 1440. Moving work between
+// 128 in bf16 take 3.75 to 4.05 ms by the board, 1086 to 1174 TFLOP/s, with the MFMAs
+// busy 62 % of the cycles at 1.79 GHz. A loop of nothing but MFMAs and these LDS reads
+// reaches 1540 to 1640 TFLOP/s on random operands, and 1170 to 1220 with the softmax's
+// instructions between them (1180 to 1206 on 16 x 16 x 32 MFMAs); the library's 8192^3
+// product 1185 to 1440. Moving work between
 // the MFMAs, reading further ahead or raising waves' priorities changes it by less
 // than 1 %. Fewer instructions do: a lazy reference, a row sum by dot products of
 // the packed words. Two workgroups a CU, so that the two waves of a SIMD wait at
@@ -402,8 +403,9 @@ __device__ __forceinline__ void packed_careful(const PackedParams& p, char* tile
 // and, the last of them, between the first that add block j's values; between
 // the others it takes block j + 1's maximum. K of block j + 1 and V of block j are
 // read in a step, so K's copies run a step ahead of V's. The order is laid out
-// product by product (left to the compiler, all fragments are read at once, which
-// spills, and the VALU's work follows the MFMAs').
+// product by product (left to the compiler, all fragments are read at once, whose
+// registers spill, and the VALU's work follows the MFMAs'). As laid out the 128-wide
+// kernels still spill 6 to 10 registers, the others none.
 template <int DT, int DP, bool CAUSAL, bool SPLIT>
 __global__ __launch_bounds__(64 * kPackWaves, DP > 128 ? 1 : 2) void packed_attention_kernel(PackedParams p) {
   using W = Packed<DT, DP, CAUSAL, SPLIT>;
